@@ -315,7 +315,7 @@ def _handles(s):
     if case["op"] == "select":
         s["workspace"] = ti.select_pages_workspace(be, s["q"], s["kb"], s["block_tables"])
     elif case["op"] == "attend":
-        s["workspace"] = ti.sparse_attention_workspace(be, s["q"], s["k"], s["tables"])
+        s["workspace"] = ti.sparse_attention_workspace(be, s["q"], s["k"], s["tables"], s["max_new"])
     elif case["op"] == "verify":
         s["workspace"] = ti.verify_draft_workspace(be, s["target"])
 
@@ -340,7 +340,7 @@ def _own(s, op):
         return s["tables"], s["lengths"]
     if op == "attend":
         return ti.sparse_attention_(be, s["out"], s["workspace"], s["q"], s["k"], s["v"], s["tables"], s["lengths"],
-                                    1 / math.sqrt(case["head_dim"]))
+                                    1 / math.sqrt(case["head_dim"]), s["starts"], s["max_new"])
     ti.verify_draft_(be, s["accepted"], s["tokens"], s["workspace"], s["drafted"], s["target"], s["draft"], s["uniforms"], s["counts"])
     return s["accepted"], s["tokens"]
 
