@@ -221,6 +221,129 @@ int ti_attention_inputs(int dtype, void *q_out, const ti_kv_cache *cache, const 
                         int table_len, const int32_t *positions, const int32_t *slots, int n,
                         int q_heads, float eps, void *stream);
 
+/* ---- attention over chosen pages, and draft verification ----------------------------------
+ * No counterpart in the reference's ops: a long context read in part, and the end of the verify step
+ * that its speculative engine makes of attention calls.
+ * Rows of the packed token arrays that belong to no sequence (before query_start_loc[0], from
+ * query_start_loc[num_seqs] on) are left as they were by all of them. */
+
+/* Bounds of the keys of a layer's pages, kept beside its cache: for each page and KV head the keys'
+ * largest (first row) and smallest element in each dimension, rounded outward to whole multiples
+ * of the page's power of two `scale`. 16-byte aligned. */
+typedef struct {
+    int8_t *bounds;             /* [num_pages][Hk][2][D] */
+    float *scale;               /* [num_pages][Hk] */
+} ti_key_bounds;
+
+/*
+ * Refresh the bounds of the pages that hold the positions of a step (those of the step's queries, as
+ * in ti_attention_args: sequence b's n_b positions from positions[qsl[b]] on), from all keys that
+ * the cache holds in them up to the step's end. Called after the step's keys are written
+ * (ti_attention_inputs, ti_store_kv). The result depends on the cached keys alone, so a step that
+ * is taken back and written again needs no other call. For an INT8 cache a key is its value times
+ * scale times smoothing, rounded to float after each product. A page with a key that is not finite
+ * gets bounds 127 and -127 and an infinite scale, and is kept by every selection that reaches
+ * its score. Pages whose id lies outside the pool, or past the block-table row, are skipped. Two
+ * sequences of a call that write into one page are not supported: its bounds are one of the two's.
+ * head_dim 64 or 128. dtype: of dense pools.
+ */
+int ti_update_key_bounds(int dtype, const ti_kv_cache *cache, const ti_key_bounds *bounds,
+                         const int32_t *block_tables, int block_table_stride, const int32_t *positions,
+                         const int32_t *query_start_loc, int num_seqs, int max_query_len, int total_tokens,
+                         void *stream);
+
+/* Arguments of ti_select_pages; the step as in ti_attention_args. */
+typedef struct {
+    int32_t dtype;                    /* ti_dtype of q */
+    int32_t q_heads, kv_heads;        /* q_heads % kv_heads == 0, at most 64 query heads per KV head */
+    int32_t head_dim;                 /* 64 or 128 */
+    int32_t page_size, num_pages;
+    int32_t num_seqs, max_query_len, total_tokens;
+    int32_t block_table_stride;
+    int32_t keep;                     /* pages kept: the width of a table */
+    int32_t sinks, window;            /* the first and last pages always kept: sinks >= 0, window >= 1,
+                                         sinks + window <= keep */
+    int32_t causal;                   /* 1: a query sees the pages up to its own position's */
+    const void *q;                    /* [total_tokens][Hq][D] */
+    ti_key_bounds bounds;
+    const int32_t *positions, *query_start_loc, *block_tables;
+    int32_t *tables;                  /* [total_tokens][Hk][keep]: out */
+    int32_t *lengths;                 /* [total_tokens][Hk]: out */
+    void *workspace;                  /* 16-byte aligned */
+    size_t workspace_bytes;
+} ti_select_args;
+
+/*
+ * For each query token and KV head the `keep` pages of its sequence whose keys can matter most.
+ * A query head is taken as whole numbers w = rint(q / 2^e) (to even), 2^e the least power of two
+ * (from 2^-126 on) with |q| <= 127 2^e; a page's score is the largest over the KV head's query heads of
+ * 2^e scale sum_d (w_d hi_d where w_d > 0, else w_d lo_d), which no key inside the bounds exceeds
+ * (it is the sum of max(w_d hi_d, w_d lo_d), since hi_d >= lo_d). The first `sinks`
+ * and the last `window` visible pages are kept, then pages by score, equal ones in order; the sums
+ * are exact, so which are kept does not depend on how they are made. A query head with an element
+ * that is not finite scores 0 everywhere.
+ * tables: the kept pages' ids in order of position, zero-padded; lengths: the keys they hold up to
+ * the last visible one, as ti_sparse_attention takes them. All visible pages are kept while there
+ * are at most `keep`.
+ */
+int ti_select_pages_workspace_bytes(const ti_select_args *args, size_t *bytes);
+int ti_select_pages(const ti_select_args *args, void *stream);
+
+/* Arguments of ti_sparse_attention. */
+typedef struct {
+    int32_t dtype;                    /* ti_dtype of q, out (and dense pools) */
+    int32_t q_heads;                  /* q_heads % kv_heads == 0; bf16: at most 64 per KV head */
+    int32_t total_tokens;
+    int32_t table_width;              /* entries per table */
+    int32_t num_seqs, max_query_len;  /* the step that the tokens are: rows next to each other that belong
+                                         to one sequence are worked on together (max_query_len > 1);
+                                         results are the same within rounding */
+    const void *q;                    /* [total_tokens][Hq][D] */
+    void *out;                        /* [total_tokens][Hq][D] */
+    const int32_t *tables;            /* [total_tokens][Hk][table_width] 1-based page ids */
+    const int32_t *lengths;           /* [total_tokens][Hk] keys, at most table_width * page_size */
+    const int32_t *query_start_loc;   /* [num_seqs + 1], or NULL: every row belongs to a sequence */
+    float scale;                      /* softmax scale: finite and > 0 */
+    void *workspace;                  /* 16-byte aligned */
+    size_t workspace_bytes;
+} ti_sparse_attention_args;
+
+/*
+ * Attention of each query token and KV head over keys 0 .. length - 1 of its own table of pages, all
+ * of them visible: the last entry in use may hold fewer than page_size keys. A token without keys
+ * (length <= 0) gets zeros; longer lengths read as table_width * page_size. An entry outside the
+ * pool is clamped into it, as in ti_attention; a page that a table names twice counts twice.
+ */
+int ti_sparse_attention_workspace_bytes(const ti_sparse_attention_args *args, const ti_kv_cache *cache, size_t *bytes);
+int ti_sparse_attention(const ti_sparse_attention_args *args, const ti_kv_cache *cache, void *stream);
+
+/* Arguments of ti_verify_draft. */
+typedef struct {
+    int32_t dtype;                    /* ti_dtype of target and draft */
+    int32_t num_seqs, max_drafts;     /* B, N >= 0 */
+    int32_t vocab;                    /* V */
+    const int32_t *draft_tokens;      /* [B][N] 0-based */
+    const int32_t *draft_lens;        /* [B] drafts of each sequence (clamped to 0 .. N), or NULL: N */
+    const void *target;               /* [B][N + 1][V] the target's probabilities */
+    const void *draft;                /* [B][N][V] the drafter's, or NULL: it gave its tokens alone */
+    const float *uniforms;            /* [B][N + 1] in [0, 1): one per draft, the last for the drawn token */
+    int32_t *accepted;                /* [B]: out */
+    int32_t *tokens;                  /* [B][N + 1]: out, the accepted drafts, the drawn token, then -1 */
+    void *workspace;                  /* 16-byte aligned */
+    size_t workspace_bytes;
+} ti_verify_args;
+
+/*
+ * Speculative sampling: draft i is accepted while u_i q_i(x_i) < p_i(x_i) (q = 1 without a drafter's
+ * probabilities); after a of them one token is drawn with the last uniform from max(p_a - q_a, 0), or
+ * p_a without x_a, where a draft was rejected, and from p_a where none was: the lowest token with
+ * weight whose running sum exceeds u times the sum of all. Products and sums in double. Entries that
+ * are not positive and finite have no weight; without any weight p_a itself is taken, and -1 where
+ * that has none. A draft token outside [0, V) is rejected.
+ */
+int ti_verify_draft_workspace_bytes(const ti_verify_args *args, size_t *bytes);
+int ti_verify_draft(const ti_verify_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -94,6 +94,68 @@ long long prefill_grid_y(const ti_prefill_plan &pl) {
     return pl.pair ? (pl.qtiles + 1LL) / 2 : (long long)pl.qtiles * pl.splits;
 }
 
+bool misaligned(const void *p) { return ((uintptr_t)p & 15) != 0; }
+
+// A step's query tokens: uniform counts fill the packed arrays, grids hold the sequences.
+int check_step(int num_seqs, int max_query_len, int total_tokens, bool ragged) {
+    if (num_seqs <= 0 || max_query_len <= 0 || total_tokens <= 0) return TI_ERR_INVALID_ARG;
+    if (!ragged && (long long)num_seqs * max_query_len != total_tokens) return TI_ERR_INVALID_ARG;
+    return num_seqs > 65535 ? TI_ERR_UNSUPPORTED : TI_OK;
+}
+
+int check_select(const ti_select_args *a) {
+    if (!a || bad_dtype(a->dtype)) return TI_ERR_INVALID_ARG;
+    if (a->q_heads <= 0 || a->kv_heads <= 0 || a->q_heads % a->kv_heads || a->page_size <= 0 || a->num_pages <= 0 ||
+        a->block_table_stride <= 0 || a->keep <= 0)
+        return TI_ERR_INVALID_ARG;
+    if (a->sinks < 0 || a->window < 1 || (long long)a->sinks + a->window > a->keep) return TI_ERR_INVALID_ARG;
+    if (a->causal != 0 && a->causal != 1) return TI_ERR_INVALID_ARG;
+    if (!a->q || !a->bounds.bounds || !a->bounds.scale || !a->positions || !a->block_tables || !a->tables || !a->lengths)
+        return TI_ERR_INVALID_ARG;
+    if (misaligned(a->bounds.bounds)) return TI_ERR_INVALID_ARG;
+    const int st = check_step(a->num_seqs, a->max_query_len, a->total_tokens, a->query_start_loc);
+    if (st) return st;
+    if (a->head_dim != 64 && a->head_dim != 128) return TI_ERR_UNSUPPORTED;
+    // lengths are 32-bit
+    if (a->q_heads / a->kv_heads > 64 || (long long)a->keep * a->page_size > 0x7fffffffLL) return TI_ERR_UNSUPPORTED;
+    return TI_OK;
+}
+
+int check_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
+    if (!a || bad_cache(c) || bad_dtype(a->dtype)) return TI_ERR_INVALID_ARG;
+    if (c->head_dim != 64 && c->head_dim != 128) return TI_ERR_UNSUPPORTED;
+    if (a->q_heads <= 0 || a->q_heads % c->kv_heads || a->table_width <= 0) return TI_ERR_INVALID_ARG;
+    if (!a->q || !a->out || !a->tables || !a->lengths) return TI_ERR_INVALID_ARG;
+    if (!(a->scale > 0.0f) || a->scale == INFINITY) return TI_ERR_INVALID_ARG;
+    const int st = check_step(a->num_seqs, a->max_query_len, a->total_tokens, a->query_start_loc);
+    if (st) return st;
+    // lengths, work-groups (at most 16 a pair) and rows of q are counted in 32 bits; query heads take grid y
+    if ((long long)a->table_width * c->page_size > 0x7fffffffLL ||
+        (long long)a->total_tokens * a->q_heads * 16 > 0x7fffffffLL || a->q_heads > 65535)
+        return TI_ERR_UNSUPPORTED;
+    return a->dtype == TI_BF16 && a->q_heads / c->kv_heads > 64 ? TI_ERR_UNSUPPORTED : TI_OK;
+}
+
+int check_verify(const ti_verify_args *a) {
+    if (!a || bad_dtype(a->dtype)) return TI_ERR_INVALID_ARG;
+    if (a->num_seqs <= 0 || a->max_drafts < 0 || a->vocab <= 0) return TI_ERR_INVALID_ARG;
+    if (!a->target || !a->uniforms || !a->accepted || !a->tokens) return TI_ERR_INVALID_ARG;
+    if (a->max_drafts > 0 && !a->draft_tokens) return TI_ERR_INVALID_ARG;
+    // entries of a row are counted in 32 bits, sequences take grid y
+    return a->num_seqs > 65535 || a->vocab > 0x7fff0000 || a->max_drafts > 0xffff ? TI_ERR_UNSUPPORTED : TI_OK;
+}
+
+int check_workspace(const void *ws, size_t have, size_t need) {
+    if (need == 0) return TI_OK;
+    if (!ws || have < need) return TI_ERR_WORKSPACE;
+    return misaligned(ws) ? TI_ERR_INVALID_ARG : TI_OK;
+}
+
+size_t sparse_bytes(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
+    const int sp = ti_sparse_splits(a, c);
+    return sp == 1 ? 0 : (size_t)a->total_tokens * a->q_heads * sp * (c->head_dim + 2) * sizeof(float);
+}
+
 }  // namespace
 
 extern "C" {
@@ -225,6 +287,63 @@ int ti_attention_inputs(int dtype, void *q_out, const ti_kv_cache *c, const void
     if (!q_out || !qkv || !cos_sin || !positions || !slots) return TI_ERR_INVALID_ARG;
     return ti_launch_attention_inputs(dtype, q_out, c, qkv, q_norm, k_norm, cos_sin, table_len,
                                       positions, slots, n, q_heads, eps, (hipStream_t)stream);
+}
+
+int ti_update_key_bounds(int dtype, const ti_kv_cache *c, const ti_key_bounds *kb, const int32_t *block_tables,
+                         int block_table_stride, const int32_t *positions, const int32_t *query_start_loc,
+                         int num_seqs, int max_query_len, int total_tokens, void *stream) {
+    if (bad_dtype(dtype) || bad_cache(c) || !kb || !kb->bounds || !kb->scale) return TI_ERR_INVALID_ARG;
+    if (!block_tables || block_table_stride <= 0 || !positions || misaligned(kb->bounds)) return TI_ERR_INVALID_ARG;
+    const int st = check_step(num_seqs, max_query_len, total_tokens, query_start_loc);
+    if (st) return st;
+    if (c->head_dim != 64 && c->head_dim != 128) return TI_ERR_UNSUPPORTED;
+    return ti_launch_key_bounds(dtype, c, kb, block_tables, block_table_stride, positions, query_start_loc, num_seqs,
+                                max_query_len, total_tokens, (hipStream_t)stream);
+}
+
+int ti_select_pages_workspace_bytes(const ti_select_args *a, size_t *bytes) {
+    if (!bytes) return TI_ERR_INVALID_ARG;
+    *bytes = 0;
+    const int st = check_select(a);
+    if (st) return st;
+    *bytes = ti_select_bytes(a);
+    return TI_OK;
+}
+
+int ti_select_pages(const ti_select_args *a, void *stream) {
+    int st = check_select(a);
+    if (!st) st = check_workspace(a->workspace, a->workspace_bytes, ti_select_bytes(a));
+    return st ? st : ti_launch_select_pages(a, (hipStream_t)stream);
+}
+
+int ti_sparse_attention_workspace_bytes(const ti_sparse_attention_args *a, const ti_kv_cache *c, size_t *bytes) {
+    if (!bytes) return TI_ERR_INVALID_ARG;
+    *bytes = 0;
+    const int st = check_sparse(a, c);
+    if (st) return st;
+    *bytes = sparse_bytes(a, c);
+    return TI_OK;
+}
+
+int ti_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, void *stream) {
+    int st = check_sparse(a, c);
+    if (!st) st = check_workspace(a->workspace, a->workspace_bytes, sparse_bytes(a, c));
+    return st ? st : ti_launch_sparse_attention(a, c, (hipStream_t)stream);
+}
+
+int ti_verify_draft_workspace_bytes(const ti_verify_args *a, size_t *bytes) {
+    if (!bytes) return TI_ERR_INVALID_ARG;
+    *bytes = 0;
+    const int st = check_verify(a);
+    if (st) return st;
+    *bytes = ti_verify_bytes(a);
+    return TI_OK;
+}
+
+int ti_verify_draft(const ti_verify_args *a, void *stream) {
+    int st = check_verify(a);
+    if (!st) st = check_workspace(a->workspace, a->workspace_bytes, ti_verify_bytes(a));
+    return st ? st : ti_launch_verify_draft(a, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -177,3 +177,16 @@ int ti_launch_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, const
 // fp32 path: its key splits and workspace bytes (host shapes only).
 int ti_plan_generic(const ti_attention_args *a, const ti_kv_cache *c, size_t *bytes);
 int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStream_t s);
+
+// Attention over chosen pages (pa_sparse.hip, its fp32 kernels in pa_generic.hip).
+int ti_sparse_splits(const ti_sparse_attention_args *a, const ti_kv_cache *c);
+int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, hipStream_t s);
+int ti_launch_sparse_f32(const ti_sparse_attention_args *a, const ti_kv_cache *c, int splits, hipStream_t s);
+// Page bounds and the selection by them (page_bounds.hip).
+int ti_launch_key_bounds(int dtype, const ti_kv_cache *c, const ti_key_bounds *kb, const int32_t *bt, int bt_stride,
+                         const int32_t *positions, const int32_t *qsl, int num_seqs, int nmax, int total, hipStream_t s);
+size_t ti_select_bytes(const ti_select_args *a);
+int ti_launch_select_pages(const ti_select_args *a, hipStream_t s);
+// Draft verification (verify_draft.hip).
+size_t ti_verify_bytes(const ti_verify_args *a);
+int ti_launch_verify_draft(const ti_verify_args *a, hipStream_t s);

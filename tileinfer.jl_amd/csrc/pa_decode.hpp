@@ -64,6 +64,7 @@ struct DecodeParams {
     int B, flat;   // flat: work-groups per KV head shared by all sequences (0: `splits` each)
     int min_tiles;   // > 0: splits of at least this many 16-key tiles (f32_active_splits)
     float scale_log2;
+    const int32_t *lengths;   // SPARSE: keys of each (token, KV head); bt holds a table row for each
 };
 
 // Flat mode: the W = p.flat work-groups of a KV head are shared out over the B sequences
@@ -274,7 +275,10 @@ __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodePara
     }
 }
 
-template <int D, int ROWB, bool INT8, bool PG16, int NW, int RS, bool JOINT = false>
+// SPARSE: every (token, KV head) pair has a table of pages and a length of its own (pa_sparse.hip);
+// a pair is a sequence of one token whose last key is at lengths - 1, and a 1-D grid holds the
+// pairs' splits, KV heads innermost.
+template <int D, int ROWB, bool INT8, bool PG16, int NW, int RS, bool JOINT = false, bool SPARSE = false>
 __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     constexpr int NKB = D / 32;          // 32-wide head-dim blocks (QK MFMAs per tile)
     constexpr int NDT = D / 16;          // 16-wide head-dim tiles (PV MFMAs per tile)
@@ -303,10 +307,26 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     // RS = 2: waves pair up on the same keys, wave w holding rows MP*(w%2) .. + MP.
     const int rslice = RS == 2 ? (w & 1) : 0, kw = RS == 2 ? (w >> 1) : w;
     const int row0 = rslice * MP;
-    const int h = blockIdx.y;
+    const int pair = SPARSE ? (int)(blockIdx.x / (unsigned)p.splits) : 0;
+    const int h = SPARSE ? pair % p.Hk : (int)blockIdx.y;
     int s, b, nsp, tok0, nb, start;
     size_t unit;   // this work-group's partial slot
-    if (p.flat) {
+    if constexpr (SPARSE) {
+        s = (int)blockIdx.x - pair * p.splits;
+        b = pair;
+        nsp = p.splits;
+        tok0 = pair / p.Hk;
+        nb = 1;
+        unit = blockIdx.x;
+        if (p.qsl && (tok0 < p.qsl[0] || tok0 >= p.qsl[p.B])) return;   // a row of no sequence
+        start = min(p.lengths[pair], p.bt_stride * p.P) - 1;
+        if (start < 0) {   // no keys: zeros (the combine's, where the keys are split)
+            if (nsp == 1)
+                for (int i = threadIdx.x; i < p.G * D / 4; i += NW * 64)
+                    *reinterpret_cast<u32x2 *>(p.out + ((size_t)tok0 * p.Hq + h * p.G) * D + 4 * i) = (u32x2){0u, 0u};
+            return;
+        }
+    } else if (p.flat) {
         const FlatPiece f = flat_piece(p, blockIdx.x, lane);
         b = f.b;
         s = blockIdx.x - f.lo;

@@ -27,22 +27,36 @@ struct GenericParams {
     float *part;                 // split partials [B][Hk][splits][G nmax][D + 2]
     int bt_stride, num_pages, P, Hk, Hq, G, nmax, causal, splits;
     float scale_log2;
+    const int32_t *lengths;      // SPARSE: keys of each (token, KV head)
+    int B;
 };
 
-template <typename T, bool INT8, int D>
+// SPARSE: (token, KV head) pairs with a table row and a length each (pa_sparse.hip), grid
+// (tokens x splits, Hq); the token's own row of partials.
+template <typename T, bool INT8, int D, bool SPARSE = false>
 __global__ void __launch_bounds__(64) generic_attention_kernel(GenericParams p) {
     using E = Elt<T>;
-    const int t = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
-    const int hq = blockIdx.y, b = blockIdx.z, lane = threadIdx.x;
-    const int tok0 = p.qsl ? p.qsl[b] : b * p.nmax;
-    const int nb = p.qsl ? min(p.qsl[b + 1] - tok0, p.nmax) : p.nmax;   // at most max_query_len
-    if (t >= nb) return;
-    const int start = max(p.positions[tok0], 0), len = start + nb;   // a negative position reads as 0
-    const int last = p.causal ? start + t : len - 1;
+    const int t0 = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
+    const int hq = blockIdx.y, lane = threadIdx.x;
+    const int g = hq / p.G;
+    const int b = SPARSE ? t0 * p.Hk + g : (int)blockIdx.z, t = SPARSE ? 0 : t0;
+    int tok0, len, last;
+    if constexpr (SPARSE) {
+        tok0 = t0;
+        if (p.qsl && (tok0 < p.qsl[0] || tok0 >= p.qsl[p.B])) return;   // a row of no sequence
+        len = max(min(p.lengths[b], p.bt_stride * p.P), 0);
+        last = len - 1;
+    } else {
+        tok0 = p.qsl ? p.qsl[b] : b * p.nmax;
+        const int nb = p.qsl ? min(p.qsl[b + 1] - tok0, p.nmax) : p.nmax;   // at most max_query_len
+        if (t >= nb) return;
+        const int start = max(p.positions[tok0], 0);   // a negative position reads as 0
+        len = start + nb;
+        last = p.causal ? start + t : len - 1;
+    }
     // this split's keys: [k0, k1) of the sequence's len, cut at the query's last key
     const int per = (len + p.splits - 1) / p.splits;
     const int k0 = split * per, k1 = min(k0 + per, last + 1);
-    const int g = hq / p.G;
     const int32_t *bt = p.bt + (size_t)b * p.bt_stride;
     const size_t half_q = (size_t)p.num_pages * p.Hk * p.P * D;
     const size_t half_s = (size_t)p.num_pages * p.Hk * p.P;
@@ -107,8 +121,9 @@ __global__ void __launch_bounds__(64) generic_attention_kernel(GenericParams p) 
     if (p.splits > 1) {
         // (acc, m, l) of packed row (hq mod G) + G t of KV head g; a split without keys
         // leaves m = NEG_BIG, l = 0, acc = 0, which the combine weights to zero.
-        const int M = p.G * p.nmax, r = (hq - g * p.G) + p.G * t;
-        float *dst = p.part + ((((size_t)b * p.Hk + g) * p.splits + split) * M + r) * (D + 2);
+        const int M = p.G * p.nmax, r = (hq - g * p.G) + p.G * t;   // SPARSE: nmax = 1
+        const size_t pair = SPARSE ? (size_t)b : (size_t)b * p.Hk + g;
+        float *dst = p.part + ((pair * p.splits + split) * M + r) * (D + 2);
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int d = lane + WAVE * j;
@@ -124,7 +139,7 @@ __global__ void __launch_bounds__(64) generic_attention_kernel(GenericParams p) 
 #pragma unroll
     for (int j = 0; j < PER; j++) {
         const int d = lane + WAVE * j;
-        if (d < D) E::st(o, d, acc[j] / l);
+        if (d < D) E::st(o, d, SPARSE && l == 0.0f ? 0.0f : acc[j] / l);   // SPARSE: no keys, zeros
     }
 }
 
@@ -155,13 +170,16 @@ struct F32Params {
     int sshift;      // log2(splits)
     int xcd;         // 1-D grid, work-groups of one (sequence, KV head) on one XCD (pairs % 8 == 0)
     float scale_log2;
+    const int32_t *lengths;   // SPARSE: keys of each (token, KV head)
 };
 
 // Each split takes at least this many 16-key tiles (one per wave), so short contexts run on
 // fewer work-groups than the launch holds.
 constexpr int F32_MIN_TILES = 4;
 
-template <int D, bool QT>   // QT: more than one q-tile per (sequence, KV head)
+// QT: more than one q-tile per (sequence, KV head). SPARSE (one q-tile): (token, KV head) pairs with a
+// table row and a length each (pa_sparse.hip), 1-D grid of the pairs' splits.
+template <int D, bool QT, bool SPARSE = false>
 __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     constexpr int NJ = D / 16, NDB = D / 16, NW = 4, MROW = D + 4;
     __shared__ __attribute__((aligned(16))) float slab[NW * 16 * MROW];
@@ -173,7 +191,11 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     // the items of one (sequence, KV head) pair take indices that share their residue mod 8,
     // run on one XCD and read the pair's keys and values through one L2.
     int item, h, b;
-    if (QT && p.xcd) {
+    if constexpr (SPARSE) {
+        b = (int)(blockIdx.x / (unsigned)p.splits);   // the pair: row of bt, partials and lengths
+        item = (int)blockIdx.x - b * p.splits;
+        h = b % p.Hk;
+    } else if (QT && p.xcd) {
         const int QX = p.splits * p.qtiles, k = blockIdx.x >> 3;
         const int pair = (int)(blockIdx.x & 7) + 8 * (k / QX);
         item = k % QX;
@@ -193,11 +215,26 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         const int u = item >> p.sshift, half = (p.qtiles + 1) >> 1;
         qt = u < half ? p.qtiles - 1 - u : u - half;
     }
-    const int tok0 = p.qsl ? p.qsl[b] : b * p.nmax;
-    const int nb = p.qsl ? min(p.qsl[b + 1] - tok0, p.nmax) : p.nmax;   // at most max_query_len
+    int tok0, nb, start;
     const int t_first = QT ? 16 * qt / p.G : 0;
-    if (t_first >= nb) return;   // the q-tile holds no token of this sequence
-    const int start = max(p.positions[tok0], 0), len = start + nb;   // a negative position reads as 0
+    if constexpr (SPARSE) {
+        tok0 = b / p.Hk;
+        nb = 1;
+        if (p.qsl && (tok0 < p.qsl[0] || tok0 >= p.qsl[p.B])) return;   // a row of no sequence
+        start = min(p.lengths[b], p.bt_stride * p.P) - 1;
+        if (start < 0) {   // no keys: zeros (the combine's, where the keys are split)
+            if (p.splits == 1)
+                for (int i = threadIdx.x; i < p.G * D / 4; i += 256)
+                    *reinterpret_cast<f32x4 *>(p.out + ((size_t)tok0 * p.Hq + h * p.G) * D + 4 * i) = (f32x4){0.f, 0.f, 0.f, 0.f};
+            return;
+        }
+    } else {
+        tok0 = p.qsl ? p.qsl[b] : b * p.nmax;
+        nb = p.qsl ? min(p.qsl[b + 1] - tok0, p.nmax) : p.nmax;   // at most max_query_len
+        if (t_first >= nb) return;   // the q-tile holds no token of this sequence
+        start = max(p.positions[tok0], 0);   // a negative position reads as 0
+    }
+    const int len = start + nb;
     // splits cut the sequence's 16-key tiles (the combine derives the same count); this
     // q-tile's keys end after its last token's position
     const ActiveSplits as = f32_active_splits((len + 15) >> 4, p.splits, F32_MIN_TILES);
@@ -315,7 +352,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         }
     }
     __syncthreads();
-    const size_t unit = ((size_t)b * p.Hk + h) * p.splits + s;
+    const size_t unit = SPARSE ? (size_t)blockIdx.x : ((size_t)b * p.Hk + h) * p.splits + s;
     const int mrows = QT ? 16 : p.M;   // one q-tile: the M <= 16 rows
     for (int it = threadIdx.x; it < mrows * (D / 4); it += NW * 64) {
         const int rr = it / (D / 4), d4 = (it % (D / 4)) * 4, r = 16 * qt + rr;
@@ -472,4 +509,70 @@ int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStrea
     if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
     return p.splits > 1 ? ti_launch_combine(a, c, a->q_heads / c->kv_heads * a->max_query_len, p.splits, s)
                         : TI_OK;
+}
+
+// fp32 attention over chosen pages (pa_sparse.hip): the matrix-core kernel where its shape limits
+// allow and one 16-row tile holds a KV head's query heads, else the VALU kernel. Returns the least
+// 16-key tiles of a split (0: every split writes a partial), or -1 if the launch failed.
+int ti_launch_sparse_f32(const ti_sparse_attention_args *a, const ti_kv_cache *c, int splits, hipStream_t s) {
+    const int G = a->q_heads / c->kv_heads;
+    if (c->kind == TI_KV_DENSE && G <= 16 && c->page_size >= 16 && (c->page_size & (c->page_size - 1)) == 0) {
+        F32Params f{};
+        f.q = (const float *)a->q;
+        f.out = (float *)a->out;
+        f.kp = (const float *)c->k_pages;
+        f.vp = (const float *)c->v_pages;
+        f.qsl = a->query_start_loc;
+        f.B = a->num_seqs;
+        f.bt = a->tables;
+        f.lengths = a->lengths;
+        f.part = (float *)a->workspace;
+        f.bt_stride = a->table_width;
+        f.num_pages = c->num_pages;
+        f.P = c->page_size;
+        f.pshift = __builtin_ctz(c->page_size);
+        f.Hk = c->kv_heads;
+        f.Hq = a->q_heads;
+        f.G = f.M = G;
+        f.nmax = 1;
+        f.qtiles = 1;
+        f.splits = splits;
+        f.scale_log2 = a->scale * LOG2E;
+        const unsigned grid = (unsigned)((long long)a->total_tokens * c->kv_heads * splits);
+        if (c->head_dim == 128) attn_f32_kernel<128, false, true><<<grid, 256, 0, s>>>(f);
+        else attn_f32_kernel<64, false, true><<<grid, 256, 0, s>>>(f);
+        return hipGetLastError() == hipSuccess ? F32_MIN_TILES : -1;
+    }
+    GenericParams p{};
+    p.q = a->q;
+    p.out = a->out;
+    p.kp = c->k_pages;
+    p.vp = c->v_pages;
+    p.lq = c->layer_q;
+    p.ls = c->layer_scale;
+    p.smooth = c->smooth;
+    p.qsl = a->query_start_loc;
+    p.B = a->num_seqs;
+    p.bt = a->tables;
+    p.lengths = a->lengths;
+    p.part = (float *)a->workspace;
+    p.bt_stride = a->table_width;
+    p.num_pages = c->num_pages;
+    p.P = c->page_size;
+    p.Hk = c->kv_heads;
+    p.Hq = a->q_heads;
+    p.G = G;
+    p.nmax = 1;
+    p.splits = splits;
+    p.scale_log2 = a->scale * LOG2E;
+    const dim3 grid((unsigned)((long long)a->total_tokens * splits), a->q_heads);
+    const bool int8 = c->kind == TI_KV_INT8;
+    if (c->head_dim == 128) {
+        if (int8) generic_attention_kernel<float, true, 128, true><<<grid, 64, 0, s>>>(p);
+        else generic_attention_kernel<float, false, 128, true><<<grid, 64, 0, s>>>(p);
+    } else {
+        if (int8) generic_attention_kernel<float, true, 64, true><<<grid, 64, 0, s>>>(p);
+        else generic_attention_kernel<float, false, 64, true><<<grid, 64, 0, s>>>(p);
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
 }

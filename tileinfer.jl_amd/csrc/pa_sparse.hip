@@ -1,0 +1,154 @@
+// Attention over chosen pages: every query token and KV head has a table of page ids and a number
+// of keys of its own (page_select.hip makes them), and the token's G query heads attend to keys
+// 0 .. length - 1 through that table.
+//
+// The kernels are the paged decode kernels with a table row, a length and a split count per
+// (token, KV head) pair in place of one per sequence (SPARSE in pa_decode.hpp and
+// pa_generic.hip): the keys of a pair are all visible to its rows, so only the last tile is masked.
+// Pairs take consecutive work-groups with the KV heads innermost: with 8 KV heads (a multiple of
+// the 8 XCDs in general) all tokens of a KV head run on one XCD, and the pages that the tokens of
+// a step share are read through one L2.
+#include "pa_decode.hpp"
+
+using namespace ti;
+using namespace ti_decode;
+
+namespace {
+
+// Merge a pair's split partials [pair][splits][G][D + 2]: one wave per query row. Loads of up to
+// SB splits are issued before any arithmetic. A pair without keys writes zeros.
+template <int D, typename T, int SB>
+__global__ void __launch_bounds__(256) sparse_combine_kernel(DecodeParams p, int rows) {
+    constexpr int PER = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int row = (int)(blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));   // token * Hq + head
+    if (row >= rows) return;
+    const int tok = row / p.Hq, hq = row - tok * p.Hq, h = hq / p.G, pair = tok * p.Hk + h;
+    const int len = min(p.lengths[pair], p.bt_stride * p.P);
+    const int q0 = p.qsl ? p.qsl[0] : 0, q1 = p.qsl ? p.qsl[p.B] : tok + 1;
+    const int splits = p.min_tiles > 0 && len > 0 ? f32_active_splits((len + 15) >> 4, p.splits, p.min_tiles).active : p.splits;
+    const size_t stride = (size_t)p.G * (D + 2);
+    const float *base = p.part + (size_t)pair * p.splits * stride + (size_t)(hq - h * p.G) * (D + 2);
+    float mx = NEG_BIG, lsum = 0.0f, acc[PER];
+#pragma unroll
+    for (int k = 0; k < PER; k++) acc[k] = 0.0f;
+    for (int sp0 = 0; sp0 < splits; sp0 += SB) {
+        float2 ml[SB];
+        float dv[SB][PER];
+#pragma unroll
+        for (int j = 0; j < SB; j++) {
+            const float *src = base + min(sp0 + j, splits - 1) * stride;
+            ml[j] = *reinterpret_cast<const float2 *>(src + D);
+#pragma unroll
+            for (int k = 0; k < PER; k++) dv[j][k] = src[lane + 64 * k];
+        }
+        float bm = mx;
+#pragma unroll
+        for (int j = 0; j < SB; j++)
+            if (sp0 + j < splits) bm = fmaxf(bm, ml[j].x);
+        const float alpha = fast_exp2(mx - bm);
+        mx = bm;
+        lsum *= alpha;
+#pragma unroll
+        for (int k = 0; k < PER; k++) acc[k] *= alpha;
+#pragma unroll
+        for (int j = 0; j < SB; j++) {
+            const float wgt = sp0 + j < splits ? fast_exp2(ml[j].x - mx) : 0.0f;
+            lsum += ml[j].y * wgt;
+#pragma unroll
+            for (int k = 0; k < PER; k++) acc[k] += dv[j][k] * wgt;
+        }
+    }
+    if (tok < q0 || tok >= q1) return;         // a row of no sequence
+    if (len > 0 && splits == 1) return;        // its one split wrote the output
+    T *o = reinterpret_cast<T *>(p.out) + (size_t)row * D;
+#pragma unroll
+    for (int k = 0; k < PER; k++) Elt<T>::st(o, lane + 64 * k, len > 0 ? acc[k] / lsum : 0.0f);
+}
+
+template <int D, typename T>
+void launch_combine(const DecodeParams &p, int rows, hipStream_t s) {
+    const dim3 grid((rows + 3) / 4);
+    if (p.splits <= 2) sparse_combine_kernel<D, T, 2><<<grid, 256, 0, s>>>(p, rows);
+    else if (p.splits <= 4) sparse_combine_kernel<D, T, 4><<<grid, 256, 0, s>>>(p, rows);
+    else if (p.splits <= 8) sparse_combine_kernel<D, T, 8><<<grid, 256, 0, s>>>(p, rows);
+    else sparse_combine_kernel<D, T, 16><<<grid, 256, 0, s>>>(p, rows);
+}
+
+template <int D, bool INT8, bool PG16>
+void launch_sparse_p(const DecodeParams &p, unsigned grid, hipStream_t s) {
+    if constexpr (INT8 && D == 128) {   // the decode launch's rule for joint steps
+        if (p.G <= 16 && grid <= 256) {
+            decode_kernel<D, 1, INT8, PG16, 4, 1, true, true><<<grid, 256, 0, s>>>(p);
+            return;
+        }
+    }
+    if (p.G <= 16) decode_kernel<D, 1, INT8, PG16, 4, 1, false, true><<<grid, 256, 0, s>>>(p);
+    else if (p.G <= 32) decode_kernel<D, 2, INT8, PG16, 4, 1, false, true><<<grid, 256, 0, s>>>(p);
+    else decode_kernel<D, 2, INT8, PG16, 4, 2, false, true><<<grid, 256, 0, s>>>(p);
+}
+
+template <int D>
+void launch_sparse_d(const DecodeParams &p, bool int8, unsigned grid, hipStream_t s) {
+    const bool pg16 = p.pshift >= 4;
+    if (int8) pg16 ? launch_sparse_p<D, true, true>(p, grid, s) : launch_sparse_p<D, true, false>(p, grid, s);
+    else pg16 ? launch_sparse_p<D, false, true>(p, grid, s) : launch_sparse_p<D, false, false>(p, grid, s);
+}
+
+}  // namespace
+
+// Splits of a pair's keys: as the decode launch, while there are fewer than 256 work-groups, at
+// most 16 and at least four 16-key tiles of a full table each (one per wave).
+int ti_sparse_splits(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
+    const long long pairs = (long long)a->total_tokens * c->kv_heads;
+    const long long tiles = ((long long)a->table_width * c->page_size + 15) / 16;
+    int sp = 1;
+    while (sp < 16 && pairs * sp < 256 && tiles >= 8 * sp) sp <<= 1;
+    return sp;
+}
+
+int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, hipStream_t s) {
+    DecodeParams p{};
+    p.q = (const uint16_t *)a->q;
+    p.out = (uint16_t *)a->out;
+    p.kp = (const uint16_t *)c->k_pages;
+    p.vp = (const uint16_t *)c->v_pages;
+    p.lq = c->layer_q;
+    p.ls = c->layer_scale;
+    p.smooth = c->smooth;
+    p.qsl = a->query_start_loc;
+    p.B = a->num_seqs;
+    p.bt = a->tables;
+    p.lengths = a->lengths;
+    p.part = (float *)a->workspace;
+    p.bt_stride = a->table_width;
+    p.num_pages = c->num_pages;
+    p.P = c->page_size;
+    p.pshift = (c->page_size & (c->page_size - 1)) == 0 ? __builtin_ctz(c->page_size) : -1;
+    p.Hk = c->kv_heads;
+    p.Hq = a->q_heads;
+    p.G = p.M = a->q_heads / c->kv_heads;
+    p.nmax = 1;
+    p.splits = ti_sparse_splits(a, c);
+    p.scale_log2 = a->scale * LOG2E;
+    const unsigned grid = (unsigned)((long long)a->total_tokens * c->kv_heads * p.splits);
+    if (a->dtype == TI_F32) {
+        p.min_tiles = ti_launch_sparse_f32(a, c, p.splits, s);
+        if (p.min_tiles < 0) return TI_ERR_LAUNCH;
+    } else {
+        const bool int8 = c->kind == TI_KV_INT8;
+        if (c->head_dim == 128) launch_sparse_d<128>(p, int8, grid, s);
+        else launch_sparse_d<64>(p, int8, grid, s);
+    }
+    if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
+    if (p.splits == 1) return TI_OK;
+    const int rows = a->total_tokens * a->q_heads;
+    if (c->head_dim == 128) {
+        if (a->dtype == TI_F32) launch_combine<128, float>(p, rows, s);
+        else launch_combine<128, uint16_t>(p, rows, s);
+    } else {
+        if (a->dtype == TI_F32) launch_combine<64, float>(p, rows, s);
+        else launch_combine<64, uint16_t>(p, rows, s);
+    }
+    return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
+}

@@ -22,7 +22,10 @@ TI_KV_DENSE, TI_KV_INT8 = 0, 1
 
 # Every symbol include/tileinfer_hip.h declares.
 EXPORTS = ("ti_version", "ti_status_string", "ti_attention_workspace_bytes", "ti_attention",
-           "ti_attention_noalloc", "ti_store_kv", "ti_rmsnorm", "ti_rope", "ti_attention_inputs")
+           "ti_attention_noalloc", "ti_store_kv", "ti_rmsnorm", "ti_rope", "ti_attention_inputs",
+           "ti_update_key_bounds", "ti_select_pages_workspace_bytes", "ti_select_pages",
+           "ti_sparse_attention_workspace_bytes", "ti_sparse_attention",
+           "ti_verify_draft_workspace_bytes", "ti_verify_draft")
 NOALLOC_SCRATCH_BYTES = 32 << 20   # TI_NOALLOC_SCRATCH_BYTES
 
 
@@ -45,6 +48,41 @@ class AttentionArgs(ctypes.Structure):
                 ("block_tables", ctypes.c_void_p), ("scale", ctypes.c_float),
                 ("causal", ctypes.c_int32), ("path", ctypes.c_int32),
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class KeyBoundsArgs(ctypes.Structure):
+    """ti_key_bounds: the bounds of a layer's pages (device pointers)."""
+    _fields_ = [("bounds", ctypes.c_void_p), ("scale", ctypes.c_void_p)]
+
+
+def _fields(*groups):
+    return [(n, t) for t, names in groups for n in names.split()]
+
+
+class SelectArgs(ctypes.Structure):
+    """ti_select_args."""
+    _fields_ = _fields(
+        (ctypes.c_int32, "dtype q_heads kv_heads head_dim page_size num_pages num_seqs max_query_len total_tokens "
+                         "block_table_stride keep sinks window causal"),
+        (ctypes.c_void_p, "q"), (KeyBoundsArgs, "bounds"),
+        (ctypes.c_void_p, "positions query_start_loc block_tables tables lengths workspace"),
+        (ctypes.c_size_t, "workspace_bytes"))
+
+
+class SparseAttentionArgs(ctypes.Structure):
+    """ti_sparse_attention_args."""
+    _fields_ = _fields(
+        (ctypes.c_int32, "dtype q_heads total_tokens table_width num_seqs max_query_len"),
+        (ctypes.c_void_p, "q out tables lengths query_start_loc"), (ctypes.c_float, "scale"),
+        (ctypes.c_void_p, "workspace"), (ctypes.c_size_t, "workspace_bytes"))
+
+
+class VerifyArgs(ctypes.Structure):
+    """ti_verify_args."""
+    _fields_ = _fields(
+        (ctypes.c_int32, "dtype num_seqs max_drafts vocab"),
+        (ctypes.c_void_p, "draft_tokens draft_lens target draft uniforms accepted tokens workspace"),
+        (ctypes.c_size_t, "workspace_bytes"))
 
 
 _lib = None
@@ -78,6 +116,16 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     L.ti_attention_inputs.restype = i32
     L.ti_attention_inputs.argtypes = [i32, vp, P(KVCache), vp, vp, vp, vp, i32, vp, vp, i32, i32,
                                       ctypes.c_float, vp]
+    size = P(ctypes.c_size_t)
+    for name, types in (("ti_update_key_bounds", [i32, P(KVCache), P(KeyBoundsArgs), vp, i32, vp, vp, i32, i32, i32, vp]),
+                        ("ti_select_pages_workspace_bytes", [P(SelectArgs), size]),
+                        ("ti_select_pages", [P(SelectArgs), vp]),
+                        ("ti_sparse_attention_workspace_bytes", [P(SparseAttentionArgs), P(KVCache), size]),
+                        ("ti_sparse_attention", [P(SparseAttentionArgs), P(KVCache), vp]),
+                        ("ti_verify_draft_workspace_bytes", [P(VerifyArgs), size]),
+                        ("ti_verify_draft", [P(VerifyArgs), vp])):
+        getattr(L, name).restype = i32
+        getattr(L, name).argtypes = types
     _bind_calls(L)
     _lib = L
     return L

@@ -20,8 +20,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import ArgumentError, AttentionArgs, KVCache, check
-from .kv import Int8Pages, layer_arrays
+from ._lib import ArgumentError, AttentionArgs, KeyBoundsArgs, KVCache, SelectArgs, SparseAttentionArgs, VerifyArgs, check
+from .kv import Int8Pages, KeyBounds, layer_arrays
 from .rope import RotaryTable
 
 
@@ -41,7 +41,9 @@ class HipBackend:
         return "HipBackend()"
 
 
-_OPS = {"attention", "attention!", "store_kv!", "rmsnorm", "rmsnorm!", "rope", "rope!", "attention_inputs!"}
+_OPS = {"attention", "attention!", "store_kv!", "rmsnorm", "rmsnorm!", "rope", "rope!", "attention_inputs!",
+        "update_key_bounds!", "select_pages", "select_pages!", "sparse_attention", "sparse_attention!", "verify_draft",
+        "verify_draft!"}
 
 
 def supports_graphs(be: HipBackend) -> bool:
@@ -290,3 +292,249 @@ def attention_inputs_(be: HipBackend, q, k_pages, v_pages, qkv, q_norm, k_norm,
         _ptr(table.cos_sin), table.cos_sin.shape[0], _ptr(positions), _ptr(slots), n, nq,
         float(eps), _stream(q)))
     return q
+
+
+# ---- attention over chosen pages, and draft verification ---------------------------------------
+
+def _one_device(first: torch.Tensor, *ts):
+    """All on the GPU of `first` and contiguous; a context with that GPU as the current one, where the
+    library launches."""
+    _dev(first, *ts)
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ArgumentError("tensors must be on one GPU")
+    return torch.cuda.device(first.device)
+
+
+def _cache_tensors(k_pages, v_pages):
+    if isinstance(k_pages, Int8Pages) or isinstance(v_pages, Int8Pages):
+        return layer_arrays(k_pages, v_pages)
+    return k_pages, v_pages
+
+
+def _step(block_tables, positions, query_start_loc, max_query_len):
+    """(block tables as rows, sequences, most queries of one) of a step, as paged_attention_ takes it."""
+    bts = block_tables if block_tables.dim() == 2 else block_tables.view(1, -1)
+    B, T = bts.shape[0], positions.numel()
+    _i32(bts, "block_tables")
+    _i32(positions, "positions")
+    if query_start_loc is not None:
+        _i32(query_start_loc, "query_start_loc")
+        if max_query_len is None:
+            raise ArgumentError("max_query_len is required with query_start_loc")
+        if query_start_loc.numel() != B + 1:
+            raise ArgumentError("query_start_loc must hold an offset per sequence and the end")
+    return bts, B, max_query_len if max_query_len is not None else T // max(B, 1)
+
+
+def _workspace(size_of, device, *args):
+    size = ctypes.c_size_t(0)
+    check(size_of(*args, ctypes.byref(size)))
+    return None if size.value == 0 else torch.empty(size.value, dtype=torch.uint8, device=device)
+
+
+def _give_workspace(a, workspace):
+    a.workspace = _ptr(workspace)
+    a.workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+
+
+def update_key_bounds_(be: HipBackend, bounds: KeyBounds, k_pages, v_pages, block_tables, positions,
+                       query_start_loc: Optional[torch.Tensor] = None, max_query_len: Optional[int] = None):
+    """Refresh the bounds of the pages that hold the step's positions, from every key that the cache
+    holds in them up to the step's end; the step as paged_attention_ takes it, its keys already
+    written. It depends on the cached keys alone: after truncate() and another step on the same
+    pages there is nothing else to call. Returns bounds."""
+    on = _one_device(bounds.bounds, bounds.scale, *_cache_tensors(k_pages, v_pages), block_tables, positions, query_start_loc)
+    bts, B, n = _step(block_tables, positions, query_start_loc, max_query_len)
+    c = kv_cache_struct(k_pages, v_pages)
+    if bounds.shape != (c.num_pages, c.kv_heads, c.page_size, c.head_dim):
+        raise ArgumentError("bounds do not belong to pools of this shape")
+    dtype = _lib.TI_BF16 if c.kind == _lib.TI_KV_INT8 else _dtype(k_pages)
+    kb = KeyBoundsArgs(_ptr(bounds.bounds), _ptr(bounds.scale))
+    with on:
+        check(_lib.load().ti_update_key_bounds(
+            dtype, ctypes.byref(c), ctypes.byref(kb), _ptr(bts), bts.shape[1], _ptr(positions), _ptr(query_start_loc), B, n,
+            positions.numel(), _stream(positions)))
+    return bounds
+
+
+def _select_args(q, bounds: KeyBounds, stride, B, n, keep, sinks, window, causal) -> SelectArgs:
+    pages, H, P, D = bounds.shape
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % H:
+        raise ArgumentError("q must be [n][heads][D] with the bounds' head_dim and a multiple of their KV heads")
+    a = SelectArgs()
+    a.dtype, a.q_heads, a.kv_heads, a.head_dim, a.page_size, a.num_pages = _dtype(q), q.shape[1], H, D, P, pages
+    a.num_seqs, a.max_query_len, a.total_tokens, a.block_table_stride = B, n, q.shape[0], stride
+    a.keep, a.sinks, a.window, a.causal = keep, sinks, window, int(bool(causal))
+    return a
+
+
+def select_pages_workspace(be: HipBackend, q, bounds: KeyBounds, block_tables):
+    """Scratch of select_pages_ for queries shaped like q: a byte tensor (4 bytes per query token, KV head
+    and block-table entry)."""
+    a = _select_args(q, bounds, block_tables.shape[-1], 1, q.shape[0], 1, 0, 1, True)
+    a.q = a.bounds.bounds = a.bounds.scale = a.positions = a.block_tables = a.tables = a.lengths = 16
+    return _workspace(_lib.load().ti_select_pages_workspace_bytes, q.device, ctypes.byref(a))
+
+
+def select_pages_(be: HipBackend, tables, lengths, workspace, q, bounds: KeyBounds, block_tables, positions,
+                  sinks: int = 1, window: int = 1, causal: bool = True,
+                  query_start_loc: Optional[torch.Tensor] = None, max_query_len: Optional[int] = None):
+    """The tables.shape[2] pages of its sequence that each query token of the step attends to, per KV head,
+    by the bounds of their keys; the step as paged_attention_ takes it. tables [n][kv_heads][keep]
+    int32: 1-based page ids in order of position, zero-padded; lengths [n][kv_heads] int32: the
+    keys they hold, as sparse_attention_ takes both. The first `sinks` and the last `window` visible
+    pages are always kept, the others by the largest product that a key inside their bounds could have
+    with any of the KV head's queries (rounded to whole numbers); equal ones in order. Rows that belong
+    to no sequence are left as they were. Returns (tables, lengths)."""
+    on = _one_device(q, bounds.bounds, bounds.scale, block_tables, positions, query_start_loc, tables, lengths, workspace)
+    bts, B, n = _step(block_tables, positions, query_start_loc, max_query_len)
+    _i32(tables, "tables")
+    _i32(lengths, "lengths")
+    if positions.numel() != q.shape[0]:
+        raise ArgumentError("one position per query token")
+    H = bounds.shape[1]
+    if tables.dim() != 3 or tables.shape[:2] != (q.shape[0], H) or lengths.shape != (q.shape[0], H):
+        raise ArgumentError("tables must be [n][kv_heads][keep] and lengths [n][kv_heads]")
+    a = _select_args(q, bounds, bts.shape[1], B, n, tables.shape[2], int(sinks), int(window), causal)
+    a.q, a.bounds.bounds, a.bounds.scale, a.positions = _ptr(q), _ptr(bounds.bounds), _ptr(bounds.scale), _ptr(positions)
+    a.query_start_loc, a.block_tables, a.tables, a.lengths = _ptr(query_start_loc), _ptr(bts), _ptr(tables), _ptr(lengths)
+    _give_workspace(a, workspace)
+    with on:
+        check(_lib.load().ti_select_pages(ctypes.byref(a), _stream(q)))
+    return tables, lengths
+
+
+def select_pages(be: HipBackend, q, bounds: KeyBounds, block_tables, positions, keep: int, sinks: int = 1, window: int = 1,
+                 causal: bool = True, query_start_loc: Optional[torch.Tensor] = None, max_query_len: Optional[int] = None):
+    """Allocating select_pages_: rows that belong to no sequence get empty tables."""
+    H = bounds.shape[1]
+    tables = torch.zeros((q.shape[0], H, int(keep)), dtype=torch.int32, device=q.device)
+    lengths = torch.zeros((q.shape[0], H), dtype=torch.int32, device=q.device)
+    return select_pages_(be, tables, lengths, select_pages_workspace(be, q, bounds, block_tables), q, bounds, block_tables,
+                         positions, sinks, window, causal, query_start_loc, max_query_len)
+
+
+def _sparse_args(q, width, B, n, scale) -> SparseAttentionArgs:
+    a = SparseAttentionArgs()
+    a.dtype, a.q_heads, a.total_tokens, a.table_width, a.num_seqs, a.max_query_len = _dtype(q), q.shape[1], q.shape[0], width, B, n
+    a.scale = float(scale)
+    return a
+
+
+def _sparse_step(q, query_start_loc, max_query_len):
+    n = int(max_query_len) if max_query_len is not None else 1
+    if query_start_loc is None:
+        if n <= 0 or q.shape[0] % n:
+            raise ArgumentError("without query_start_loc every sequence has max_query_len tokens")
+        return q.shape[0] // n, n
+    if max_query_len is None:
+        raise ArgumentError("max_query_len is required with query_start_loc")
+    _i32(query_start_loc, "query_start_loc")
+    return query_start_loc.numel() - 1, n
+
+
+def sparse_attention_workspace(be: HipBackend, q, k_pages, tables, max_query_len: int = 1):
+    """Scratch of sparse_attention_ for queries shaped like q and tables of this width, or None. A byte
+    tensor; enough for every batch of as many tokens."""
+    c = KVCache()
+    if isinstance(k_pages, Int8Pages):
+        c.kind, c.layer_q, c.layer_scale, c.smooth = _lib.TI_KV_INT8, 16, 16, 16
+    else:
+        c.kind, c.k_pages, c.v_pages = _lib.TI_KV_DENSE, 16, 16
+    c.num_pages, c.kv_heads, c.page_size, c.head_dim = k_pages.shape
+    a = _sparse_args(q, tables.shape[-1], 1, int(max_query_len), 1.0)
+    a.q = a.out = a.tables = a.lengths = a.query_start_loc = 16
+    return _workspace(_lib.load().ti_sparse_attention_workspace_bytes, q.device, ctypes.byref(a), ctypes.byref(c))
+
+
+def sparse_attention_(be: HipBackend, out, workspace, q, k_pages, v_pages, tables, lengths, scale: float,
+                      query_start_loc: Optional[torch.Tensor] = None, max_query_len: Optional[int] = None):
+    """Attention of each query token and KV head over the keys 0 .. lengths - 1 of its own table of pages
+    (select_pages_, or any other choice), all of them visible. tables [n][kv_heads][width] int32 1-based
+    page ids, lengths [n][kv_heads] int32. A token without keys gets zeros. With query_start_loc, rows
+    that belong to no sequence are left as they were. max_query_len (1 without query_start_loc: every
+    token a sequence) says that up to so many rows next to each other are one sequence's step, whose
+    tables share pages."""
+    on = _one_device(q, out, *_cache_tensors(k_pages, v_pages), tables, lengths, query_start_loc, workspace)
+    _i32(tables, "tables")
+    _i32(lengths, "lengths")
+    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype:
+        raise ArgumentError("q and out must be matching [n][heads][D] tensors")
+    c = kv_cache_struct(k_pages, v_pages, None if isinstance(k_pages, Int8Pages) else q.dtype)
+    if q.shape[2] != c.head_dim:
+        raise ArgumentError("q's head_dim differs from the pools'")
+    if tables.dim() != 3 or tables.shape[:2] != (q.shape[0], c.kv_heads) or lengths.shape != (q.shape[0], c.kv_heads):
+        raise ArgumentError("tables must be [n][kv_heads][width] and lengths [n][kv_heads]")
+    B, n = _sparse_step(q, query_start_loc, max_query_len)
+    a = _sparse_args(q, tables.shape[2], B, n, scale)
+    a.q, a.out, a.tables, a.lengths, a.query_start_loc = _ptr(q), _ptr(out), _ptr(tables), _ptr(lengths), _ptr(query_start_loc)
+    _give_workspace(a, workspace)
+    with on:
+        check(_lib.load().ti_sparse_attention(ctypes.byref(a), ctypes.byref(c), _stream(q)))
+    return out
+
+
+def sparse_attention(be: HipBackend, q, k_pages, v_pages, tables, lengths, scale: float,
+                     query_start_loc: Optional[torch.Tensor] = None, max_query_len: Optional[int] = None):
+    """Allocating sparse_attention_: rows that belong to no sequence are zero."""
+    out = torch.empty_like(q) if query_start_loc is None else torch.zeros_like(q)
+    ws = sparse_attention_workspace(be, q, k_pages, tables, 1 if max_query_len is None else max_query_len)
+    return sparse_attention_(be, out, ws, q, k_pages, v_pages, tables, lengths, scale, query_start_loc, max_query_len)
+
+
+def _verify_args(target) -> VerifyArgs:
+    if target.dim() != 3:
+        raise ArgumentError("target must be [sequences][drafts + 1][vocabulary]")
+    a = VerifyArgs()
+    a.dtype, a.num_seqs, a.max_drafts, a.vocab = _dtype(target), target.shape[0], target.shape[1] - 1, target.shape[2]
+    return a
+
+
+def verify_draft_workspace(be: HipBackend, target):
+    """Scratch of verify_draft_ for target probabilities of this shape: a byte tensor."""
+    a = _verify_args(target)
+    a.draft_tokens = a.target = a.uniforms = a.accepted = a.tokens = 16
+    return _workspace(_lib.load().ti_verify_draft_workspace_bytes, target.device, ctypes.byref(a))
+
+
+def verify_draft_(be: HipBackend, accepted, tokens, workspace, draft_tokens, target, draft, uniforms,
+                  draft_lens: Optional[torch.Tensor] = None):
+    """End of a verify step: how many drafts of each sequence are accepted, and its next tokens.
+    draft_tokens [B][N] int32 (0-based), target [B][N + 1][V] probabilities at the positions before
+    each draft and after the last, draft [B][N][V] the drafter's (None: it gave its tokens alone),
+    uniforms [B][N + 1] float32 in [0, 1), draft_lens [B] int32 (None: N each). Draft i is accepted while
+    u_i draft_i(x_i) < target_i(x_i); one token more is drawn with the last uniform, from max(target -
+    draft, 0) where a draft was rejected (without the drafter's probabilities: the target's but for the
+    draft), else from the target's. accepted [B] int32; tokens [B][N + 1] int32: the accepted drafts, the
+    drawn token, -1 behind it. truncate() takes the rejected positions out of the cache. Returns
+    (accepted, tokens)."""
+    on = _one_device(target, accepted, tokens, workspace, draft_tokens, draft, uniforms, draft_lens)
+    a = _verify_args(target)
+    B, N, V = a.num_seqs, a.max_drafts, a.vocab
+    for t, name in ((accepted, "accepted"), (tokens, "tokens"), (draft_tokens, "draft_tokens")):
+        _i32(t, name)
+    if draft_tokens.shape != (B, N) or tokens.shape != (B, N + 1) or accepted.shape != (B,):
+        raise ArgumentError("draft_tokens must be [B][N], tokens [B][N + 1] and accepted [B]")
+    if draft is not None and (draft.shape != (B, N, V) or draft.dtype != target.dtype):
+        raise ArgumentError("draft must be [B][N][V] in target's element type")
+    if uniforms.shape != (B, N + 1) or uniforms.dtype != torch.float32:
+        raise ArgumentError("uniforms must be float32 [B][N + 1]")
+    if draft_lens is not None:
+        _i32(draft_lens, "draft_lens")
+        if draft_lens.shape != (B,):
+            raise ArgumentError("draft_lens must be [B]")
+    a.draft_tokens, a.draft_lens, a.target, a.draft = _ptr(draft_tokens), _ptr(draft_lens), _ptr(target), _ptr(draft)
+    a.uniforms, a.accepted, a.tokens = _ptr(uniforms), _ptr(accepted), _ptr(tokens)
+    _give_workspace(a, workspace)
+    with on:
+        check(_lib.load().ti_verify_draft(ctypes.byref(a), _stream(target)))
+    return accepted, tokens
+
+
+def verify_draft(be: HipBackend, draft_tokens, target, draft, uniforms, draft_lens: Optional[torch.Tensor] = None):
+    """Allocating verify_draft_."""
+    B, N1 = target.shape[:2]
+    accepted = torch.empty(B, dtype=torch.int32, device=target.device)
+    tokens = torch.empty((B, N1), dtype=torch.int32, device=target.device)
+    return verify_draft_(be, accepted, tokens, verify_draft_workspace(be, target), draft_tokens, target, draft, uniforms, draft_lens)

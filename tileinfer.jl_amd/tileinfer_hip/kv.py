@@ -143,15 +143,43 @@ def layer_arrays(k: Int8Pages, v: Int8Pages):
     return k.layer_q, k.layer_scale, k.smooth
 
 
+class KeyBounds:
+    """Bounds of the keys of a layer's pages, beside its pools of either kind: for each page and KV
+    head the keys' largest and smallest element in each dimension as whole multiples of the page's
+    power of two. `bounds` [pages][H][2][D] int8 (largest first), `scale` [pages][H] f32;
+    update_key_bounds_ writes them, select_pages_ scores pages by them."""
+
+    def __init__(self, bounds: torch.Tensor, scale: torch.Tensor, page_size: int):
+        if bounds.dtype != torch.int8 or scale.dtype != torch.float32 or bounds.dim() != 4 or bounds.shape[2] != 2 \
+                or scale.shape != bounds.shape[:2] or page_size <= 0:
+            raise ArgumentError("bounds must be int8 [pages][kv_heads][2][D] and scale float32 [pages][kv_heads]")
+        self.bounds, self.scale, self.page_size = bounds, scale, int(page_size)
+
+    @property
+    def shape(self):
+        """(pages, kv_heads, page_size, D), as the pools the bounds belong to."""
+        pages, H, _, D = self.bounds.shape
+        return (pages, H, self.page_size, D)
+
+
+def key_bounds(head_dim: int, page_size: int, kv_heads: int, num_pages: int, device="cuda") -> KeyBounds:
+    """The zeroed KeyBounds of one layer."""
+    return KeyBounds(torch.zeros((num_pages, kv_heads, 2, head_dim), dtype=torch.int8, device=device),
+                     torch.zeros((num_pages, kv_heads), dtype=torch.float32, device=device), page_size)
+
+
 class PagedKVCache:
     """Key/value pools for every layer and their page allocator (src/kv/paged_cache.jl:18-36).
-    quantize=None: pools in `dtype`; quantize="int8": Int8Pages pairs."""
+    quantize=None: pools in `dtype`; quantize="int8": Int8Pages pairs. bounds=True: a KeyBounds
+    for every layer in `bounds`, for attention over chosen pages."""
 
     def __init__(self, num_layers: int, head_dim: int, kv_heads: int, num_pages: int,
                  page_size: int = DEFAULT_PAGE_SIZE, dtype=torch.bfloat16, quantize=None,
-                 key_smoothing=None, device="cuda"):
+                 key_smoothing=None, device="cuda", bounds: bool = False):
         self.blocks = BlockManager(num_pages, page_size)
         self.quantize = quantize
+        self.bounds = [key_bounds(head_dim, page_size, kv_heads, num_pages, device) for _ in range(num_layers)] \
+            if bounds else None
         if quantize is None:
             shape = (num_pages, kv_heads, page_size, head_dim)
             self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
@@ -177,7 +205,8 @@ class PagedKVCache:
 
 def bytes_per_token(num_layers: int, kv_heads: int, head_dim: int, elt_bytes: int = 2,
                     quantize=None) -> int:
-    """Cache bytes per cached position (src/kv/paged_cache.jl:43-47)."""
+    """Cache bytes per cached position (src/kv/paged_cache.jl:43-47), without KeyBounds (2 head_dim + 4
+    bytes a page, layer and KV head)."""
     if quantize == "int8":
         return 2 * num_layers * kv_heads * (head_dim + 4)
     return 2 * num_layers * kv_heads * head_dim * elt_bytes
