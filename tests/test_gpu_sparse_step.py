@@ -215,3 +215,22 @@ def test_two_calls_at_once(gpu):
     for i in (0, 2):
         for x, y in zip(results(steps[i]), results(steps[i + 1])):
             assert torch.equal(x, y)
+
+
+def test_native_calls_and_ctypes_agree(gpu, monkeypatch):
+    """Every op of the step through the native call path, and through backend.py's own checks."""
+    from test_gpu_calls import _Counted, _NotPlain
+    from tileinfer_hip import _lib
+    ti.load_library()
+    real = _lib.calls
+    for kv in ("bf16", "int8", "fp32"):
+        got = []
+        for calls in (_Counted(real), _NotPlain()):
+            monkeypatch.setattr(_lib, "calls", calls)
+            s = make_step(kv, 2, 4, 10, 8, [900, 500])
+            set_step(s, [800, 400], 4)
+            run_step(s, workspaces(s))
+            got.append(results(s))
+            assert isinstance(calls, _NotPlain) or calls.made == 5, "an op was left to ctypes"
+        for a, b in zip(*got):
+            assert torch.equal(a, b)

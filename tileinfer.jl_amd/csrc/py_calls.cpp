@@ -12,6 +12,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -24,7 +25,12 @@ decltype(&ti_attention_inputs) f_inputs;
 decltype(&ti_store_kv) f_store_kv;
 decltype(&ti_rope) f_rope;
 decltype(&ti_rmsnorm) f_rmsnorm;
-PyObject *int8_pages, *n_layer_q, *n_layer_scale, *n_smooth, *n_half, *n_cos_sin;   // Int8Pages, attribute names
+decltype(&ti_update_key_bounds) f_bounds;
+decltype(&ti_select_pages) f_select;
+decltype(&ti_sparse_attention) f_sparse;
+decltype(&ti_verify_draft) f_verify;
+PyObject *int8_pages, *key_bounds;   // Int8Pages, KeyBounds
+PyObject *n_layer_q, *n_layer_scale, *n_smooth, *n_half, *n_cos_sin, *n_bounds, *n_scale, *n_page_size;   // attribute names
 
 struct NotPlain {};   // leave the call to backend.py
 
@@ -96,6 +102,61 @@ ti_kv_cache cache_of(PyObject *k, PyObject *v, at::ScalarType like) {
     c.page_size = (int32_t)kt.size(2), c.head_dim = (int32_t)kt.size(3);
     return c;
 }
+
+// The GPU that the calls below launch on: the current one, and that of all their tensors (backend.py
+// makes another one current).
+struct OneGpu {
+    c10::Device d;
+    OneGpu(const at::Tensor &t) : d(t.device()) { require(d.index() == c10::hip::current_device()); }
+    const at::Tensor &operator()(PyObject *o) const {
+        const at::Tensor &t = dev(o);
+        require(t.device() == d);
+        return t;
+    }
+    const at::Tensor *or_none(PyObject *o) const { return o == Py_None ? nullptr : &(*this)(o); }
+    // The layer's cache with its tensors on this GPU.
+    ti_kv_cache cache(PyObject *k, PyObject *v, at::ScalarType like) const {
+        const ti_kv_cache c = cache_of(k, v, like);
+        if (c.kind == TI_KV_DENSE) {
+            (*this)(k), (*this)(v);
+        } else {
+            Attr q(k, n_layer_q), s(k, n_layer_scale), m(k, n_smooth);
+            (*this)(q.o), (*this)(s.o), (*this)(m.o);
+        }
+        return c;
+    }
+};
+
+// The tensors of a KeyBounds; its shape is (pages, kv_heads, page_size, D).
+struct Bounds {
+    Attr b, s;
+    ti_key_bounds ptr;
+    int64_t pages, heads, page, D;
+    Bounds(PyObject *o, const OneGpu &gpu)
+        : b((require((PyObject *)Py_TYPE(o) == key_bounds), o), n_bounds), s(o, n_scale) {
+        const at::Tensor &bt = gpu(b.o), &st = gpu(s.o);
+        const Attr p(o, n_page_size);
+        require(bt.dim() == 4 && bt.scalar_type() == at::kChar && st.scalar_type() == at::kFloat && bt.size(2) == 2);
+        require(st.dim() == 2 && st.size(0) == bt.size(0) && st.size(1) == bt.size(1));
+        pages = bt.size(0), heads = bt.size(1), page = integer(p.o), D = bt.size(3);
+        ptr = {static_cast<int8_t *>(bt.data_ptr()), static_cast<float *>(st.data_ptr())};
+    }
+};
+
+// The step of query tokens that block_tables, positions, query_start_loc and max_query_len give.
+struct StepArgs {
+    const int32_t *tables, *positions, *qsl;
+    int seqs, n, total, stride;
+    StepArgs(const OneGpu &gpu, PyObject *o_tables, PyObject *o_positions, PyObject *o_qsl, PyObject *o_n) {
+        const at::Tensor &bt = gpu(o_tables), &pos = gpu(o_positions), *q = gpu.or_none(o_qsl);
+        tables = i32(bt), positions = i32(pos), qsl = q ? i32(*q) : nullptr;
+        require(bt.dim() == 1 || bt.dim() == 2);
+        const int64_t B = bt.dim() == 2 ? bt.size(0) : 1;
+        require(B > 0 && (!q || (o_n != Py_None && q->numel() == B + 1)));
+        seqs = (int)B, total = (int)pos.numel(), stride = (int)bt.size(-1);
+        n = (int)(o_n != Py_None ? integer(o_n) : total / B);
+    }
+};
 
 // Runs `body` (checks, then the call without the interpreter lock) and returns its status.
 template <typename F>
@@ -224,14 +285,118 @@ PyObject *py_rmsnorm(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     });
 }
 
-// bind(Int8Pages, addresses of ti_attention, ti_attention_inputs, ti_store_kv, ti_rope, ti_rmsnorm)
+// (bounds, k_pages, v_pages, block_tables, positions, query_start_loc, max_query_len)
+PyObject *py_bounds(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded(nargs, 7, [&]() -> long {
+        const at::Tensor &pos = dev(a[4]);
+        const OneGpu gpu(pos);
+        const Bounds b(a[0], gpu);
+        const bool dense = THPVariable_CheckExact(a[1]);
+        const at::ScalarType like = dense ? THPVariable_Unpack(a[1]).scalar_type() : at::kBFloat16;
+        const ti_kv_cache c = gpu.cache(a[1], a[2], like);
+        require(b.pages == c.num_pages && b.heads == c.kv_heads && b.page == c.page_size && b.D == c.head_dim);
+        const int dtype = dense ? dtype_of(THPVariable_Unpack(a[1])) : TI_BF16;
+        const StepArgs t(gpu, a[3], a[4], a[5], a[6]);
+        void *s = stream_of(pos);
+        return unlocked([&] { return f_bounds(dtype, &c, &b.ptr, t.tables, t.stride, t.positions, t.qsl, t.seqs, t.n, t.total, s); });
+    });
+}
+
+// (tables, lengths, workspace, q, bounds, block_tables, positions, sinks, window, causal, query_start_loc, max_query_len)
+PyObject *py_select(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded(nargs, 12, [&]() -> long {
+        const at::Tensor &q = dev(a[3]);
+        const OneGpu gpu(q);
+        const at::Tensor &tables = gpu(a[0]), &lengths = gpu(a[1]), &ws = gpu(a[2]);
+        const Bounds b(a[4], gpu);
+        const StepArgs t(gpu, a[5], a[6], a[10], a[11]);
+        require(q.dim() == 3 && q.size(2) == b.D && t.total == q.size(0) && PyBool_Check(a[9]));
+        require(tables.dim() == 3 && tables.size(0) == q.size(0) && tables.size(1) == b.heads);
+        require(lengths.dim() == 2 && lengths.size(0) == q.size(0) && lengths.size(1) == b.heads);
+        ti_select_args g{};
+        g.dtype = dtype_of(q);
+        g.q_heads = (int32_t)q.size(1), g.kv_heads = (int32_t)b.heads, g.head_dim = (int32_t)b.D;
+        g.page_size = (int32_t)b.page, g.num_pages = (int32_t)b.pages;
+        g.num_seqs = t.seqs, g.max_query_len = t.n, g.total_tokens = t.total, g.block_table_stride = t.stride;
+        g.keep = (int32_t)tables.size(2), g.sinks = (int32_t)integer(a[7]), g.window = (int32_t)integer(a[8]), g.causal = a[9] == Py_True;
+        g.q = q.data_ptr(), g.bounds = b.ptr;
+        g.positions = t.positions, g.query_start_loc = t.qsl, g.block_tables = t.tables;
+        g.tables = const_cast<int32_t *>(i32(tables)), g.lengths = const_cast<int32_t *>(i32(lengths));
+        g.workspace = ws.data_ptr(), g.workspace_bytes = (size_t)ws.nbytes();
+        void *s = stream_of(q);
+        return unlocked([&] { return f_select(&g, s); });
+    });
+}
+
+// (out, workspace, q, k_pages, v_pages, tables, lengths, scale, query_start_loc, max_query_len)
+PyObject *py_sparse(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded(nargs, 10, [&]() -> long {
+        const at::Tensor &q = dev(a[2]);
+        const OneGpu gpu(q);
+        const at::Tensor &out = gpu(a[0]), *ws = gpu.or_none(a[1]), &tables = gpu(a[5]), &lengths = gpu(a[6]), *qsl = gpu.or_none(a[8]);
+        require(q.dim() == 3 && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type());
+        const ti_kv_cache c = gpu.cache(a[3], a[4], q.scalar_type());
+        require(q.size(2) == c.head_dim && (!qsl || a[9] != Py_None));
+        require(tables.dim() == 3 && tables.size(0) == q.size(0) && tables.size(1) == c.kv_heads);
+        require(lengths.dim() == 2 && lengths.size(0) == q.size(0) && lengths.size(1) == c.kv_heads);
+        ti_sparse_attention_args g{};
+        g.dtype = dtype_of(q);
+        g.max_query_len = a[9] == Py_None ? 1 : (int32_t)integer(a[9]);
+        require(g.max_query_len > 0 && (qsl || q.size(0) % g.max_query_len == 0));
+        g.num_seqs = (int32_t)(qsl ? qsl->numel() - 1 : q.size(0) / g.max_query_len);
+        g.q_heads = (int32_t)q.size(1), g.total_tokens = (int32_t)q.size(0), g.table_width = (int32_t)tables.size(2);
+        g.q = q.data_ptr(), g.out = out.data_ptr();
+        g.tables = i32(tables), g.lengths = i32(lengths), g.query_start_loc = qsl ? i32(*qsl) : nullptr;
+        g.scale = number(a[7]);
+        g.workspace = ws ? ws->data_ptr() : nullptr, g.workspace_bytes = ws ? (size_t)ws->nbytes() : 0;
+        void *s = stream_of(q);
+        return unlocked([&] { return f_sparse(&g, &c, s); });
+    });
+}
+
+// (accepted, tokens, workspace, draft_tokens, target, draft, uniforms, draft_lens)
+PyObject *py_verify(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded(nargs, 8, [&]() -> long {
+        const at::Tensor &p = dev(a[4]);
+        const OneGpu gpu(p);
+        const at::Tensor &acc = gpu(a[0]), &tok = gpu(a[1]), &ws = gpu(a[2]), &x = gpu(a[3]), *q = gpu.or_none(a[5]), &u = gpu(a[6]),
+                         *n = gpu.or_none(a[7]);
+        require(p.dim() == 3 && p.size(1) > 0);
+        const int64_t B = p.size(0), N = p.size(1) - 1, V = p.size(2);
+        require(x.dim() == 2 && x.size(0) == B && x.size(1) == N && tok.dim() == 2 && tok.size(0) == B && tok.size(1) == N + 1);
+        require(acc.dim() == 1 && acc.size(0) == B && u.dim() == 2 && u.size(0) == B && u.size(1) == N + 1 && u.scalar_type() == at::kFloat);
+        require(!q || (q->dim() == 3 && q->size(0) == B && q->size(1) == N && q->size(2) == V && q->scalar_type() == p.scalar_type()));
+        require(!n || (n->dim() == 1 && n->size(0) == B));
+        ti_verify_args g{};
+        g.dtype = dtype_of(p);
+        g.num_seqs = (int32_t)B, g.max_drafts = (int32_t)N, g.vocab = (int32_t)V;
+        g.draft_tokens = i32(x), g.draft_lens = n ? i32(*n) : nullptr;
+        g.target = p.data_ptr(), g.draft = q ? q->data_ptr() : nullptr;
+        g.uniforms = static_cast<const float *>(u.data_ptr());
+        g.accepted = const_cast<int32_t *>(i32(acc)), g.tokens = const_cast<int32_t *>(i32(tok));
+        g.workspace = ws.data_ptr(), g.workspace_bytes = (size_t)ws.nbytes();
+        void *s = stream_of(p);
+        return unlocked([&] { return f_verify(&g, s); });
+    });
+}
+
+// bind(Int8Pages, KeyBounds, addresses of ti_attention, ti_attention_inputs, ti_store_kv, ti_rope, ti_rmsnorm,
+//      ti_update_key_bounds, ti_select_pages, ti_sparse_attention, ti_verify_draft)
 PyObject *py_bind(PyObject *, PyObject *args) {
-    PyObject *pages;
-    unsigned long long f[5];
-    if (!PyArg_ParseTuple(args, "OKKKKK", &pages, &f[0], &f[1], &f[2], &f[3], &f[4])) return nullptr;
+    PyObject *pages, *bounds;
+    unsigned long long f[9];
+    if (!PyArg_ParseTuple(args, "OOKKKKKKKKK", &pages, &bounds, &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6], &f[7], &f[8]))
+        return nullptr;
     Py_INCREF(pages);
     Py_XDECREF(int8_pages);
     int8_pages = pages;
+    Py_INCREF(bounds);
+    Py_XDECREF(key_bounds);
+    key_bounds = bounds;
+    f_bounds = reinterpret_cast<decltype(f_bounds)>(f[5]);
+    f_select = reinterpret_cast<decltype(f_select)>(f[6]);
+    f_sparse = reinterpret_cast<decltype(f_sparse)>(f[7]);
+    f_verify = reinterpret_cast<decltype(f_verify)>(f[8]);
     f_attention = reinterpret_cast<decltype(f_attention)>(f[0]);
     f_inputs = reinterpret_cast<decltype(f_inputs)>(f[1]);
     f_store_kv = reinterpret_cast<decltype(f_store_kv)>(f[2]);
@@ -242,7 +407,8 @@ PyObject *py_bind(PyObject *, PyObject *args) {
 
 #define FAST(name, f) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST("attention", py_attention), FAST("attention_inputs", py_inputs), FAST("store_kv", py_store_kv),
-                         FAST("rope", py_rope), FAST("rmsnorm", py_rmsnorm), {"bind", py_bind, METH_VARARGS, nullptr},
+                         FAST("rope", py_rope), FAST("rmsnorm", py_rmsnorm), FAST("update_key_bounds", py_bounds),
+                         FAST("select_pages", py_select), FAST("sparse_attention", py_sparse), FAST("verify_draft", py_verify), {"bind", py_bind, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods};
 
@@ -254,6 +420,9 @@ PyMODINIT_FUNC PyInit__calls() {
     n_smooth = PyUnicode_InternFromString("smooth");
     n_half = PyUnicode_InternFromString("half");
     n_cos_sin = PyUnicode_InternFromString("cos_sin");
+    n_bounds = PyUnicode_InternFromString("bounds");
+    n_scale = PyUnicode_InternFromString("scale");
+    n_page_size = PyUnicode_InternFromString("page_size");
     PyObject *m = PyModule_Create(&module);
     // the torch and Python whose layouts this was compiled for; _lib.py compares
     if (m && PyModule_AddStringConstant(m, "built_for", BUILT_FOR) < 0) {

@@ -147,7 +147,7 @@ def _bind_calls(L: ctypes.CDLL) -> None:
     ctypes, with a warning."""
     global calls
     import torch
-    from .kv import Int8Pages
+    from .kv import Int8Pages, KeyBounds
     here = f"torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
     try:
         from . import _calls
@@ -158,8 +158,9 @@ def _bind_calls(L: ctypes.CDLL) -> None:
                       "build it with `python tileinfer.jl_amd/build.py`", RuntimeWarning, stacklevel=2)
         calls = _NoCalls()
         return
-    _calls.bind(Int8Pages, *(ctypes.cast(f, ctypes.c_void_p).value for f in
-                             (L.ti_attention, L.ti_attention_inputs, L.ti_store_kv, L.ti_rope, L.ti_rmsnorm)))
+    _calls.bind(Int8Pages, KeyBounds, *(ctypes.cast(f, ctypes.c_void_p).value for f in
+                                        (L.ti_attention, L.ti_attention_inputs, L.ti_store_kv, L.ti_rope, L.ti_rmsnorm,
+                                         L.ti_update_key_bounds, L.ti_select_pages, L.ti_sparse_attention, L.ti_verify_draft)))
     calls = _calls
 
 

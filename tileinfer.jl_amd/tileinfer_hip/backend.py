@@ -344,6 +344,8 @@ def update_key_bounds_(be: HipBackend, bounds: KeyBounds, k_pages, v_pages, bloc
     holds in them up to the step's end; the step as paged_attention_ takes it, its keys already
     written. It depends on the cached keys alone: after truncate() and another step on the same
     pages there is nothing else to call. Returns bounds."""
+    if _done(_lib.native().update_key_bounds(bounds, k_pages, v_pages, block_tables, positions, query_start_loc, max_query_len)):
+        return bounds
     on = _one_device(bounds.bounds, bounds.scale, *_cache_tensors(k_pages, v_pages), block_tables, positions, query_start_loc)
     bts, B, n = _step(block_tables, positions, query_start_loc, max_query_len)
     c = kv_cache_struct(k_pages, v_pages)
@@ -387,6 +389,9 @@ def select_pages_(be: HipBackend, tables, lengths, workspace, q, bounds: KeyBoun
     pages are always kept, the others by the largest product that a key inside their bounds could have
     with any of the KV head's queries (rounded to whole numbers); equal ones in order. Rows that belong
     to no sequence are left as they were. Returns (tables, lengths)."""
+    if _done(_lib.native().select_pages(tables, lengths, workspace, q, bounds, block_tables, positions, sinks, window, causal,
+                                        query_start_loc, max_query_len)):
+        return tables, lengths
     on = _one_device(q, bounds.bounds, bounds.scale, block_tables, positions, query_start_loc, tables, lengths, workspace)
     bts, B, n = _step(block_tables, positions, query_start_loc, max_query_len)
     _i32(tables, "tables")
@@ -456,6 +461,9 @@ def sparse_attention_(be: HipBackend, out, workspace, q, k_pages, v_pages, table
     that belong to no sequence are left as they were. max_query_len (1 without query_start_loc: every
     token a sequence) says that up to so many rows next to each other are one sequence's step, whose
     tables share pages."""
+    if _done(_lib.native().sparse_attention(out, workspace, q, k_pages, v_pages, tables, lengths, scale, query_start_loc,
+                                            max_query_len)):
+        return out
     on = _one_device(q, out, *_cache_tensors(k_pages, v_pages), tables, lengths, query_start_loc, workspace)
     _i32(tables, "tables")
     _i32(lengths, "lengths")
@@ -509,6 +517,8 @@ def verify_draft_(be: HipBackend, accepted, tokens, workspace, draft_tokens, tar
     draft), else from the target's. accepted [B] int32; tokens [B][N + 1] int32: the accepted drafts, the
     drawn token, -1 behind it. truncate() takes the rejected positions out of the cache. Returns
     (accepted, tokens)."""
+    if _done(_lib.native().verify_draft(accepted, tokens, workspace, draft_tokens, target, draft, uniforms, draft_lens)):
+        return accepted, tokens
     on = _one_device(target, accepted, tokens, workspace, draft_tokens, draft, uniforms, draft_lens)
     a = _verify_args(target)
     B, N, V = a.num_seqs, a.max_drafts, a.vocab
