@@ -15,168 +15,227 @@
 // are all zero (probabilities that contradict each other) fall back to p_a, and a row p_a without
 // any weight draws nothing (-1).
 //
-// Work. All that is read is one value of p and q per draft and then row a of both (V entries), so a
-// sequence's row is shared out over work-groups of CHUNK entries: sum_kernel finds a for itself
-// (64 drafts per wave step, all loads of a step at once) and sums its chunk, draw_kernel takes the
-// chunk in which the sum passes the goal, and scans that. Every sum has one fixed order.
+// Work. All that is read is one value of p and q per draft and then row a of both (V entries).
+// sum_kernel: a wave sums pieces of PIECE entries of a sequence's row (PER per lane, 16-byte loads),
+// after finding a for itself (the drafts of a sequence one per lane, their loads together); one wave per
+// piece, and `rep` pieces per wave where there are more pieces than the chip holds waves. draw_kernel:
+// one work-group per sequence takes the piece in which the running sum passes the goal, and scans that
+// one piece. Every sum has one fixed order. The sum kernel is bound by the read of the two rows, or where
+// that is short by its chain of dependent loads (drafts, their probabilities, the row).
 #include "common.hpp"
 
 using namespace ti;
 
 namespace {
 
-constexpr int CHUNK = 4096;    // entries per work-group: 256 threads of 16
-constexpr int PER = CHUNK / 256;
+constexpr int PIECE = 1024;         // entries summed together: one wave, PER entries per lane
+constexpr int PER = PIECE / 64;
 
 struct VerifyParams {
     const void *target, *draft;
     const int32_t *drafted, *counts;
     const float *uniforms;
     int32_t *accepted, *tokens;
-    double *sums;   // [B][chunks][2]: the weights' sum and p_a's
-    int N, V, chunks;
+    double *sums;   // [B][pieces][2]: the weights' sum and p_a's
+    int N, V, pieces, rep;
 };
 
-// Accepted drafts of sequence b; every lane gets the count. *n: the sequence's drafts.
+// Accepted drafts of sequence b; every lane gets the count. *count: the sequence's drafts.
 template <typename T>
 __device__ __forceinline__ int accepted_of(const VerifyParams &p, int b, int lane, int *count) {
-    const int n = p.counts ? min(max(p.counts[b], 0), p.N) : p.N;
-    *count = n;
-    int i0 = 0;
-    for (; i0 < n; i0 += 64) {
-        const int i = i0 + lane;
+    int n = p.N;
+    if (p.counts) n = p.counts[b];
+    for (int i0 = 0;; i0 += 64) {
+        const int i = min(i0 + lane, p.N - 1);   // loads before the count is known stay inside the row
+        int x = -1;
+        float u = 0.0f;
+        if (p.N > 0) {
+            x = p.drafted[(size_t)b * p.N + i];
+            u = p.uniforms[(size_t)b * (p.N + 1) + i];
+        }
+        n = min(max(n, 0), p.N);
+        *count = n;
         bool ok = false;
-        if (i < n) {
-            const int x = p.drafted[(size_t)b * p.N + i];
-            const float u = p.uniforms[(size_t)b * (p.N + 1) + i];
-            if (x >= 0 && x < p.V) {   // a token that does not exist is not accepted
-                const float pv = Elt<T>::ld((const T *)p.target, ((size_t)b * (p.N + 1) + i) * p.V + x);
-                const float qv = p.draft ? Elt<T>::ld((const T *)p.draft, ((size_t)b * p.N + i) * p.V + x) : 1.0f;
-                ok = (double)u * (double)qv < (double)pv;
-            }
+        if (i0 + lane < n && x >= 0 && x < p.V) {   // a token that does not exist is not accepted
+            const float pv = Elt<T>::ld((const T *)p.target, ((size_t)b * (p.N + 1) + i) * p.V + x);
+            const float qv = p.draft ? Elt<T>::ld((const T *)p.draft, ((size_t)b * p.N + i) * p.V + x) : 1.0f;
+            ok = (double)u * (double)qv < (double)pv;
         }
         const unsigned long long no = __ballot(!ok);   // lanes past the last draft say no
         if (no) return i0 + __builtin_ctzll(no);
     }
-    return n;
 }
 
 __device__ __forceinline__ double positive(double w) { return w > 0.0 && w < INFINITY ? w : 0.0; }
 
-// PER consecutive entries of row a from v0 on: their weights w and target probabilities pv.
-template <typename T>
-__device__ __forceinline__ void weights(const VerifyParams &p, int b, int a, int n, int v0, double (&w)[PER], float (&pv)[PER]) {
-    const T *row = (const T *)p.target + ((size_t)b * (p.N + 1) + a) * p.V;
-    const bool rejected = a < n;
-    const T *qrow = rejected && p.draft ? (const T *)p.draft + ((size_t)b * p.N + a) * p.V : nullptr;
-    const int gone = rejected && !p.draft ? p.drafted[(size_t)b * p.N + a] : -1;
-    float qv[PER];
+// Four entries from v on (0 past the row's end), one load where all are inside. Rows of an odd
+// vocabulary are aligned to their elements only, which a vector load here allows.
+template <typename T> __device__ __forceinline__ void load4(const T *row, int v, int V, float (&x)[4]) {
+    if (v + 4 <= V) {
+        if constexpr (sizeof(T) == 4) {
+            typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+            const f32x4u w = *reinterpret_cast<const f32x4u *>(row + v);
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int v = v0 + i;
-        pv[i] = v < p.V ? Elt<T>::ld(row, v) : 0.0f;
-        qv[i] = qrow && v < p.V ? Elt<T>::ld(qrow, v) : 0.0f;
+            for (int i = 0; i < 4; i++) x[i] = w[i];
+        } else {
+            typedef uint16_t u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+            const u16x4u w = *reinterpret_cast<const u16x4u *>(row + v);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = bf2f(w[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = v + i < V ? Elt<T>::ld(row, v + i) : 0.0f;
     }
-#pragma unroll
-    for (int i = 0; i < PER; i++) w[i] = v0 + i == gone ? 0.0 : positive((double)pv[i] - (double)qv[i]);
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
+// The rows that the token after a drafts is drawn from: p_a, and q_a or the draft without weight.
+template <typename T> struct Rows {
+    const T *p, *q;
+    int gone, V;
+    __device__ Rows(const VerifyParams &v, int b, int a, int n) : V(v.V) {
+        p = (const T *)v.target + ((size_t)b * (v.N + 1) + a) * v.V;
+        q = a < n && v.draft ? (const T *)v.draft + ((size_t)b * v.N + a) * v.V : nullptr;
+        gone = a < n && !v.draft ? v.drafted[(size_t)b * v.N + a] : -1;
+    }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(256) sum_kernel(VerifyParams p) {
-    __shared__ double part[4][2];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, b = blockIdx.y;
+    const int lane = threadIdx.x & 63, b = blockIdx.y;
+    const int w = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int n;
     const int a = accepted_of<T>(p, b, lane, &n);
-    double w[PER], sw = 0.0, sp = 0.0;
-    float pv[PER];
-    weights<T>(p, b, a, n, blockIdx.x * CHUNK + tid * PER, w, pv);
+    if (w == 0 && lane == 0) p.accepted[b] = a;
+    const Rows<T> r(p, b, a, n);
+    for (int k = w * p.rep; k < min((w + 1) * p.rep, p.pieces); k++) {
+        const int v0 = k * PIECE + 4 * lane;   // entries v0 + 256 j .. + 3
+        float pv[PER / 4][4], qv[PER / 4][4];
 #pragma unroll
-    for (int i = 0; i < PER; i++) sw += w[i], sp += positive(pv[i]);
-    sw = wave_sum64(sw);
-    sp = wave_sum64(sp);
-    if (lane == 0) part[wv][0] = sw, part[wv][1] = sp;
-    __syncthreads();
-    if (tid == 0) {
-        double *dst = p.sums + ((size_t)b * p.chunks + blockIdx.x) * 2;
-        dst[0] = (part[0][0] + part[1][0]) + (part[2][0] + part[3][0]);
-        dst[1] = (part[0][1] + part[1][1]) + (part[2][1] + part[3][1]);
+        for (int j = 0; j < PER / 4; j++) load4(r.p, v0 + 256 * j, p.V, pv[j]);
+        if (r.q) {
+#pragma unroll
+            for (int j = 0; j < PER / 4; j++) load4(r.q, v0 + 256 * j, p.V, qv[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER / 4; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) qv[j][i] = 0.0f;
+        }
+        double sw = 0.0, sp = 0.0;
+#pragma unroll
+        for (int j = 0; j < PER / 4; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const double x = pv[j][i];
+                sp += positive(x);
+                sw += v0 + 256 * j + i == r.gone ? 0.0 : positive(x - (double)qv[j][i]);
+            }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            sw += __shfl_xor(sw, o);
+            sp += __shfl_xor(sp, o);
+        }
+        if (lane == 0) {
+            double *dst = p.sums + ((size_t)b * p.pieces + k) * 2;
+            dst[0] = sw;
+            dst[1] = sp;
+        }
     }
+}
+
+// Sum of the 256 threads' values before this one's, and of all.
+__device__ __forceinline__ double block_before(double own, double *part, int lane, int wv, double *all) {
+    double incl = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double v = __shfl_up(incl, o);
+        if (lane >= o) incl += v;
+    }
+    __syncthreads();   // earlier reads of part are done
+    if (lane == 63) part[wv] = incl;
+    __syncthreads();
+    double before = incl - own, total = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (i < wv) before += part[i];
+        total += part[i];
+    }
+    *all = total;
+    return before;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) draw_kernel(VerifyParams p) {
-    __shared__ double part[4], goal_s, before_s;
-    __shared__ int chunk_s, found, last, plain_s;
+    __shared__ double part[4], before_s;
+    __shared__ int first_piece, last_piece, first, last;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, b = blockIdx.x;
-    int n;
-    const int a = accepted_of<T>(p, b, lane, &n);
-    const double *sums = p.sums + (size_t)b * p.chunks * 2;
-    if (tid == 0) {
-        double tw = 0.0, tp = 0.0;
-        for (int c = 0; c < p.chunks; c++) tw += sums[2 * c], tp += sums[2 * c + 1];
-        const int plain = !(tw > 0.0);   // no weight left: the target's own row
-        const double goal = (double)p.uniforms[(size_t)b * (p.N + 1) + p.N] * (plain ? tp : tw);
-        double run = 0.0, before = 0.0;
-        int chunk = -1;
-        for (int c = 0; c < p.chunks; c++) {
-            const double s = sums[2 * c + plain];
-            if (!(s > 0.0)) continue;
-            chunk = c;   // the last chunk with weight, where none passes the goal
-            before = run;
-            run += s;
-            if (run > goal) break;
-        }
-        goal_s = goal;
-        before_s = before;
-        chunk_s = chunk;
-        plain_s = plain;
-        found = CHUNK;
-        last = -1;
+    if (tid == 0) first_piece = first = 0x7fffffff, last_piece = last = -1;
+    const double u = (double)p.uniforms[(size_t)b * (p.N + 1) + p.N];
+    const int a = p.accepted[b];
+    const int n = p.counts ? min(max(p.counts[b], 0), p.N) : p.N;
+    const double2 *sums = reinterpret_cast<const double2 *>(p.sums) + (size_t)b * p.pieces;
+    // thread t holds pieces [t each, (t + 1) each)
+    const int each = (p.pieces + 255) / 256, k0 = min(tid * each, p.pieces), k1 = min(k0 + each, p.pieces);
+    double own = 0.0, total, before;
+    for (int k = k0; k < k1; k++) own += sums[k].x;
+    before = block_before(own, part, lane, wv, &total);
+    const bool plain = !(total > 0.0);   // no weight left: the target's own row
+    if (plain) {
+        own = 0.0;
+        for (int k = k0; k < k1; k++) own += sums[k].y;
+        before = block_before(own, part, lane, wv, &total);
     }
+    const double goal = u * total;
+    // the first piece whose running sum passes the goal, or the last with weight where none does
+    int mine = 0x7fffffff, top = -1;
+    double run = before, mine_before = 0.0, top_before = 0.0;
+    for (int k = k0; k < k1; k++) {
+        const double s = plain ? sums[k].y : sums[k].x;
+        if (s > 0.0) {
+            top = k;
+            top_before = run;
+            if (run + s > goal && mine == 0x7fffffff) {
+                mine = k;
+                mine_before = run;
+            }
+        }
+        run += s;
+    }
+    if (mine != 0x7fffffff) atomicMin(&first_piece, mine);
+    if (top >= 0) atomicMax(&last_piece, top);
     __syncthreads();
-    const int chunk = chunk_s;
+    const int piece = first_piece != 0x7fffffff ? first_piece : last_piece;
     int token = -1;
-    if (chunk >= 0) {
-        double w[PER], own = 0.0;
-        float pv[PER];
-        weights<T>(p, b, a, n, chunk * CHUNK + tid * PER, w, pv);
-        int top = -1;
+    if (piece >= 0) {
+        if (mine == piece) before_s = mine_before;
+        else if (top == piece && first_piece == 0x7fffffff) before_s = top_before;
+        const Rows<T> r(p, b, a, n);
+        const int v0 = piece * PIECE + 4 * tid;
+        float pv[4], qv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        load4(r.p, v0, p.V, pv);
+        if (r.q && !plain) load4(r.q, v0, p.V, qv);
+        double w[4], sum = 0.0, all;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            if (plain_s) w[i] = positive(pv[i]);
-            own += w[i];
-            if (w[i] > 0.0) top = tid * PER + i;
+        for (int i = 0; i < 4; i++) {
+            w[i] = !plain && v0 + i == r.gone ? 0.0 : positive((double)pv[i] - (double)qv[i]);
+            sum += w[i];
         }
-        double incl = own;
+        double c = block_before(sum, part, lane, wv, &all) + before_s;
+        int hit = 0x7fffffff, held = -1;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double v = __shfl_up(incl, o);
-            if (lane >= o) incl += v;
+        for (int i = 0; i < 4; i++) {
+            c += w[i];
+            if (w[i] > 0.0) {
+                held = v0 + i;
+                if (c > goal && hit == 0x7fffffff) hit = v0 + i;
+            }
         }
-        if (lane == 63) part[wv] = incl;
+        if (hit != 0x7fffffff) atomicMin(&first, hit);
+        if (held >= 0) atomicMax(&last, held);
         __syncthreads();
-        double run = before_s + (incl - own);
-        for (int i = 0; i < wv; i++) run += part[i];
-        int hit = CHUNK;
-#pragma unroll
-        for (int i = PER - 1; i >= 0; i--) {
-            double c = run;
-#pragma unroll
-            for (int j = 0; j <= i; j++) c += w[j];
-            if (w[i] > 0.0 && c > goal_s) hit = tid * PER + i;
-        }
-        if (hit < CHUNK) atomicMin(&found, hit);
-        if (top >= 0) atomicMax(&last, top);
-        __syncthreads();
-        token = chunk * CHUNK + (found < CHUNK ? found : last);
+        token = first != 0x7fffffff ? first : last;
     }
-    if (tid == 0) p.accepted[b] = a;
     for (int i = tid; i <= p.N; i += 256)
         p.tokens[(size_t)b * (p.N + 1) + i] = i < a ? p.drafted[(size_t)b * p.N + i] : (i == a ? token : -1);
 }
@@ -184,7 +243,7 @@ __global__ void __launch_bounds__(256) draw_kernel(VerifyParams p) {
 }  // namespace
 
 size_t ti_verify_bytes(const ti_verify_args *a) {
-    return (size_t)a->num_seqs * ((a->vocab + (size_t)CHUNK - 1) / CHUNK) * 2 * sizeof(double);
+    return (size_t)a->num_seqs * ((a->vocab + (size_t)PIECE - 1) / PIECE) * 2 * sizeof(double);
 }
 
 int ti_launch_verify_draft(const ti_verify_args *a, hipStream_t s) {
@@ -199,8 +258,10 @@ int ti_launch_verify_draft(const ti_verify_args *a, hipStream_t s) {
     p.sums = (double *)a->workspace;
     p.N = a->max_drafts;
     p.V = a->vocab;
-    p.chunks = (int)((a->vocab + (long long)CHUNK - 1) / CHUNK);
-    const dim3 grid(p.chunks, a->num_seqs);
+    p.pieces = (int)((a->vocab + (long long)PIECE - 1) / PIECE);
+    // about 16 waves on each of 256 CUs, so that the drafts' chain of loads is paid once
+    p.rep = (int)min((long long)p.pieces, max(1LL, (long long)p.pieces * a->num_seqs / 4096));
+    const dim3 grid((p.pieces + 4 * p.rep - 1) / (4 * p.rep), a->num_seqs);
     if (a->dtype == TI_F32) {
         sum_kernel<float><<<grid, 256, 0, s>>>(p);
         if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
