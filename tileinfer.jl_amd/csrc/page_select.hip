@@ -9,10 +9,10 @@
 // on how the work is split.
 //
 // Scores become 32-bit keys in the scores' order, 0 for pages that are not up for choice (those kept
-// anyway, and those past the last visible one). The key of the last page kept by score is found by
-// bisection between the smallest and the largest key, counting the keys above the middle: it ends
-// when the count is right, after about log2 of the pages and a few steps, and at the latest after 32
-// (equal keys). Then one pass over the pages in order writes the kept ones.
+// anyway, and those past the last visible one). The key of the last page kept by score is found by one
+// wave, by bisection between the smallest and the largest key, counting the keys above the middle: it
+// ends when the count is right, after about log2 of the pages and a few steps, and at the latest after
+// 32 (equal keys). Then one pass over the pages in order writes the kept ones.
 //
 // Two forms. select_kernel holds a token tile's keys in LDS and does both steps in one launch.
 // scores_kernel and keep_kernel share a tile's pages out over several work-groups, the keys going
@@ -26,8 +26,8 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int WAVES = 16, THREADS = WAVES * 64;
 constexpr int ROUND = 256;   // keys read by a wave at once: rows of keys are padded to it with zeros
+constexpr int ONE = 8 * ROUND;   // the most keys that one wave searches
 
 struct SelectParams {
     const void *q;
@@ -36,7 +36,7 @@ struct SelectParams {
     const int32_t *positions, *qsl, *bt;
     int32_t *tables, *lengths;
     uint32_t *keys;   // two launches: [total][Hk][pitch]
-    int bt_stride, num_pages, P, Hk, Hq, G, nmax, total, keep, sinks, window, causal, f32;
+    int bt_stride, num_pages, P, Hk, Hq, G, nmax, total, keep, sinks, window, causal, f32, pshift;
     int pitch, split;   // keys per (token, KV head); work-groups that share a token tile's pages
 };
 
@@ -45,7 +45,7 @@ struct Seen {
     int last, seen, c0, c1, kept, need;
     __device__ Seen(const SelectParams &p, const Step &st, int t) {
         last = st.start + (p.causal ? t : st.n - 1);
-        seen = min(last / p.P + 1, p.bt_stride);
+        seen = min((p.pshift >= 0 ? last >> p.pshift : last / p.P) + 1, p.bt_stride);
         c0 = min(p.sinks, seen);
         c1 = max(c0, seen - p.window);
         kept = min(seen, p.keep);
@@ -53,23 +53,30 @@ struct Seen {
     }
 };
 
-// Larger score, larger key, never 0; NaN (an infinite page scale times 0) counts as the largest.
+// Larger score, larger key, never 0; NaN (an infinite page scale times 0) counts as infinite.
 __device__ __forceinline__ uint32_t order_key(float x) {
-    x += 0.0f;   // -0 and 0 are one score
-    const uint32_t u = __float_as_uint(x);
-    return x != x ? 0xffffffffu : ((int32_t)u < 0 ? ~u : u | 0x80000000u);
+    x = x != x ? INFINITY : x + 0.0f;   // -0 and 0 are one score
+    const int32_t u = (int32_t)__float_as_uint(x);
+    return (uint32_t)(u ^ (u >> 31 | (int32_t)0x80000000));
 }
 
-// The largest of GP neighbouring lanes, in all of them (GP a power of two up to 16).
-template <int CTRL> __device__ __forceinline__ float dpp_max(float x) {
-    return fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, false)));
+template <int CTRL> __device__ __forceinline__ int dpp(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, false); }
+// Sum of a wave's values, wave-uniform: within rows of 16 lanes by mirrored halves, across them by lane reads.
+__device__ __forceinline__ int wave_total(int x) {
+    x += dpp<0xb1>(x);    // quad_perm 1 0 3 2
+    x += dpp<0x4e>(x);    // quad_perm 2 3 0 1
+    x += dpp<0x141>(x);   // row_half_mirror
+    x += dpp<0x140>(x);   // row_mirror
+    return (__builtin_amdgcn_readlane(x, 0) + __builtin_amdgcn_readlane(x, 16)) +
+           (__builtin_amdgcn_readlane(x, 32) + __builtin_amdgcn_readlane(x, 48));
 }
-template <int GP> __device__ __forceinline__ float group_max(float x) {
-    if (GP >= 2) x = dpp_max<0xb1>(x);    // quad_perm 1 0 3 2
-    if (GP >= 4) x = dpp_max<0x4e>(x);    // quad_perm 2 3 0 1
-    if (GP >= 8) x = dpp_max<0x141>(x);   // row_half_mirror: the other quad of eight lanes
-    if (GP >= 16) x = dpp_max<0x140>(x);  // row_mirror: the other half of sixteen
-    return x;
+__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
+    x = max(x, (uint32_t)dpp<0xb1>((int)x));
+    x = max(x, (uint32_t)dpp<0x4e>((int)x));
+    x = max(x, (uint32_t)dpp<0x141>((int)x));
+    x = max(x, (uint32_t)dpp<0x140>((int)x));
+    return max(max((uint32_t)__builtin_amdgcn_readlane((int)x, 0), (uint32_t)__builtin_amdgcn_readlane((int)x, 16)),
+               max((uint32_t)__builtin_amdgcn_readlane((int)x, 32), (uint32_t)__builtin_amdgcn_readlane((int)x, 48)));
 }
 
 // A tile of RT x 16 query rows: rows of a token are its G heads, padded to GP (a power of two up to 16);
@@ -79,12 +86,12 @@ template <int GP, int RT, bool WIDE> struct Tile {
 };
 
 // The whole-number operands of a tile's rows in LDS: relu(w) then min(w, 0), and 2^e (a row that is not
-// finite: zeros). 16 lanes per row.
-template <int D, int GP, int RT, bool WIDE>
+// finite: zeros; a row that pads the heads: NaN, which no maximum takes). 16 lanes per row.
+template <int D, int GP, int RT, bool WIDE, int W>
 __device__ __forceinline__ void quantize_rows(const SelectParams &p, const Step &st, int h, int t0, int tid, int8_t (*w)[2 * D],
                                               float *forth) {
     constexpr int E = D / 16;
-    for (int r = tid / 16; r < RT * 16; r += THREADS / 16) {
+    for (int r = tid / 16; r < RT * 16; r += W * 4) {
         const int t = WIDE ? t0 : t0 + r / GP, g = WIDE ? r : r % GP, c = (tid & 15) * E;
         const bool ok = t < st.n && g < p.G;
         const size_t src = ((size_t)(st.tok0 + (ok ? t : t0)) * p.Hq + h * p.G + (ok ? g : 0)) * D + c;
@@ -121,40 +128,37 @@ __device__ __forceinline__ void quantize_rows(const SelectParams &p, const Step 
             *reinterpret_cast<uint32_t *>(&w[r][c + 4 * i]) = up[i];
             *reinterpret_cast<uint32_t *>(&w[r][D + c + 4 * i]) = dn[i];
         }
-        if ((tid & 15) == 0) forth[r] = power(e);
+        if ((tid & 15) == 0) forth[r] = g < p.G ? power(e) : NAN;
     }
 }
 
 // The keys of a tile's tokens for the 16-page tiles j = first, first + step, ... < ntiles, by one wave:
-// S = bounds W on v_mfma_i32_16x16x64_i8 (A: lane l holds page l % 16's bytes 16 (l / 16) .. + 16 of each
-// 64; B: a query row's, the same way), so lane l gets row l % 16's products with pages 4 (l / 16) .. + 3,
-// and the heads of a token are neighbouring lanes. dst(t, page) is where four keys of token t0 + t go.
+// S = W bounds on v_mfma_i32_16x16x64_i8 (A: lane l holds row l % 16's bytes 16 (l / 16) .. + 16 of each
+// 64; B: a page's, the same way), so lane l gets the products of page l % 16 with rows 4 (l / 16) .. + 3:
+// the heads of a token are a lane's registers (and those of other 16-lane groups for GP > 4), its page's
+// scale is at hand, and few vector instructions are left beside the loads: with the operands the other
+// way round (heads in lanes) they bound the kernel (512 tokens on 64k: 17 us of scores, 2048 pages
+// 11.6). dst(t, page) is where the key of token t0 + t goes.
 template <int D, int GP, int RT, bool WIDE, typename Dst>
-__device__ __forceinline__ void score_pages(const SelectParams &p, const Step &st, int b, int h, int t0, int lane, int first, int step,
-                                            int ntiles, int most, const int8_t (*w)[2 * D], const float *forth, Dst dst) {
+__device__ __forceinline__ void score_pages(const SelectParams &p, int b, int h, int tokens, int lane, int first, int step, int ntiles,
+                                            int most, const int8_t (*w)[2 * D], const float *forth, Dst dst) {
     constexpr int NK = 2 * D / 64;
-    constexpr int TPB = WIDE ? 1 : 16 / GP;   // tokens per 16-row block
+    constexpr int HL = GP < 4 ? GP : 4, TL = 4 / HL;   // heads and tokens of a lane's four rows
     const int r16 = lane & 15, kg = lane >> 4;
     const int32_t *bt = p.bt + (size_t)b * p.bt_stride;
     i32x4 q[RT][NK];
-    float f[RT];
-    int c0[RT], c1[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
+    for (int rt = 0; rt < RT; rt++)
 #pragma unroll
         for (int i = 0; i < NK; i++) q[rt][i] = *reinterpret_cast<const i32x4 *>(&w[rt * 16 + r16][i * 64 + kg * 16]);
-        f[rt] = forth[rt * 16 + r16];
-        const int t = WIDE ? t0 : t0 + rt * TPB + r16 / GP;
-        const Seen s(p, st, min(t, st.n - 1));
-        c0[rt] = s.c0;
-        c1[rt] = t < st.n ? s.c1 : 0;
-    }
     struct Page {
         i32x4 b[NK];
         float scale;
     };
-    auto load = [&](int j, Page &pg) {
-        const int id = page_of(bt, min(j * 16 + r16, most - 1), p.bt_stride, p.num_pages);
+    // a tile's page ids are loaded a tile ahead of its bounds, so that one wait does not follow another
+    auto ids = [&](int j) { return bt[min(j * 16 + r16, most - 1)]; };
+    auto load = [&](int raw, Page &pg) {
+        const int id = clamp_page(raw, p.num_pages);
         const size_t at = (size_t)id * p.Hk + h;
         const int8_t *src = p.bounds + at * 2 * D + kg * 16;
 #pragma unroll
@@ -162,51 +166,52 @@ __device__ __forceinline__ void score_pages(const SelectParams &p, const Step &s
         pg.scale = p.scale[at];
     };
     auto use = [&](int j, const Page &pg) {
-        float ps[4], s[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) ps[k] = __shfl(pg.scale, 4 * kg + k);
+        float s[TL];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < NK; i++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(pg.b[i], q[rt][i], acc, 0, 0, 0);
-            const bool head = (WIDE ? rt * 16 + r16 : r16 % GP) < p.G;   // a padding row counts for nothing
+            for (int i = 0; i < NK; i++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[rt][i], pg.b[i], acc, 0, 0, 0);
+            const f32x4 f = *reinterpret_cast<const f32x4 *>(&forth[rt * 16 + 4 * kg]);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const float x = head ? (float)acc[k] * f[rt] : -INFINITY;
-                s[k] = WIDE && rt > 0 ? fmaxf(s[k], x) : x;
+                const float x = (float)acc[k] * f[k];
+                s[k / HL] = k % HL || (WIDE && rt) ? fmaxf(s[k / HL], x) : x;
             }
             if (WIDE && rt < RT - 1) continue;
-            u32x4 key;
+            if (GP >= 8) s[0] = fmaxf(s[0], __shfl_xor(s[0], 16));
+            if (GP >= 16) s[0] = fmaxf(s[0], __shfl_xor(s[0], 32));
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int page = j * 16 + 4 * kg + k;
-                const uint32_t o = order_key(group_max<GP>(s[k]) * ps[k]);
-                key[k] = page >= c0[rt] && page < c1[rt] ? o : 0u;
+            for (int n = 0; n < TL; n++) {
+                const int t = WIDE ? 0 : (rt * 16 + 4 * kg + n * HL) / GP;
+                if (4 * kg % GP == 0 && t < tokens) *dst(t, j * 16 + r16) = order_key(s[n] * pg.scale);
             }
-            const int t = WIDE ? 0 : rt * TPB + r16 / GP;
-            if (r16 % GP == 0 && t0 + t < st.n) *reinterpret_cast<u32x4 *>(dst(t, j * 16 + 4 * kg)) = key;
         }
     };
     int j = first;
-    if constexpr (RT > 1) {   // its operands leave no registers for a second set
+    if (j >= ntiles) return;
+    int ia = ids(j), ib = ids(j + step);
+    if constexpr (RT > 1) {   // its operands leave no registers for a second set of bounds
         Page pg;
         for (; j < ntiles; j += step) {
-            load(j, pg);
+            load(ia, pg);
+            ia = ib;
+            ib = ids(j + 2 * step);
             use(j, pg);
         }
-        return;
-    }
-    // two sets in turn: the next tile's loads are issued before this one is worked on
-    Page pa, pb;
-    if (j < ntiles) {
-        load(j, pa);
+    } else {
+        // two sets in turn: the next tile's loads are issued before this one is worked on
+        Page pa, pb;
+        load(ia, pa);
+        ia = ids(j + 2 * step);
         while (true) {
-            load(min(j + step, ntiles - 1), pb);
+            if (j + step < ntiles) load(ib, pb);
+            ib = ids(j + 3 * step);
             use(j, pa);
             j += step;
             if (j >= ntiles) break;
-            load(min(j + step, ntiles - 1), pa);
+            if (j + step < ntiles) load(ia, pa);
+            ia = ids(j + 3 * step);
             use(j, pb);
             j += step;
             if (j >= ntiles) break;
@@ -214,86 +219,112 @@ __device__ __forceinline__ void score_pages(const SelectParams &p, const Step &s
     }
 }
 
-__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+// The last page kept by score: keys above `limit` are kept, and `ties` of those equal to it.
+struct Limit {
+    uint32_t limit;
+    int ties;
+};
+// Joins what the W waves that search together found: `red` holds 4 W words of LDS, used in halves in
+// turn, so that one barrier is enough.
+template <int W> struct Join {
+    int *red;
+    int lane, w, turn;
+    __device__ int sum(int v) {
+        if constexpr (W == 1) return v;
+        return wave_total(swap(v, 0));
+    }
+    __device__ uint32_t most(uint32_t v) {
+        if constexpr (W == 1) return v;
+        return wave_umax((uint32_t)swap((int)v, 0));
+    }
+    __device__ int swap(int v, int none) {
+        int *r = red + (turn ^= 1) * W;
+        if (lane == 0) r[w] = v;
+        __syncthreads();
+        return lane < W ? r[lane] : none;
+    }
+};
+
+// The search over keys in groups of four per lane, group(n) the n-th of this wave's `groups`.
+template <typename Group, typename J> __device__ __forceinline__ Limit bisect(int need, int groups, Group group, J join) {
+    uint32_t top = 0, low = 0xffffffffu;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-    return v;
+    for (int n = 0; n < groups; n++) {
+        const u32x4 k = group(n);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            top = max(top, k[e]);
+            low = min(low, k[e] - 1);   // 0 wraps to the largest
+        }
+    }
+    top = join.most(wave_umax(top));
+    low = ~join.most(wave_umax(~low)) + 1;
+    int above = 0;   // keys > top: fewer than need; keys >= low: at least need
+    while (low < top) {
+        const uint32_t d = top - low, mid = low + d / 2 + (d & 1);
+        int c = 0;
+#pragma unroll
+        for (int n = 0; n < groups; n++) {
+            const u32x4 k = group(n);
+#pragma unroll
+            for (int e = 0; e < 4; e++) c += __popcll(__ballot(k[e] >= mid));
+        }
+        c = join.sum(c);
+        if (c == need) return {mid - 1, 0};
+        if (c > need) {
+            low = mid;
+        } else {
+            top = mid - 1;
+            above = c;
+        }
+    }
+    return {low, need - above};
+}
+// Up to NG groups a wave in registers: the search is all arithmetic.
+template <int NG, int W, typename J>
+__device__ __forceinline__ Limit bisect_held(int need, const uint32_t *keys, int span, int lane, int w, J join) {
+    u32x4 k[NG];
+#pragma unroll
+    for (int n = 0; n < NG; n++) {
+        const int i = (n * W + w) * ROUND;
+        k[n] = i < span ? *reinterpret_cast<const u32x4 *>(keys + i + 4 * lane) : (u32x4){0u, 0u, 0u, 0u};
+    }
+    return bisect(need, NG, [&](int n) { return k[n]; }, join);
 }
 
-// Writes one token's kept pages and its number of keys. keys: `span` of them (a multiple of ROUND).
-// NW waves share the work (1: no barrier is passed; else all of the work-group call it together,
-// red holding 3 NW + 3 words of LDS).
-template <int NW, typename Keys>
-__device__ __forceinline__ void keep_pages(const SelectParams &p, const Seen &s, Keys keys, int span, size_t pair, const int32_t *bt,
-                                           int lane, int w, int *red) {
-    // limit: keys above it are kept, and `ties` of those equal to it
-    uint32_t limit = 1;
-    int ties = 0x7fffffff, parity = 0;
-    auto total = [&](int v) {   // the sum over the waves, alternating between two cells
-        if constexpr (NW == 1) return v;
-        parity ^= 1;
-        if (lane == 0) red[parity * NW + w] = v;
-        __syncthreads();
-        int sum = 0;
-#pragma unroll
-        for (int i = 0; i < NW; i++) sum += red[parity * NW + i];
-        return sum;
-    };
-    const int stride = NW * ROUND;
-    if (s.need < s.c1 - s.c0 && s.need > 0) {
-        uint32_t top = 0, low = 0xffffffffu;
-        for (int i = w * ROUND + 4 * lane; i < span; i += stride) {
-            const u32x4 k = *reinterpret_cast<const u32x4 *>(keys + i);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                top = max(top, k[e]);
-                low = min(low, k[e] - 1);   // 0 wraps to the largest: not up for choice
-            }
-        }
-        top = wave_umax(top);
-        low = ~wave_umax(~low);
-        if constexpr (NW > 1) {
-            uint32_t *r = reinterpret_cast<uint32_t *>(red);
-            if (lane == 0) r[w] = top, r[2 * NW + w] = low;   // cells that total() writes after a barrier
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < NW; i++) top = max(top, r[i]), low = min(low, r[2 * NW + i]);
-        }
-        low++;
-        int above = 0;   // keys > top: fewer than need; keys >= low: at least need
-        bool exact = false;
-        while (low < top && !exact) {
-            const uint32_t d = top - low, mid = low + d / 2 + (d & 1);
-            int c = 0;
-            for (int i = w * ROUND + 4 * lane; i < span; i += stride) {
-                const u32x4 k = *reinterpret_cast<const u32x4 *>(keys + i);
-#pragma unroll
-                for (int e = 0; e < 4; e++) c += __popcll(__ballot(k[e] >= mid));
-            }
-            c = total(c);
-            if (c >= s.need) {
-                low = mid;
-                exact = c == s.need;
-            } else {
-                top = mid - 1;
-                above = c;
-            }
-        }
-        limit = low;
-        ties = exact ? 0x7fffffff : s.need - above;
-    } else if (s.need <= 0) {
-        limit = 0xffffffffu;   // none by score
-        ties = 0;
+// By W waves (all of the work-group where W > 1), over `span` keys (a multiple of ROUND); those that are
+// not up for choice become 0. One wave takes up to ONE keys, all in registers (512 keys 1.6 us, 2048 2.0;
+// 8192 through LDS took 45), more waves 512 each before they read them from LDS at every step.
+template <int W>
+__device__ __forceinline__ Limit find_limit(const Seen &s, uint32_t *keys, int span, int lane, int w, int *red) {
+    for (int i = w * 64 + lane; i < s.c0; i += W * 64) keys[i] = 0;
+    for (int i = s.c1 + w * 64 + lane; i < span; i += W * 64) keys[i] = 0;
+    if (W > 1) __syncthreads();
+    if (s.need >= s.c1 - s.c0) return {0, 0};   // every candidate
+    if (s.need <= 0) return {0xffffffffu, 0};     // none
+    const Join<W> join{red, lane, w, 0};
+    if (span <= 2 * W * ROUND) return bisect_held<2, W>(s.need, keys, span, lane, w, join);
+    if constexpr (W == 1) {
+        if (span <= 5 * ROUND) return bisect_held<5, W>(s.need, keys, span, lane, w, join);
+        return bisect_held<8, W>(s.need, keys, span, lane, w, join);
     }
-    // pages in order: wave w takes [i0, i1)
-    const int seen64 = (s.seen + 63) & ~63, part = NW == 1 ? seen64 : ((seen64 / 64 + NW - 1) / NW) * 64;
-    const int i0 = min(w * part, seen64), i1 = min(i0 + part, seen64);
+    const int all = span / ROUND, mine = (all - w + W - 1) / W;
+    return bisect(s.need, mine, [&](int n) { return *reinterpret_cast<const u32x4 *>(keys + (n * W + w) * ROUND + 4 * lane); }, join);
+}
+
+// Writes one token's kept pages in order, zeros behind them, and its number of keys; NW waves share the
+// pages (all of the work-group where NW > 1: red holds 2 NW words of LDS).
+template <int NW>
+__device__ __forceinline__ void write_pages(const SelectParams &p, const Seen &s, const Limit &l, const uint32_t *keys, size_t pair,
+                                            const int32_t *bt, int lane, int w, int *red) {
+    const int steps = (s.seen + 63) >> 6, part = NW == 1 ? steps : (steps + NW - 1) / NW;
+    const int i0 = min(w * part, steps) * 64, i1 = min((w + 1) * part, steps) * 64;
     int base = 0, eq = 0;
     auto page = [&](int i, bool &sure, bool &even) {
         const uint32_t k = keys[i];
         const bool cand = i >= s.c0 && i < s.c1;
-        sure = i < s.seen && (!cand || k > limit);
-        even = cand && k == limit;
+        sure = i < s.seen && (!cand || k > l.limit);
+        even = cand && k == l.limit;
     };
     if constexpr (NW > 1) {
         int ns = 0, ne = 0;
@@ -303,37 +334,59 @@ __device__ __forceinline__ void keep_pages(const SelectParams &p, const Seen &s,
             ns += __popcll(__ballot(sure));
             ne += __popcll(__ballot(even));
         }
-        __syncthreads();
         if (lane == 0) red[w] = ns, red[NW + w] = ne;
         __syncthreads();
-        for (int i = 0; i < w; i++) base += red[i], eq += red[NW + i];
+        base = wave_total(lane < w ? red[lane] : 0);
+        eq = wave_total(lane < w ? red[NW + lane] : 0);
     }
     int32_t *out = p.tables + pair * p.keep;
     const unsigned long long below = (1ull << lane) - 1;
+    int next = bt[min(i0 + lane, s.seen - 1)];
     for (int i = i0; i < i1; i += 64) {
+        const int id = next;
+        next = bt[min(i + 64 + lane, s.seen - 1)];
         bool sure, even;
         page(i + lane, sure, even);
         const unsigned long long ms = __ballot(sure), me = __ballot(even);
         // pages written before this one: the sure ones, and the equal ones while there was room
-        const int q = eq + __popcll(me & below), at = base + __popcll(ms & below) + min(q, ties);
-        if ((sure || (even && q < ties)) && at < s.kept) out[at] = bt[i + lane];
+        const int q = eq + __popcll(me & below), at = base + __popcll(ms & below) + min(q, l.ties);
+        if ((sure || (even && q < l.ties)) && at < s.kept) out[at] = id;
         base += __popcll(ms);
         eq += __popcll(me);
     }
     for (int i = s.kept + w * 64 + lane; i < p.keep; i += NW * 64) out[i] = 0;
     if (w == 0 && lane == 0) {
-        const long long l = (long long)(s.kept - 1) * p.P + min(s.last + 1 - (s.seen - 1) * p.P, p.P);
-        p.lengths[pair] = (int)l;
+        const long long n = (long long)(s.kept - 1) * p.P + min(s.last + 1 - (s.seen - 1) * p.P, p.P);
+        p.lengths[pair] = (int)n;
     }
 }
 
+// One token's pages by the whole work-group of W waves: up to ONE keys are searched by one wave (no
+// barriers: 2048 keys 31 us for the call against 34.5 by 16 waves), more by all; all write. red: 4 W + 2 words of LDS.
+template <int W>
+__device__ __forceinline__ void keep_together(const SelectParams &p, const Seen &s, uint32_t *keys, int span, size_t pair,
+                                              const int32_t *bt, int lane, int w, int *red) {
+    Limit l;
+    if (span <= ONE) {
+        if (w == 0) {
+            l = find_limit<1>(s, keys, span, lane, 0, red);
+            if (lane == 0) red[0] = (int)l.limit, red[1] = l.ties;
+        }
+        __syncthreads();
+        l = Limit{(uint32_t)red[0], red[1]};
+    } else {
+        l = find_limit<W>(s, keys, span, lane, w, red + 2);
+    }
+    write_pages<W>(p, s, l, keys, pair, bt, lane, w, red + 2 + 2 * W);
+}
+
 // Grid (Hk, token tiles, B), the keys of the tile's tokens in LDS.
-template <int D, int GP, int RT, bool WIDE>
-__global__ void __launch_bounds__(THREADS) select_kernel(SelectParams p) {
+template <int D, int GP, int RT, bool WIDE, int W>
+__global__ void __launch_bounds__(W * 64) select_kernel(SelectParams p) {
     using TL = Tile<GP, RT, WIDE>;
     __shared__ __attribute__((aligned(16))) int8_t w[TL::ROWS][2 * D];
     __shared__ float forth[TL::ROWS];
-    __shared__ int red[3 * WAVES + 3];
+    __shared__ int red[4 * W + 2];
     extern __shared__ __attribute__((aligned(16))) uint32_t keys[];   // [TT][pitch]
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x, b = blockIdx.z;
@@ -343,27 +396,30 @@ __global__ void __launch_bounds__(THREADS) select_kernel(SelectParams p) {
         const int tokens = min(TL::TT, st.n - t0);
         const int most = Seen(p, st, t0 + tokens - 1).seen, ntiles = (most + 15) >> 4;
         const int span = (most + ROUND - 1) / ROUND * ROUND;
-        quantize_rows<D, GP, RT, WIDE>(p, st, h, t0, tid, w, forth);
-        for (int i = ntiles * 16 + tid; i < span; i += THREADS)
-            for (int t = 0; t < tokens; t++) keys[t * p.pitch + i] = 0;
+        quantize_rows<D, GP, RT, WIDE, W>(p, st, h, t0, tid, w, forth);
         __syncthreads();
-        score_pages<D, GP, RT, WIDE>(p, st, b, h, t0, lane, wv, WAVES, ntiles, most, w, forth,
+        score_pages<D, GP, RT, WIDE>(p, b, h, tokens, lane, wv, W, ntiles, most, w, forth,
                                      [&](int t, int page) { return keys + t * p.pitch + page; });
         __syncthreads();
         const int32_t *bt = p.bt + (size_t)b * p.bt_stride;
-        if constexpr (TL::TT == 1) {
-            keep_pages<WAVES>(p, Seen(p, st, t0), (const uint32_t *)keys, span, (size_t)(st.tok0 + t0) * p.Hk + h, bt, lane, wv, red);
+        if (tokens == 1 || span > ONE) {
+            for (int t = 0; t < tokens; t++) {
+                keep_together<W>(p, Seen(p, st, t0 + t), keys + t * p.pitch, span, (size_t)(st.tok0 + t0 + t) * p.Hk + h, bt, lane, wv, red);
+                __syncthreads();   // red is read
+            }
         } else {
-            for (int t = wv; t < tokens; t += WAVES)
-                keep_pages<1>(p, Seen(p, st, t0 + t), (const uint32_t *)keys + t * p.pitch, span,
-                              (size_t)(st.tok0 + t0 + t) * p.Hk + h, bt, lane, 0, red);
+            for (int t = wv; t < tokens; t += W) {
+                const Seen s(p, st, t0 + t);
+                const Limit l = find_limit<1>(s, keys + t * p.pitch, span, lane, 0, red);
+                write_pages<1>(p, s, l, keys + t * p.pitch, (size_t)(st.tok0 + t0 + t) * p.Hk + h, bt, lane, 0, red);
+            }
         }
     }
 }
 
 // The keys of a token tile to the workspace: grid (Hk x split, token tiles, B).
-template <int D, int GP, int RT, bool WIDE>
-__global__ void __launch_bounds__(THREADS) scores_kernel(SelectParams p) {
+template <int D, int GP, int RT, bool WIDE, int W>
+__global__ void __launch_bounds__(W * 64) scores_kernel(SelectParams p) {
     using TL = Tile<GP, RT, WIDE>;
     __shared__ __attribute__((aligned(16))) int8_t w[TL::ROWS][2 * D];
     __shared__ float forth[TL::ROWS];
@@ -374,37 +430,47 @@ __global__ void __launch_bounds__(THREADS) scores_kernel(SelectParams p) {
         __syncthreads();
         const int tokens = min(TL::TT, st.n - t0);
         const int most = Seen(p, st, t0 + tokens - 1).seen, ntiles = (most + 15) >> 4;
-        const int span = (most + ROUND - 1) / ROUND * ROUND;
-        quantize_rows<D, GP, RT, WIDE>(p, st, h, t0, tid, w, forth);
-        auto at = [&](int t, int page) { return p.keys + ((size_t)(st.tok0 + t0 + t) * p.Hk + h) * p.pitch + page; };
-        if (part == 0)
-            for (int i = ntiles * 16 + tid; i < span; i += THREADS)
-                for (int t = 0; t < tokens; t++) *at(t, i) = 0;
+        quantize_rows<D, GP, RT, WIDE, W>(p, st, h, t0, tid, w, forth);
         __syncthreads();
-        score_pages<D, GP, RT, WIDE>(p, st, b, h, t0, lane, part * WAVES + wv, p.split * WAVES, ntiles, most, w, forth, at);
+        score_pages<D, GP, RT, WIDE>(p, b, h, tokens, lane, part * W + wv, p.split * W, ntiles, most, w, forth, [&](int t, int page) {
+            return p.keys + ((size_t)(st.tok0 + t0 + t) * p.Hk + h) * p.pitch + page;
+        });
     }
 }
 
-// Kept pages of one token and KV head from the workspace: grid (Hk, tokens, B). `tt` is the scores'
-// token tile: rows of keys are padded to the last visible page of their tile.
-__global__ void __launch_bounds__(THREADS) keep_kernel(SelectParams p, int tt) {
-    __shared__ int red[3 * WAVES + 3];
+// Kept pages of one token and KV head from the workspace: grid (Hk, tokens, B). The keys are read into LDS
+// where it holds them (`lds` of them).
+template <int W> __global__ void __launch_bounds__(W * 64) keep_kernel(SelectParams p, int lds) {
+    __shared__ int red[4 * W + 2];
+    extern __shared__ __attribute__((aligned(16))) uint32_t held[];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x, b = blockIdx.z;
     const Step st = step_of(p.qsl, p.positions, b, p.nmax, p.total);
     for (int t = blockIdx.y; t < st.n; t += gridDim.y) {
-        const int most = Seen(p, st, min(t / tt * tt + tt, st.n) - 1).seen, span = (most + ROUND - 1) / ROUND * ROUND;
+        const Seen s(p, st, t);
+        const int span = (s.seen + ROUND - 1) / ROUND * ROUND;
         const size_t pair = (size_t)(st.tok0 + t) * p.Hk + h;
-        __syncthreads();   // the token before this one is done with red
-        keep_pages<WAVES>(p, Seen(p, st, t), (const uint32_t *)p.keys + pair * p.pitch, span, pair, p.bt + (size_t)b * p.bt_stride,
-                          lane, wv, red);
+        uint32_t *keys = p.keys + pair * p.pitch;
+        __syncthreads();   // the token before this one is done with LDS
+        const int32_t *bt = p.bt + (size_t)b * p.bt_stride;
+        if (span <= lds) {
+            for (int i = 4 * tid; i < span; i += W * 256)
+                *reinterpret_cast<u32x4 *>(held + i) = *reinterpret_cast<const u32x4 *>(keys + i);
+            __syncthreads();
+            keep_together<W>(p, s, held, span, pair, bt, lane, wv, red);
+        } else {
+            keep_together<W>(p, s, keys, span, pair, bt, lane, wv, red);
+        }
     }
 }
 
 // LDS that select_kernel's keys may take: one work-group of 16 waves and its operands on a CU.
 constexpr int LDS_KEYS = 136 << 10;
+bool allow_lds(const void *kernel, size_t bytes) {
+    return bytes <= (32u << 10) || hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
+}
 
-template <int D, int GP, int RT, bool WIDE>
+template <int D, int GP, int RT, bool WIDE, int W>
 int launch(SelectParams p, int num_seqs, hipStream_t s) {
     constexpr int TT = Tile<GP, RT, WIDE>::TT;
     const long long tiles = (p.nmax + (long long)TT - 1) / TT, groups = tiles * num_seqs * p.Hk;
@@ -412,35 +478,41 @@ int launch(SelectParams p, int num_seqs, hipStream_t s) {
     const size_t bytes = (size_t)TT * p.pitch * sizeof(uint32_t);
     // One launch while the keys fit LDS and either the launch's work-groups fill half of the chip or a
     // table is short; a wide table's pages are shared out over work-groups otherwise.
-    if (bytes <= (size_t)LDS_KEYS && (groups >= 128 || p.bt_stride <= 2048)) {
-        auto kernel = select_kernel<D, GP, RT, WIDE>;
-        if (bytes > (48u << 10) &&
-            hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess)
-            return TI_ERR_LAUNCH;
-        kernel<<<dim3(p.Hk, y, num_seqs), THREADS, bytes, s>>>(p);
+    if (bytes <= (size_t)LDS_KEYS && (groups >= 128 || p.bt_stride <= 1024)) {
+        auto kernel = select_kernel<D, GP, RT, WIDE, W>;
+        if (!allow_lds((const void *)kernel, bytes)) return TI_ERR_LAUNCH;
+        kernel<<<dim3(p.Hk, y, num_seqs), W * 64, bytes, s>>>(p);
         return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
     }
     p.split = 1;
-    while (groups * p.split < 256 && p.split * WAVES * 32 < p.bt_stride) p.split <<= 1;
-    scores_kernel<D, GP, RT, WIDE><<<dim3(p.Hk * p.split, y, num_seqs), THREADS, 0, s>>>(p);
+    while (groups * p.split < 256 && p.split * W * 32 < p.bt_stride) p.split <<= 1;
+    scores_kernel<D, GP, RT, WIDE, W><<<dim3(p.Hk * p.split, y, num_seqs), W * 64, 0, s>>>(p);
     if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
-    keep_kernel<<<dim3(p.Hk, min(p.nmax, 32768), num_seqs), THREADS, 0, s>>>(p, TT);
+    const size_t held = min((size_t)p.pitch * sizeof(uint32_t), (size_t)LDS_KEYS);
+    if (!allow_lds((const void *)keep_kernel<W>, held)) return TI_ERR_LAUNCH;
+    keep_kernel<W><<<dim3(p.Hk, min(p.nmax, 32768), num_seqs), W * 64, held, s>>>(p, (int)(held / sizeof(uint32_t)));
     return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
 }
 
-// Query rows per tile: 64 where the steps' tokens fill them and the launch still has work-groups for
-// every CU (bounds are then read once for four blocks of rows), else 16.
+// Query rows per tile: 64 (32 where a token's heads do not fill a lane's four rows or go past them: 64
+// spill there) where the steps' tokens fill them and the launch still has work-groups for every CU
+// (bounds are then read once for several blocks of rows), else 16.
+constexpr int W4_PAGES = 256;
 template <int D, int GP>
 int launch_rows(const SelectParams &p, int num_seqs, hipStream_t s) {
-    constexpr int TT = Tile<GP, 4, false>::TT;
+    constexpr int RT = GP == 4 || GP == 16 ? 4 : 2, TT = Tile<GP, RT, false>::TT;
     const long long groups = ((long long)p.nmax + TT - 1) / TT * num_seqs * p.Hk;
-    if (groups >= 256 && p.nmax >= TT && (size_t)TT * p.pitch * 4 <= (size_t)LDS_KEYS) return launch<D, GP, 4, false>(p, num_seqs, s);
-    return launch<D, GP, 1, false>(p, num_seqs, s);
+    const long long groups1 = (p.nmax + 16LL / GP - 1) / (16 / GP) * num_seqs * p.Hk;
+    if (groups >= 256 && p.nmax >= TT && (size_t)TT * p.pitch * 4 <= (size_t)LDS_KEYS) return launch<D, GP, RT, false, 16>(p, num_seqs, s);
+    // 4 waves for tables that give no more than two 16-page tiles to each and a launch of several work-groups
+    // per CU, 16 otherwise.
+    if (p.bt_stride <= W4_PAGES && groups1 >= 512) return launch<D, GP, 1, false, 4>(p, num_seqs, s);
+    return launch<D, GP, 1, false, 16>(p, num_seqs, s);
 }
 
 template <int D>
 int launch_heads(const SelectParams &p, int num_seqs, hipStream_t s) {
-    if (p.G > 16) return launch<D, 16, 4, true>(p, num_seqs, s);
+    if (p.G > 16) return launch<D, 16, 4, true, 16>(p, num_seqs, s);
     if (p.G > 8) return launch_rows<D, 16>(p, num_seqs, s);
     if (p.G > 4) return launch_rows<D, 8>(p, num_seqs, s);
     if (p.G > 2) return launch_rows<D, 4>(p, num_seqs, s);
@@ -470,6 +542,7 @@ int ti_launch_select_pages(const ti_select_args *a, hipStream_t s) {
     p.bt_stride = a->block_table_stride;
     p.num_pages = a->num_pages;
     p.P = a->page_size;
+    p.pshift = (p.P & (p.P - 1)) == 0 ? __builtin_ctz(p.P) : -1;
     p.Hk = a->kv_heads;
     p.Hq = a->q_heads;
     p.G = a->q_heads / a->kv_heads;
