@@ -41,6 +41,7 @@ class Cache:
             self.hk = (q[0].float() * s[0][..., None] * self.smooth).double().numpy()    # rounded as specified
             self.raw = q[0].double().numpy() * s[0][..., None].double().numpy()           # without smoothing
             self.hv = q[1].double().numpy() * s[1][..., None].double().numpy()
+            self.scales = s.double().numpy()
         else:
             k = torch.randn((self.pages, H, P, D), generator=g).to(T[kv])
             v = torch.randn((self.pages, H, P, D), generator=g).to(T[kv])
@@ -281,8 +282,11 @@ def check_attend(c, q, tables, lengths, scale=None, qsl=None, n=None, out=None):
     lo, hi = (0, rows) if qsl is None else (int(qsl[0]), int(qsl[-1]))
     half = torch.finfo(q.dtype).eps / 2
     if c.kv == "int8":
-        # the kernel's queries: rounded to bf16 after smoothing; weights times value scales in fp16
-        qd = (q.float().cpu() * c.smooth).to(torch.bfloat16).double().numpy()
+        # the kernel's queries: smoothed, then rounded to fp16's 11 bits (a row's largest scaled into [2^14, 2^15),
+        # where every float of 2^-28 of it is normal); weights times value scales in fp16
+        x = (q.float().cpu() * c.smooth).double()
+        e = 15 - torch.frexp(x.abs().amax(2, keepdim=True)).exponent
+        qd = torch.ldexp(torch.ldexp(x, e).to(torch.float16).double(), -e).numpy()
     keys_of = c.raw if c.kv == "int8" else c.hk
     p_eps = {"bf16": 2.0 ** -8, "int8": 2.0 ** -11 + 2.0 ** -23, "fp32": 0.0, "int8_fp32": 2.0 ** -22}[c.kv]
     for r in range(rows):
@@ -297,7 +301,19 @@ def check_attend(c, q, tables, lengths, scale=None, qsl=None, n=None, out=None):
             page = np.clip(table[r, h][at // c.P] - 1, 0, c.pages - 1)
             k, v = keys_of[page, h, at % c.P], c.hv[page, h, at % c.P]
             want, weight, size = ref.attend(rows_, k, v, scale)
-            tol = ref.attention_tolerance(want, weight, size, D + (3 if c.kv == "int8_fp32" else 0), m, p_eps, half)
+            bias = 0.0
+            if c.kv == "int8" and m:
+                # The kernel multiplies biased values: sums of q (1152 + b) and p s (1152 + b), from which 1152 sum(q)
+                # and 1152 sum(p s) come off. |b| <= 127, so every partial sum is at most 1279 (1152) times sum |q|
+                # (sum p s), and each of its additions, the other sum's and the subtraction round by 2^-24 of that:
+                # 2431 sum |q| s scale takes the place of the scores' size, and 2431 (keys + 2) 2^-24 sum(p s) is
+                # added to the output. A weight p s (p <= 1 of the largest, whose own is at least 1 of the sum) below
+                # fp16's normal range 2^-14 rounds to a multiple of 2^-24: off by 2^-25 of |b| per key.
+                ks, vs = c.scales[0][page, h, at % c.P], c.scales[1][page, h, at % c.P]
+                size = 2431 * np.abs(rows_).sum(1).max() * ks.max() * scale
+                bias = 2431 * (m + 2) * 2.0 ** -24 * ref.attend(rows_, k, vs[:, None], scale)[0] \
+                    + 2.0 ** -25 * np.abs(v / vs[:, None]).sum(0)
+            tol = bias + ref.attention_tolerance(want, weight, size, D + (3 if c.kv == "int8_fp32" else 0), m, p_eps, half)
             worst = np.max(np.abs(mine - want) / tol)
             assert worst <= 1, f"row {r} head {h}: {worst:.2f} times the tolerance"
     return got
@@ -394,6 +410,98 @@ def test_attend_does_not_see_past_the_last_key(gpu, kv):
             c.k[i, :, 7:], c.v[i, :, 7:] = math.nan, math.inf
     check_attend(c, q, tables, lengths)
     check_attend(c, q, tables, lengths, n=6)
+
+
+def shared(c, rows, width, seed, common=0.8):
+    """Tables as the tokens of a step select them: most pages are the same from token to token, and every
+    token's last page is partly filled, to another position."""
+    g = torch.Generator().manual_seed(seed)
+    liked = torch.rand((c.H, c.pages), generator=g)
+    t = torch.zeros((rows, c.H, width), dtype=torch.int32)
+    for r in range(rows):
+        rank = common * liked + (1 - common) * torch.rand((c.H, c.pages), generator=g)
+        t[r] = torch.sort(torch.topk(rank, width, dim=1).indices, dim=1).values + 1
+    n = torch.randint(1, width * c.P + 1, (rows, c.H), generator=g)
+    n[: rows // 2] = (width - 1) * c.P + torch.randint(1, c.P + 1, (rows // 2, c.H), generator=g)
+    return t.cuda().contiguous(), n.to(torch.int32).cuda().contiguous()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G,P", [(4, 16), (4, 64), (1, 16), (2, 32), (3, 16), (7, 64), (8, 16), (12, 16), (16, 32)])
+@pytest.mark.parametrize("rows", [2, 16, 33])
+def test_attend_steps_that_share_pages(gpu, kv, D, G, P, rows):
+    c = Cache(kv, D, 2, P, [40 * P], seed=G + P)
+    torch.manual_seed(G)
+    q = torch.randn((rows, 2 * G, D), device="cuda", dtype=T[kv])
+    tables, lengths = shared(c, rows, 13, seed=G)
+    check_attend(c, q, tables, lengths, n=rows)
+    lengths[0], lengths[rows // 2, 0], lengths[-1] = 0, 1, 13 * P
+    check_attend(c, q, tables, lengths, n=rows)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("width", [1, 5, 70, 200, 600, 1100])
+def test_attend_steps_of_any_width(gpu, kv, width):
+    """As many tokens as their tables leave room for: 32 rows, 16, fewer tokens than fill them, one."""
+    c = Cache(kv, 64, 8, 16, [16 * (width + 40)], seed=width)
+    torch.manual_seed(width)
+    rows = 520 if width <= 5 else 12
+    q = torch.randn((rows, 32, 64), device="cuda", dtype=T[kv])
+    tables, lengths = shared(c, rows, width, seed=width)
+    check_attend(c, q, tables, lengths, n=rows)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("rows,heads", [(6, 2), (300, 8)])
+def test_attend_values_that_are_not_finite_stay_with_their_tokens(gpu, value, where, rows, heads):
+    """A key or value that is not finite in a page that some tokens of a step keep, or behind the last key
+    of others: tokens that do not see it are as without it, those that do are as their own attention."""
+    c = Cache("bf16", 128, heads, 16, [60 * 16], seed=31)
+    torch.manual_seed(31)
+    q = torch.randn((rows, heads * 4, 128), device="cuda", dtype=torch.bfloat16)
+    tables, lengths = shared(c, rows, 9, seed=31)
+    lengths[:] = 8 * 16 + 9
+    bad = tables[1, 0, 2].item()
+    last = tables[3, 1, 8].item()
+    pool = c.k if where == "k" else c.v
+    pool[bad - 1, :, 5, 17] = value
+    pool[last - 1, :, 9, 3] = value                # seen where this page is not the last one
+    alone = torch.empty_like(q)
+    ti.sparse_attention_(BE, alone, ti.sparse_attention_workspace(BE, q, c.k, tables), q, c.k, c.v, tables, lengths, 0.09)
+    got = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09, None, rows)
+    touched = (((tables == bad) | (tables == last)) & ~((tables == last) & (torch.arange(9, device="cuda") == 8)
+                                                     & (tables != bad))).any(2)
+    touched = touched.repeat_interleave(4, 1)
+    assert touched.any() and not touched.all()
+    clean = pool.clone()
+    clean[bad - 1, :, 5, 17], clean[last - 1, :, 9, 3] = 0, 0
+    k, v = (clean, c.v) if where == "k" else (c.k, clean)
+    want = ti.sparse_attention(BE, q, k, v, tables, lengths, 0.09, None, rows)
+    # rows of the wave-by-row path round otherwise: each is within 2^-7 of the exact weights and output
+    assert torch.isfinite(got[~touched]).all()
+    tol = 4 * 2.0 ** -8 * c.v[torch.isfinite(c.v)].float().abs().max()
+    assert (got[~touched].float() - want[~touched].float()).abs().max() <= tol
+    a, b = alone[touched].float(), got[touched].float()
+    assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.isinf(a), torch.isinf(b))
+    fine = torch.isfinite(a)
+    assert ((a[fine] - b[fine]).abs() <= tol).all()
+
+
+def test_attend_sequences_do_not_touch_each_other(gpu):
+    """Steps of several sequences whose rows fall into one group: NaN in one sequence's cache."""
+    c = Cache("bf16", 128, 2, 16, [160, 160, 160], seed=32)
+    torch.manual_seed(32)
+    q = torch.randn((9, 8, 128), device="cuda", dtype=torch.bfloat16)
+    kb = ti.key_bounds(128, 16, 2, c.pages)
+    pos = positions([157, 157, 157], [3, 3, 3])
+    for i in c.rows[1]:
+        c.k[i - 1], c.v[i - 1] = math.nan, math.nan
+    ti.update_key_bounds_(BE, kb, c.k, c.v, c.tables, positions([0, 0, 0], [160] * 3), max_query_len=160)
+    tables, lengths = ti.select_pages(BE, q, kb, c.tables, pos, 6, max_query_len=3)
+    got = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09, None, 3)
+    assert torch.isnan(got[3:6]).all() and torch.isfinite(got[:3]).all() and torch.isfinite(got[6:]).all()
 
 
 def test_attend_large_and_small_scores(gpu):

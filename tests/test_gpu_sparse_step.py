@@ -26,7 +26,7 @@ class View:
             self.kv, self.smooth = "int8", self.k.smooth.cpu()
             q, s = self.k.layer_q.cpu().double().numpy(), self.k.layer_scale.cpu().double().numpy()
             self.hk = (self.k.q.float() * self.k.scale[..., None] * self.k.smooth).double().cpu().numpy()
-            self.raw, self.hv = q[0] * s[0][..., None], q[1] * s[1][..., None]
+            self.raw, self.hv, self.scales = q[0] * s[0][..., None], q[1] * s[1][..., None], s
         else:
             self.kv = "bf16"
             self.hk, self.hv = self.k.double().cpu().numpy(), self.v.double().cpu().numpy()

@@ -151,11 +151,6 @@ int check_workspace(const void *ws, size_t have, size_t need) {
     return misaligned(ws) ? TI_ERR_INVALID_ARG : TI_OK;
 }
 
-size_t sparse_bytes(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
-    const int sp = ti_sparse_splits(a, c);
-    return sp == 1 ? 0 : (size_t)a->total_tokens * a->q_heads * sp * (c->head_dim + 2) * sizeof(float);
-}
-
 }  // namespace
 
 extern "C" {
@@ -321,13 +316,13 @@ int ti_sparse_attention_workspace_bytes(const ti_sparse_attention_args *a, const
     *bytes = 0;
     const int st = check_sparse(a, c);
     if (st) return st;
-    *bytes = sparse_bytes(a, c);
+    *bytes = ti_sparse_bytes(a, c);
     return TI_OK;
 }
 
 int ti_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, void *stream) {
     int st = check_sparse(a, c);
-    if (!st) st = check_workspace(a->workspace, a->workspace_bytes, sparse_bytes(a, c));
+    if (!st) st = check_workspace(a->workspace, a->workspace_bytes, ti_sparse_bytes(a, c));
     return st ? st : ti_launch_sparse_attention(a, c, (hipStream_t)stream);
 }
 

@@ -179,7 +179,12 @@ int ti_plan_generic(const ti_attention_args *a, const ti_kv_cache *c, size_t *by
 int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStream_t s);
 
 // Attention over chosen pages (pa_sparse.hip, its fp32 kernels in pa_generic.hip).
-int ti_sparse_splits(const ti_sparse_attention_args *a, const ti_kv_cache *c);
+struct ti_sparse_plan {
+    int tg;       // neighbouring tokens worked on together
+    int splits;   // work-groups that share the keys of a (group of tokens, KV head)
+};
+ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c);
+size_t ti_sparse_bytes(const ti_sparse_attention_args *a, const ti_kv_cache *c);
 int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, hipStream_t s);
 int ti_launch_sparse_f32(const ti_sparse_attention_args *a, const ti_kv_cache *c, int splits, hipStream_t s);
 // Page bounds and the selection by them (page_bounds.hip).

@@ -41,6 +41,8 @@
 // w_s = exp2(m_s - max m), o = sum acc_s w_s / sum l_s w_s.
 #pragma once
 
+#include <stddef.h>
+
 #include <type_traits>
 
 #include "common.hpp"
@@ -65,6 +67,7 @@ struct DecodeParams {
     int min_tiles;   // > 0: splits of at least this many 16-key tiles (f32_active_splits)
     float scale_log2;
     const int32_t *lengths;   // SPARSE: keys of each (token, KV head); bt holds a table row for each
+    int tg, total;            // GROUP: tokens of a group, tokens of the call
 };
 
 // Flat mode: the W = p.flat work-groups of a KV head are shared out over the B sequences
@@ -195,11 +198,33 @@ struct RowMap {
         const int pg = page_of_s(bt, pos >> pshift, bt_stride, num_pages);
         return ((long long)pg * Hk + h) * P + (pos & (P - 1));
     }
+    __device__ __forceinline__ int last(int pos) const { return len - 1 - pos; }   // last key of the tile at pos
 };
 
-template <int D, bool INT8, bool PG16>
+// The same over the pages of a group's tokens (GROUP, see group_pages): page u holds `most` keys that
+// one of the tokens sees. Tiles past them read the page's last tile that has some.
+struct GroupMap {
+    const int2 *pages;   // LDS: {page, most}
+    int P, pshift, Hk, h, len;
+    __device__ __forceinline__ int2 page(int pos) const {
+        const int2 e = pages[pos >> pshift];
+        return make_int2(__builtin_amdgcn_readfirstlane(e.x), __builtin_amdgcn_readfirstlane(e.y));
+    }
+    __device__ __forceinline__ int first(int pos, int most) const { return min(pos & (P - 1), (most - 1) & ~15); }
+    __device__ __forceinline__ long long row_s(int pos) const {
+        const int2 e = page(pos);
+        return ((long long)e.x * Hk + h) * P + first(pos, e.y);
+    }
+    __device__ __forceinline__ int last(int pos) const {
+        const int most = page(pos).y;
+        return most - 1 - first(pos, most);
+    }
+    __device__ __forceinline__ long long row(int) const { return 0; }   // whole tiles only
+};
+
+template <int D, bool INT8, bool PG16, typename Map>
 __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodeParams &p,
-                                          const RowMap &rm, int j, int r16, int kg, int vg,
+                                          const Map &rm, int j, int r16, int kg, int vg,
                                           int vc, size_t half_q, size_t half_s) {
     constexpr int NKB = TileRegs<D, INT8>::NKB, KPL = TileRegs<D, INT8>::KPL;
     if (PG16) {
@@ -208,7 +233,7 @@ __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodePara
         // valid key's row, whose finite values meet p = 0 (never stale memory that could
         // hold NaN).
         const long long r0 = rm.row_s(j * 16);
-        const int last = rm.len - 1 - j * 16;
+        const int last = rm.last(j * 16);
         const uint32_t kr = (uint32_t)min(r16, last);
         uint32_t vr[KPL];
 #pragma unroll
@@ -275,10 +300,155 @@ __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodePara
     }
 }
 
+// Groups of tokens over chosen pages. The tables of up to GROUP_PAGES entries in all are joined into one
+// list of pages in LDS, each with the number of its keys that each token sees (0: not in its table), so
+// that a page that several tokens keep is read and multiplied once for all their rows. An entry's place is
+// that of its first mention (position in the table first, then token): found with a hash table in LDS whose
+// slots keep the smallest mention, so the list does not depend on the order of the threads. Where a token
+// names a page twice, every entry is a page of its own.
+constexpr int GROUP_PAGES = 1024, GROUP_SLOTS = 2 * GROUP_PAGES;
+struct GroupLds {
+    int2 pages[GROUP_PAGES];             // {page, keys that some token sees}
+    union {
+        struct {                         // while the list is made
+            int id[GROUP_SLOTS], first[GROUP_SLOTS];
+            uint32_t seen[GROUP_SLOTS];
+        } slot;
+        char rest[1];                    // then the value tiles
+    };
+};
+
+template <int NT>
+__device__ int group_pages(const DecodeParams &p, GroupLds &g, uint16_t *lim, int *red, int tok0, int h, int q0, int q1) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, K = p.bt_stride, TG = p.tg, entries = TG * K;
+    for (int i = tid; i < GROUP_SLOTS; i += NT) g.slot.id[i] = -1, g.slot.first[i] = 0x7fffffff, g.slot.seen[i] = 0;
+    for (int i = tid; i < entries * TG; i += NT) lim[i] = 0;
+    if (tid == 0) red[0] = 0;
+    __syncthreads();
+    constexpr int EACH = GROUP_PAGES / NT;
+    int id[EACH], slot[EACH], keys[EACH];
+#pragma unroll
+    for (int n = 0; n < EACH; n++) {
+        const int x = n * NT + tid, a = x / TG, tok = tok0 + x - a * TG;
+        keys[n] = 0;
+        if (x < entries && tok >= q0 && tok < q1) {
+            const int len = min(p.lengths[tok * p.Hk + h], K * p.P);
+            keys[n] = min(len - a * p.P, p.P);
+            if (keys[n] > 0) id[n] = clamp_page(p.bt[((size_t)tok * p.Hk + h) * K + a], p.num_pages);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < EACH; n++) {
+        if (keys[n] <= 0) continue;
+        const int x = n * NT + tid;
+        int s = (int)(((uint32_t)id[n] * 2654435761u) >> 21) & (GROUP_SLOTS - 1);
+        while (true) {   // fewer entries than slots: a free one or the page's own is found
+            const int was = atomicCAS(&g.slot.id[s], -1, id[n]);
+            if (was == -1 || was == id[n]) break;
+            s = (s + 1) & (GROUP_SLOTS - 1);
+        }
+        slot[n] = s;
+        atomicMin(&g.slot.first[s], x);
+        const uint32_t bit = 1u << (x % TG);
+        if (atomicOr(&g.slot.seen[s], bit) & bit) red[0] = 1;   // named twice by one token
+    }
+    __syncthreads();
+    const bool apart = red[0] != 0;
+    // places in order of mention
+    int base = 0;
+#pragma unroll
+    for (int n = 0; n < EACH; n++) {
+        const int x = n * NT + tid;
+        const bool first = keys[n] > 0 && (apart || g.slot.first[slot[n]] == x);
+        const unsigned long long m = __ballot(first);
+        __syncthreads();
+        if (lane == 0) red[1 + w] = __popcll(m);
+        __syncthreads();
+        int at = base + __popcll(m & ((1ull << lane) - 1));
+#pragma unroll
+        for (int i = 0; i < NT / 64; i++) {
+            if (i < w) at += red[1 + i];
+            base += red[1 + i];
+        }
+        if (first) {
+            g.pages[at] = make_int2(id[n], 0);
+            if (!apart) g.slot.first[slot[n]] = -1 - at;   // its mentions find the place here
+            else slot[n] = at;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < EACH; n++) {
+        if (keys[n] <= 0) continue;
+        const int x = n * NT + tid, at = apart ? slot[n] : -1 - g.slot.first[slot[n]];
+        lim[at * TG + x % TG] = (uint16_t)keys[n];
+        atomicMax(&g.pages[at].y, keys[n]);
+    }
+    __syncthreads();   // the slots' LDS is free for the value tiles
+    return base;
+}
+
+// A group's rows one by one on the vector ALUs, over the same tiles: where the matrix products of a dense
+// cache met a value that is not finite. There a row's weight of 0 times such a value of a page that only
+// other rows see is NaN; here a key that a row does not see is not touched. (INT8 values are finite, and
+// a key's scales enter its own rows' weights only.)
+template <int D>
+__device__ __forceinline__ void group_rows(const DecodeParams &p, const int2 *pages, const uint16_t *lim, int tok0, int h, int q0, int q1,
+                                           int j0, int j1, int nsp, size_t unit, int w, int nw, int lane) {
+    constexpr int PER = D / 64;
+    for (int r = w; r < p.M; r += nw) {
+        const int t = r / p.G, tok = tok0 + t;
+        if (tok < q0 || tok >= q1) continue;
+        const size_t qrow = (size_t)tok * p.Hq + h * p.G + (r - t * p.G);
+        float m = NEG_BIG, l = 0.0f, acc[PER];
+#pragma unroll
+        for (int k = 0; k < PER; k++) acc[k] = 0.0f;
+        for (int j = j0; j < j1; j += 4) {
+            const int pos = (j + (lane >> 4)) * 16 + (lane & 15);
+            bool see = (j + (lane >> 4)) < j1;
+            const int u = see ? pos >> p.pshift : 0, off = pos & (p.P - 1);
+            see = see && off < lim[u * p.tg + t];
+            const long long row = ((long long)pages[u].x * p.Hk + h) * p.P + off;
+            float s = -INFINITY;
+            if (see) {
+                float dot = 0.0f;
+                for (int d = 0; d < D; d++) dot += bf2f(p.q[qrow * D + d]) * bf2f(p.kp[row * D + d]);
+                s = dot * p.scale_log2;
+            }
+            const float mn = fmaxf(m, wave_max(s));
+            const float alpha = fast_exp2(m - mn), pr = see ? fast_exp2(s - mn) : 0.0f;
+            m = mn;
+            l = l * alpha + wave_sum(pr);
+#pragma unroll
+            for (int k = 0; k < PER; k++) acc[k] *= alpha;
+            for (int i = 0; i < 64; i++) {
+                if (!__shfl((int)see, i)) continue;
+                const float pi = __shfl(pr, i);
+                const long long ri = __shfl(row, i);
+#pragma unroll
+                for (int k = 0; k < PER; k++) acc[k] += pi * bf2f(p.vp[ri * D + lane + 64 * k]);
+            }
+        }
+        if (nsp == 1) {
+#pragma unroll
+            for (int k = 0; k < PER; k++) p.out[qrow * D + lane + 64 * k] = l == 0.0f ? 0 : f2bf(acc[k] / l);
+        } else {
+            float *dst = p.part + (unit * (size_t)p.M + r) * (D + 2);
+#pragma unroll
+            for (int k = 0; k < PER; k++) dst[lane + 64 * k] = acc[k];
+            if (lane == 0) {
+                dst[D] = m;
+                dst[D + 1] = l;
+            }
+        }
+    }
+}
+
 // SPARSE: every (token, KV head) pair has a table of pages and a length of its own (pa_sparse.hip);
 // a pair is a sequence of one token whose last key is at lengths - 1, and a 1-D grid holds the
-// pairs' splits, KV heads innermost.
-template <int D, int ROWB, bool INT8, bool PG16, int NW, int RS, bool JOINT = false, bool SPARSE = false>
+// pairs' splits, KV heads innermost. GROUP (SPARSE, whole tiles): p.tg neighbouring tokens' pairs at a time
+// over the joined list of their pages, packed rows g + G t of the group.
+template <int D, int ROWB, bool INT8, bool PG16, int NW, int RS, bool JOINT = false, bool SPARSE = false, bool GROUP = false>
 __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     constexpr int NKB = D / 32;          // 32-wide head-dim blocks (QK MFMAs per tile)
     constexpr int NDT = D / 16;          // 16-wide head-dim tiles (PV MFMAs per tile)
@@ -297,8 +467,12 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     constexpr int VROW = vtile_row<D>();
     constexpr int VT_BYTES = NW * JT * 16 * VROW * 2;
     constexpr int SLAB_BYTES = NW * MP * MROW * 4;
-    __shared__ __attribute__((aligned(16))) char smem_raw[VT_BYTES > SLAB_BYTES ? VT_BYTES : SLAB_BYTES];
-    uint16_t (*vt)[JT * 16 * VROW] = reinterpret_cast<uint16_t (*)[JT * 16 * VROW]>(smem_raw);
+    // GROUP: the joined pages in front of the value tiles, the tokens' keys of each in dynamic LDS
+    constexpr int LIST_BYTES = GROUP ? (int)offsetof(GroupLds, rest) : 0;
+    constexpr int LOOP_BYTES = GROUP && LIST_BYTES + VT_BYTES < (int)sizeof(GroupLds) ? (int)sizeof(GroupLds) : LIST_BYTES + VT_BYTES;
+    __shared__ __attribute__((aligned(16))) char smem_raw[LOOP_BYTES > SLAB_BYTES ? LOOP_BYTES : SLAB_BYTES];
+    uint16_t (*vt)[JT * 16 * VROW] = reinterpret_cast<uint16_t (*)[JT * 16 * VROW]>(smem_raw + LIST_BYTES);
+    extern __shared__ __attribute__((aligned(16))) uint16_t lim[];   // GROUP: [pages][tg]
     float *mslab = reinterpret_cast<float *>(smem_raw);
 
     const int lane = threadIdx.x & 63;
@@ -318,8 +492,12 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
         tok0 = pair / p.Hk;
         nb = 1;
         unit = blockIdx.x;
-        if (p.qsl && (tok0 < p.qsl[0] || tok0 >= p.qsl[p.B])) return;   // a row of no sequence
-        start = min(p.lengths[pair], p.bt_stride * p.P) - 1;
+        if constexpr (GROUP) {
+            tok0 *= p.tg;
+            nb = p.tg;
+        }
+        if (p.qsl && (tok0 + nb <= p.qsl[0] || tok0 >= p.qsl[p.B])) return;   // rows of no sequence
+        start = GROUP ? 0 : min(p.lengths[pair], p.bt_stride * p.P) - 1;
         if (start < 0) {   // no keys: zeros (the combine's, where the keys are split)
             if (nsp == 1)
                 for (int i = threadIdx.x; i < p.G * D / 4; i += NW * 64)
@@ -347,13 +525,21 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
         start = max(p.positions[tok0], 0);   // a negative position reads as 0
         unit = ((size_t)b * p.Hk + h) * p.splits + s;
     }
-    const int len = start + nb;
+    const int q0 = GROUP && p.qsl ? max(p.qsl[0], 0) : 0, q1 = GROUP ? (p.qsl ? min(p.qsl[p.B], p.total) : p.total) : 0;
+    int len = start + nb;
+    if constexpr (GROUP) {
+        __shared__ int red[1 + NW];
+        len = group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem_raw), lim, red, tok0, h, q0, q1) * p.P;
+    }
     const int ntiles = (len + 15) >> 4;
     const int per = (ntiles + nsp - 1) / nsp;
     const int j0 = s * per, j1 = min(j0 + per, ntiles);
     const size_t half_q = (size_t)p.num_pages * p.Hk * p.P * D;
     const size_t half_s = (size_t)p.num_pages * p.Hk * p.P;
-    const RowMap rm{p.bt + (size_t)b * p.bt_stride, p.P, p.pshift, p.Hk, h, p.num_pages, len, p.bt_stride};
+    const auto rm = [&] {
+        if constexpr (GROUP) return GroupMap{reinterpret_cast<const int2 *>(smem_raw), p.P, p.pshift, p.Hk, h, len};
+        else return RowMap{p.bt + (size_t)b * p.bt_stride, p.P, p.pshift, p.Hk, h, p.num_pages, len, p.bt_stride};
+    }();
     // Keys up to mask_from are visible to every row; later tiles need the mask.
     const int mask_from = p.causal ? start : len - 1;
 
@@ -367,8 +553,8 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
 #pragma unroll
     for (int rb = 0; rb < ROWB; rb++) {
         const int r = row0 + rb * 16 + r16, t = r / p.G, g = r - t * p.G;
-        const bool ok = r < p.M && t < nb;
-        qpos[rb] = p.causal && ok ? start + t : len - 1;
+        const bool ok = r < p.M && t < nb && (!GROUP || (tok0 + t >= q0 && tok0 + t < q1));
+        qpos[rb] = GROUP ? min(t, p.tg - 1) : (p.causal && ok ? start + t : len - 1);   // GROUP: the row's token
         const uint16_t *qr = p.q + ((size_t)(tok0 + t) * p.Hq + h * p.G + g) * D;
         if constexpr (!INT8) {
 #pragma unroll
@@ -383,8 +569,12 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     // bf16(q * smooth) (attention.jl:90-95), kept as float
-                    qf[i][2 * e] = bf2f(f2bf(__uint_as_float(raw[e] << 16) * p.smooth[d0 + 2 * e]));
-                    qf[i][2 * e + 1] = bf2f(f2bf(__uint_as_float(raw[e] & 0xffff0000u) * p.smooth[d0 + 2 * e + 1]));
+                    qf[i][2 * e] = __uint_as_float(raw[e] << 16) * p.smooth[d0 + 2 * e];
+                    qf[i][2 * e + 1] = __uint_as_float(raw[e] & 0xffff0000u) * p.smooth[d0 + 2 * e + 1];
+                    if constexpr (!SPARSE) {   // SPARSE: rounded once, to fp16's 11 bits
+                        qf[i][2 * e] = bf2f(f2bf(qf[i][2 * e]));
+                        qf[i][2 * e + 1] = bf2f(f2bf(qf[i][2 * e + 1]));
+                    }
                     amax = fmaxf(amax, fmaxf(fabsf(qf[i][2 * e]), fabsf(qf[i][2 * e + 1])));
                 }
             }
@@ -473,7 +663,20 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
         // it by more than RESCALE_LOG2 (then p <= 2^RESCALE_LOG2, safe in bf16 and fp32);
         // l and O always use the same reference, so the result is exact. INT8 moves m
         // with every larger max (p <= 1, so p times a value scale stays within fp16).
-        const bool need_mask = (j + NT) * 16 - 1 > mask_from;
+        int seen[ROWB], off = 0;   // GROUP: keys of the page that the row sees, the tile's first one
+        bool need_mask = (j + NT) * 16 - 1 > mask_from;
+        if constexpr (GROUP) {
+            static_assert(!GROUP || NT == 1);
+            const int u = j * 16 >> p.pshift;
+            off = j * 16 & (p.P - 1);
+            bool whole = true;
+#pragma unroll
+            for (int rb = 0; rb < ROWB; rb++) {
+                seen[rb] = lim[u * p.tg + qpos[rb]];
+                whole &= off + 16 <= seen[rb];
+            }
+            need_mask = !__all(whole);
+        }
         s16x4 pop[NT][ROWB];
         float x[ROWB][4 * NT], mt[ROWB];
         bool grow = false;
@@ -485,7 +688,9 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
                 float v = sc[e >> 2][rb][e & 3];
                 if (INT8) v = (v - qcorr[rb]) * skk[e >> 2][e & 3] * qsl[rb];
                 else v *= p.scale_log2;
-                if (need_mask) {
+                if constexpr (GROUP) {
+                    if (need_mask) v = off + kg * 4 + e < seen[rb] ? v : -INFINITY;
+                } else if (need_mask) {
                     const int kp = (j + (e >> 2)) * 16 + kg * 4 + (e & 3);
                     v = (kp <= qpos[rb] && kp < len) ? v : -INFINITY;
                 }
@@ -517,7 +722,8 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
                 for (int e = 0; e < 4; e++) {
                     pe[e] = fast_exp2(x[rb][4 * n + e] - m[rb]);
                     ps += pe[e];
-                    if (INT8) pe[e] *= svk[n][e];
+                    if (INT8 && GROUP && need_mask) pe[e] = x[rb][4 * n + e] == -INFINITY ? 0.0f : pe[e] * svk[n][e];
+                    else if (INT8) pe[e] *= svk[n][e];
                 }
                 l[rb] += ps;
                 if (INT8) {
@@ -608,6 +814,7 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
         }
     }
     __syncthreads();
+    bool fine = true;   // GROUP: no value that is not finite has come in
     for (int item = threadIdx.x; item < p.M * (D / 4); item += NW * 64) {
         const int r = item / (D / 4), d4 = (item % (D / 4)) * 4;
         const int rs = RS == 2 ? r / MP : 0, rr = r - rs * MP;   // row slice, row in slab
@@ -623,11 +830,16 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
             lsum += src[D + 1] * wgt;
             acc += *reinterpret_cast<const f32x4 *>(src + d4) * wgt;
         }
+        if constexpr (GROUP && !INT8) {
+            fine &= fabsf(lsum) < INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4; e++) fine &= fabsf(acc[e]) < INFINITY;
+        }
         if (nsp == 1) {
             // One split: this group saw every key; normalize and write the output rows.
             const int t = r / p.G, g = r - t * p.G;
-            if (t < nb) {
-                const float inv = 1.0f / lsum;
+            if (t < nb && (!GROUP || (tok0 + t >= q0 && tok0 + t < q1))) {
+                const float inv = GROUP && lsum == 0.0f ? 0.0f : 1.0f / lsum;
                 uint16_t *o16 = p.out + ((size_t)(tok0 + t) * p.Hq + h * p.G + g) * D + d4;
                 *reinterpret_cast<u32x2 *>(o16) = (u32x2){pack_bf16x2(acc[0] * inv, acc[1] * inv),
                                                           pack_bf16x2(acc[2] * inv, acc[3] * inv)};
@@ -641,6 +853,14 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
                 dst[D] = mx;
                 dst[D + 1] = lsum;
             }
+        }
+    }
+    if constexpr (GROUP && !INT8) {
+        // The slabs have overwritten the joined list: it is made again.
+        if (__syncthreads_or(!fine)) {
+            __shared__ int red[1 + NW];
+            group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem_raw), lim, red, tok0, h, q0, q1);
+            group_rows<D>(p, reinterpret_cast<const int2 *>(smem_raw), lim, tok0, h, q0, q1, j0, j1, nsp, unit, w, NW, lane);
         }
     }
 }

@@ -5,6 +5,11 @@
 // The kernels are the paged decode kernels with a table row, a length and a split count per
 // (token, KV head) pair in place of one per sequence (SPARSE in pa_decode.hpp and
 // pa_generic.hip): the keys of a pair are all visible to its rows, so only the last tile is masked.
+// Steps of several tokens a sequence (max_query_len > 1) take neighbouring tokens in groups: their tables
+// are joined into one list in LDS, and a page that several of them keep is read and multiplied once for
+// all their rows (GROUP in pa_decode.hpp). Token by token such a step is bound by the L2's rate (512
+// tokens of 2048 keys and 8 KV heads: 4.3 GB in 300 us).
+//
 // Pairs take consecutive work-groups with the KV heads innermost: with 8 KV heads (a multiple of
 // the 8 XCDs in general) all tokens of a KV head run on one XCD, and the pages that the tokens of
 // a step share are read through one L2.
@@ -15,7 +20,7 @@ using namespace ti_decode;
 
 namespace {
 
-// Merge a pair's split partials [pair][splits][G][D + 2]: one wave per query row. Loads of up to
+// Merge split partials [pair or group of pairs][splits][rows][D + 2]: one wave per query row. Loads of up to
 // SB splits are issued before any arithmetic. A pair without keys writes zeros.
 template <int D, typename T, int SB>
 __global__ void __launch_bounds__(256) sparse_combine_kernel(DecodeParams p, int rows) {
@@ -24,11 +29,13 @@ __global__ void __launch_bounds__(256) sparse_combine_kernel(DecodeParams p, int
     const int row = (int)(blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));   // token * Hq + head
     if (row >= rows) return;
     const int tok = row / p.Hq, hq = row - tok * p.Hq, h = hq / p.G, pair = tok * p.Hk + h;
+    const int group = tok / p.tg;   // p.tg tokens share a unit of partials, packed rows g + G t
     const int len = min(p.lengths[pair], p.bt_stride * p.P);
     const int q0 = p.qsl ? p.qsl[0] : 0, q1 = p.qsl ? p.qsl[p.B] : tok + 1;
     const int splits = p.min_tiles > 0 && len > 0 ? f32_active_splits((len + 15) >> 4, p.splits, p.min_tiles).active : p.splits;
-    const size_t stride = (size_t)p.G * (D + 2);
-    const float *base = p.part + (size_t)pair * p.splits * stride + (size_t)(hq - h * p.G) * (D + 2);
+    const size_t stride = (size_t)p.M * (D + 2);
+    const float *base = p.part + ((size_t)group * p.Hk + h) * p.splits * stride +
+                        (size_t)(hq - h * p.G + (tok - group * p.tg) * p.G) * (D + 2);
     float mx = NEG_BIG, lsum = 0.0f, acc[PER];
 #pragma unroll
     for (int k = 0; k < PER; k++) acc[k] = 0.0f;
@@ -95,16 +102,43 @@ void launch_sparse_d(const DecodeParams &p, bool int8, unsigned grid, hipStream_
     else pg16 ? launch_sparse_p<D, false, true>(p, grid, s) : launch_sparse_p<D, false, false>(p, grid, s);
 }
 
+template <int D, bool INT8>
+void launch_group_d(const DecodeParams &p, unsigned grid, hipStream_t s) {
+    const size_t lds = (size_t)p.tg * p.tg * p.bt_stride * sizeof(uint16_t);
+    if (p.M <= 16) decode_kernel<D, 1, INT8, true, 4, 1, false, true, true><<<grid, 256, lds, s>>>(p);
+    else decode_kernel<D, 2, INT8, true, 4, 1, false, true, true><<<grid, 256, lds, s>>>(p);
+}
+
 }  // namespace
 
-// Splits of a pair's keys: as the decode launch, while there are fewer than 256 work-groups, at
-// most 16 and at least four 16-key tiles of a full table each (one per wave).
-int ti_sparse_splits(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
-    const long long pairs = (long long)a->total_tokens * c->kv_heads;
-    const long long tiles = ((long long)a->table_width * c->page_size + 15) / 16;
-    int sp = 1;
-    while (sp < 16 && pairs * sp < 256 && tiles >= 8 * sp) sp <<= 1;
-    return sp;
+// Tokens worked on together, and splits of their keys.
+// Groups: bf16 steps of several tokens a sequence over pages of whole 16-key tiles, as many tokens as fill 16
+// rows, or 32 where there are then still two work-groups for every CU; their tables are joined from at most
+// GROUP_PAGES entries (512 for 32 rows, whose LDS two work-groups of a CU share).
+// Splits: as the decode launch, while there are fewer than 256 work-groups, at most 16 and at least four
+// 16-key tiles of a full table each (one per wave).
+ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
+    const int G = a->q_heads / c->kv_heads, P = c->page_size;
+    ti_sparse_plan pl{1, 1};
+    if (a->dtype == TI_BF16 && a->max_query_len > 1 && P >= 16 && P <= 32768 && (P & (P - 1)) == 0 && G <= 16) {
+        auto tokens = [&](int rows, int entries) {
+            return max(1, min(min(rows / G, a->max_query_len), entries / min(a->table_width, entries + 1)));
+        };
+        pl.tg = tokens(16, GROUP_PAGES);
+        const int wide = tokens(32, GROUP_PAGES / 2);
+        if (wide > pl.tg && (long long)a->total_tokens / wide * c->kv_heads >= 512) pl.tg = wide;
+    }
+    const long long pairs = (((long long)a->total_tokens + pl.tg - 1) / pl.tg) * c->kv_heads;
+    const long long tiles = ((long long)a->table_width * P + 15) / 16;
+    while (pl.splits < 16 && pairs * pl.splits < 256 && tiles >= 8 * pl.splits) pl.splits <<= 1;
+    return pl;
+}
+
+size_t ti_sparse_bytes(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
+    const ti_sparse_plan pl = ti_plan_sparse(a, c);
+    if (pl.splits == 1) return 0;
+    const size_t groups = ((size_t)a->total_tokens + pl.tg - 1) / pl.tg;
+    return groups * pl.tg * a->q_heads * pl.splits * (c->head_dim + 2) * sizeof(float);
 }
 
 int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, hipStream_t s) {
@@ -127,17 +161,24 @@ int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_ca
     p.pshift = (c->page_size & (c->page_size - 1)) == 0 ? __builtin_ctz(c->page_size) : -1;
     p.Hk = c->kv_heads;
     p.Hq = a->q_heads;
-    p.G = p.M = a->q_heads / c->kv_heads;
+    const ti_sparse_plan pl = ti_plan_sparse(a, c);
+    p.G = a->q_heads / c->kv_heads;
+    p.tg = pl.tg;
+    p.M = pl.tg * p.G;
+    p.total = a->total_tokens;
     p.nmax = 1;
-    p.splits = ti_sparse_splits(a, c);
+    p.splits = pl.splits;
     p.scale_log2 = a->scale * LOG2E;
-    const unsigned grid = (unsigned)((long long)a->total_tokens * c->kv_heads * p.splits);
+    const unsigned grid = (unsigned)(((long long)a->total_tokens + pl.tg - 1) / pl.tg * c->kv_heads * p.splits);
     if (a->dtype == TI_F32) {
         p.min_tiles = ti_launch_sparse_f32(a, c, p.splits, s);
         if (p.min_tiles < 0) return TI_ERR_LAUNCH;
     } else {
         const bool int8 = c->kind == TI_KV_INT8;
-        if (c->head_dim == 128) launch_sparse_d<128>(p, int8, grid, s);
+        if (pl.tg > 1) {
+            if (c->head_dim == 128) int8 ? launch_group_d<128, true>(p, grid, s) : launch_group_d<128, false>(p, grid, s);
+            else int8 ? launch_group_d<64, true>(p, grid, s) : launch_group_d<64, false>(p, grid, s);
+        } else if (c->head_dim == 128) launch_sparse_d<128>(p, int8, grid, s);
         else launch_sparse_d<64>(p, int8, grid, s);
     }
     if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
