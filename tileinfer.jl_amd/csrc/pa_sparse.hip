@@ -113,24 +113,29 @@ void launch_group_d(const DecodeParams &p, unsigned grid, hipStream_t s) {
 
 // Tokens worked on together, and splits of their keys.
 // Groups: bf16 steps of several tokens a sequence over pages of whole 16-key tiles, as many tokens as fill 16
-// rows, or 32 where there are then still two work-groups for every CU; their tables are joined from at most
-// GROUP_PAGES entries (512 for 32 rows, whose LDS two work-groups of a CU share).
-// Splits: as the decode launch, while there are fewer than 256 work-groups, at most 16 and at least four
-// 16-key tiles of a full table each (one per wave).
+// query rows. 32 rows read a page for twice the tokens at half the work-groups, and pay once 16 would give
+// 256 work-groups (8 steps of 16 tokens, 4096 keys each: 65.7 -> 50.3 us; 512 tokens 126 -> 74; below it
+// one step of 16 18.5 against 19.0-21.4), INT8 caches 512 (8 x 16 39.6 us against 46.6; 512 tokens 126 ->
+// 101). Their tables are joined from at most GROUP_PAGES entries, 512 for 32 rows, whose LDS two work-groups
+// of a CU share.
+// Splits: while there are fewer work-groups than CUs (twice as many for joined INT8 tables: 8 x 16 46.7 ->
+// 39.6 us, one step of 8 18.5 -> 16.9), at most 16 and at least four 16-key tiles of a full table each (one
+// per wave).
 ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
     const int G = a->q_heads / c->kv_heads, P = c->page_size;
+    const bool int8 = c->kind == TI_KV_INT8;
     ti_sparse_plan pl{1, 1};
+    auto pairs = [&](int tg) { return ((long long)a->total_tokens + tg - 1) / tg * c->kv_heads; };
     if (a->dtype == TI_BF16 && a->max_query_len > 1 && P >= 16 && P <= 32768 && (P & (P - 1)) == 0 && G <= 16) {
         auto tokens = [&](int rows, int entries) {
             return max(1, min(min(rows / G, a->max_query_len), entries / min(a->table_width, entries + 1)));
         };
         pl.tg = tokens(16, GROUP_PAGES);
         const int wide = tokens(32, GROUP_PAGES / 2);
-        if (wide > pl.tg && (long long)a->total_tokens / wide * c->kv_heads >= 512) pl.tg = wide;
+        if (wide > pl.tg && pairs(pl.tg) >= (int8 ? 512 : 256)) pl.tg = wide;
     }
-    const long long pairs = (((long long)a->total_tokens + pl.tg - 1) / pl.tg) * c->kv_heads;
-    const long long tiles = ((long long)a->table_width * P + 15) / 16;
-    while (pl.splits < 16 && pairs * pl.splits < 256 && tiles >= 8 * pl.splits) pl.splits <<= 1;
+    const long long tiles = ((long long)a->table_width * P + 15) / 16, target = int8 && pl.tg > 1 ? 512 : 256;
+    while (pl.splits < 16 && pairs(pl.tg) * pl.splits < target && tiles >= 8 * pl.splits) pl.splits <<= 1;
     return pl;
 }
 

@@ -144,18 +144,31 @@ __global__ void __launch_bounds__(256) sum_kernel(VerifyParams p) {
     }
 }
 
-// Sum of the 256 threads' values before this one's, and of all.
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double x) {
+    union {
+        double d;
+        int i[2];
+    } v{x}, u;
+    u.i[0] = __builtin_amdgcn_update_dpp(0, v.i[0], CTRL, ROWS, 0xf, false);   // lanes without a source add 0
+    u.i[1] = __builtin_amdgcn_update_dpp(0, v.i[1], CTRL, ROWS, 0xf, false);
+    return x + u.d;
+}
+// Sum of the lanes up to this one: within rows of 16 by shifts, then each row's total into those behind it.
+__device__ __forceinline__ double wave_upto(double x) {
+    x = dpp_add<0x111, 0xf>(x);   // row_shr 1
+    x = dpp_add<0x112, 0xf>(x);   // row_shr 2
+    x = dpp_add<0x114, 0xf>(x);   // row_shr 4
+    x = dpp_add<0x118, 0xf>(x);   // row_shr 8
+    x = dpp_add<0x142, 0xa>(x);   // row_bcast 15 into rows 1 and 3
+    return dpp_add<0x143, 0xc>(x);   // row_bcast 31 into rows 2 and 3
+}
+
+// Sum of the 256 threads' values before this one's, and of all. part: 4 doubles of LDS of this call's own.
 __device__ __forceinline__ double block_before(double own, double *part, int lane, int wv, double *all) {
-    double incl = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double v = __shfl_up(incl, o);
-        if (lane >= o) incl += v;
-    }
-    __syncthreads();   // earlier reads of part are done
-    if (lane == 63) part[wv] = incl;
+    const double upto = wave_upto(own);
+    if (lane == 63) part[wv] = upto;
     __syncthreads();
-    double before = incl - own, total = 0.0;
+    double before = upto - own, total = 0.0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if (i < wv) before += part[i];
@@ -165,52 +178,70 @@ __device__ __forceinline__ double block_before(double own, double *part, int lan
     return before;
 }
 
+// The value (>= 0) of the first thread of the work-group that `has` one, or of the last; -1 where none has.
+// cells: 4 words of LDS of this call's own. (An LDS atomic per lane is worked off lane by lane: 3 us each.)
+template <bool LAST> __device__ __forceinline__ int end_of(bool has, int v, int *cells, int lane, int wv) {
+    const unsigned long long m = __ballot(has);
+    const int mine = m ? __builtin_amdgcn_readlane(v, LAST ? 63 - __builtin_clzll(m) : __builtin_ctzll(m)) : -1;
+    if (lane == 0) cells[wv] = mine;
+    __syncthreads();
+    int end = -1;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int c = cells[LAST ? i : 3 - i];
+        if (c >= 0) end = c;
+    }
+    return end;
+}
+
+// The drawn token of a sequence, one work-group: bound by its chain of dependent loads (the sums and the
+// accepted count, one piece of the rows) and the scans between them, so what does not depend on them is
+// loaded in front, and a thread's first piece stays in registers.
 template <typename T>
 __global__ void __launch_bounds__(256) draw_kernel(VerifyParams p) {
-    __shared__ double part[4], before_s;
-    __shared__ int first_piece, last_piece, first, last;
+    __shared__ double part[3][4], before_s;
+    __shared__ int cells[4][4];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, b = blockIdx.x;
-    if (tid == 0) first_piece = first = 0x7fffffff, last_piece = last = -1;
-    const double u = (double)p.uniforms[(size_t)b * (p.N + 1) + p.N];
-    const int a = p.accepted[b];
-    const int n = p.counts ? min(max(p.counts[b], 0), p.N) : p.N;
     const double2 *sums = reinterpret_cast<const double2 *>(p.sums) + (size_t)b * p.pieces;
     // thread t holds pieces [t each, (t + 1) each)
     const int each = (p.pieces + 255) / 256, k0 = min(tid * each, p.pieces), k1 = min(k0 + each, p.pieces);
-    double own = 0.0, total, before;
-    for (int k = k0; k < k1; k++) own += sums[k].x;
-    before = block_before(own, part, lane, wv, &total);
+    const double2 s0 = k0 < k1 ? sums[k0] : make_double2(0.0, 0.0);
+    const int x0 = tid < p.N ? p.drafted[(size_t)b * p.N + tid] : -1;
+    const double u = (double)p.uniforms[(size_t)b * (p.N + 1) + p.N];
+    const int a = p.accepted[b];
+    const int n = p.counts ? min(max(p.counts[b], 0), p.N) : p.N;
+    const Rows<T> r(p, b, a, n);
+    double own = s0.x, total, before;
+    for (int k = k0 + 1; k < k1; k++) own += sums[k].x;
+    before = block_before(own, part[0], lane, wv, &total);
     const bool plain = !(total > 0.0);   // no weight left: the target's own row
     if (plain) {
-        own = 0.0;
-        for (int k = k0; k < k1; k++) own += sums[k].y;
-        before = block_before(own, part, lane, wv, &total);
+        own = s0.y;
+        for (int k = k0 + 1; k < k1; k++) own += sums[k].y;
+        before = block_before(own, part[1], lane, wv, &total);
     }
     const double goal = u * total;
     // the first piece whose running sum passes the goal, or the last with weight where none does
-    int mine = 0x7fffffff, top = -1;
+    int mine = -1, top = -1;
     double run = before, mine_before = 0.0, top_before = 0.0;
     for (int k = k0; k < k1; k++) {
-        const double s = plain ? sums[k].y : sums[k].x;
+        const double2 sk = k == k0 ? s0 : sums[k];
+        const double s = plain ? sk.y : sk.x;
         if (s > 0.0) {
             top = k;
             top_before = run;
-            if (run + s > goal && mine == 0x7fffffff) {
+            if (run + s > goal && mine < 0) {
                 mine = k;
                 mine_before = run;
             }
         }
         run += s;
     }
-    if (mine != 0x7fffffff) atomicMin(&first_piece, mine);
-    if (top >= 0) atomicMax(&last_piece, top);
-    __syncthreads();
-    const int piece = first_piece != 0x7fffffff ? first_piece : last_piece;
-    int token = -1;
+    int piece = end_of<false>(mine >= 0, mine, cells[0], lane, wv), token = -1;
+    const bool passed = piece >= 0;
+    if (!passed) piece = end_of<true>(top >= 0, top, cells[1], lane, wv);
     if (piece >= 0) {
-        if (mine == piece) before_s = mine_before;
-        else if (top == piece && first_piece == 0x7fffffff) before_s = top_before;
-        const Rows<T> r(p, b, a, n);
+        if (passed ? mine == piece : top == piece) before_s = passed ? mine_before : top_before;
         const int v0 = piece * PIECE + 4 * tid;
         float pv[4], qv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         load4(r.p, v0, p.V, pv);
@@ -221,23 +252,22 @@ __global__ void __launch_bounds__(256) draw_kernel(VerifyParams p) {
             w[i] = !plain && v0 + i == r.gone ? 0.0 : positive((double)pv[i] - (double)qv[i]);
             sum += w[i];
         }
-        double c = block_before(sum, part, lane, wv, &all) + before_s;
-        int hit = 0x7fffffff, held = -1;
+        double c = block_before(sum, part[2], lane, wv, &all) + before_s;
+        int hit = -1, held = -1;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             c += w[i];
             if (w[i] > 0.0) {
                 held = v0 + i;
-                if (c > goal && hit == 0x7fffffff) hit = v0 + i;
+                if (c > goal && hit < 0) hit = v0 + i;
             }
         }
-        if (hit != 0x7fffffff) atomicMin(&first, hit);
-        if (held >= 0) atomicMax(&last, held);
-        __syncthreads();
-        token = first != 0x7fffffff ? first : last;
+        // the first entry that passes the goal; the last with weight where rounding leaves none
+        token = end_of<false>(hit >= 0, hit, cells[2], lane, wv);
+        if (token < 0) token = end_of<true>(held >= 0, held, cells[3], lane, wv);
     }
     for (int i = tid; i <= p.N; i += 256)
-        p.tokens[(size_t)b * (p.N + 1) + i] = i < a ? p.drafted[(size_t)b * p.N + i] : (i == a ? token : -1);
+        p.tokens[(size_t)b * (p.N + 1) + i] = i < a ? (i == tid ? x0 : p.drafted[(size_t)b * p.N + i]) : (i == a ? token : -1);
 }
 
 }  // namespace
