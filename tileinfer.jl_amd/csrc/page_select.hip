@@ -245,8 +245,12 @@ template <int W> struct Join {
     }
 };
 
-// The search over keys in groups of four per lane, group(n) the n-th of this wave's `groups`.
-template <typename Group, typename J> __device__ __forceinline__ Limit bisect(int need, int groups, Group group, J join) {
+// The search over keys in groups of four per lane, group(n) the n-th of this wave's `groups`; `all` keys are up
+// for choice. A step takes 0.2 us for 512 keys and 0.4 for 2048, and 11 are usual (counting lane
+// masks, or several middles at a time in 16 waves, was no faster). Where few keys are left between the
+// ends, these close in on them: equal keys end the search then and not after all 24 halvings of their digits.
+template <typename Group, typename J>
+__device__ __forceinline__ Limit bisect(int need, int all, int groups, Group group, J join) {
     uint32_t top = 0, low = 0xffffffffu;
 #pragma unroll
     for (int n = 0; n < groups; n++) {
@@ -259,20 +263,38 @@ template <typename Group, typename J> __device__ __forceinline__ Limit bisect(in
     }
     top = join.most(wave_umax(top));
     low = ~join.most(wave_umax(~low)) + 1;
-    int above = 0;   // keys > top: fewer than need; keys >= low: at least need
+    int from = all, above = 0;   // keys >= low: at least need; keys > top: fewer
+    bool closed = false;
     while (low < top) {
+        if (!closed && from - above <= 4) {
+            closed = true;
+            uint32_t most = 0, least = 0xffffffffu;
+#pragma unroll
+            for (int n = 0; n < groups; n++) {
+                const u32x4 k = group(n);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    most = max(most, k[e] <= top ? k[e] : 0u);
+                    least = min(least, k[e] >= low ? k[e] : 0xffffffffu);
+                }
+            }
+            top = join.most(wave_umax(most));
+            low = ~join.most(wave_umax(~least));
+            continue;
+        }
         const uint32_t d = top - low, mid = low + d / 2 + (d & 1);
-        int c = 0;
+        int count = 0;
 #pragma unroll
         for (int n = 0; n < groups; n++) {
             const u32x4 k = group(n);
 #pragma unroll
-            for (int e = 0; e < 4; e++) c += __popcll(__ballot(k[e] >= mid));
+            for (int e = 0; e < 4; e++) count += k[e] >= mid;
         }
-        c = join.sum(c);
+        const int c = join.sum(wave_total(count));
         if (c == need) return {mid - 1, 0};
         if (c > need) {
             low = mid;
+            from = c;
         } else {
             top = mid - 1;
             above = c;
@@ -282,19 +304,19 @@ template <typename Group, typename J> __device__ __forceinline__ Limit bisect(in
 }
 // Up to NG groups a wave in registers: the search is all arithmetic.
 template <int NG, int W, typename J>
-__device__ __forceinline__ Limit bisect_held(int need, const uint32_t *keys, int span, int lane, int w, J join) {
+__device__ __forceinline__ Limit bisect_held(int need, int all, const uint32_t *keys, int span, int lane, int w, J join) {
     u32x4 k[NG];
 #pragma unroll
     for (int n = 0; n < NG; n++) {
         const int i = (n * W + w) * ROUND;
         k[n] = i < span ? *reinterpret_cast<const u32x4 *>(keys + i + 4 * lane) : (u32x4){0u, 0u, 0u, 0u};
     }
-    return bisect(need, NG, [&](int n) { return k[n]; }, join);
+    return bisect(need, all, NG, [&](int n) { return k[n]; }, join);
 }
 
 // By W waves (all of the work-group where W > 1), over `span` keys (a multiple of ROUND); those that are
-// not up for choice become 0. One wave takes up to ONE keys, all in registers (512 keys 1.6 us, 2048 2.0;
-// 8192 through LDS took 45), more waves 512 each before they read them from LDS at every step.
+// not up for choice become 0. One wave takes up to ONE keys, all in registers (8192 through LDS
+// took 45 us), more waves 512 each before they read them from LDS at every step.
 template <int W>
 __device__ __forceinline__ Limit find_limit(const Seen &s, uint32_t *keys, int span, int lane, int w, int *red) {
     for (int i = w * 64 + lane; i < s.c0; i += W * 64) keys[i] = 0;
@@ -303,13 +325,13 @@ __device__ __forceinline__ Limit find_limit(const Seen &s, uint32_t *keys, int s
     if (s.need >= s.c1 - s.c0) return {0, 0};   // every candidate
     if (s.need <= 0) return {0xffffffffu, 0};     // none
     const Join<W> join{red, lane, w, 0};
-    if (span <= 2 * W * ROUND) return bisect_held<2, W>(s.need, keys, span, lane, w, join);
+    if (span <= 2 * W * ROUND) return bisect_held<2, W>(s.need, s.c1 - s.c0, keys, span, lane, w, join);
     if constexpr (W == 1) {
-        if (span <= 5 * ROUND) return bisect_held<5, W>(s.need, keys, span, lane, w, join);
-        return bisect_held<8, W>(s.need, keys, span, lane, w, join);
+        if (span <= 5 * ROUND) return bisect_held<5, W>(s.need, s.c1 - s.c0, keys, span, lane, w, join);
+        return bisect_held<8, W>(s.need, s.c1 - s.c0, keys, span, lane, w, join);
     }
     const int all = span / ROUND, mine = (all - w + W - 1) / W;
-    return bisect(s.need, mine, [&](int n) { return *reinterpret_cast<const u32x4 *>(keys + (n * W + w) * ROUND + 4 * lane); }, join);
+    return bisect(s.need, s.c1 - s.c0, mine, [&](int n) { return *reinterpret_cast<const u32x4 *>(keys + (n * W + w) * ROUND + 4 * lane); }, join);
 }
 
 // Writes one token's kept pages in order, zeros behind them, and its number of keys; NW waves share the
