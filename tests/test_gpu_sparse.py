@@ -426,7 +426,7 @@ def shared(c, rows, width, seed, common=0.8):
     return t.cuda().contiguous(), n.to(torch.int32).cuda().contiguous()
 
 
-@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("kv", ["bf16", "int8", "fp32"])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("G,P", [(4, 16), (4, 64), (1, 16), (2, 32), (3, 16), (7, 64), (8, 16), (12, 16), (16, 32)])
 @pytest.mark.parametrize("rows", [2, 16, 33])
@@ -440,7 +440,7 @@ def test_attend_steps_that_share_pages(gpu, kv, D, G, P, rows):
     check_attend(c, q, tables, lengths, n=rows)
 
 
-@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("kv", ["bf16", "int8", "fp32"])
 @pytest.mark.parametrize("width", [1, 5, 70, 200, 600, 1100])
 def test_attend_steps_of_any_width(gpu, kv, width):
     """As many tokens as their tables leave room for: 32 rows, 16, fewer tokens than fill them, one."""
@@ -454,13 +454,13 @@ def test_attend_steps_of_any_width(gpu, kv, width):
 
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("where", ["k", "v"])
-@pytest.mark.parametrize("rows,heads", [(6, 2), (300, 8)])
-def test_attend_values_that_are_not_finite_stay_with_their_tokens(gpu, value, where, rows, heads):
+@pytest.mark.parametrize("rows,heads,kv", [(6, 2, "bf16"), (300, 8, "bf16"), (6, 2, "fp32"), (300, 8, "fp32")])
+def test_attend_values_that_are_not_finite_stay_with_their_tokens(gpu, value, where, rows, heads, kv):
     """A key or value that is not finite in a page that some tokens of a step keep, or behind the last key
     of others: tokens that do not see it are as without it, those that do are as their own attention."""
-    c = Cache("bf16", 128, heads, 16, [60 * 16], seed=31)
+    c = Cache(kv, 128, heads, 16, [60 * 16], seed=31)
     torch.manual_seed(31)
-    q = torch.randn((rows, heads * 4, 128), device="cuda", dtype=torch.bfloat16)
+    q = torch.randn((rows, heads * 4, 128), device="cuda", dtype=T[kv])
     tables, lengths = shared(c, rows, 9, seed=31)
     lengths[:] = 8 * 16 + 9
     bad = tables[1, 0, 2].item()
@@ -477,8 +477,8 @@ def test_attend_values_that_are_not_finite_stay_with_their_tokens(gpu, value, wh
     assert touched.any() and not touched.all()
     clean = pool.clone()
     clean[bad - 1, :, 5, 17], clean[last - 1, :, 9, 3] = 0, 0
-    k, v = (clean, c.v) if where == "k" else (c.k, clean)
-    want = ti.sparse_attention(BE, q, k, v, tables, lengths, 0.09, None, rows)
+    k, clean_v = (clean, c.v) if where == "k" else (c.k, clean)
+    want = ti.sparse_attention(BE, q, k, clean_v, tables, lengths, 0.09, None, rows)
     # rows of the wave-by-row path round otherwise: each is within 2^-7 of the exact weights and output
     assert torch.isfinite(got[~touched]).all()
     tol = 4 * 2.0 ** -8 * c.v[torch.isfinite(c.v)].float().abs().max()

@@ -186,7 +186,8 @@ struct ti_sparse_plan {
 ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c);
 size_t ti_sparse_bytes(const ti_sparse_attention_args *a, const ti_kv_cache *c);
 int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, hipStream_t s);
-int ti_launch_sparse_f32(const ti_sparse_attention_args *a, const ti_kv_cache *c, int splits, hipStream_t s);
+bool ti_sparse_f32_mfma(const ti_sparse_attention_args *a, const ti_kv_cache *c);
+int ti_launch_sparse_f32(const ti_sparse_attention_args *a, const ti_kv_cache *c, const ti_sparse_plan &pl, hipStream_t s);
 // Page bounds and the selection by them (page_bounds.hip).
 int ti_launch_key_bounds(int dtype, const ti_kv_cache *c, const ti_key_bounds *kb, const int32_t *bt, int bt_stride,
                          const int32_t *positions, const int32_t *qsl, int num_seqs, int nmax, int total, hipStream_t s);

@@ -11,9 +11,12 @@
 // combine kernel merges the splits.
 // Semantics as attention(::RefBackend) (src/ops/reference.jl:95-121): key i visible to
 // query t iff i <= start + t (causal) or i < start + n (not causal).
-#include "common.hpp"
+#include <stddef.h>
+
+#include "pa_group.hpp"
 
 using namespace ti;
+using namespace ti_group;
 
 namespace {
 
@@ -171,6 +174,7 @@ struct F32Params {
     int xcd;         // 1-D grid, work-groups of one (sequence, KV head) on one XCD (pairs % 8 == 0)
     float scale_log2;
     const int32_t *lengths;   // SPARSE: keys of each (token, KV head)
+    int tg, total;            // GROUP: tokens of a group, tokens of the call
 };
 
 // Each split takes at least this many 16-key tiles (one per wave), so short contexts run on
@@ -178,11 +182,16 @@ struct F32Params {
 constexpr int F32_MIN_TILES = 4;
 
 // QT: more than one q-tile per (sequence, KV head). SPARSE (one q-tile): (token, KV head) pairs with a
-// table row and a length each (pa_sparse.hip), 1-D grid of the pairs' splits.
-template <int D, bool QT, bool SPARSE = false>
+// table row and a length each (pa_sparse.hip), 1-D grid of the pairs' splits. GROUP (SPARSE): p.tg
+// neighbouring tokens' pairs at a time over the joined list of their pages (pa_group.hpp), packed rows g + G t.
+template <int D, bool QT, bool SPARSE = false, bool GROUP = false>
 __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     constexpr int NJ = D / 16, NDB = D / 16, NW = 4, MROW = D + 4;
-    __shared__ __attribute__((aligned(16))) float slab[NW * 16 * MROW];
+    // GROUP: the joined list, in the merge's LDS; the tokens' keys of each page in dynamic LDS
+    constexpr int SLAB = NW * 16 * MROW * 4, LDS = GROUP && SLAB < (int)sizeof(GroupLds) ? (int)sizeof(GroupLds) : SLAB;
+    __shared__ __attribute__((aligned(16))) char smem[LDS];
+    float *slab = reinterpret_cast<float *>(smem);
+    extern __shared__ __attribute__((aligned(16))) uint16_t lim[];
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, kg = lane >> 4;
@@ -218,10 +227,10 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     int tok0, nb, start;
     const int t_first = QT ? 16 * qt / p.G : 0;
     if constexpr (SPARSE) {
-        tok0 = b / p.Hk;
-        nb = 1;
-        if (p.qsl && (tok0 < p.qsl[0] || tok0 >= p.qsl[p.B])) return;   // a row of no sequence
-        start = min(p.lengths[b], p.bt_stride * p.P) - 1;
+        nb = GROUP ? p.tg : 1;
+        tok0 = b / p.Hk * nb;
+        if (p.qsl && (tok0 + nb <= p.qsl[0] || tok0 >= p.qsl[p.B])) return;   // rows of no sequence
+        start = GROUP ? 0 : min(p.lengths[b], p.bt_stride * p.P) - 1;
         if (start < 0) {   // no keys: zeros (the combine's, where the keys are split)
             if (p.splits == 1)
                 for (int i = threadIdx.x; i < p.G * D / 4; i += 256)
@@ -234,21 +243,28 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         if (t_first >= nb) return;   // the q-tile holds no token of this sequence
         start = max(p.positions[tok0], 0);   // a negative position reads as 0
     }
-    const int len = start + nb;
-    // splits cut the sequence's 16-key tiles (the combine derives the same count); this
-    // q-tile's keys end after its last token's position
-    const ActiveSplits as = f32_active_splits((len + 15) >> 4, p.splits, F32_MIN_TILES);
+    int len = start + nb;
+    const int q0 = GROUP && p.qsl ? max(p.qsl[0], 0) : 0, q1 = GROUP ? (p.qsl ? min(p.qsl[p.B], p.total) : p.total) : 0;
+    if constexpr (GROUP) {
+        __shared__ int red[1 + NW];
+        len = group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem), lim, red, tok0, h, q0, q1) * p.P;
+    }
+    // splits cut the sequence's 16-key tiles (the combine derives the same count; GROUP: every split writes a
+    // partial); this q-tile's keys end after its last token's position
+    ActiveSplits as = f32_active_splits((len + 15) >> 4, p.splits, F32_MIN_TILES);
+    if constexpr (GROUP) as = ActiveSplits{((len >> 4) + p.splits - 1) / p.splits, p.splits};
     if (s >= as.active) return;   // no keys for this split
     const int t_last = QT ? min((16 * qt + 15) / p.G, nb - 1) : nb - 1;
     const int kend = p.causal ? start + t_last + 1 : len;
+    const GroupMap gm{reinterpret_cast<const int2 *>(smem), p.P, p.pshift, p.Hk, h, len};
     const int j0 = s * as.per, j1 = min(j0 + as.per, (kend + 15) >> 4);   // may be empty: (m, l) = (NEG_BIG, 0)
     const int r = 16 * qt + r16, t = r / p.G, g = r - t * p.G;
-    const bool ok = r < p.M && t < nb;
+    const bool ok = r < p.M && t < nb && (!GROUP || (tok0 + t >= q0 && tok0 + t < q1));
     const int qpos = p.causal && ok ? start + t : len - 1;
     const int mask_from = p.causal ? start + t_first : len - 1;   // keys up to here are visible to every row
     f32x4 qv[NJ];
     {
-        const float *qr = p.q + ((size_t)(tok0 + (ok ? t : 0)) * p.Hq + h * p.G + g) * D + 4 * kg;
+        const float *qr = p.q + ((size_t)(ok ? tok0 + t : tok0) * p.Hq + h * p.G + g) * D + 4 * kg;
 #pragma unroll
         for (int j = 0; j < NJ; j++)
             qv[j] = ok ? *reinterpret_cast<const f32x4 *>(qr + 16 * j) : (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -263,9 +279,17 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         float v[4][NDB];
     };
     auto load = [&](int j, Tile &tl) {
-        const int pos0 = j * 16, last = len - 1 - pos0;   // keys past len read the last key's row
-        const int pg = page_of_s(bt, pos0 >> p.pshift, p.bt_stride, p.num_pages);
-        const long long rbase = ((long long)pg * p.Hk + h) * p.P + (pos0 & (p.P - 1));
+        const int pos0 = j * 16;
+        int last;   // keys past it read its row
+        long long rbase;
+        if constexpr (GROUP) {
+            last = gm.last(pos0);
+            rbase = gm.row_s(pos0);
+        } else {
+            last = len - 1 - pos0;
+            const int pg = page_of_s(bt, pos0 >> p.pshift, p.bt_stride, p.num_pages);
+            rbase = ((long long)pg * p.Hk + h) * p.P + (pos0 & (p.P - 1));
+        }
         const float *krow = p.kp + (rbase + min(r16, last)) * D + 4 * kg;
 #pragma unroll
         for (int jj = 0; jj < NJ; jj++) tl.k[jj] = *reinterpret_cast<const f32x4 *>(krow + 16 * jj);
@@ -284,11 +308,17 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
 #pragma unroll
             for (int c = 0; c < 4; c++) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(tl.k[jj][c], qv[jj][c], sc, 0, 0, 0);
         const bool need_mask = pos0 + 15 > mask_from;
+        int seen = 0, off = 0;   // GROUP: keys of the page that the row sees, the tile's first one
+        if constexpr (GROUP) {
+            seen = lim[(pos0 >> p.pshift) * p.tg + min(t, p.tg - 1)];
+            off = pos0 & (p.P - 1);
+        }
         float x[4], mt = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const int kpos = pos0 + 4 * kg + e;
-            x[e] = need_mask && kpos > qpos ? -INFINITY : sc[e];
+            if constexpr (GROUP) x[e] = off + 4 * kg + e < seen ? sc[e] : -INFINITY;
+            else x[e] = need_mask && kpos > qpos ? -INFINITY : sc[e];
             mt = fmaxf(mt, x[e]);
         }
         mt *= p.scale_log2;
@@ -313,7 +343,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
 #pragma unroll
             for (int db = 0; db < NDB; db++) o[db] = __builtin_amdgcn_mfma_f32_16x16x4f32(tl.v[e][db], pe[e], o[db], 0, 0, 0);
     };
-    if constexpr (QT) {
+    if constexpr (QT || GROUP) {
         // multi-token q-tiles walk many tiles per wave: the next tile's loads are issued
         // before this one's arithmetic (two register sets; past the last tile the prefetch
         // re-reads it, unused)
@@ -342,6 +372,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     // merge the four waves' states (same rows, disjoint keys) through LDS
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+    if constexpr (GROUP) __syncthreads();   // the joined list is read
     {
         float *my = slab + ((size_t)w * 16 + r16) * MROW;
 #pragma unroll
@@ -354,6 +385,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     __syncthreads();
     const size_t unit = SPARSE ? (size_t)blockIdx.x : ((size_t)b * p.Hk + h) * p.splits + s;
     const int mrows = QT ? 16 : p.M;   // one q-tile: the M <= 16 rows
+    bool fine = true;   // GROUP: no value that is not finite has come in
     for (int it = threadIdx.x; it < mrows * (D / 4); it += NW * 64) {
         const int rr = it / (D / 4), d4 = (it % (D / 4)) * 4, r = 16 * qt + rr;
         if (r >= p.M) continue;
@@ -370,9 +402,14 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
             acc += *reinterpret_cast<const f32x4 *>(src + d4) * wgt;
         }
         const int tr = r / p.G, gr = r - tr * p.G;
-        if (tr >= nb) continue;
+        if (tr >= nb || (GROUP && (tok0 + tr < q0 || tok0 + tr >= q1))) continue;
+        if constexpr (GROUP) {
+            fine &= fabsf(lsum) < INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4; e++) fine &= fabsf(acc[e]) < INFINITY;
+        }
         if (as.active == 1) {
-            const float inv = 1.0f / lsum;
+            const float inv = GROUP && lsum == 0.0f ? 0.0f : 1.0f / lsum;
             *reinterpret_cast<f32x4 *>(p.out + ((size_t)(tok0 + tr) * p.Hq + h * p.G + gr) * D + d4) = acc * inv;
         } else {
             float *dst = p.part + (unit * (size_t)p.M + r) * (D + 2);
@@ -382,6 +419,14 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
                 dst[D] = mx;
                 dst[D + 1] = lsum;
             }
+        }
+    }
+    if constexpr (GROUP) {
+        // as the bf16 kernel: the slabs have overwritten the joined list, which is made again
+        if (__syncthreads_or(!fine)) {
+            __shared__ int red[1 + NW];
+            group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem), lim, red, tok0, h, q0, q1);
+            group_rows<D>(p, reinterpret_cast<const int2 *>(smem), lim, tok0, h, q0, q1, j0, j1, p.splits, unit, w, NW, lane);
         }
     }
 }
@@ -514,9 +559,12 @@ int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStrea
 // fp32 attention over chosen pages (pa_sparse.hip): the matrix-core kernel where its shape limits
 // allow and one 16-row tile holds a KV head's query heads, else the VALU kernel. Returns the least
 // 16-key tiles of a split (0: every split writes a partial), or -1 if the launch failed.
-int ti_launch_sparse_f32(const ti_sparse_attention_args *a, const ti_kv_cache *c, int splits, hipStream_t s) {
-    const int G = a->q_heads / c->kv_heads;
-    if (c->kind == TI_KV_DENSE && G <= 16 && c->page_size >= 16 && (c->page_size & (c->page_size - 1)) == 0) {
+bool ti_sparse_f32_mfma(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
+    return c->kind == TI_KV_DENSE && a->q_heads / c->kv_heads <= 16 && c->page_size >= 16 && (c->page_size & (c->page_size - 1)) == 0;
+}
+int ti_launch_sparse_f32(const ti_sparse_attention_args *a, const ti_kv_cache *c, const ti_sparse_plan &pl, hipStream_t s) {
+    const int G = a->q_heads / c->kv_heads, splits = pl.splits;
+    if (ti_sparse_f32_mfma(a, c)) {
         F32Params f{};
         f.q = (const float *)a->q;
         f.out = (float *)a->out;
@@ -533,12 +581,21 @@ int ti_launch_sparse_f32(const ti_sparse_attention_args *a, const ti_kv_cache *c
         f.pshift = __builtin_ctz(c->page_size);
         f.Hk = c->kv_heads;
         f.Hq = a->q_heads;
-        f.G = f.M = G;
+        f.G = G;
+        f.tg = pl.tg;
+        f.M = pl.tg * G;
+        f.total = a->total_tokens;
         f.nmax = 1;
         f.qtiles = 1;
         f.splits = splits;
         f.scale_log2 = a->scale * LOG2E;
-        const unsigned grid = (unsigned)((long long)a->total_tokens * c->kv_heads * splits);
+        const unsigned grid = (unsigned)(((long long)a->total_tokens + pl.tg - 1) / pl.tg * c->kv_heads * splits);
+        if (pl.tg > 1) {
+            const size_t lds = (size_t)pl.tg * pl.tg * a->table_width * sizeof(uint16_t);
+            if (c->head_dim == 128) attn_f32_kernel<128, false, true, true><<<grid, 256, lds, s>>>(f);
+            else attn_f32_kernel<64, false, true, true><<<grid, 256, lds, s>>>(f);
+            return hipGetLastError() == hipSuccess ? 0 : -1;
+        }
         if (c->head_dim == 128) attn_f32_kernel<128, false, true><<<grid, 256, 0, s>>>(f);
         else attn_f32_kernel<64, false, true><<<grid, 256, 0, s>>>(f);
         return hipGetLastError() == hipSuccess ? F32_MIN_TILES : -1;

@@ -126,16 +126,17 @@ ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cac
     const bool int8 = c->kind == TI_KV_INT8;
     ti_sparse_plan pl{1, 1};
     auto pairs = [&](int tg) { return ((long long)a->total_tokens + tg - 1) / tg * c->kv_heads; };
-    if (a->dtype == TI_BF16 && a->max_query_len > 1 && P >= 16 && P <= 32768 && (P & (P - 1)) == 0 && G <= 16) {
+    const bool f32 = a->dtype == TI_F32;
+    if (a->max_query_len > 1 && P >= 16 && P <= 32768 && (P & (P - 1)) == 0 && G <= 16 && (!f32 || ti_sparse_f32_mfma(a, c))) {
         auto tokens = [&](int rows, int entries) {
             return max(1, min(min(rows / G, a->max_query_len), entries / min(a->table_width, entries + 1)));
         };
         pl.tg = tokens(16, GROUP_PAGES);
         const int wide = tokens(32, GROUP_PAGES / 2);
-        if (wide > pl.tg && pairs(pl.tg) >= (int8 ? 512 : 256)) pl.tg = wide;
+        if (!f32 && wide > pl.tg && pairs(pl.tg) >= (int8 ? 512 : 256)) pl.tg = wide;
     }
-    const long long tiles = ((long long)a->table_width * P + 15) / 16, target = int8 && pl.tg > 1 ? 512 : 256;
-    while (pl.splits < 16 && pairs(pl.tg) * pl.splits < target && tiles >= 8 * pl.splits) pl.splits <<= 1;
+    const long long tiles = ((long long)a->table_width * P + 15) / 16, target = f32 || (int8 && pl.tg > 1) ? 512 : 256;
+    while (pl.splits < (f32 ? 32 : 16) && pairs(pl.tg) * pl.splits < target && tiles >= 8 * pl.splits) pl.splits <<= 1;
     return pl;
 }
 
@@ -176,7 +177,7 @@ int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_ca
     p.scale_log2 = a->scale * LOG2E;
     const unsigned grid = (unsigned)(((long long)a->total_tokens + pl.tg - 1) / pl.tg * c->kv_heads * p.splits);
     if (a->dtype == TI_F32) {
-        p.min_tiles = ti_launch_sparse_f32(a, c, p.splits, s);
+        p.min_tiles = ti_launch_sparse_f32(a, c, pl, s);
         if (p.min_tiles < 0) return TI_ERR_LAUNCH;
     } else {
         const bool int8 = c->kind == TI_KV_INT8;
