@@ -585,3 +585,98 @@ def test_refusals(gpu):
     refused(ti.sparse_attention_, out, sws, q, c.k, c.v, tables, lengths, 0.1, None, 3)
     refused(ti.sparse_attention_, out, sws, q, c.k, c.v, tables.cpu(), lengths, 0.1)
     refused(ti.sparse_attention_, out.cpu(), sws, q, c.k, c.v, tables, lengths, 0.1)
+
+
+# ---- largest sizes and launch limits ---------------------------------------------------------------
+
+@pytest.mark.parametrize("B,width", [(64, 34000), (1, 34000), (1, 40000), (2, 2100)])
+def test_select_wide_tables(gpu, B, width):
+    """Tables as wide as LDS holds in one launch and in two, wider than it holds, and with several tokens of one
+    sequence; one sequence is long, the others short."""
+    P, pages, H, n = 1, 3000, 2, 2
+    g = torch.Generator().manual_seed(width + B)
+    tables = torch.randint(1, pages + 1, (B, width), generator=g, dtype=torch.int32).cuda()
+    kb = random_bounds(pages, H, 64, P, width)
+    torch.manual_seed(B)
+    starts = [width - n] + [5 + b for b in range(1, B)]
+    q = torch.randn((B * n, H * 4, 64), device="cuda", dtype=torch.bfloat16)
+    check_select(kb, tables, starts, [n] * B, q, 70, 2, 3, True)
+
+
+def test_select_captured_with_much_lds(gpu):
+    """A launch that needs more LDS than a kernel gets by default, recorded in a graph and replayed."""
+    P, pages, B = 16, 9000, 64
+    tables = tables_for([140000] + [300] * (B - 1), P, pages, 3)
+    kb = random_bounds(pages, 2, 128, P, 3)
+    torch.manual_seed(3)
+    q = torch.randn((B, 8, 128), device="cuda", dtype=torch.bfloat16)
+    pos = i32([139999] + [250] * (B - 1))
+    out, lengths = torch.zeros((B, 2, 32), dtype=torch.int32, device="cuda"), torch.zeros((B, 2), dtype=torch.int32, device="cuda")
+    ws = ti.select_pages_workspace(BE, q, kb, tables)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ti.select_pages_(BE, out, lengths, ws, q, kb, tables, pos)
+    for i in range(3):
+        q.normal_()
+        pos[1:] += 7
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone(), lengths.clone()
+        want = ti.select_pages(BE, q, kb, tables, pos, 32)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8", "fp32"])
+@pytest.mark.parametrize("rows,heads,width", [(16, 2, 64), (256, 16, 16), (32, 2, 32)])
+def test_attend_groups_of_many_tokens(gpu, kv, rows, heads, width):
+    """One query head per KV head: 16 and 32 tokens in a group, whose lists take the most LDS."""
+    c = Cache(kv, 128, heads, 16, [16 * (width + 30)], seed=width)
+    torch.manual_seed(width)
+    q = torch.randn((rows, heads, 128), device="cuda", dtype=T[kv])
+    tables, lengths = shared(c, rows, width, seed=width)
+    check_attend(c, q, tables, lengths, n=rows)
+
+
+@pytest.mark.parametrize("n", [1, 4])
+def test_offsets_past_32_bits(gpu, n):
+    """Pools of more than 2^31 elements: pages at their end, through bounds, selection and attention."""
+    P, H, D = 16, 8, 128
+    pages = 2 ** 31 // (P * H * D) + 64
+    c = Cache("bf16", D, H, P, [300], seed=40)
+    k = torch.zeros((pages, H, P, D), dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    k[-c.pages:], v[-c.pages:] = c.k, c.v
+    tables = torch.where(c.tables > 0, c.tables + (pages - c.pages), 0).to(torch.int32)
+    pos = positions([300 - n], [n])
+    torch.manual_seed(40)
+    q = torch.randn((n, 32, D), device="cuda", dtype=torch.bfloat16)
+    results = []
+    for kp, vp, t in ((k, v, tables), (c.k, c.v, c.tables)):
+        kb = ti.key_bounds(D, P, H, kp.shape[0])
+        ti.update_key_bounds_(BE, kb, kp, vp, t, positions([0], [300]), max_query_len=300)
+        chosen, lengths = ti.select_pages(BE, q, kb, t, pos, 9, max_query_len=n)
+        out = ti.sparse_attention(BE, q, kp, vp, chosen, lengths, 0.09, None, n)
+        results.append((kb.bounds[-c.pages:], kb.scale[-c.pages:], chosen, lengths, out))
+    a, b = results
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(a[3], b[3])
+    assert torch.equal(torch.where(b[2] > 0, b[2] + (pages - c.pages), 0), a[2])
+    if n == 1:
+        assert torch.equal(a[4], b[4])
+    else:       # the joined list's order is that of the tables, whatever the ids
+        assert torch.equal(a[4], b[4])
+
+
+def test_long_step(gpu):
+    """More query tokens than a launch's grid holds tiles for one by one."""
+    n, P = 70000, 64
+    tables = tables_for([n], P, 1200, 41)
+    kb = random_bounds(1200, 1, 64, P, 41)
+    torch.manual_seed(41)
+    q = torch.randn((n, 16, 64), device="cuda", dtype=torch.bfloat16)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    out, lengths = ti.select_pages(BE, q, kb, tables, pos, 6, max_query_len=n)
+    b, s, table = kb.bounds.cpu().numpy(), kb.scale.cpu().numpy(), tables[0].cpu().numpy()
+    for t in (0, 63, 64, 32767, 32768, 32769, 65535, 65536, n - 1):
+        want, want_len = ref.select(q[t].double().cpu().numpy(), b, s, table, t, P, 6, 1, 1)
+        assert np.array_equal(out[t].cpu().numpy(), want) and np.array_equal(lengths[t].cpu().numpy(), want_len), t
+    assert (lengths > 0).all()
