@@ -603,6 +603,22 @@ def test_select_wide_tables(gpu, B, width):
     check_select(kb, tables, starts, [n] * B, q, 70, 2, 3, True)
 
 
+@pytest.mark.parametrize("B,H,pages", [(64, 8, 256), (1, 2, 900), (2, 2, 9000)])
+def test_select_infinite_scores(gpu, B, H, pages):
+    """Many pages of infinite scores of either sign beside finite ones, more of the largest than are kept."""
+    kb = random_bounds(pages, H, 64, 16, B)
+    kb.bounds[:], sign = kb.bounds.abs(), torch.arange(pages, device="cuda") % 5
+    kb.scale[sign > 0] = math.inf
+    kb.bounds[sign == 1] *= -1
+    tables = tables_for([16 * (pages - 20 - b) for b in range(B)], 16, pages, B)
+    torch.manual_seed(B)
+    q = torch.rand((B, H * 4, 64), device="cuda", dtype=torch.bfloat16) + 0.25
+    check_select(kb, tables, [16 * (pages - 20 - b) - 1 for b in range(B)], [1] * B, q, 40, 1, 1, True)
+    kb.scale[sign > 1] = 2.0 ** -120
+    kb.scale[sign == 2] = 2.0 ** 100
+    check_select(kb, tables, [16 * (pages - 20 - b) - 1 for b in range(B)], [1] * B, q, pages // 2, 1, 1, True)
+
+
 def test_select_captured_with_much_lds(gpu):
     """A launch that needs more LDS than a kernel gets by default, recorded in a graph and replayed."""
     P, pages, B = 16, 9000, 64

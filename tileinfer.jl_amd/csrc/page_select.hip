@@ -9,10 +9,9 @@
 // on how the work is split.
 //
 // Scores become 32-bit keys in the scores' order, 0 for pages that are not up for choice (those kept
-// anyway, and those past the last visible one). The key of the last page kept by score is found by one
-// wave, by bisection between the smallest and the largest key, counting the keys above the middle: it
-// ends when the count is right, after about log2 of the pages and a few steps, and at the latest after
-// 32 (equal keys). Then one pass over the pages in order writes the kept ones.
+// anyway, and those past the last visible one). The key of the last page kept by score is found by counting keys
+// in parts of their range: in halves by one wave where a work-group has a token for each, in as many parts as
+// it has threads where it has one token. Then one pass over the pages in order writes the kept ones.
 //
 // Two forms. select_kernel holds a token tile's keys in LDS and does both steps in one launch.
 // scores_kernel and keep_kernel share a tile's pages out over several work-groups, the keys going
@@ -27,7 +26,7 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int ROUND = 256;   // keys read by a wave at once: rows of keys are padded to it with zeros
-constexpr int ONE = 8 * ROUND;   // the most keys that one wave searches
+constexpr int ONE = 8 * ROUND;   // the most keys that one wave searches (they stay in registers)
 
 struct SelectParams {
     const void *q;
@@ -224,75 +223,49 @@ struct Limit {
     uint32_t limit;
     int ties;
 };
-// Joins what the W waves that search together found: `red` holds 4 W words of LDS, used in halves in
-// turn, so that one barrier is enough.
-template <int W> struct Join {
-    int *red;
-    int lane, w, turn;
-    __device__ int sum(int v) {
-        if constexpr (W == 1) return v;
-        return wave_total(swap(v, 0));
-    }
-    __device__ uint32_t most(uint32_t v) {
-        if constexpr (W == 1) return v;
-        return wave_umax((uint32_t)swap((int)v, 0));
-    }
-    __device__ int swap(int v, int none) {
-        int *r = red + (turn ^= 1) * W;
-        if (lane == 0) r[w] = v;
-        __syncthreads();
-        return lane < W ? r[lane] : none;
-    }
-};
-
-// The search over keys in groups of four per lane, group(n) the n-th of this wave's `groups`; `all` keys are up
-// for choice. A step takes 0.2 us for 512 keys and 0.4 for 2048, and 11 are usual (counting lane
-// masks, or several middles at a time in 16 waves, was no faster). Where few keys are left between the
-// ends, these close in on them: equal keys end the search then and not after all 24 halvings of their digits.
-template <typename Group, typename J>
-__device__ __forceinline__ Limit bisect(int need, int all, int groups, Group group, J join) {
+// The search by one wave that holds all keys, by halves between the smallest and the largest: a step takes
+// 0.2 us for 512 keys and 0.4 for 2048, and 11 are usual. Where few keys are left between the ends, these
+// close in on them: equal keys end the search then and not after all 24 halvings of their digits.
+template <int NG> __device__ __forceinline__ Limit bisect(const Seen &s, const uint32_t *keys, int span, int lane) {
+    u32x4 k[NG];
     uint32_t top = 0, low = 0xffffffffu;
 #pragma unroll
-    for (int n = 0; n < groups; n++) {
-        const u32x4 k = group(n);
+    for (int n = 0; n < NG; n++) {
+        k[n] = n * ROUND < span ? *reinterpret_cast<const u32x4 *>(keys + n * ROUND + 4 * lane) : (u32x4){0u, 0u, 0u, 0u};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            top = max(top, k[e]);
-            low = min(low, k[e] - 1);   // 0 wraps to the largest
+            top = max(top, k[n][e]);
+            low = min(low, k[n][e] - 1);   // 0 wraps to the largest
         }
     }
-    top = join.most(wave_umax(top));
-    low = ~join.most(wave_umax(~low)) + 1;
-    int from = all, above = 0;   // keys >= low: at least need; keys > top: fewer
+    top = wave_umax(top);
+    low = ~wave_umax(~low) + 1;
+    int from = s.c1 - s.c0, above = 0;   // keys >= low: at least need; keys > top: fewer
     bool closed = false;
     while (low < top) {
         if (!closed && from - above <= 4) {
             closed = true;
             uint32_t most = 0, least = 0xffffffffu;
 #pragma unroll
-            for (int n = 0; n < groups; n++) {
-                const u32x4 k = group(n);
+            for (int n = 0; n < NG; n++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    most = max(most, k[e] <= top ? k[e] : 0u);
-                    least = min(least, k[e] >= low ? k[e] : 0xffffffffu);
+                    most = max(most, k[n][e] <= top ? k[n][e] : 0u);
+                    least = min(least, k[n][e] >= low ? k[n][e] : 0xffffffffu);
                 }
-            }
-            top = join.most(wave_umax(most));
-            low = ~join.most(wave_umax(~least));
+            top = wave_umax(most);
+            low = ~wave_umax(~least);
             continue;
         }
         const uint32_t d = top - low, mid = low + d / 2 + (d & 1);
-        int count = 0;
+        int c = 0;
 #pragma unroll
-        for (int n = 0; n < groups; n++) {
-            const u32x4 k = group(n);
+        for (int n = 0; n < NG; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) count += k[e] >= mid;
-        }
-        const int c = join.sum(wave_total(count));
-        if (c == need) return {mid - 1, 0};
-        if (c > need) {
+            for (int e = 0; e < 4; e++) c += k[n][e] >= mid;
+        c = wave_total(c);
+        if (c == s.need) return {mid - 1, 0};
+        if (c > s.need) {
             low = mid;
             from = c;
         } else {
@@ -300,38 +273,115 @@ __device__ __forceinline__ Limit bisect(int need, int all, int groups, Group gro
             above = c;
         }
     }
-    return {low, need - above};
-}
-// Up to NG groups a wave in registers: the search is all arithmetic.
-template <int NG, int W, typename J>
-__device__ __forceinline__ Limit bisect_held(int need, int all, const uint32_t *keys, int span, int lane, int w, J join) {
-    u32x4 k[NG];
-#pragma unroll
-    for (int n = 0; n < NG; n++) {
-        const int i = (n * W + w) * ROUND;
-        k[n] = i < span ? *reinterpret_cast<const u32x4 *>(keys + i + 4 * lane) : (u32x4){0u, 0u, 0u, 0u};
-    }
-    return bisect(need, all, NG, [&](int n) { return k[n]; }, join);
+    return {low, s.need - above};
 }
 
-// By W waves (all of the work-group where W > 1), over `span` keys (a multiple of ROUND); those that are
-// not up for choice become 0. One wave takes up to ONE keys, all in registers (8192 through LDS
-// took 45 us), more waves 512 each before they read them from LDS at every step.
+// Keys that are not up for choice become 0; *found: there is nothing to search.
+__device__ __forceinline__ Limit begin_search(const Seen &s, uint32_t *keys, int span, int tid, int threads, bool *found) {
+    for (int i = tid; i < s.c0; i += threads) keys[i] = 0;
+    for (int i = s.c1 + tid; i < span; i += threads) keys[i] = 0;
+    *found = s.need >= s.c1 - s.c0 || s.need <= 0;
+    return Limit{s.need <= 0 ? 0xffffffffu : 0u, 0};   // none, or every candidate
+}
+
+// By one wave, up to ONE keys.
+__device__ __forceinline__ Limit find_limit(const Seen &s, uint32_t *keys, int span, int lane) {
+    bool found;
+    const Limit l = begin_search(s, keys, span, lane, 64, &found);
+    if (found) return l;
+    if (span <= 2 * ROUND) return bisect<2>(s, keys, span, lane);
+    if (span <= 5 * ROUND) return bisect<5>(s, keys, span, lane);
+    return bisect<8>(s, keys, span, lane);
+}
+
+// The words of LDS that the waves of a work-group search with.
+template <int W> struct SearchLds {
+    int hist[W * 64];   // keys in each part of the range; then the keys of one part
+    int sum[2 * W];
+    int part, above, held, listed;
+};
+
+// By the W waves of a work-group, any number of keys: they are counted in as many equal parts of their range as
+// there are threads, and the part that holds the last one kept is searched on: with up to 64 keys (the usual
+// case, after one round) each lane ranks one of them, else as the range was. The waves' barriers and not the
+// keys are the cost: 8192 keys take what 512 do.
 template <int W>
-__device__ __forceinline__ Limit find_limit(const Seen &s, uint32_t *keys, int span, int lane, int w, int *red) {
-    for (int i = w * 64 + lane; i < s.c0; i += W * 64) keys[i] = 0;
-    for (int i = s.c1 + w * 64 + lane; i < span; i += W * 64) keys[i] = 0;
-    if (W > 1) __syncthreads();
-    if (s.need >= s.c1 - s.c0) return {0, 0};   // every candidate
-    if (s.need <= 0) return {0xffffffffu, 0};     // none
-    const Join<W> join{red, lane, w, 0};
-    if (span <= 2 * W * ROUND) return bisect_held<2, W>(s.need, s.c1 - s.c0, keys, span, lane, w, join);
-    if constexpr (W == 1) {
-        if (span <= 5 * ROUND) return bisect_held<5, W>(s.need, s.c1 - s.c0, keys, span, lane, w, join);
-        return bisect_held<8, W>(s.need, s.c1 - s.c0, keys, span, lane, w, join);
+__device__ __forceinline__ Limit find_limit_together(const Seen &s, uint32_t *keys, int span, int lane, int w, SearchLds<W> &m) {
+    constexpr int BINS = W * 64, BITS = __builtin_ctz(BINS);
+    const int tid = w * 64 + lane;
+    bool found;
+    const Limit l = begin_search(s, keys, span, tid, BINS, &found);
+    m.hist[tid] = 0;
+    if (tid == 0) m.listed = 0;
+    __syncthreads();   // (keys may be in global memory)
+    if (found) return l;
+    uint32_t top = 0, low = 0xffffffffu;
+    for (int i = 4 * tid; i < span; i += 4 * BINS) {
+        const u32x4 k = *reinterpret_cast<const u32x4 *>(keys + i);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            top = max(top, k[e]);
+            low = min(low, k[e] - 1);   // 0 wraps to the largest
+        }
     }
-    const int all = span / ROUND, mine = (all - w + W - 1) / W;
-    return bisect(s.need, s.c1 - s.c0, mine, [&](int n) { return *reinterpret_cast<const u32x4 *>(keys + (n * W + w) * ROUND + 4 * lane); }, join);
+    top = wave_umax(top);
+    low = wave_umax(~low);
+    if (lane == 0) m.sum[w] = (int)top, m.sum[W + w] = (int)low;
+    __syncthreads();
+    top = wave_umax(lane < W ? (uint32_t)m.sum[lane] : 0u);
+    low = ~wave_umax(lane < W ? (uint32_t)m.sum[W + lane] : 0u) + 1;
+    int need = s.need;   // of the keys in [low, top]; larger ones are all kept
+    while (low < top) {
+        const int shift = max(32 - __builtin_clz(top - low) - BITS, 0);
+        for (int i = 4 * tid; i < span; i += 4 * BINS) {
+            const u32x4 k = *reinterpret_cast<const u32x4 *>(keys + i);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (k[e] >= low && k[e] <= top) atomicAdd(&m.hist[(k[e] - low) >> shift], 1);
+        }
+        __syncthreads();
+        const int part = BINS - 1 - tid, c = m.hist[part];
+        m.hist[part] = 0;
+        int upto = c;   // keys of this part and the ones above it
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(upto, o);
+            if (lane >= o) upto += v;
+        }
+        if (lane == 63) m.sum[w] = upto;
+        __syncthreads();
+        upto += wave_total(lane < w ? m.sum[lane] : 0);
+        if (upto >= need && upto - c < need) {
+            m.part = part;
+            m.above = upto - c;
+            m.held = c;
+        }
+        __syncthreads();
+        need -= m.above;
+        low += (uint32_t)m.part << shift;
+        top = low + min(top - low, (1u << shift) - 1);
+        if (need == m.held) return {low - 1, 0};
+        if (m.held > 64) continue;
+        const int held = m.held;
+        for (int i = 4 * tid; i < span; i += 4 * BINS) {
+            const u32x4 k = *reinterpret_cast<const u32x4 *>(keys + i);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (k[e] >= low && k[e] <= top) m.hist[atomicAdd(&m.listed, 1)] = (int)k[e];
+        }
+        __syncthreads();
+        const uint32_t mine = lane < held ? (uint32_t)m.hist[lane] : 0u;
+        int more = 0, same = 0;
+        for (int j = 0; j < held; j++) {
+            const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
+            more += other > mine;
+            same += other == mine;
+        }
+        const unsigned long long last = __ballot(lane < held && more < need && more + same >= need);
+        const int at = __builtin_ctzll(last);
+        return {(uint32_t)__builtin_amdgcn_readlane((int)mine, at), need - __builtin_amdgcn_readlane(more, at)};
+    }
+    return {low, need};
 }
 
 // Writes one token's kept pages in order, zeros behind them, and its number of keys; NW waves share the
@@ -383,23 +433,22 @@ __device__ __forceinline__ void write_pages(const SelectParams &p, const Seen &s
     }
 }
 
-// One token's pages by the whole work-group of W waves: up to ONE keys are searched by one wave (no
-// barriers: 2048 keys 31 us for the call against 34.5 by 16 waves), more by all; all write. red: 4 W + 2 words of LDS.
+// The search as a call, for tiles of several blocks of rows, where it is the exception: in line it would take
+// registers from the scores' loop, which spills then (31.3 and 32.9 us for 512 tokens on 64k keys).
 template <int W>
+__device__ __attribute__((noinline)) Limit find_limit_apart(const Seen &s, uint32_t *keys, int span, int lane, int w, SearchLds<W> &m) {
+    return find_limit_together<W>(s, keys, span, lane, w, m);
+}
+
+// One token's pages by the whole work-group of W waves.
+template <int W, bool APART>
 __device__ __forceinline__ void keep_together(const SelectParams &p, const Seen &s, uint32_t *keys, int span, size_t pair,
-                                              const int32_t *bt, int lane, int w, int *red) {
+                                              const int32_t *bt, int lane, int w, SearchLds<W> &m) {
     Limit l;
-    if (span <= ONE) {
-        if (w == 0) {
-            l = find_limit<1>(s, keys, span, lane, 0, red);
-            if (lane == 0) red[0] = (int)l.limit, red[1] = l.ties;
-        }
-        __syncthreads();
-        l = Limit{(uint32_t)red[0], red[1]};
-    } else {
-        l = find_limit<W>(s, keys, span, lane, w, red + 2);
-    }
-    write_pages<W>(p, s, l, keys, pair, bt, lane, w, red + 2 + 2 * W);
+    if constexpr (APART) l = find_limit_apart<W>(s, keys, span, lane, w, m);
+    else l = find_limit_together<W>(s, keys, span, lane, w, m);
+    __syncthreads();   // m is read
+    write_pages<W>(p, s, l, keys, pair, bt, lane, w, m.sum);
 }
 
 // Grid (Hk, token tiles, B), the keys of the tile's tokens in LDS.
@@ -408,7 +457,7 @@ __global__ void __launch_bounds__(W * 64) select_kernel(SelectParams p) {
     using TL = Tile<GP, RT, WIDE>;
     __shared__ __attribute__((aligned(16))) int8_t w[TL::ROWS][2 * D];
     __shared__ float forth[TL::ROWS];
-    __shared__ int red[4 * W + 2];
+    __shared__ SearchLds<W> search;
     extern __shared__ __attribute__((aligned(16))) uint32_t keys[];   // [TT][pitch]
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x, b = blockIdx.z;
@@ -426,14 +475,15 @@ __global__ void __launch_bounds__(W * 64) select_kernel(SelectParams p) {
         const int32_t *bt = p.bt + (size_t)b * p.bt_stride;
         if (tokens == 1 || span > ONE) {
             for (int t = 0; t < tokens; t++) {
-                keep_together<W>(p, Seen(p, st, t0 + t), keys + t * p.pitch, span, (size_t)(st.tok0 + t0 + t) * p.Hk + h, bt, lane, wv, red);
-                __syncthreads();   // red is read
+                keep_together<W, (RT > 1 && !WIDE)>(p, Seen(p, st, t0 + t), keys + t * p.pitch, span, (size_t)(st.tok0 + t0 + t) * p.Hk + h, bt, lane,
+                                               wv, search);
+                __syncthreads();   // its LDS is read
             }
         } else {
             for (int t = wv; t < tokens; t += W) {
                 const Seen s(p, st, t0 + t);
-                const Limit l = find_limit<1>(s, keys + t * p.pitch, span, lane, 0, red);
-                write_pages<1>(p, s, l, keys + t * p.pitch, (size_t)(st.tok0 + t0 + t) * p.Hk + h, bt, lane, 0, red);
+                const Limit l = find_limit(s, keys + t * p.pitch, span, lane);
+                write_pages<1>(p, s, l, keys + t * p.pitch, (size_t)(st.tok0 + t0 + t) * p.Hk + h, bt, lane, 0, nullptr);
             }
         }
     }
@@ -463,7 +513,7 @@ __global__ void __launch_bounds__(W * 64) scores_kernel(SelectParams p) {
 // Kept pages of one token and KV head from the workspace: grid (Hk, tokens, B). The keys are read into LDS
 // where it holds them (`lds` of them).
 template <int W> __global__ void __launch_bounds__(W * 64) keep_kernel(SelectParams p, int lds) {
-    __shared__ int red[4 * W + 2];
+    __shared__ SearchLds<W> search;
     extern __shared__ __attribute__((aligned(16))) uint32_t held[];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x, b = blockIdx.z;
@@ -479,15 +529,15 @@ template <int W> __global__ void __launch_bounds__(W * 64) keep_kernel(SelectPar
             for (int i = 4 * tid; i < span; i += W * 256)
                 *reinterpret_cast<u32x4 *>(held + i) = *reinterpret_cast<const u32x4 *>(keys + i);
             __syncthreads();
-            keep_together<W>(p, s, held, span, pair, bt, lane, wv, red);
+            keep_together<W, false>(p, s, held, span, pair, bt, lane, wv, search);
         } else {
-            keep_together<W>(p, s, keys, span, pair, bt, lane, wv, red);
+            keep_together<W, false>(p, s, keys, span, pair, bt, lane, wv, search);
         }
     }
 }
 
 // LDS that select_kernel's keys may take: one work-group of 16 waves and its operands on a CU.
-constexpr int LDS_KEYS = 136 << 10;
+constexpr int LDS_KEYS = 128 << 10;
 bool allow_lds(const void *kernel, size_t bytes) {
     return bytes <= (32u << 10) || hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
 }
