@@ -589,7 +589,7 @@ def test_refusals(gpu):
 
 # ---- largest sizes and launch limits ---------------------------------------------------------------
 
-@pytest.mark.parametrize("B,width", [(64, 34000), (1, 34000), (1, 40000), (2, 2100)])
+@pytest.mark.parametrize("B,width", [(64, 34000), (64, 16300), (130, 16300), (1, 34000), (1, 40000), (2, 2100), (4, 760), (64, 2040), (130, 4000)])
 def test_select_wide_tables(gpu, B, width):
     """Tables as wide as LDS holds in one launch and in two, wider than it holds, and with several tokens of one
     sequence; one sequence is long, the others short."""

@@ -542,49 +542,65 @@ bool allow_lds(const void *kernel, size_t bytes) {
     return bytes <= (32u << 10) || hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
 }
 
+// Keys of a tile, in LDS.
+size_t key_bytes(const SelectParams &p, int tile) { return (size_t)min(tile, p.nmax) * p.pitch * sizeof(uint32_t); }
+
+// One launch while the keys fit LDS and either there is a work-group for every CU or a table is short: one token
+// over 512 pages takes 11.0 us so and 13.0 in two launches, over 1024 15.4 and 13.2, over 2048 23.7 and 13.8;
+// 256 work-groups over 2048 pages each 39.7 and 45.4, 128 26.2 and 24.0.
+template <int TT> bool fits_one_launch(const SelectParams &p, long long groups) {
+    return key_bytes(p, TT) <= (size_t)LDS_KEYS && (groups >= 256 || p.bt_stride <= 768);
+}
+
 template <int D, int GP, int RT, bool WIDE, int W>
-int launch(SelectParams p, int num_seqs, hipStream_t s) {
-    constexpr int TT = Tile<GP, RT, WIDE>::TT;
-    const long long tiles = (p.nmax + (long long)TT - 1) / TT, groups = tiles * num_seqs * p.Hk;
-    const unsigned y = (unsigned)min(tiles, 32768LL);   // longer steps loop
-    const size_t bytes = (size_t)TT * p.pitch * sizeof(uint32_t);
-    // One launch while the keys fit LDS and either the launch's work-groups fill half of the chip or a
-    // table is short; a wide table's pages are shared out over work-groups otherwise.
-    if (bytes <= (size_t)LDS_KEYS && (groups >= 128 || p.bt_stride <= 1024)) {
-        auto kernel = select_kernel<D, GP, RT, WIDE, W>;
-        if (!allow_lds((const void *)kernel, bytes)) return TI_ERR_LAUNCH;
-        kernel<<<dim3(p.Hk, y, num_seqs), W * 64, bytes, s>>>(p);
-        return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
-    }
-    p.split = 1;
-    while (groups * p.split < 256 && p.split * W * 32 < p.bt_stride) p.split <<= 1;
-    scores_kernel<D, GP, RT, WIDE, W><<<dim3(p.Hk * p.split, y, num_seqs), W * 64, 0, s>>>(p);
-    if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
-    const size_t held = min((size_t)p.pitch * sizeof(uint32_t), (size_t)LDS_KEYS);
-    if (!allow_lds((const void *)keep_kernel<W>, held)) return TI_ERR_LAUNCH;
-    keep_kernel<W><<<dim3(p.Hk, min(p.nmax, 32768), num_seqs), W * 64, held, s>>>(p, (int)(held / sizeof(uint32_t)));
+int launch_one(const SelectParams &p, unsigned y, int num_seqs, hipStream_t s) {
+    const size_t bytes = key_bytes(p, Tile<GP, RT, WIDE>::TT);
+    auto kernel = select_kernel<D, GP, RT, WIDE, W>;
+    if (!allow_lds((const void *)kernel, bytes)) return TI_ERR_LAUNCH;
+    kernel<<<dim3(p.Hk, y, num_seqs), W * 64, bytes, s>>>(p);
     return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
 }
 
-// Query rows per tile: 64 (32 where a token's heads do not fill a lane's four rows or go past them: 64
-// spill there) where the steps' tokens fill them and the launch still has work-groups for every CU
-// (bounds are then read once for several blocks of rows), else 16.
-constexpr int W4_PAGES = 256;
+template <int D, int GP, int RT, bool WIDE>
+int launch(SelectParams p, int num_seqs, hipStream_t s) {
+    constexpr int TT = Tile<GP, RT, WIDE>::TT, W = 16;
+    const long long tiles = (p.nmax + (long long)TT - 1) / TT, groups = tiles * num_seqs * p.Hk;
+    const unsigned y = (unsigned)min(tiles, 32768LL);   // longer steps loop
+    if (fits_one_launch<TT>(p, groups)) {
+        // 4 waves for short tables, whose pages give 16 waves little to do, and for several work-groups per CU,
+        // which wait for each other less (while LDS holds four): 128 pages and 64 work-groups 7.1 us and 7.8 with
+        // 16, 512 and 512 19.2 and 25.2, 2048 and 512 68 and 76; 2048 and 128 27.7 and 25.9.
+        if constexpr (RT == 1)
+            if (key_bytes(p, TT) <= (32u << 10) && (p.bt_stride <= 512 || groups >= 512)) return launch_one<D, GP, RT, WIDE, 4>(p, y, num_seqs, s);
+        return launch_one<D, GP, RT, WIDE, W>(p, y, num_seqs, s);
+    }
+    if constexpr (RT == 1 || WIDE) {   // launch_rows takes tiles of several tokens' blocks for one launch only
+        p.split = 1;
+        while (groups * p.split < 256 && p.split * W * 32 < p.bt_stride) p.split <<= 1;
+        scores_kernel<D, GP, RT, WIDE, W><<<dim3(p.Hk * p.split, y, num_seqs), W * 64, 0, s>>>(p);
+        if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
+        const size_t held = min((size_t)p.pitch * sizeof(uint32_t), (size_t)LDS_KEYS);
+        if (!allow_lds((const void *)keep_kernel<W>, held)) return TI_ERR_LAUNCH;
+        keep_kernel<W><<<dim3(p.Hk, min(p.nmax, 32768), num_seqs), W * 64, held, s>>>(p, (int)(held / sizeof(uint32_t)));
+        return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
+    }
+    return TI_ERR_LAUNCH;
+}
+
+// Query rows per tile: 64 (32 where a token's heads do not fill a lane's four rows or go past them: 64 spill
+// there) where the steps' tokens fill them and the launch still has work-groups for every CU (bounds are then
+// read once for several blocks of rows: 512 tokens on 64k keys 31 us, 91 with 16), else 16 (128 tokens 25 and 30).
 template <int D, int GP>
 int launch_rows(const SelectParams &p, int num_seqs, hipStream_t s) {
     constexpr int RT = GP == 4 || GP == 16 ? 4 : 2, TT = Tile<GP, RT, false>::TT;
     const long long groups = ((long long)p.nmax + TT - 1) / TT * num_seqs * p.Hk;
-    const long long groups1 = (p.nmax + 16LL / GP - 1) / (16 / GP) * num_seqs * p.Hk;
-    if (groups >= 256 && p.nmax >= TT && (size_t)TT * p.pitch * 4 <= (size_t)LDS_KEYS) return launch<D, GP, RT, false, 16>(p, num_seqs, s);
-    // 4 waves for tables that give no more than two 16-page tiles to each and a launch of several work-groups
-    // per CU, 16 otherwise.
-    if (p.bt_stride <= W4_PAGES && groups1 >= 512) return launch<D, GP, 1, false, 4>(p, num_seqs, s);
-    return launch<D, GP, 1, false, 16>(p, num_seqs, s);
+    if (groups >= 256 && p.nmax >= TT && key_bytes(p, TT) <= (size_t)LDS_KEYS) return launch<D, GP, RT, false>(p, num_seqs, s);
+    return launch<D, GP, 1, false>(p, num_seqs, s);
 }
 
 template <int D>
 int launch_heads(const SelectParams &p, int num_seqs, hipStream_t s) {
-    if (p.G > 16) return launch<D, 16, 4, true, 16>(p, num_seqs, s);
+    if (p.G > 16) return launch<D, 16, 4, true>(p, num_seqs, s);
     if (p.G > 8) return launch_rows<D, 16>(p, num_seqs, s);
     if (p.G > 4) return launch_rows<D, 8>(p, num_seqs, s);
     if (p.G > 2) return launch_rows<D, 4>(p, num_seqs, s);
