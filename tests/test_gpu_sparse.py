@@ -653,6 +653,45 @@ def test_attend_groups_of_many_tokens(gpu, kv, rows, heads, width):
     check_attend(c, q, tables, lengths, n=rows)
 
 
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("D,P,heads,G,rows,width", [(128, 16, 32, 4, 131, 5), (128, 64, 32, 4, 128, 3), (128, 16, 64, 2, 260, 4),
+                                                    (128, 32, 64, 3, 84, 6), (128, 16, 128, 12, 11, 9), (64, 16, 64, 4, 131, 5),
+                                                    (64, 16, 64, 16, 67, 3), (128, 16, 128, 8, 35, 130)])
+def test_attend_many_rows_in_a_group(gpu, kv, D, P, heads, G, rows, width):
+    """Steps with so many tokens and KV heads that a group has up to 64 query rows; the last group is not full."""
+    c = Cache(kv, D, heads, P, [P * (width + 20)], seed=rows)
+    torch.manual_seed(rows)
+    q = torch.randn((rows, heads * G, D), device="cuda", dtype=T[kv])
+    tables, lengths = shared(c, rows, width, seed=rows)
+    lengths[3], lengths[5, 1] = 0, 1
+    check_attend(c, q, tables, lengths, n=rows)
+    check_attend(c, q, tables, lengths, scale=0.05, qsl=i32([2, rows // 2, rows - 1]), n=rows)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_attend_many_rows_with_values_that_are_not_finite(gpu, value, where):
+    rows, heads = 64, 64
+    c = Cache("bf16", 128, heads, 16, [40 * 16], seed=32)
+    torch.manual_seed(32)
+    q = torch.randn((rows, heads * 4, 128), device="cuda", dtype=torch.bfloat16)
+    tables, lengths = shared(c, rows, 4, seed=32)
+    bad = tables[1, 0, 2].item()
+    pool = c.k if where == "k" else c.v
+    want = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09, None, rows)
+    pool[bad - 1, :, 5, 17] = value
+    got = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09, None, rows)
+    used = torch.arange(4, device="cuda") * 16 < lengths[..., None]
+    touched = ((tables == bad) & used).any(2).repeat_interleave(4, 1)
+    assert touched.any() and not touched.all()
+    assert torch.isfinite(got[~touched]).all()
+    # rows of the wave-by-row path round otherwise: each is within 2^-7 of the exact weights and output
+    size = c.v[torch.isfinite(c.v)].abs().max().item()
+    assert (got[~touched].float() - want[~touched].float()).abs().max().item() <= 2 * 2.0 ** -7 * size
+    alone = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09)
+    assert torch.equal(torch.isfinite(got), torch.isfinite(alone))
+
+
 @pytest.mark.parametrize("n", [1, 4])
 def test_offsets_past_32_bits(gpu, n):
     """Pools of more than 2^31 elements: pages at their end, through bounds, selection and attention."""

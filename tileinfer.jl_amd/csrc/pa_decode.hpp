@@ -166,6 +166,15 @@ __device__ __forceinline__ f32x4 pv_mfma(s16x4 v, s16x4 pt, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v, pt, c, 0, 0, 0);
 }
 
+// The same on two tiles of keys: a lane's first four elements of the depth are the first tile's keys 4 k .. 4 k + 3,
+// its last four the second's, in both operands.
+template <bool INT8>
+__device__ __forceinline__ f32x4 pv_mfma2(s16x4 v0, s16x4 v1, s16x4 p0, s16x4 p1, f32x4 c) {
+    const u32x2 a0 = __builtin_bit_cast(u32x2, v0), a1 = __builtin_bit_cast(u32x2, v1);
+    const u32x2 b0 = __builtin_bit_cast(u32x2, p0), b1 = __builtin_bit_cast(u32x2, p1);
+    return qk_mfma<INT8>((u32x4){a0[0], a0[1], a1[0], a1[1]}, (u32x4){b0[0], b0[1], b1[0], b1[1]}, c);
+}
+
 // One 16-key tile's raw loads, held in registers from issue to use (software pipeline).
 template <int D, bool INT8>
 struct TileRegs {
@@ -202,7 +211,8 @@ struct RowMap {
     __device__ __forceinline__ int last(int pos) const { return len - 1 - pos; }   // last key of the tile at pos
 };
 
-template <int D, bool INT8, bool PG16, typename Map>
+// PART: 1 the keys, 2 the values, 3 both (1 and 2 for dense caches and whole tiles).
+template <int D, bool INT8, bool PG16, int PART = 3, typename Map>
 __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodeParams &p,
                                           const Map &rm, int j, int r16, int kg, int vg,
                                           int vc, size_t half_q, size_t half_s) {
@@ -225,10 +235,10 @@ __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodePara
         if (!INT8) {
             const uint16_t *kb = p.kp + r0 * D, *vb = p.vp + r0 * D;
 #pragma unroll
-            for (int i = 0; i < NKB; i++)
+            for (int i = 0; i < (PART & 1 ? NKB : 0); i++)
                 t.k[i] = *reinterpret_cast<const u32x4 *>(kb + (kr * D + i * 32 + kg * 8));
 #pragma unroll
-            for (int e = 0; e < KPL; e++)
+            for (int e = 0; e < (PART & 2 ? KPL : 0); e++)
                 t.v[e] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vb + (vr[e] * D + vc * 8)));
         } else {
             const int8_t *kb = p.lq + r0 * D, *vb = p.lq + half_q + r0 * D;
@@ -294,15 +304,16 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     constexpr int NKW = NW / RS;         // waves splitting the keys (RS row slices each)
     // Tiles loaded per step (TPI: see the loop) and worked on together (JT). JOINT: a whole step
     // runs its tiles through one softmax, so their score chains overlap and one max decides the
-    // rescale.
-    constexpr int TPI = INT8 ? (ROWB == 1 ? 3 : 2) : 1, JT = JOINT ? TPI : 1;
+    // rescale. GROUP: two, whose values are one product of depth 32 (INT8, 512 tokens: 100 -> 88 us).
+    constexpr int TPI = GROUP ? 2 : INT8 ? (ROWB == 1 ? 3 : 2) : 1, JT = JOINT || GROUP ? TPI : 1;
 
     // Per-wave transposed V tiles during the key loop; afterwards the same LDS holds each
     // wave's (O, m, l) slab for the merge (rows of D + 4 floats, 16-B aligned).
     constexpr int MROW = D + 4;
     constexpr int VROW = vtile_row<D>();
     constexpr int VT_BYTES = NW * JT * 16 * VROW * 2;
-    constexpr int SLAB_BYTES = NW * MP * MROW * 4;
+    constexpr int HB = ROWB > 2 ? 2 : ROWB, HP = HB * 16;   // blocks and rows merged at once (LDS)
+    constexpr int SLAB_BYTES = NW * HP * MROW * 4;
     // GROUP: the joined pages in front of the value tiles, the tokens' keys of each in dynamic LDS
     constexpr int LIST_BYTES = GROUP ? (int)offsetof(GroupLds, rest) : 0;
     constexpr int LOOP_BYTES = GROUP && LIST_BYTES + VT_BYTES < (int)sizeof(GroupLds) ? (int)sizeof(GroupLds) : LIST_BYTES + VT_BYTES;
@@ -439,7 +450,7 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     }
 
     f32x4 o[ROWB][NDT];
-    f32x4 psum[ROWB];   // INT8: sum of the fp16 probabilities (every element: the row's)
+    f32x4 psum[ROWB];   // INT8 and GROUP: sum of the rounded probabilities (every element: the row's)
     float m[ROWB], l[ROWB];
 #pragma unroll
     for (int rb = 0; rb < ROWB; rb++) {
@@ -454,8 +465,9 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     const int vc = lane % CPR, vg = lane / CPR;   // V load: chunk, key group
 
     // NT tiles j .. j + NT - 1: their scores, one softmax over them, their values.
-    auto compute = [&](const TileRegs<D, INT8> *t, int j, auto count) {
+    auto compute = [&](const TileRegs<D, INT8> *t, int j, auto count, auto next) {
         constexpr int NT = decltype(count)::value;
+        constexpr bool PAIR = GROUP && NT == 2;   // the values of two tiles in one product of depth 32
         // ---- V rows -> row-major LDS tiles (INT8: biased fp16, exact) ----
         u32x4 vrows[NT][KPL];
 #pragma unroll
@@ -494,22 +506,25 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
                     svk[n][e] = __shfl(t[n].sv, kg * 4 + e);
                 }
         }
+        next();   // the tiles' registers are free
         // ---- online softmax + P^T operands ----
         // Lazy rescaling: m is a reference max that only moves when a step's max exceeds
         // it by more than RESCALE_LOG2 (then p <= 2^RESCALE_LOG2, safe in bf16 and fp32);
         // l and O always use the same reference, so the result is exact. INT8 moves m
         // with every larger max (p <= 1, so p times a value scale stays within fp16).
-        int seen[ROWB], off = 0;   // GROUP: keys of the page that the row sees, the tile's first one
+        int seen[NT][ROWB], off[NT];   // GROUP: keys of the page that the row sees, the tile's first one
         bool need_mask = (j + NT) * 16 - 1 > mask_from;
         if constexpr (GROUP) {
-            static_assert(!GROUP || NT == 1);
-            const int u = j * 16 >> p.pshift;
-            off = j * 16 & (p.P - 1);
             bool whole = true;
 #pragma unroll
-            for (int rb = 0; rb < ROWB; rb++) {
-                seen[rb] = lim[u * p.tg + qpos[rb]];
-                whole &= off + 16 <= seen[rb];
+            for (int n = 0; n < NT; n++) {
+                const int at = min(j + n, j1 - 1) * 16, u = at >> p.pshift;
+                off[n] = at & (p.P - 1);
+#pragma unroll
+                for (int rb = 0; rb < ROWB; rb++) {
+                    seen[n][rb] = j + n < j1 ? lim[u * p.tg + qpos[rb]] : 0;   // none of a pair's tile past the end
+                    whole &= off[n] + 16 <= seen[n][rb];
+                }
             }
             need_mask = !__all(whole);
         }
@@ -525,7 +540,7 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
                 if (INT8) v = (v - qcorr[rb]) * skk[e >> 2][e & 3] * qsl[rb];
                 else v *= p.scale_log2;
                 if constexpr (GROUP) {
-                    if (need_mask) v = off + kg * 4 + e < seen[rb] ? v : -INFINITY;
+                    if (need_mask) v = off[e >> 2] + kg * 4 + (e & 3) < seen[e >> 2][rb] ? v : -INFINITY;
                 } else if (need_mask) {
                     const int kp = (j + (e >> 2)) * 16 + kg * 4 + (e & 3);
                     v = (kp <= qpos[rb] && kp < len) ? v : -INFINITY;
@@ -569,7 +584,8 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
                                                                    __builtin_bit_cast(uint32_t, h1)});
                     // the row's sum of these fp16 probabilities, for the values' bias
                     const s16x4 ones = __builtin_bit_cast(s16x4, (u32x2){0x3c003c00u, 0x3c003c00u});
-                    psum[rb] = pv_mfma<true>(ones, pop[n][rb], psum[rb]);
+                    if constexpr (!PAIR) psum[rb] = pv_mfma<true>(ones, pop[n][rb], psum[rb]);
+                    else if (n == 1) psum[rb] = pv_mfma2<true>(ones, ones, pop[0][rb], pop[1][rb], psum[rb]);
                 } else {
                     pop[n][rb] = __builtin_bit_cast(s16x4, (u32x2){pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3])});
                 }
@@ -577,13 +593,112 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
         // ---- O^T += V^T P^T ----
         lds_fence();   // this step's V^T is in LDS
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < (PAIR ? 1 : NT); n++)
 #pragma unroll
             for (int dt = 0; dt < NDT; dt++) {
                 const s16x4 a = lds_tr16(myvt + n * 16 * VROW + (4 * kg + (r16 >> 2)) * VROW + dt * 16 + 4 * (r16 & 3));
+                if constexpr (PAIR) {
+                    const s16x4 c = lds_tr16(myvt + 16 * VROW + (4 * kg + (r16 >> 2)) * VROW + dt * 16 + 4 * (r16 & 3));
 #pragma unroll
-                for (int rb = 0; rb < ROWB; rb++) o[rb][dt] = pv_mfma<INT8>(a, pop[n][rb], o[rb][dt]);
+                    for (int rb = 0; rb < ROWB; rb++) o[rb][dt] = pv_mfma2<INT8>(a, c, pop[0][rb], pop[1][rb], o[rb][dt]);
+                } else {
+#pragma unroll
+                    for (int rb = 0; rb < ROWB; rb++) o[rb][dt] = pv_mfma<INT8>(a, pop[n][rb], o[rb][dt]);
+                }
             }
+    };
+
+    // GROUP over a dense cache: two tiles at a time, the row blocks one behind the other, so that each block's softmax
+    // is on the vector ALUs between the products of the next block's scores and of the last one's with the values,
+    // which the matrix cores work on meanwhile. A wave's issue slots bound this loop, and the softmax is short in them:
+    // scores stay unscaled up to exp2(scale s - m), one fused multiply-add; a row that sees none of a tile has m = inf there; the sum of a row's weights is a product with ones,
+    // of the weights as rounded for the values. The next tiles are loaded as soon as
+    // their registers are free: values once these are in LDS, keys after the last product of scores.
+    auto compute_blocks = [&](const TileRegs<D, INT8> *t, int j, auto next_keys, auto next_values) {
+        lds_fence();   // the previous step's reads of myvt are done before overwriting
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int e = 0; e < KPL; e++)
+                *reinterpret_cast<u32x4 *>(myvt + n * 16 * VROW + (vg * KPL + e) * VROW + vc * 8) = t[n].v[e];
+        next_values();
+        // keys of each tile that the row sees: 16 or more all, 0 or fewer none
+        int rem[2][ROWB];
+        const int u0 = j * 16 >> p.pshift, u1 = min(j + 1, j1 - 1) * 16 >> p.pshift;
+        const int off0 = j * 16 & (p.P - 1), off1 = j + 1 < j1 ? (j + 1) * 16 & (p.P - 1) : p.P;   // past the end: none
+#pragma unroll
+        for (int rb = 0; rb < ROWB; rb++) rem[0][rb] = rem[1][rb] = lim[u0 * p.tg + qpos[rb]];
+        if (u1 != u0) {
+#pragma unroll
+            for (int rb = 0; rb < ROWB; rb++) rem[1][rb] = lim[u1 * p.tg + qpos[rb]];
+        }
+        f32x4 sc[3][2];
+        auto qk = [&](int rb) {
+#pragma unroll
+            for (int n = 0; n < 2; n++) sc[rb % 3][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NKB; i++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) sc[rb % 3][n] = qk_mfma<INT8>(t[n].k[i], qreg[rb][i], sc[rb % 3][n]);
+        };
+        s16x4 va[NDT][2], pop[2][2];
+        auto pv = [&](int rb) {
+            const s16x4 ones = __builtin_bit_cast(s16x4, (u32x2){0x3f803f80u, 0x3f803f80u});
+            psum[rb] = pv_mfma2<INT8>(ones, ones, pop[rb & 1][0], pop[rb & 1][1], psum[rb]);
+#pragma unroll
+            for (int dt = 0; dt < NDT; dt++) o[rb][dt] = pv_mfma2<INT8>(va[dt][0], va[dt][1], pop[rb & 1][0], pop[rb & 1][1], o[rb][dt]);
+        };
+        qk(0);
+        if (ROWB > 1) qk(1);
+        if (ROWB <= 2) next_keys();
+        bool part = false;
+#pragma unroll
+        for (int rb = 0; rb < ROWB; rb++) {
+            rem[0][rb] -= off0;
+            rem[1][rb] -= off1;
+            part |= (uint32_t)(rem[0][rb] - 1) < 15u || (uint32_t)(rem[1][rb] - 1) < 15u;
+        }
+        const bool some = __any(part);
+        lds_fence();   // this step's V^T is in LDS
+#pragma unroll
+        for (int dt = 0; dt < NDT; dt++)
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+                va[dt][n] = lds_tr16(myvt + n * 16 * VROW + (4 * kg + (r16 >> 2)) * VROW + dt * 16 + 4 * (r16 & 3));
+#pragma unroll
+        for (int rb = 0; rb < ROWB; rb++) {
+            if (rb > 0) pv(rb - 1);
+            f32x4 *x = sc[rb % 3];
+            if (some) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e >> 2][e & 3] = kg * 4 + (e & 3) < rem[e >> 2][rb] ? x[e >> 2][e & 3] : -INFINITY;
+            }
+            const bool see0 = rem[0][rb] > 0, see1 = rem[1][rb] > 0;
+            float t0 = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), x[0][2]), x[0][3]) * p.scale_log2;
+            float t1 = fmaxf(fmaxf(fmaxf(x[1][0], x[1][1]), x[1][2]), x[1][3]) * p.scale_log2;
+            const float mt = fmaxf(see0 ? t0 : -INFINITY, see1 ? t1 : -INFINITY);
+            if (__any(mt > m[rb] + RESCALE_LOG2)) {
+                float t2 = fmaxf(mt, __shfl_xor(mt, 16));
+                t2 = fmaxf(t2, __shfl_xor(t2, 32));
+                const float mn = fmaxf(m[rb], t2);
+                const float alpha = fast_exp2(m[rb] - mn);
+                m[rb] = mn;
+                psum[rb] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < NDT; dt++) o[rb][dt] *= alpha;
+            }
+            if (rb + 2 < ROWB) qk(rb + 2);
+            if (rb + 3 == ROWB) next_keys();
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const float mm = (n ? see1 : see0) ? m[rb] : INFINITY;
+                float pe[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) pe[e] = fast_exp2(__builtin_fmaf(x[n][e], p.scale_log2, -mm));
+                pop[rb & 1][n] = __builtin_bit_cast(s16x4, (u32x2){pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3])});
+            }
+        }
+        pv(ROWB - 1);
     };
 
     // Two register sets, ping-ponged: the next group of TPI tiles is loading while the
@@ -602,14 +717,42 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     };
     auto run = [&](const TileRegs<D, INT8> (&t)[TPI], int jj) {
         if constexpr (JT > 1) {
-            if (jj + JT <= j1) return compute(t, jj, std::integral_constant<int, JT>{});
+            if (jj + JT <= j1) return compute(t, jj, std::integral_constant<int, JT>{}, [] {});
         }
 #pragma unroll
         for (int e = 0; e < TPI; e++)
-            if (jj + e < j1) compute(t + e, jj + e, std::integral_constant<int, 1>{});
+            if (jj + e < j1) compute(t + e, jj + e, std::integral_constant<int, 1>{}, [] {});
     };
     int j = j0 + TPI * kw;
-    if (j < j1) {
+    if constexpr (GROUP && !INT8 && ROWB == 1) {   // few steps a wave: two sets, as below (one: 21.7 -> 22.3 us)
+        if (j < j1) {
+            ld(ta, j);
+            while (true) {
+                ld(tb, j + STRIDE);
+                compute_blocks(ta, j, [] {}, [] {});
+                j += STRIDE;
+                if (j >= j1) break;
+                ld(ta, j + STRIDE);
+                compute_blocks(tb, j, [] {}, [] {});
+                j += STRIDE;
+                if (j >= j1) break;
+            }
+        }
+    } else if constexpr (GROUP) {   // one set of registers, loaded again as soon as they are free
+        if (j < j1) ld(ta, j);
+        for (; j < j1; j += STRIDE) {
+            if constexpr (INT8) {
+                compute(ta, j, std::integral_constant<int, JT>{}, [&] { ld(ta, j + STRIDE); });
+            } else {
+                auto part = [&](auto which) {
+#pragma unroll
+                    for (int e = 0; e < TPI; e++)
+                        load_tile<D, INT8, PG16, decltype(which)::value>(ta[e], p, rm, min(j + STRIDE + e, j1 - 1), r16, kg, vg, vc, half_q, half_s);
+                };
+                compute_blocks(ta, j, [&] { part(std::integral_constant<int, 1>{}); }, [&] { part(std::integral_constant<int, 2>{}); });
+            }
+        }
+    } else if (j < j1) {
         ld(ta, j);
         while (true) {
             ld(tb, j + STRIDE);
@@ -634,60 +777,67 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     // ---- merge the waves' states (same rows, disjoint keys) through LDS slabs ----
 #pragma unroll
     for (int rb = 0; rb < ROWB; rb++) {
+        if (GROUP && !INT8) {
+            l[rb] = psum[rb][0];
+            continue;
+        }
         l[rb] += __shfl_xor(l[rb], 16);
         l[rb] += __shfl_xor(l[rb], 32);
     }
-    __syncthreads();   // every wave is done with its V tile
-#pragma unroll
-    for (int rb = 0; rb < ROWB; rb++) {
-        float *my = mslab + ((size_t)w * MP + rb * 16 + r16) * MROW;
-#pragma unroll
-        for (int dt = 0; dt < NDT; dt++)
-            *reinterpret_cast<f32x4 *>(my + dt * 16 + kg * 4) = o[rb][dt];
-        if (kg == 0) {
-            my[D] = m[rb];
-            my[D + 1] = l[rb];
-        }
-    }
-    __syncthreads();
     bool fine = true;   // GROUP: no value that is not finite has come in
-    for (int item = threadIdx.x; item < p.M * (D / 4); item += NW * 64) {
-        const int r = item / (D / 4), d4 = (item % (D / 4)) * 4;
-        const int rs = RS == 2 ? r / MP : 0, rr = r - rs * MP;   // row slice, row in slab
-        float mx = NEG_BIG;
 #pragma unroll
-        for (int wi = 0; wi < NKW; wi++) mx = fmaxf(mx, mslab[((size_t)(wi * RS + rs) * MP + rr) * MROW + D]);
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        float lsum = 0.0f;
+    for (int hb = 0; hb < ROWB; hb += HB) {
+        __syncthreads();   // every wave is done with its V tile
 #pragma unroll
-        for (int wi = 0; wi < NKW; wi++) {
-            const float *src = mslab + ((size_t)(wi * RS + rs) * MP + rr) * MROW;
-            const float wgt = fast_exp2(src[D] - mx);
-            lsum += src[D + 1] * wgt;
-            acc += *reinterpret_cast<const f32x4 *>(src + d4) * wgt;
-        }
-        if constexpr (GROUP && !INT8) {
-            fine &= fabsf(lsum) < INFINITY;
+        for (int rb = hb; rb < hb + HB; rb++) {
+            float *my = mslab + ((size_t)w * HP + (rb - hb) * 16 + r16) * MROW;
 #pragma unroll
-            for (int e = 0; e < 4; e++) fine &= fabsf(acc[e]) < INFINITY;
-        }
-        if (nsp == 1) {
-            // One split: this group saw every key; normalize and write the output rows.
-            const int t = r / p.G, g = r - t * p.G;
-            if (t < nb && (!GROUP || (tok0 + t >= q0 && tok0 + t < q1))) {
-                const float inv = GROUP && lsum == 0.0f ? 0.0f : 1.0f / lsum;
-                uint16_t *o16 = p.out + ((size_t)(tok0 + t) * p.Hq + h * p.G + g) * D + d4;
-                *reinterpret_cast<u32x2 *>(o16) = (u32x2){pack_bf16x2(acc[0] * inv, acc[1] * inv),
-                                                          pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+            for (int dt = 0; dt < NDT; dt++)
+                *reinterpret_cast<f32x4 *>(my + dt * 16 + kg * 4) = o[rb][dt];
+            if (kg == 0) {
+                my[D] = m[rb];
+                my[D + 1] = l[rb];
             }
-        } else {
-            // The split's partial: part[unit][r][D + 2] = (acc, m, l).
-            float *dst = p.part + (unit * (size_t)p.M + r) * (D + 2);
+        }
+        __syncthreads();
+        for (int item = threadIdx.x; item < (HB < ROWB ? min(p.M - hb * 16, HP) : p.M) * (D / 4); item += NW * 64) {
+            const int rl = item / (D / 4), r = hb * 16 + rl, d4 = (item % (D / 4)) * 4;
+            const int rs = RS == 2 ? r / MP : 0, rr = rl - rs * MP;   // row slice, row in slab
+            float mx = NEG_BIG;
 #pragma unroll
-            for (int e = 0; e < 4; e++) dst[d4 + e] = acc[e];
-            if (d4 == 0) {
-                dst[D] = mx;
-                dst[D + 1] = lsum;
+            for (int wi = 0; wi < NKW; wi++) mx = fmaxf(mx, mslab[((size_t)(wi * RS + rs) * HP + rr) * MROW + D]);
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            float lsum = 0.0f;
+#pragma unroll
+            for (int wi = 0; wi < NKW; wi++) {
+                const float *src = mslab + ((size_t)(wi * RS + rs) * HP + rr) * MROW;
+                const float wgt = fast_exp2(src[D] - mx);
+                lsum += src[D + 1] * wgt;
+                acc += *reinterpret_cast<const f32x4 *>(src + d4) * wgt;
+            }
+            if constexpr (GROUP && !INT8) {
+                fine &= fabsf(lsum) < INFINITY;
+#pragma unroll
+                for (int e = 0; e < 4; e++) fine &= fabsf(acc[e]) < INFINITY;
+            }
+            if (nsp == 1) {
+                // One split: this group saw every key; normalize and write the output rows.
+                const int t = r / p.G, g = r - t * p.G;
+                if (t < nb && (!GROUP || (tok0 + t >= q0 && tok0 + t < q1))) {
+                    const float inv = GROUP && lsum == 0.0f ? 0.0f : 1.0f / lsum;
+                    uint16_t *o16 = p.out + ((size_t)(tok0 + t) * p.Hq + h * p.G + g) * D + d4;
+                    *reinterpret_cast<u32x2 *>(o16) = (u32x2){pack_bf16x2(acc[0] * inv, acc[1] * inv),
+                                                              pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+                }
+            } else {
+                // The split's partial: part[unit][r][D + 2] = (acc, m, l).
+                float *dst = p.part + (unit * (size_t)p.M + r) * (D + 2);
+#pragma unroll
+                for (int e = 0; e < 4; e++) dst[d4 + e] = acc[e];
+                if (d4 == 0) {
+                    dst[D] = mx;
+                    dst[D + 1] = lsum;
+                }
             }
         }
     }

@@ -8,7 +8,7 @@
 // Steps of several tokens a sequence (max_query_len > 1) take neighbouring tokens in groups: their tables
 // are joined into one list in LDS, and a page that several of them keep is read and multiplied once for
 // all their rows (GROUP in pa_decode.hpp). Token by token such a step is bound by the L2's rate (512
-// tokens of 2048 keys and 8 KV heads: 4.3 GB in 300 us).
+// tokens of 2048 keys and 8 KV heads: 4.3 GB in 300 us; 64 us in groups of 16).
 //
 // Pairs take consecutive work-groups with the KV heads innermost: with 8 KV heads (a multiple of
 // the 8 XCDs in general) all tokens of a KV head run on one XCD, and the pages that the tokens of
@@ -102,11 +102,23 @@ void launch_sparse_d(const DecodeParams &p, bool int8, unsigned grid, hipStream_
     else pg16 ? launch_sparse_p<D, false, true>(p, grid, s) : launch_sparse_p<D, false, false>(p, grid, s);
 }
 
-template <int D, bool INT8>
-void launch_group_d(const DecodeParams &p, unsigned grid, hipStream_t s) {
+template <int D, bool INT8, int ROWB>
+int launch_group_r(const DecodeParams &p, unsigned grid, hipStream_t s) {
     const size_t lds = (size_t)p.tg * p.tg * p.bt_stride * sizeof(uint16_t);
-    if (p.M <= 16) decode_kernel<D, 1, INT8, true, 4, 1, false, true, true><<<grid, 256, lds, s>>>(p);
-    else decode_kernel<D, 2, INT8, true, 4, 1, false, true, true><<<grid, 256, lds, s>>>(p);
+    auto kernel = decode_kernel<D, ROWB, INT8, true, 4, 1, false, true, true>;
+    if (lds > (32u << 10) &&
+        hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+        return TI_ERR_LAUNCH;
+    kernel<<<grid, 256, lds, s>>>(p);
+    return TI_OK;
+}
+
+template <int D, bool INT8>
+int launch_group_d(const DecodeParams &p, unsigned grid, hipStream_t s) {
+    if (p.M <= 16) return launch_group_r<D, INT8, 1>(p, grid, s);
+    if constexpr (!INT8)
+        if (p.M > 32) return launch_group_r<D, INT8, 4>(p, grid, s);
+    return launch_group_r<D, INT8, 2>(p, grid, s);
 }
 
 }  // namespace
@@ -114,10 +126,12 @@ void launch_group_d(const DecodeParams &p, unsigned grid, hipStream_t s) {
 // Tokens worked on together, and splits of their keys.
 // Groups: bf16 steps of several tokens a sequence over pages of whole 16-key tiles, as many tokens as fill 16
 // query rows. 32 rows read a page for twice the tokens at half the work-groups, and pay once 16 would give
-// 256 work-groups (8 steps of 16 tokens, 4096 keys each: 65.7 -> 50.3 us; 512 tokens 126 -> 74; below it
-// one step of 16 18.5 against 19.0-21.4), INT8 caches 512 (8 x 16 39.6 us against 46.6; 512 tokens 126 ->
-// 101). Their tables are joined from at most GROUP_PAGES entries, 512 for 32 rows, whose LDS two work-groups
-// of a CU share.
+// 256 work-groups (tables of 32 pages of 64 keys: 8 steps of 16 tokens 45 -> 36 us, 256 tokens 72 -> 43, 512 tokens
+// 136 -> 80; below it one step of 16 18.5 against 19.0-21.4), INT8 caches 512 (256 tokens 57.6 and 57.3, 512
+// tokens 104 -> 89). 64 rows, dense caches only, are one work-group a CU and pay once 32 would give 512 of them
+// (512 tokens 80 -> 64 us, 1024 161 -> 127; 400 tokens 82 and 85, 256 43 and 46), with heads of 64, where two
+// work-groups of 32 rows share a CU, 1024 (1024 tokens 82 -> 66; 512 42 and 50). Their tables are joined from at
+// most GROUP_PAGES entries, 512 for 32 rows, whose LDS two work-groups of a CU share.
 // Splits: while there are fewer work-groups than CUs (twice as many for joined INT8 tables: 8 x 16 46.7 ->
 // 39.6 us, one step of 8 18.5 -> 16.9), at most 16 and at least four 16-key tiles of a full table each (one
 // per wave).
@@ -129,11 +143,13 @@ ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cac
     const bool f32 = a->dtype == TI_F32;
     if (a->max_query_len > 1 && P >= 16 && P <= 32768 && (P & (P - 1)) == 0 && G <= 16 && (!f32 || ti_sparse_f32_mfma(a, c))) {
         auto tokens = [&](int rows, int entries) {
-            return max(1, min(min(rows / G, a->max_query_len), entries / min(a->table_width, entries + 1)));
+            return max(1, min(min(min(rows / G, 32), a->max_query_len), entries / min(a->table_width, entries + 1)));
         };
         pl.tg = tokens(16, GROUP_PAGES);
         const int wide = tokens(32, GROUP_PAGES / 2);
         if (!f32 && wide > pl.tg && pairs(pl.tg) >= (int8 ? 512 : 256)) pl.tg = wide;
+        const int wider = tokens(64, GROUP_PAGES);
+        if (!f32 && !int8 && wider > pl.tg && pairs(pl.tg) >= (c->head_dim == 128 ? 512 : 1024)) pl.tg = wider;
     }
     const long long tiles = ((long long)a->table_width * P + 15) / 16, target = f32 || (int8 && pl.tg > 1) ? 512 : 256;
     while (pl.splits < (f32 ? 32 : 16) && pairs(pl.tg) * pl.splits < target && tiles >= 8 * pl.splits) pl.splits <<= 1;
@@ -182,8 +198,10 @@ int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_ca
     } else {
         const bool int8 = c->kind == TI_KV_INT8;
         if (pl.tg > 1) {
-            if (c->head_dim == 128) int8 ? launch_group_d<128, true>(p, grid, s) : launch_group_d<128, false>(p, grid, s);
-            else int8 ? launch_group_d<64, true>(p, grid, s) : launch_group_d<64, false>(p, grid, s);
+            int r;
+            if (c->head_dim == 128) r = int8 ? launch_group_d<128, true>(p, grid, s) : launch_group_d<128, false>(p, grid, s);
+            else r = int8 ? launch_group_d<64, true>(p, grid, s) : launch_group_d<64, false>(p, grid, s);
+            if (r != TI_OK) return r;
         } else if (c->head_dim == 128) launch_sparse_d<128>(p, int8, grid, s);
         else launch_sparse_d<64>(p, int8, grid, s);
     }
