@@ -2,9 +2,11 @@
  * tileinfer_hip.h — C ABI of libtileinfer_hip.so, the MI355X (gfx950) paged
  * flash-attention path of TileInfer.jl.
  *
- * Every entry point replaces one method of the reference's op interface
- * (src/ops/interface.jl) for its TileBackend kernels; each declaration cites the
- * reference function it stands in for. All pointers are device pointers unless noted;
+ * The entry points of paged attention and the cache replace one method each of the reference's
+ * op interface (src/ops/interface.jl) for its TileBackend kernels; each declaration cites the
+ * reference function it stands in for. Page bounds, page selection, attention over selected pages
+ * and draft verification (last in this file) have no counterpart there: they work on the same
+ * caches, block tables and steps. All pointers are device pointers unless noted;
  * calls enqueue work on `stream` and return without synchronizing. The library never
  * allocates device memory: the caller owns pools, inputs, outputs and the workspace.
  * Errors are returned as ti_status codes, never thrown; argument checks run on the host
@@ -244,7 +246,8 @@ typedef struct {
  * scale times smoothing, rounded to float after each product. A page with a key that is not finite
  * gets bounds 127 and -127 and an infinite scale, and is kept by every selection that reaches
  * its score. Pages whose id lies outside the pool, or past the block-table row, are skipped. Two
- * sequences of a call that write into one page are not supported: its bounds are one of the two's.
+ * sequences of a call that write into one page, or two entries of a block-table row that name one,
+ * are not supported: the page's bounds are one of the two's.
  * head_dim 64 or 128. dtype: of dense pools.
  */
 int ti_update_key_bounds(int dtype, const ti_kv_cache *cache, const ti_key_bounds *bounds,
