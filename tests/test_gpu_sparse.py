@@ -692,6 +692,30 @@ def test_attend_many_rows_with_values_that_are_not_finite(gpu, value, where):
     assert torch.equal(torch.isfinite(got), torch.isfinite(alone))
 
 
+def test_attend_captured_with_much_lds(gpu):
+    """Groups of 32 tokens whose joined tables need 64 KB of LDS beside the tiles', recorded in a graph and replayed."""
+    rows, heads, width = 36, 256, 32
+    c = Cache("bf16", 64, heads, 16, [(width + 20) * 16], seed=33)
+    torch.manual_seed(33)
+    q = torch.randn((rows, heads * 2, 64), device="cuda", dtype=torch.bfloat16)
+    tables, lengths = shared(c, rows, width, seed=33)
+    out, ws = torch.zeros_like(q), ti.sparse_attention_workspace(BE, q, c.k, tables, rows)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ti.sparse_attention_(BE, out, ws, q, c.k, c.v, tables, lengths, 0.125, None, rows)
+    size = c.v.abs().max().item()
+    for i in range(3):
+        q.normal_()
+        lengths.sub_(3)
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.125, None, rows))
+        # token by token: weights rounded to bf16 (2^-8 each, their sum too) and the output (2^-8), on either side
+        alone = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.125)
+        assert (got.float() - alone.float()).abs().max().item() <= 2 * 3 * 2.0 ** -8 * size
+
+
 @pytest.mark.parametrize("n", [1, 4])
 def test_offsets_past_32_bits(gpu, n):
     """Pools of more than 2^31 elements: pages at their end, through bounds, selection and attention."""

@@ -51,21 +51,28 @@ struct GroupLds {
 template <int NT, typename Params>
 __device__ __forceinline__ int group_pages(const Params &p, GroupLds &g, uint16_t *lim, int *red, int tok0, int h, int q0, int q1) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, K = p.bt_stride, TG = p.tg, entries = TG * K;
+    constexpr int EACH = GROUP_PAGES / NT;
+    int id[EACH], slot[EACH], keys[EACH];
+    // both loads of an entry at once, in front of the LDS's clearing
+#pragma unroll
+    for (int n = 0; n < EACH; n++) {
+        const int x = n * NT + tid, a = x / TG, tok = tok0 + x - a * TG;
+        keys[n] = id[n] = 0;
+        if (x < entries && tok < p.total) {
+            keys[n] = p.lengths[tok * p.Hk + h];
+            id[n] = p.bt[((size_t)tok * p.Hk + h) * K + a];
+        }
+    }
     for (int i = tid; i < GROUP_SLOTS; i += NT) g.slot.id[i] = -1, g.slot.first[i] = 0x7fffffff, g.slot.seen[i] = 0;
     for (int i = tid; i < entries * TG; i += NT) lim[i] = 0;
     if (tid == 0) red[0] = 0;
     __syncthreads();
-    constexpr int EACH = GROUP_PAGES / NT;
-    int id[EACH], slot[EACH], keys[EACH];
 #pragma unroll
     for (int n = 0; n < EACH; n++) {
         const int x = n * NT + tid, a = x / TG, tok = tok0 + x - a * TG;
-        keys[n] = 0;
-        if (x < entries && tok >= q0 && tok < q1) {
-            const int len = min(p.lengths[tok * p.Hk + h], K * p.P);
-            keys[n] = min(len - a * p.P, p.P);
-            if (keys[n] > 0) id[n] = clamp_page(p.bt[((size_t)tok * p.Hk + h) * K + a], p.num_pages);
-        }
+        const int len = min(keys[n], K * p.P);
+        keys[n] = x < entries && tok >= q0 && tok < q1 ? min(len - a * p.P, p.P) : 0;
+        id[n] = clamp_page(id[n], p.num_pages);
     }
 #pragma unroll
     for (int n = 0; n < EACH; n++) {
