@@ -242,6 +242,7 @@ template <int NG> __device__ __forceinline__ Limit bisect(const Seen &s, const u
     low = ~wave_umax(~low) + 1;
     int from = s.c1 - s.c0, above = 0;   // keys >= low: at least need; keys > top: fewer
     bool closed = false;
+    int step = 1;
     while (low < top) {
         if (!closed && from - above <= 4) {
             closed = true;
@@ -257,7 +258,10 @@ template <int NG> __device__ __forceinline__ Limit bisect(const Seen &s, const u
             low = ~wave_umax(~least);
             continue;
         }
-        const uint32_t d = top - low, mid = low + d / 2 + (d & 1);
+        // where the count would be right if the keys lay evenly; every fourth step halves
+        const uint32_t d = top - low;
+        const float part = step++ & 3 ? (float)(from - s.need) * __builtin_amdgcn_rcpf((float)(from - above)) : 0.5f;
+        const uint32_t mid = low + min(max((uint32_t)((float)d * part), 1u), d);
         int c = 0;
 #pragma unroll
         for (int n = 0; n < NG; n++)
@@ -384,33 +388,60 @@ __device__ __forceinline__ Limit find_limit_together(const Seen &s, uint32_t *ke
     return {low, need};
 }
 
-// Writes one token's kept pages in order, zeros behind them, and its number of keys; NW waves share the
-// pages (all of the work-group where NW > 1: red holds 2 NW words of LDS).
-template <int NW>
-__device__ __forceinline__ void write_pages(const SelectParams &p, const Seen &s, const Limit &l, const uint32_t *keys, size_t pair,
-                                            const int32_t *bt, int lane, int w, int *red) {
-    const int steps = (s.seen + 63) >> 6, part = NW == 1 ? steps : (steps + NW - 1) / NW;
-    const int i0 = min(w * part, steps) * 64, i1 = min((w + 1) * part, steps) * 64;
+// Writes a token's number of keys.
+__device__ __forceinline__ void write_length(const SelectParams &p, const Seen &s, size_t pair) {
+    const long long n = (long long)(s.kept - 1) * p.P + min(s.last + 1 - (s.seen - 1) * p.P, p.P);
+    p.lengths[pair] = (int)n;
+}
+
+// Writes one token's kept pages in order, zeros behind them, and its number of keys, by one wave. The kept
+// pages' places take the place of keys that have been read, so that one load of up to 64 ids is waited for and not
+// one for each 64 pages.
+__device__ __forceinline__ void write_pages(const SelectParams &p, const Seen &s, const Limit &l, uint32_t *keys, size_t pair,
+                                            const int32_t *bt, int lane) {
+    const unsigned long long below = (1ull << lane) - 1;
     int base = 0, eq = 0;
+    uint32_t next = keys[lane];
+    for (int i0 = 0; i0 < s.seen; i0 += 64) {
+        const uint32_t k = next;
+        const int i = i0 + lane;
+        next = keys[min(i + 64, s.seen - 1)];
+        const bool cand = i >= s.c0 && i < s.c1;
+        const bool sure = i < s.seen && (!cand || k > l.limit), even = cand && k == l.limit;
+        const unsigned long long ms = __ballot(sure), me = __ballot(even);
+        // pages kept before this one: the sure ones, and the equal ones while there was room
+        const int q = eq + __popcll(me & below), at = base + __popcll(ms & below) + min(q, l.ties);
+        if ((sure || (even && q < l.ties)) && at < s.kept) keys[at] = i;
+        base += __popcll(ms);
+        eq += __popcll(me);
+    }
+    int32_t *out = p.tables + pair * p.keep;
+    for (int i = lane; i < p.keep; i += 64) out[i] = i < s.kept ? bt[keys[i]] : 0;
+    if (lane == 0) write_length(p, s, pair);
+}
+
+// The same by the NW waves of a work-group, which share the pages; red: 2 NW words of LDS.
+template <int NW>
+__device__ __forceinline__ void write_pages_together(const SelectParams &p, const Seen &s, const Limit &l, const uint32_t *keys, size_t pair,
+                                                     const int32_t *bt, int lane, int w, int *red) {
+    const int steps = (s.seen + 63) >> 6, part = (steps + NW - 1) / NW;
+    const int i0 = min(w * part, steps) * 64, i1 = min((w + 1) * part, steps) * 64;
     auto page = [&](int i, bool &sure, bool &even) {
         const uint32_t k = keys[i];
         const bool cand = i >= s.c0 && i < s.c1;
         sure = i < s.seen && (!cand || k > l.limit);
         even = cand && k == l.limit;
     };
-    if constexpr (NW > 1) {
-        int ns = 0, ne = 0;
-        for (int i = i0; i < i1; i += 64) {
-            bool sure, even;
-            page(i + lane, sure, even);
-            ns += __popcll(__ballot(sure));
-            ne += __popcll(__ballot(even));
-        }
-        if (lane == 0) red[w] = ns, red[NW + w] = ne;
-        __syncthreads();
-        base = wave_total(lane < w ? red[lane] : 0);
-        eq = wave_total(lane < w ? red[NW + lane] : 0);
+    int ns = 0, ne = 0;
+    for (int i = i0; i < i1; i += 64) {
+        bool sure, even;
+        page(i + lane, sure, even);
+        ns += __popcll(__ballot(sure));
+        ne += __popcll(__ballot(even));
     }
+    if (lane == 0) red[w] = ns, red[NW + w] = ne;
+    __syncthreads();
+    int base = wave_total(lane < w ? red[lane] : 0), eq = wave_total(lane < w ? red[NW + lane] : 0);
     int32_t *out = p.tables + pair * p.keep;
     const unsigned long long below = (1ull << lane) - 1;
     int next = bt[min(i0 + lane, s.seen - 1)];
@@ -427,10 +458,7 @@ __device__ __forceinline__ void write_pages(const SelectParams &p, const Seen &s
         eq += __popcll(me);
     }
     for (int i = s.kept + w * 64 + lane; i < p.keep; i += NW * 64) out[i] = 0;
-    if (w == 0 && lane == 0) {
-        const long long n = (long long)(s.kept - 1) * p.P + min(s.last + 1 - (s.seen - 1) * p.P, p.P);
-        p.lengths[pair] = (int)n;
-    }
+    if (w == 0 && lane == 0) write_length(p, s, pair);
 }
 
 // The search as a call, for tiles of several blocks of rows, where it is the exception: in line it would take
@@ -448,7 +476,7 @@ __device__ __forceinline__ void keep_together(const SelectParams &p, const Seen 
     if constexpr (APART) l = find_limit_apart<W>(s, keys, span, lane, w, m);
     else l = find_limit_together<W>(s, keys, span, lane, w, m);
     __syncthreads();   // m is read
-    write_pages<W>(p, s, l, keys, pair, bt, lane, w, m.sum);
+    write_pages_together<W>(p, s, l, keys, pair, bt, lane, w, m.sum);
 }
 
 // Grid (Hk, token tiles, B), the keys of the tile's tokens in LDS.
@@ -483,7 +511,7 @@ __global__ void __launch_bounds__(W * 64) select_kernel(SelectParams p) {
             for (int t = wv; t < tokens; t += W) {
                 const Seen s(p, st, t0 + t);
                 const Limit l = find_limit(s, keys + t * p.pitch, span, lane);
-                write_pages<1>(p, s, l, keys + t * p.pitch, (size_t)(st.tok0 + t0 + t) * p.Hk + h, bt, lane, 0, nullptr);
+                write_pages(p, s, l, keys + t * p.pitch, (size_t)(st.tok0 + t0 + t) * p.Hk + h, bt, lane);
             }
         }
     }
