@@ -10,7 +10,7 @@
 //
 // Scores become 32-bit keys in the scores' order, 0 for pages that are not up for choice (those kept
 // anyway, and those past the last visible one). The key of the last page kept by score is found by counting keys
-// in parts of their range: in halves by one wave where a work-group has a token for each, in as many parts as
+// in parts of their range: in two by one wave where a work-group has a token for each, in as many parts as
 // it has threads where it has one token. Then one pass over the pages in order writes the kept ones.
 //
 // Two forms. select_kernel holds a token tile's keys in LDS and does both steps in one launch.
@@ -223,10 +223,11 @@ struct Limit {
     uint32_t limit;
     int ties;
 };
-// The search by one wave that holds all keys, by halves between the smallest and the largest: a step takes
-// 0.2 us for 512 keys and 0.4 for 2048, and 11 are usual. Where few keys are left between the ends, these
-// close in on them: equal keys end the search then and not after all 24 halvings of their digits.
-template <int NG> __device__ __forceinline__ Limit bisect(const Seen &s, const uint32_t *keys, int span, int lane) {
+// The search by one wave that holds all keys, between the smallest and the largest: a step takes 0.2 us for 512
+// keys and 0.4 for 2048, so the next one is where the count would be right if the keys lay evenly (512 tokens on
+// 64k keys 31.0 us by halves only, 29.3 so). Where few keys are left between the ends, these close in on them:
+// equal keys end the search then and not after all 24 halvings of their digits.
+template <int NG> __device__ __forceinline__ Limit narrow(const Seen &s, const uint32_t *keys, int span, int lane) {
     u32x4 k[NG];
     uint32_t top = 0, low = 0xffffffffu;
 #pragma unroll
@@ -293,9 +294,9 @@ __device__ __forceinline__ Limit find_limit(const Seen &s, uint32_t *keys, int s
     bool found;
     const Limit l = begin_search(s, keys, span, lane, 64, &found);
     if (found) return l;
-    if (span <= 2 * ROUND) return bisect<2>(s, keys, span, lane);
-    if (span <= 5 * ROUND) return bisect<5>(s, keys, span, lane);
-    return bisect<8>(s, keys, span, lane);
+    if (span <= 2 * ROUND) return narrow<2>(s, keys, span, lane);
+    if (span <= 5 * ROUND) return narrow<5>(s, keys, span, lane);
+    return narrow<8>(s, keys, span, lane);
 }
 
 // The words of LDS that the waves of a work-group search with.
@@ -462,7 +463,7 @@ __device__ __forceinline__ void write_pages_together(const SelectParams &p, cons
 }
 
 // The search as a call, for tiles of several blocks of rows, where it is the exception: in line it would take
-// registers from the scores' loop, which spills then (31.3 and 32.9 us for 512 tokens on 64k keys).
+// registers from the scores' loop, which spills then (512 tokens on 64k keys 31.3 us, in line 32.9).
 template <int W>
 __device__ __attribute__((noinline)) Limit find_limit_apart(const Seen &s, uint32_t *keys, int span, int lane, int w, SearchLds<W> &m) {
     return find_limit_together<W>(s, keys, span, lane, w, m);
@@ -617,7 +618,7 @@ int launch(SelectParams p, int num_seqs, hipStream_t s) {
 
 // Query rows per tile: 64 (32 where a token's heads do not fill a lane's four rows or go past them: 64 spill
 // there) where the steps' tokens fill them and the launch still has work-groups for every CU (bounds are then
-// read once for several blocks of rows: 512 tokens on 64k keys 31 us, 91 with 16), else 16 (128 tokens 25 and 30).
+// read once for several blocks of rows: 512 tokens on 64k keys 31 us, 91 with 16 rows), else 16 (128 tokens 25 and 30).
 template <int D, int GP>
 int launch_rows(const SelectParams &p, int num_seqs, hipStream_t s) {
     constexpr int RT = GP == 4 || GP == 16 ? 4 : 2, TT = Tile<GP, RT, false>::TT;
