@@ -131,7 +131,9 @@ int launch_group_d(const DecodeParams &p, unsigned grid, hipStream_t s) {
 // tokens 104 -> 89). 64 rows, dense caches only, are one work-group a CU and pay once 32 would give 512 of them
 // (512 tokens 80 -> 64 us, 1024 161 -> 127; 400 tokens 82 and 85, 256 43 and 46), with heads of 64, where two
 // work-groups of 32 rows share a CU, 1024 (1024 tokens 82 -> 66; 512 42 and 50). Their tables are joined from at
-// most GROUP_PAGES entries, 512 for 32 rows, whose LDS two work-groups of a CU share.
+// most GROUP_PAGES entries; 512 for 32 rows of INT8 caches or heads of 64, two work-groups of which share a CU and its
+// LDS (tables of 128 pages of 16 keys, 8 steps of 16 tokens: INT8 35 us, 41 with 1024 entries, dense 42 and 37;
+// 128 tokens with heads of 64 22 and 25).
 // Splits: while there are fewer work-groups than CUs (twice as many for joined INT8 tables: 8 x 16 46.7 ->
 // 39.6 us, one step of 8 18.5 -> 16.9), at most 16 and at least four 16-key tiles of a full table each (one
 // per wave).
@@ -146,7 +148,7 @@ ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cac
             return max(1, min(min(min(rows / G, 32), a->max_query_len), entries / min(a->table_width, entries + 1)));
         };
         pl.tg = tokens(16, GROUP_PAGES);
-        const int wide = tokens(32, GROUP_PAGES / 2);
+        const int wide = tokens(32, int8 || c->head_dim == 64 ? GROUP_PAGES / 2 : GROUP_PAGES);
         if (!f32 && wide > pl.tg && pairs(pl.tg) >= (int8 ? 512 : 256)) pl.tg = wide;
         const int wider = tokens(64, GROUP_PAGES);
         if (!f32 && !int8 && wider > pl.tg && pairs(pl.tg) >= (c->head_dim == 128 ? 512 : 1024)) pl.tg = wider;
