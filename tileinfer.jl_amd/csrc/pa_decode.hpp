@@ -211,7 +211,7 @@ struct RowMap {
     __device__ __forceinline__ int last(int pos) const { return len - 1 - pos; }   // last key of the tile at pos
 };
 
-// PART: 1 the keys, 2 the values, 3 both (1 and 2 for dense caches and whole tiles).
+// PART: 1 the keys, 2 the values, 3 both (1 and 2 for whole tiles).
 template <int D, bool INT8, bool PG16, int PART = 3, typename Map>
 __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodeParams &p,
                                           const Map &rm, int j, int r16, int kg, int vg,
@@ -246,19 +246,19 @@ __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodePara
             // 32 with 8-B pieces: 1 % faster); score MFMA 2 u + c takes bytes 64 u + 16 kg +
             // 8 c, and the queries' head dimension is gathered in the same order
 #pragma unroll
-            for (int u = 0; u < NKB / 2; u++) {
+            for (int u = 0; u < (PART & 1 ? NKB / 2 : 0); u++) {
                 const u32x4 r = *reinterpret_cast<const u32x4 *>(kb + (kr * D + u * 64 + kg * 16));
                 t.k[2 * u] = (u32x4){r[0], r[1], 0u, 0u};
                 t.k[2 * u + 1] = (u32x4){r[2], r[3], 0u, 0u};
             }
 #pragma unroll
-            for (int e = 0; e < KPL; e++) {
+            for (int e = 0; e < (PART & 2 ? KPL : 0); e++) {
                 const u32x2 r = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(vb + (vr[e] * D + vc * 8)));
                 t.v[e] = (u32x4){r[0], r[1], 0u, 0u};
             }
             const float *sb = p.ls + r0;
-            t.sk = sb[kr];
-            t.sv = sb[half_s + kr];
+            if (PART & 1) t.sk = sb[kr];
+            if (PART & 2) t.sv = sb[half_s + kr];
         }
         return;
     }
@@ -293,9 +293,10 @@ __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodePara
 // SPARSE: every (token, KV head) pair has a table of pages and a length of its own (pa_sparse.hip);
 // a pair is a sequence of one token whose last key is at lengths - 1, and a 1-D grid holds the
 // pairs' splits, KV heads innermost. GROUP (SPARSE, whole tiles): p.tg neighbouring tokens' pairs at a time
-// over the joined list of their pages, packed rows g + G t of the group.
+// over the joined list of their pages, packed rows g + G t of the group. (32 rows of INT8 caches take 8 registers
+// too many for two waves a SIMD by themselves, 112 and 72 us for 512 tokens.)
 template <int D, int ROWB, bool INT8, bool PG16, int NW, int RS, bool JOINT = false, bool SPARSE = false, bool GROUP = false>
-__global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
+__global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) decode_kernel(DecodeParams p) {
     constexpr int NKB = D / 32;          // 32-wide head-dim blocks (QK MFMAs per tile)
     constexpr int NDT = D / 16;          // 16-wide head-dim tiles (PV MFMAs per tile)
     constexpr int CPR = D / 8;           // 8-element chunks per V row
@@ -465,9 +466,8 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     const int vc = lane % CPR, vg = lane / CPR;   // V load: chunk, key group
 
     // NT tiles j .. j + NT - 1: their scores, one softmax over them, their values.
-    auto compute = [&](const TileRegs<D, INT8> *t, int j, auto count, auto next) {
+    auto compute = [&](const TileRegs<D, INT8> *t, int j, auto count) {
         constexpr int NT = decltype(count)::value;
-        constexpr bool PAIR = GROUP && NT == 2;   // the values of two tiles in one product of depth 32
         // ---- V rows -> row-major LDS tiles (INT8: biased fp16, exact) ----
         u32x4 vrows[NT][KPL];
 #pragma unroll
@@ -506,28 +506,12 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
                     svk[n][e] = __shfl(t[n].sv, kg * 4 + e);
                 }
         }
-        next();   // the tiles' registers are free
         // ---- online softmax + P^T operands ----
         // Lazy rescaling: m is a reference max that only moves when a step's max exceeds
         // it by more than RESCALE_LOG2 (then p <= 2^RESCALE_LOG2, safe in bf16 and fp32);
         // l and O always use the same reference, so the result is exact. INT8 moves m
         // with every larger max (p <= 1, so p times a value scale stays within fp16).
-        int seen[NT][ROWB], off[NT];   // GROUP: keys of the page that the row sees, the tile's first one
-        bool need_mask = (j + NT) * 16 - 1 > mask_from;
-        if constexpr (GROUP) {
-            bool whole = true;
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const int at = min(j + n, j1 - 1) * 16, u = at >> p.pshift;
-                off[n] = at & (p.P - 1);
-#pragma unroll
-                for (int rb = 0; rb < ROWB; rb++) {
-                    seen[n][rb] = j + n < j1 ? lim[u * p.tg + qpos[rb]] : 0;   // none of a pair's tile past the end
-                    whole &= off[n] + 16 <= seen[n][rb];
-                }
-            }
-            need_mask = !__all(whole);
-        }
+        const bool need_mask = (j + NT) * 16 - 1 > mask_from;
         s16x4 pop[NT][ROWB];
         float x[ROWB][4 * NT], mt[ROWB];
         bool grow = false;
@@ -539,9 +523,7 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
                 float v = sc[e >> 2][rb][e & 3];
                 if (INT8) v = (v - qcorr[rb]) * skk[e >> 2][e & 3] * qsl[rb];
                 else v *= p.scale_log2;
-                if constexpr (GROUP) {
-                    if (need_mask) v = off[e >> 2] + kg * 4 + (e & 3) < seen[e >> 2][rb] ? v : -INFINITY;
-                } else if (need_mask) {
+                if (need_mask) {
                     const int kp = (j + (e >> 2)) * 16 + kg * 4 + (e & 3);
                     v = (kp <= qpos[rb] && kp < len) ? v : -INFINITY;
                 }
@@ -573,8 +555,7 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
                 for (int e = 0; e < 4; e++) {
                     pe[e] = fast_exp2(x[rb][4 * n + e] - m[rb]);
                     ps += pe[e];
-                    if (INT8 && GROUP && need_mask) pe[e] = x[rb][4 * n + e] == -INFINITY ? 0.0f : pe[e] * svk[n][e];
-                    else if (INT8) pe[e] *= svk[n][e];
+                    if (INT8) pe[e] *= svk[n][e];
                 }
                 l[rb] += ps;
                 if (INT8) {
@@ -584,8 +565,7 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
                                                                    __builtin_bit_cast(uint32_t, h1)});
                     // the row's sum of these fp16 probabilities, for the values' bias
                     const s16x4 ones = __builtin_bit_cast(s16x4, (u32x2){0x3c003c00u, 0x3c003c00u});
-                    if constexpr (!PAIR) psum[rb] = pv_mfma<true>(ones, pop[n][rb], psum[rb]);
-                    else if (n == 1) psum[rb] = pv_mfma2<true>(ones, ones, pop[0][rb], pop[1][rb], psum[rb]);
+                    psum[rb] = pv_mfma<true>(ones, pop[n][rb], psum[rb]);
                 } else {
                     pop[n][rb] = __builtin_bit_cast(s16x4, (u32x2){pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3])});
                 }
@@ -593,22 +573,19 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
         // ---- O^T += V^T P^T ----
         lds_fence();   // this step's V^T is in LDS
 #pragma unroll
-        for (int n = 0; n < (PAIR ? 1 : NT); n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int dt = 0; dt < NDT; dt++) {
                 const s16x4 a = lds_tr16(myvt + n * 16 * VROW + (4 * kg + (r16 >> 2)) * VROW + dt * 16 + 4 * (r16 & 3));
-                if constexpr (PAIR) {
-                    const s16x4 c = lds_tr16(myvt + 16 * VROW + (4 * kg + (r16 >> 2)) * VROW + dt * 16 + 4 * (r16 & 3));
 #pragma unroll
-                    for (int rb = 0; rb < ROWB; rb++) o[rb][dt] = pv_mfma2<INT8>(a, c, pop[0][rb], pop[1][rb], o[rb][dt]);
-                } else {
-#pragma unroll
-                    for (int rb = 0; rb < ROWB; rb++) o[rb][dt] = pv_mfma<INT8>(a, pop[n][rb], o[rb][dt]);
-                }
+                for (int rb = 0; rb < ROWB; rb++) o[rb][dt] = pv_mfma<INT8>(a, pop[n][rb], o[rb][dt]);
             }
     };
 
-    // GROUP over a dense cache: two tiles at a time, the row blocks one behind the other, so that each block's softmax
+    bool tame = true;   // GROUP, INT8: see below
+#pragma unroll
+    for (int rb = 0; rb < ROWB; rb++) tame &= qsl[rb] <= 0x1p40f;
+    // GROUP: two tiles at a time, the row blocks one behind the other, so that each block's softmax
     // is on the vector ALUs between the products of the next block's scores and of the last one's with the values,
     // which the matrix cores work on meanwhile. A wave's issue slots bound this loop, and the softmax is short in them:
     // scores stay unscaled up to exp2(scale s - m), one fused multiply-add; a row that sees none of a tile has m = inf there; the sum of a row's weights is a product with ones,
@@ -620,7 +597,29 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int e = 0; e < KPL; e++)
-                *reinterpret_cast<u32x4 *>(myvt + n * 16 * VROW + (vg * KPL + e) * VROW + vc * 8) = t[n].v[e];
+                *reinterpret_cast<u32x4 *>(myvt + n * 16 * VROW + (vg * KPL + e) * VROW + vc * 8) =
+                    INT8 ? i8x8_to_f16b(t[n].v[e][0], t[n].v[e][1]) : t[n].v[e];
+        // INT8: scales of this lane's keys. One that is not finite, or so large that a score could overflow (raw
+        // scores are below 2^34), must not meet a row that does not see its key: such tiles are masked key by key
+        float skk[2][4], svk[2][4];
+        bool odd = false;
+        u32x4 kreg[2][NKB];
+        if constexpr (INT8) {
+            bool fine = tame;
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                fine &= fabsf(t[n].sk) <= 0x1p40f && fabsf(t[n].sv) < INFINITY;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    skk[n][e] = __shfl(t[n].sk, kg * 4 + e);
+                    svk[n][e] = __shfl(t[n].sv, kg * 4 + e);
+                }
+#pragma unroll
+                for (int i = 0; i < NKB; i++) kreg[n][i] = i8x8_to_f16b(t[n].k[i][0], t[n].k[i][1]);
+            }
+            odd = !__all(fine);
+            next_keys();
+        }
         next_values();
         // keys of each tile that the row sees: 16 or more all, 0 or fewer none
         int rem[2][ROWB];
@@ -639,18 +638,19 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
 #pragma unroll
             for (int i = 0; i < NKB; i++)
 #pragma unroll
-                for (int n = 0; n < 2; n++) sc[rb % 3][n] = qk_mfma<INT8>(t[n].k[i], qreg[rb][i], sc[rb % 3][n]);
+                for (int n = 0; n < 2; n++) sc[rb % 3][n] = qk_mfma<INT8>(INT8 ? kreg[n][i] : t[n].k[i], qreg[rb][i], sc[rb % 3][n]);
         };
         s16x4 va[NDT][2], pop[2][2];
         auto pv = [&](int rb) {
-            const s16x4 ones = __builtin_bit_cast(s16x4, (u32x2){0x3f803f80u, 0x3f803f80u});
+            constexpr uint32_t ONE = INT8 ? 0x3c003c00u : 0x3f803f80u;
+            const s16x4 ones = __builtin_bit_cast(s16x4, (u32x2){ONE, ONE});
             psum[rb] = pv_mfma2<INT8>(ones, ones, pop[rb & 1][0], pop[rb & 1][1], psum[rb]);
 #pragma unroll
             for (int dt = 0; dt < NDT; dt++) o[rb][dt] = pv_mfma2<INT8>(va[dt][0], va[dt][1], pop[rb & 1][0], pop[rb & 1][1], o[rb][dt]);
         };
         qk(0);
         if (ROWB > 1) qk(1);
-        if (ROWB <= 2) next_keys();
+        if (!INT8 && ROWB <= 2) next_keys();
         bool part = false;
 #pragma unroll
         for (int rb = 0; rb < ROWB; rb++) {
@@ -669,33 +669,52 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
         for (int rb = 0; rb < ROWB; rb++) {
             if (rb > 0) pv(rb - 1);
             f32x4 *x = sc[rb % 3];
-            if (some) {
+            if constexpr (INT8) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e >> 2][e & 3] = (x[e >> 2][e & 3] - qcorr[rb]) * skk[e >> 2][e & 3] * qsl[rb];
+            }
+            const float scale = INT8 ? 1.0f : p.scale_log2;   // INT8: scaled already
+            if (some || (INT8 && odd)) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) x[e >> 2][e & 3] = kg * 4 + (e & 3) < rem[e >> 2][rb] ? x[e >> 2][e & 3] : -INFINITY;
             }
             const bool see0 = rem[0][rb] > 0, see1 = rem[1][rb] > 0;
-            float t0 = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), x[0][2]), x[0][3]) * p.scale_log2;
-            float t1 = fmaxf(fmaxf(fmaxf(x[1][0], x[1][1]), x[1][2]), x[1][3]) * p.scale_log2;
+            float t0 = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), x[0][2]), x[0][3]) * scale;
+            float t1 = fmaxf(fmaxf(fmaxf(x[1][0], x[1][1]), x[1][2]), x[1][3]) * scale;
             const float mt = fmaxf(see0 ? t0 : -INFINITY, see1 ? t1 : -INFINITY);
-            if (__any(mt > m[rb] + RESCALE_LOG2)) {
+            if (__any(mt > m[rb] + (INT8 ? 0.0f : RESCALE_LOG2))) {
                 float t2 = fmaxf(mt, __shfl_xor(mt, 16));
                 t2 = fmaxf(t2, __shfl_xor(t2, 32));
                 const float mn = fmaxf(m[rb], t2);
                 const float alpha = fast_exp2(m[rb] - mn);
                 m[rb] = mn;
+                if (INT8) l[rb] *= alpha;
                 psum[rb] *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < NDT; dt++) o[rb][dt] *= alpha;
             }
             if (rb + 2 < ROWB) qk(rb + 2);
-            if (rb + 3 == ROWB) next_keys();
+            if (!INT8 && rb + 3 == ROWB) next_keys();
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 const float mm = (n ? see1 : see0) ? m[rb] : INFINITY;
                 float pe[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) pe[e] = fast_exp2(__builtin_fmaf(x[n][e], p.scale_log2, -mm));
-                pop[rb & 1][n] = __builtin_bit_cast(s16x4, (u32x2){pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3])});
+                for (int e = 0; e < 4; e++) pe[e] = fast_exp2(INT8 ? x[n][e] - mm : __builtin_fmaf(x[n][e], scale, -mm));
+                if constexpr (INT8) {
+                    l[rb] += (pe[0] + pe[1]) + (pe[2] + pe[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) pe[e] *= svk[n][e];
+                    if (odd) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) pe[e] = x[n][e] == -INFINITY ? 0.0f : pe[e];
+                    }
+                    const f16x2 h0 = __builtin_convertvector(((f32x2){pe[0], pe[1]}), f16x2);
+                    const f16x2 h1 = __builtin_convertvector(((f32x2){pe[2], pe[3]}), f16x2);
+                    pop[rb & 1][n] = __builtin_bit_cast(s16x4, (u32x2){__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1)});
+                } else {
+                    pop[rb & 1][n] = __builtin_bit_cast(s16x4, (u32x2){pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3])});
+                }
             }
         }
         pv(ROWB - 1);
@@ -717,11 +736,11 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     };
     auto run = [&](const TileRegs<D, INT8> (&t)[TPI], int jj) {
         if constexpr (JT > 1) {
-            if (jj + JT <= j1) return compute(t, jj, std::integral_constant<int, JT>{}, [] {});
+            if (jj + JT <= j1) return compute(t, jj, std::integral_constant<int, JT>{});
         }
 #pragma unroll
         for (int e = 0; e < TPI; e++)
-            if (jj + e < j1) compute(t + e, jj + e, std::integral_constant<int, 1>{}, [] {});
+            if (jj + e < j1) compute(t + e, jj + e, std::integral_constant<int, 1>{});
     };
     int j = j0 + TPI * kw;
     if constexpr (GROUP && !INT8 && ROWB == 1) {   // few steps a wave: two sets, as below (one: 21.7 -> 22.3 us)
@@ -741,16 +760,12 @@ __global__ void __launch_bounds__(NW * 64) decode_kernel(DecodeParams p) {
     } else if constexpr (GROUP) {   // one set of registers, loaded again as soon as they are free
         if (j < j1) ld(ta, j);
         for (; j < j1; j += STRIDE) {
-            if constexpr (INT8) {
-                compute(ta, j, std::integral_constant<int, JT>{}, [&] { ld(ta, j + STRIDE); });
-            } else {
-                auto part = [&](auto which) {
+            auto part = [&](auto which) {
 #pragma unroll
-                    for (int e = 0; e < TPI; e++)
-                        load_tile<D, INT8, PG16, decltype(which)::value>(ta[e], p, rm, min(j + STRIDE + e, j1 - 1), r16, kg, vg, vc, half_q, half_s);
-                };
-                compute_blocks(ta, j, [&] { part(std::integral_constant<int, 1>{}); }, [&] { part(std::integral_constant<int, 2>{}); });
-            }
+                for (int e = 0; e < TPI; e++)
+                    load_tile<D, INT8, PG16, decltype(which)::value>(ta[e], p, rm, min(j + STRIDE + e, j1 - 1), r16, kg, vg, vc, half_q, half_s);
+            };
+            compute_blocks(ta, j, [&] { part(std::integral_constant<int, 1>{}); }, [&] { part(std::integral_constant<int, 2>{}); });
         }
     } else if (j < j1) {
         ld(ta, j);

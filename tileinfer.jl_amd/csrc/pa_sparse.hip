@@ -127,8 +127,9 @@ int launch_group_d(const DecodeParams &p, unsigned grid, hipStream_t s) {
 // Groups: bf16 steps of several tokens a sequence over pages of whole 16-key tiles, as many tokens as fill 16
 // query rows. 32 rows read a page for twice the tokens at half the work-groups, and pay once 16 would give
 // 256 work-groups (tables of 32 pages of 64 keys: 8 steps of 16 tokens 45 -> 36 us, 256 tokens 72 -> 43, 512 tokens
-// 136 -> 80; below it one step of 16 18.5 against 19.0-21.4), INT8 caches 512 (256 tokens 57.6 and 57.3, 512
-// tokens 104 -> 89). 64 rows, dense caches only, are one work-group a CU and pay once 32 would give 512 of them
+// 136 -> 80; below it one step of 16 18.5 against 19.0-21.4), INT8 caches 512 (256 tokens 51 -> 48, 512
+// tokens 99 -> 72). 64 rows, dense caches only (INT8: 72 -> 118 us for 512
+// tokens), are one work-group a CU and pay once 32 would give 512 of them
 // (512 tokens 80 -> 64 us, 1024 161 -> 127; 400 tokens 82 and 85, 256 43 and 46), with heads of 64, where two
 // work-groups of 32 rows share a CU, 1024 (1024 tokens 82 -> 66; 512 42 and 50). Their tables are joined from at
 // most GROUP_PAGES entries; 512 for 32 rows of INT8 caches or heads of 64, two work-groups of which share a CU and its
