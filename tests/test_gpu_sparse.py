@@ -716,6 +716,31 @@ def test_attend_captured_with_much_lds(gpu):
         assert (got.float() - alone.float()).abs().max().item() <= 2 * 3 * 2.0 ** -8 * size
 
 
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf, 1e38])
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("rows,heads", [(6, 2), (300, 8)])
+def test_attend_int8_scales_that_are_not_finite_stay_with_their_tokens(gpu, value, half, rows, heads):
+    """INT8: a key's or value's scale that is not finite, or so large that scores overflow, in a page that some
+    tokens of a step keep and behind the last key of others: the same operations on the same numbers for the rest."""
+    c = Cache("int8", 128, heads, 16, [60 * 16], seed=34)
+    torch.manual_seed(34)
+    q = torch.randn((rows, heads * 4, 128), device="cuda", dtype=torch.bfloat16)
+    tables, lengths = shared(c, rows, 9, seed=34)
+    lengths[:] = 8 * 16 + 9
+    bad, last = tables[1, 0, 2].item(), tables[3, 1, 8].item()
+    want = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09, None, rows)
+    scales = c.k.layer_scale
+    scales[half, bad - 1, :, 5] = value
+    scales[half, last - 1, :, 12] = value              # seen where this page is not the last one
+    got = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09, None, rows)
+    end = torch.arange(9, device="cuda") == 8
+    touched = ((tables == bad) | ((tables == last) & ~end)).any(2).repeat_interleave(4, 1)
+    assert touched.any() and not touched.all()
+    assert torch.equal(got[~touched], want[~touched])
+    alone = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09)
+    assert torch.equal(torch.isfinite(got[~touched]), torch.isfinite(alone[~touched]))
+
+
 @pytest.mark.parametrize("n", [1, 4])
 def test_offsets_past_32_bits(gpu, n):
     """Pools of more than 2^31 elements: pages at their end, through bounds, selection and attention."""
