@@ -133,11 +133,11 @@ int launch_group_d(const DecodeParams &p, unsigned grid, hipStream_t s) {
 // (512 tokens 80 -> 64 us, 1024 161 -> 127; 400 tokens 82 and 85, 256 43 and 46), with heads of 64, where two
 // work-groups of 32 rows share a CU, 1024 (1024 tokens 82 -> 66; 512 42 and 50). Their tables are joined from at
 // most GROUP_PAGES entries; 512 for 32 rows of INT8 caches or heads of 64, two work-groups of which share a CU and its
-// LDS (tables of 128 pages of 16 keys, 8 steps of 16 tokens: INT8 35 us, 41 with 1024 entries, dense 42 and 37;
-// 128 tokens with heads of 64 22 and 25).
-// Splits: while there are fewer work-groups than CUs (twice as many for joined INT8 tables: 8 x 16 46.7 ->
-// 39.6 us, one step of 8 18.5 -> 16.9), at most 16 and at least four 16-key tiles of a full table each (one
-// per wave).
+// LDS (tables of 128 pages of 16 keys: INT8, 16 steps of 16 tokens 53 us, 74 with 1024 entries; dense, 8 steps of 16
+// tokens 42 and 37; 128 tokens with heads of 64 22 and 25).
+// Splits: while there are fewer work-groups than CUs (twice as many for joined INT8 tables: 8 steps of 16 tokens over
+// 128 pages of 16 keys 35.2 -> 32.6 us, 4 over 64 pages of 64 38.5 -> 31.2; dense 39.0 -> 43.5), at most 16 and at
+// least four 16-key tiles of a full table each (one per wave).
 ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
     const int G = a->q_heads / c->kv_heads, P = c->page_size;
     const bool int8 = c->kind == TI_KV_INT8;
