@@ -585,12 +585,13 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
     bool tame = true;   // GROUP, INT8: see below
 #pragma unroll
     for (int rb = 0; rb < ROWB; rb++) tame &= qsl[rb] <= 0x1p40f;
-    // GROUP: two tiles at a time, the row blocks one behind the other, so that each block's softmax
-    // is on the vector ALUs between the products of the next block's scores and of the last one's with the values,
-    // which the matrix cores work on meanwhile. A wave's issue slots bound this loop, and the softmax is short in them:
-    // scores stay unscaled up to exp2(scale s - m), one fused multiply-add; a row that sees none of a tile has m = inf there; the sum of a row's weights is a product with ones,
-    // of the weights as rounded for the values. The next tiles are loaded as soon as
-    // their registers are free: values once these are in LDS, keys after the last product of scores.
+    // GROUP: two tiles at a time, the row blocks one behind the other, so that each block's softmax is on the vector
+    // ALUs between the products of the next block's scores and of the last one's with the values, which the matrix
+    // cores work on meanwhile. A wave's issue slots bound this loop, and the softmax is short in them: dense scores
+    // stay unscaled up to exp2(scale s - m), one fused multiply-add; a row that sees none of a tile has m = inf
+    // there; the sum of a row's weights is a product with ones, of the weights as rounded for the values (INT8: the
+    // biases' sum; the weights' own is in float). The next tiles are loaded as soon as their registers are free:
+    // values once these are in LDS, keys after the last product of scores (INT8: once converted).
     auto compute_blocks = [&](const TileRegs<D, INT8> *t, int j, auto next_keys, auto next_values) {
         lds_fence();   // the previous step's reads of myvt are done before overwriting
 #pragma unroll
