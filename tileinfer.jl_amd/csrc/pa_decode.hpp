@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
             nb = p.tg;
         }
         if (p.qsl && (tok0 + nb <= p.qsl[0] || tok0 >= p.qsl[p.B])) return;   // rows of no sequence
-        start = GROUP ? 0 : min(p.lengths[pair], p.bt_stride * p.P) - 1;
+        start = GROUP ? 0 : table_keys(p.lengths[pair], p.bt_stride * p.P) - 1;
         if (start < 0) {   // no keys: zeros (the combine's, where the keys are split)
             if (nsp == 1)
                 for (int i = threadIdx.x; i < p.G * D / 4; i += NW * 64)

@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(64) generic_attention_kernel(GenericParams p) 
     if constexpr (SPARSE) {
         tok0 = t0;
         if (p.qsl && (tok0 < p.qsl[0] || tok0 >= p.qsl[p.B])) return;   // a row of no sequence
-        len = max(min(p.lengths[b], p.bt_stride * p.P), 0);
+        len = table_keys(p.lengths[b], p.bt_stride * p.P);
         last = len - 1;
     } else {
         tok0 = p.qsl ? p.qsl[b] : b * p.nmax;
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         nb = GROUP ? p.tg : 1;
         tok0 = b / p.Hk * nb;
         if (p.qsl && (tok0 + nb <= p.qsl[0] || tok0 >= p.qsl[p.B])) return;   // rows of no sequence
-        start = GROUP ? 0 : min(p.lengths[b], p.bt_stride * p.P) - 1;
+        start = GROUP ? 0 : table_keys(p.lengths[b], p.bt_stride * p.P) - 1;
         if (start < 0) {   // no keys: zeros (the combine's, where the keys are split)
             if (p.splits == 1)
                 for (int i = threadIdx.x; i < p.G * D / 4; i += 256)

@@ -9,6 +9,10 @@
 namespace ti_group {
 using namespace ti;
 
+// Keys of a table that holds `most`: lengths below 0 are none. (Clamped before anything is taken off, which
+// would wrap for lengths near -2^31.)
+__device__ __forceinline__ int table_keys(int length, int most) { return min(max(length, 0), most); }
+
 // The same over the pages of a group's tokens (GROUP, see group_pages): page u holds `most` keys that
 // one of the tokens sees. Tiles past them read the page's last tile that has some.
 struct GroupMap {
@@ -70,7 +74,7 @@ __device__ __forceinline__ int group_pages(const Params &p, GroupLds &g, uint16_
 #pragma unroll
     for (int n = 0; n < EACH; n++) {
         const int x = n * NT + tid, a = x / TG, tok = tok0 + x - a * TG;
-        const int len = min(keys[n], K * p.P);
+        const int len = table_keys(keys[n], K * p.P);
         keys[n] = x < entries && tok >= q0 && tok < q1 ? min(len - a * p.P, p.P) : 0;
         id[n] = clamp_page(id[n], p.num_pages);
     }

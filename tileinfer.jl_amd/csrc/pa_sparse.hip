@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(256) sparse_combine_kernel(DecodeParams p, int
     if (row >= rows) return;
     const int tok = row / p.Hq, hq = row - tok * p.Hq, h = hq / p.G, pair = tok * p.Hk + h;
     const int group = tok / p.tg;   // p.tg tokens share a unit of partials, packed rows g + G t
-    const int len = min(p.lengths[pair], p.bt_stride * p.P);
+    const int len = table_keys(p.lengths[pair], p.bt_stride * p.P);
     const int q0 = p.qsl ? p.qsl[0] : 0, q1 = p.qsl ? p.qsl[p.B] : tok + 1;
     const int splits = p.min_tiles > 0 && len > 0 ? f32_active_splits((len + 15) >> 4, p.splits, p.min_tiles).active : p.splits;
     const size_t stride = (size_t)p.M * (D + 2);
