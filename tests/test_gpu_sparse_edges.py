@@ -29,3 +29,30 @@ def test_lengths_at_the_ends_of_their_type(gpu, kv, rows, width):
     lengths.fill_(-2 ** 31)
     for n in (1, rows):
         assert (check_attend(c, q, tables, lengths, n=n) == 0).all()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8", "fp32"])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("rows,heads,width", [(6, 2, 7), (6, 2, 8), (300, 8, 7)])
+def test_tokens_without_keys_whose_queries_are_not_finite(gpu, kv, value, rows, heads, width):
+    """Rows that pad a batch: no keys and whatever their memory holds as queries, beside tokens with keys. They
+    get zeros, the others what they get beside queries of zeros."""
+    c = Cache(kv, 128, heads, 16, [60 * 16], seed=52)
+    torch.manual_seed(52)
+    q = torch.randn((rows, heads * 4, 128), device="cuda", dtype=T[kv])
+    tables, lengths = shared(c, rows, width, seed=52)
+    lengths[:] = width * 16                    # whole pages: no tile is masked for the others' sake
+    pad = torch.arange(rows, device="cuda") % 5 == 3
+    lengths[pad] = 0
+    q[pad] = 0
+    want = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09, None, rows)
+    q[pad, :, 17] = value
+    got = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09, None, rows)
+    assert (got[pad] == 0).all()
+    if kv == "int8":                           # the same operations on the same numbers
+        assert torch.equal(got[~pad], want[~pad])
+    else:                                      # weights rounded or not (2^-8 each, their sum too), the output (2^-8)
+        tol = 2 * 3 * 2.0 ** -8 * c.v.float().abs().max()
+        assert ((got[~pad] - want[~pad]).float().abs() <= tol).all()
+    if rows == 6:
+        check_attend(c, q, tables, lengths, n=rows)

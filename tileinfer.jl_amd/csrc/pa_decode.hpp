@@ -582,9 +582,9 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
             }
     };
 
-    bool tame = true;   // GROUP, INT8: see below
+    bool tame = true;   // GROUP, INT8: the rows' own part of `fine` below
 #pragma unroll
-    for (int rb = 0; rb < ROWB; rb++) tame &= qsl[rb] <= 0x1p40f;
+    for (int rb = 0; rb < ROWB; rb++) tame &= qsl[rb] <= 0x1p40f && fabsf(qcorr[rb]) < INFINITY;
     // GROUP: two tiles at a time, the row blocks one behind the other, so that each block's softmax is on the vector
     // ALUs between the products of the next block's scores and of the last one's with the values, which the matrix
     // cores work on meanwhile. A wave's issue slots bound this loop, and the softmax is short in them: dense scores
@@ -601,7 +601,8 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
                 *reinterpret_cast<u32x4 *>(myvt + n * 16 * VROW + (vg * KPL + e) * VROW + vc * 8) =
                     INT8 ? i8x8_to_f16b(t[n].v[e][0], t[n].v[e][1]) : t[n].v[e];
         // INT8: scales of this lane's keys. One that is not finite, or so large that a score could overflow (raw
-        // scores are below 2^34), must not meet a row that does not see its key: such tiles are masked key by key
+        // scores are below 2^34), must not meet a row that does not see its key, nor must a query that is not
+        // finite (a row without keys may hold anything): such tiles are masked key by key
         float skk[2][4], svk[2][4];
         bool odd = false;
         u32x4 kreg[2][NKB];
