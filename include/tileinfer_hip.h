@@ -316,8 +316,13 @@ typedef struct {
  * of them visible: the last entry in use may hold fewer than page_size keys. A token without keys
  * (length <= 0) gets zeros; longer lengths read as table_width * page_size. An entry outside the
  * pool is clamped into it, as in ti_attention; a page that a table names twice counts twice.
+ * ti_sparse_attention_workspace_bytes is what a call of exactly these sizes needs: fewer tokens, or another
+ * max_query_len, may need more, because keys are split where work-groups are few. ..._workspace_bound is enough
+ * for every call with these heads, types and pages of at most total_tokens tokens, max_query_len tokens a sequence
+ * and table_width entries, for a workspace that is made once.
  */
 int ti_sparse_attention_workspace_bytes(const ti_sparse_attention_args *args, const ti_kv_cache *cache, size_t *bytes);
+int ti_sparse_attention_workspace_bound(const ti_sparse_attention_args *args, const ti_kv_cache *cache, size_t *bytes);
 int ti_sparse_attention(const ti_sparse_attention_args *args, const ti_kv_cache *cache, void *stream);
 
 /* Arguments of ti_verify_draft. */

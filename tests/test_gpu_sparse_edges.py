@@ -56,3 +56,22 @@ def test_tokens_without_keys_whose_queries_are_not_finite(gpu, kv, value, rows, 
         assert ((got[~pad] - want[~pad]).float().abs() <= tol).all()
     if rows == 6:
         check_attend(c, q, tables, lengths, n=rows)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8", "fp32"])
+def test_one_workspace_for_all_batches(gpu, kv):
+    """Made for the largest batch and block, used by every smaller call, whatever they split."""
+    c = Cache(kv, 128, 8, 16, [40 * 16], seed=54)
+    torch.manual_seed(54)
+    q = torch.randn((48, 32, 128), device="cuda", dtype=T[kv])
+    tables, lengths = shared(c, 48, 30, seed=54)
+    ws = ti.sparse_attention_workspace(BE, q, c.k, tables, 16)
+    for rows in (48, 33, 32, 31, 16, 15, 4, 1):
+        for n in (1, 4, 16):
+            for width in (30, 9):
+                if rows % n:
+                    continue
+                t, m = tables[:rows, :, :width].contiguous(), lengths[:rows].clamp(max=16 * width)
+                out = torch.empty_like(q[:rows])
+                ti.sparse_attention_(BE, out, ws, q[:rows], c.k, c.v, t, m, 0.09, None, n)
+                assert torch.equal(out, ti.sparse_attention(BE, q[:rows], c.k, c.v, t, m, 0.09, None, n))

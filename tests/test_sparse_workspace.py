@@ -1,0 +1,80 @@
+"""Workspaces that a serving loop makes once: the sizes hold for every smaller call, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+import tileinfer_hip as ti
+from tileinfer_hip import _lib
+
+BE = ti.HipBackend()
+PTR = 0x1000
+
+
+def attend_size(name, tokens, n, width, heads=32, kv_heads=8, D=128, P=16, dtype=1, int8=False):
+    c = _lib.KVCache()
+    c.kind, c.head_dim, c.page_size, c.kv_heads, c.num_pages = int(int8), D, P, kv_heads, 4096
+    c.k_pages = c.v_pages = c.layer_q = c.layer_scale = c.smooth = PTR
+    a = _lib.SparseAttentionArgs()
+    a.dtype, a.q_heads, a.total_tokens, a.table_width, a.num_seqs, a.max_query_len = dtype, heads, tokens, width, 1, n
+    a.q = a.out = a.tables = a.lengths = a.query_start_loc = PTR
+    a.scale = 0.1
+    size = ctypes.c_size_t(7)
+    assert getattr(ti.load_library(), name)(ctypes.byref(a), ctypes.byref(c), ctypes.byref(size)) == 0
+    return size.value
+
+
+TYPES = [dict(), dict(int8=True), dict(dtype=0), dict(dtype=0, int8=True)]
+SHAPES = [dict(), dict(P=64), dict(P=5), dict(heads=8), dict(heads=24), dict(heads=96, kv_heads=4), dict(heads=64, kv_heads=2),
+          dict(heads=256, kv_heads=256), dict(heads=600, kv_heads=600), dict(D=64), dict(D=64, heads=16, P=64)]
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attend_bound_holds_for_smaller_calls(types, shape):
+    """For every plan up to its sizes, and it grows with them."""
+    kw = {**types, **shape}
+    exact = lambda *a: attend_size("ti_sparse_attention_workspace_bytes", *a, **kw)
+    bound = lambda *a: attend_size("ti_sparse_attention_workspace_bound", *a, **kw)
+    counts = list(range(1, 70)) + [100, 127, 128, 129, 255, 256, 257, 511, 512, 513, 2048, 5000]
+    last = {}
+    for T in counts:
+        for n in (1, 2, 3, 4, 7, 8, 16, 33):
+            for width in (1, 2, 7, 8, 31, 33, 64, 130, 300, 700, 1500):
+                b = bound(T, n, width)
+                assert exact(T, n, width) <= b
+                for smaller in ((T, max(1, n // 2), width), (T, n, max(1, width // 2))):
+                    assert bound(*smaller) <= b
+                assert last.get((n, width), 0) <= b
+                last[n, width] = b
+    for T, n, width in ((300, 16, 700), (64, 8, 64)):     # against all that is smaller
+        b = bound(T, n, width)
+        for t in range(1, T + 1, 7):
+            for m in range(1, n + 1):
+                for w in (1, 3, 8, 30, 64, 100, 256, 300, 512, 513, 700):
+                    if w <= width:
+                        assert exact(t, m, w) <= b
+
+
+def test_attend_workspace_is_made_once():
+    """The workspace of the largest batch serves the smaller and the drafted ones: as the batch shrinks, its keys
+    are split more, so a launch of 32 tokens needs nothing where one of 31 does."""
+    k = torch.zeros((64, 8, 16, 128), dtype=torch.bfloat16)
+    q, tables = torch.zeros((32, 32, 128), dtype=torch.bfloat16), torch.zeros((32, 8, 64), dtype=torch.int32)
+    assert attend_size("ti_sparse_attention_workspace_bytes", 32, 1, 64) == 0
+    have = ti.sparse_attention_workspace(BE, q, k, tables)
+    for t in range(1, 33):
+        assert have.numel() >= attend_size("ti_sparse_attention_workspace_bytes", t, 1, 64)
+    have = ti.sparse_attention_workspace(BE, q, k, tables, 4)
+    for t in range(1, 33):
+        for n in range(1, 5):
+            assert have.numel() >= attend_size("ti_sparse_attention_workspace_bytes", t, n, 64)
+    assert ti.sparse_attention_workspace(BE, q, k, tables[:, :, :1]) is None      # too short to split
+
+
+def test_attend_bound_refuses_as_the_call():
+    L, size = ti.load_library(), ctypes.c_size_t(7)
+    c, a = _lib.KVCache(), _lib.SparseAttentionArgs()
+    assert L.ti_sparse_attention_workspace_bound(ctypes.byref(a), ctypes.byref(c), ctypes.byref(size)) == _lib.TI_ERR_INVALID_ARG
+    assert size.value == 0
+    assert L.ti_sparse_attention_workspace_bound(ctypes.byref(a), ctypes.byref(c), None) == _lib.TI_ERR_INVALID_ARG

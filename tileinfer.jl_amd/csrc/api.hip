@@ -320,6 +320,15 @@ int ti_sparse_attention_workspace_bytes(const ti_sparse_attention_args *a, const
     return TI_OK;
 }
 
+int ti_sparse_attention_workspace_bound(const ti_sparse_attention_args *a, const ti_kv_cache *c, size_t *bytes) {
+    if (!bytes) return TI_ERR_INVALID_ARG;
+    *bytes = 0;
+    const int st = check_sparse(a, c);
+    if (st) return st;
+    *bytes = ti_sparse_bound(a, c);
+    return TI_OK;
+}
+
 int ti_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, void *stream) {
     int st = check_sparse(a, c);
     if (!st) st = check_workspace(a->workspace, a->workspace_bytes, ti_sparse_bytes(a, c));

@@ -185,6 +185,7 @@ struct ti_sparse_plan {
 };
 ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c);
 size_t ti_sparse_bytes(const ti_sparse_attention_args *a, const ti_kv_cache *c);
+size_t ti_sparse_bound(const ti_sparse_attention_args *a, const ti_kv_cache *c);
 int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, hipStream_t s);
 bool ti_sparse_f32_mfma(const ti_sparse_attention_args *a, const ti_kv_cache *c);
 int ti_launch_sparse_f32(const ti_sparse_attention_args *a, const ti_kv_cache *c, const ti_sparse_plan &pl, hipStream_t s);

@@ -121,6 +121,24 @@ int launch_group_d(const DecodeParams &p, unsigned grid, hipStream_t s) {
     return launch_group_r<D, INT8, 2>(p, grid, s);
 }
 
+// Steps that are worked on in groups of tokens.
+bool groups_allowed(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
+    const int P = c->page_size;
+    return a->max_query_len > 1 && P >= 16 && P <= 32768 && (P & (P - 1)) == 0 && a->q_heads / c->kv_heads <= 16 &&
+           (a->dtype != TI_F32 || ti_sparse_f32_mfma(a, c));
+}
+
+// Work-groups below which keys are split, for groups of tg tokens.
+long long split_target(bool f32, bool int8, int tg) { return f32 || (int8 && tg > 1) ? 512 : 256; }
+
+// The most splits of a table: at most 16 (Float32 32), of at least four 16-key tiles each.
+int most_splits(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
+    const long long tiles = ((long long)a->table_width * c->page_size + 15) / 16;
+    int s = 1;
+    while (s < (a->dtype == TI_F32 ? 32 : 16) && tiles >= 8 * s) s <<= 1;
+    return s;
+}
+
 }  // namespace
 
 // Tokens worked on together, and splits of their keys.
@@ -144,7 +162,7 @@ ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cac
     ti_sparse_plan pl{1, 1};
     auto pairs = [&](int tg) { return ((long long)a->total_tokens + tg - 1) / tg * c->kv_heads; };
     const bool f32 = a->dtype == TI_F32;
-    if (a->max_query_len > 1 && P >= 16 && P <= 32768 && (P & (P - 1)) == 0 && G <= 16 && (!f32 || ti_sparse_f32_mfma(a, c))) {
+    if (groups_allowed(a, c)) {
         auto tokens = [&](int rows, int entries) {
             return max(1, min(min(min(rows / G, 32), a->max_query_len), entries / min(a->table_width, entries + 1)));
         };
@@ -154,8 +172,8 @@ ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cac
         const int wider = tokens(64, GROUP_PAGES);
         if (!f32 && !int8 && wider > pl.tg && pairs(pl.tg) >= (c->head_dim == 128 ? 512 : 1024)) pl.tg = wider;
     }
-    const long long tiles = ((long long)a->table_width * P + 15) / 16, target = f32 || (int8 && pl.tg > 1) ? 512 : 256;
-    while (pl.splits < (f32 ? 32 : 16) && pairs(pl.tg) * pl.splits < target && tiles >= 8 * pl.splits) pl.splits <<= 1;
+    const int most = most_splits(a, c);
+    while (pl.splits < most && pairs(pl.tg) * pl.splits < split_target(f32, int8, pl.tg)) pl.splits <<= 1;
     return pl;
 }
 
@@ -164,6 +182,20 @@ size_t ti_sparse_bytes(const ti_sparse_attention_args *a, const ti_kv_cache *c) 
     if (pl.splits == 1) return 0;
     const size_t groups = ((size_t)a->total_tokens + pl.tg - 1) / pl.tg;
     return groups * pl.tg * a->q_heads * pl.splits * (c->head_dim + 2) * sizeof(float);
+}
+
+// Enough for every plan of at most as many tokens, query tokens a sequence and table entries: one of s > 1 splits has
+// fewer than split_target work-groups with s / 2 of them, and no more groups and splits than the largest step.
+size_t ti_sparse_bound(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
+    const int G = a->q_heads / c->kv_heads, splits = most_splits(a, c);
+    const bool f32 = a->dtype == TI_F32, int8 = c->kind == TI_KV_INT8;
+    const int rows = f32 ? 16 : int8 ? 32 : 64, most = groups_allowed(a, c) ? max(1, min(min(rows / G, 32), a->max_query_len)) : 1;
+    long long tokens = 0;   // times splits
+    for (int tg = 1; splits > 1 && tg <= most; tg++) {
+        const long long groups = ((long long)a->total_tokens + tg - 1) / tg;
+        tokens = max(tokens, tg * min(groups * splits, (split_target(f32, int8, tg) - 1) / c->kv_heads * 2));
+    }
+    return (size_t)tokens * a->q_heads * (c->head_dim + 2) * sizeof(float);
 }
 
 int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, hipStream_t s) {

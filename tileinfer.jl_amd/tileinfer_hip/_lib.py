@@ -24,7 +24,7 @@ TI_KV_DENSE, TI_KV_INT8 = 0, 1
 EXPORTS = ("ti_version", "ti_status_string", "ti_attention_workspace_bytes", "ti_attention",
            "ti_attention_noalloc", "ti_store_kv", "ti_rmsnorm", "ti_rope", "ti_attention_inputs",
            "ti_update_key_bounds", "ti_select_pages_workspace_bytes", "ti_select_pages",
-           "ti_sparse_attention_workspace_bytes", "ti_sparse_attention",
+           "ti_sparse_attention_workspace_bytes", "ti_sparse_attention_workspace_bound", "ti_sparse_attention",
            "ti_verify_draft_workspace_bytes", "ti_verify_draft")
 NOALLOC_SCRATCH_BYTES = 32 << 20   # TI_NOALLOC_SCRATCH_BYTES
 
@@ -121,6 +121,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
                         ("ti_select_pages_workspace_bytes", [P(SelectArgs), size]),
                         ("ti_select_pages", [P(SelectArgs), vp]),
                         ("ti_sparse_attention_workspace_bytes", [P(SparseAttentionArgs), P(KVCache), size]),
+                        ("ti_sparse_attention_workspace_bound", [P(SparseAttentionArgs), P(KVCache), size]),
                         ("ti_sparse_attention", [P(SparseAttentionArgs), P(KVCache), vp]),
                         ("ti_verify_draft_workspace_bytes", [P(VerifyArgs), size]),
                         ("ti_verify_draft", [P(VerifyArgs), vp])):

@@ -439,9 +439,7 @@ def _sparse_step(q, query_start_loc, max_query_len):
     return query_start_loc.numel() - 1, n
 
 
-def sparse_attention_workspace(be: HipBackend, q, k_pages, tables, max_query_len: int = 1):
-    """Scratch of sparse_attention_ for queries shaped like q and tables of this width, or None. A byte
-    tensor; enough for every batch of as many tokens."""
+def _sparse_workspace(size_of, q, k_pages, tables, max_query_len):
     c = KVCache()
     if isinstance(k_pages, Int8Pages):
         c.kind, c.layer_q, c.layer_scale, c.smooth = _lib.TI_KV_INT8, 16, 16, 16
@@ -450,7 +448,14 @@ def sparse_attention_workspace(be: HipBackend, q, k_pages, tables, max_query_len
     c.num_pages, c.kv_heads, c.page_size, c.head_dim = k_pages.shape
     a = _sparse_args(q, tables.shape[-1], 1, int(max_query_len), 1.0)
     a.q = a.out = a.tables = a.lengths = a.query_start_loc = 16
-    return _workspace(_lib.load().ti_sparse_attention_workspace_bytes, q.device, ctypes.byref(a), ctypes.byref(c))
+    return _workspace(size_of, q.device, ctypes.byref(a), ctypes.byref(c))
+
+
+def sparse_attention_workspace(be: HipBackend, q, k_pages, tables, max_query_len: int = 1):
+    """Scratch of sparse_attention_, or None where no such call needs any: a byte tensor, enough for every call with
+    q's heads of at most as many tokens as q has, at most max_query_len of them a sequence and tables at most
+    as wide."""
+    return _sparse_workspace(_lib.load().ti_sparse_attention_workspace_bound, q, k_pages, tables, max_query_len)
 
 
 def sparse_attention_(be: HipBackend, out, workspace, q, k_pages, v_pages, tables, lengths, scale: float,
@@ -487,7 +492,8 @@ def sparse_attention(be: HipBackend, q, k_pages, v_pages, tables, lengths, scale
                      query_start_loc: Optional[torch.Tensor] = None, max_query_len: Optional[int] = None):
     """Allocating sparse_attention_: rows that belong to no sequence are zero."""
     out = torch.empty_like(q) if query_start_loc is None else torch.zeros_like(q)
-    ws = sparse_attention_workspace(be, q, k_pages, tables, 1 if max_query_len is None else max_query_len)
+    ws = _sparse_workspace(_lib.load().ti_sparse_attention_workspace_bytes, q, k_pages, tables,
+                           1 if max_query_len is None else max_query_len)
     return sparse_attention_(be, out, ws, q, k_pages, v_pages, tables, lengths, scale, query_start_loc, max_query_len)
 
 
