@@ -288,6 +288,8 @@ typedef struct {
  * tables: the kept pages' ids in order of position, zero-padded; lengths: the keys they hold up to
  * the last visible one, as ti_sparse_attention takes them. All visible pages are kept while there
  * are at most `keep`.
+ * The workspace is 4 bytes per token, KV head and (rounded to 256) table entry, up to 128 MiB (at least one token's). It
+ * grows with total_tokens and block_table_stride and depends on neither num_seqs nor max_query_len.
  */
 int ti_select_pages_workspace_bytes(const ti_select_args *args, size_t *bytes);
 int ti_select_pages(const ti_select_args *args, void *stream);

@@ -2,11 +2,13 @@
 without keys, garbage in whatever a table does not name."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
+import sparse_ref as ref
 import tileinfer_hip as ti
-from test_gpu_sparse import Cache, T, check_attend, i32, shared
+from test_gpu_sparse import Cache, T, check_attend, i32, offsets, positions, random_bounds, shared
 
 pytestmark = pytest.mark.gpu
 BE = ti.HipBackend()
@@ -75,3 +77,36 @@ def test_one_workspace_for_all_batches(gpu, kv):
                 out = torch.empty_like(q[:rows])
                 ti.sparse_attention_(BE, out, ws, q[:rows], c.k, c.v, t, m, 0.09, None, n)
                 assert torch.equal(out, ti.sparse_attention(BE, q[:rows], c.k, c.v, t, m, 0.09, None, n))
+
+
+@pytest.mark.parametrize("G,D", [(4, 64), (20, 64)])
+def test_selection_in_parts(gpu, G, D):
+    """Tables wider than LDS holds and more tokens than the workspace: worked on in parts, which begin inside a
+    tile and a sequence; each sequence alone (one part) gives the same."""
+    P, pages, H, width = 1, 3000, 8, 34000
+    counts, starts = [67, 1, 0, 70, 5, 66, 130], [33000, 20, 0, 30000, 33990, 100, 33500]
+    total, spare = sum(counts), 3
+    g = torch.Generator().manual_seed(55)
+    tables = torch.randint(1, pages + 1, (len(counts), width), generator=g, dtype=torch.int32).cuda()
+    kb = random_bounds(pages, H, D, P, 55)
+    torch.manual_seed(55)
+    q = torch.randn((total + spare, H * G, D), device="cuda", dtype=torch.bfloat16)
+    pos = torch.cat([positions(starts, counts), i32([0] * spare)])
+    out = torch.full((total + spare, H, 40), -5, dtype=torch.int32, device="cuda")
+    lengths = torch.full((total + spare, H), -5, dtype=torch.int32, device="cuda")
+    ws = ti.select_pages_workspace(BE, q, kb, tables)
+    assert ws.numel() < (total * H * width * 4) // 2
+    ti.select_pages_(BE, out, lengths, ws, q, kb, tables, pos, 2, 3, True, offsets(counts), max(counts))
+    row = 0
+    for b, n in enumerate(counts):
+        for t0 in range(0, n, 65):
+            m = min(65, n - t0)
+            a = slice(row + t0, row + t0 + m)
+            want = ti.select_pages(BE, q[a], kb, tables[b:b + 1], pos[a], 40, 2, 3, True, None, m)
+            assert torch.equal(out[a], want[0]) and torch.equal(lengths[a], want[1])
+        row += n
+    assert (out[row:] == -5).all() and (lengths[row:] == -5).all()
+    hb, hs, ht = kb.bounds.cpu().numpy(), kb.scale.cpu().numpy(), tables.cpu().numpy()
+    for r, b, t in ((0, 0, 0), (140, 4, 2), (total - 1, 6, 129)):
+        want, want_len = ref.select(q[r].double().cpu().numpy(), hb, hs, ht[b], starts[b] + t, P, 40, 2, 3)
+        assert np.array_equal(out[r].cpu().numpy(), want) and np.array_equal(lengths[r].cpu().numpy(), want_len)

@@ -78,3 +78,31 @@ def test_attend_bound_refuses_as_the_call():
     assert L.ti_sparse_attention_workspace_bound(ctypes.byref(a), ctypes.byref(c), ctypes.byref(size)) == _lib.TI_ERR_INVALID_ARG
     assert size.value == 0
     assert L.ti_sparse_attention_workspace_bound(ctypes.byref(a), ctypes.byref(c), None) == _lib.TI_ERR_INVALID_ARG
+
+
+def select_size(tokens, stride, seqs=1, n=None, heads=32, kv_heads=8):
+    a = _lib.SelectArgs()
+    a.dtype, a.q_heads, a.kv_heads, a.head_dim, a.page_size, a.num_pages = 1, heads, kv_heads, 128, 16, 4096
+    a.num_seqs, a.max_query_len, a.total_tokens, a.block_table_stride = seqs, tokens if n is None else n, tokens, stride
+    a.keep, a.sinks, a.window, a.causal = 8, 1, 2, 1
+    a.q = a.bounds.bounds = a.bounds.scale = a.positions = a.block_tables = a.tables = a.lengths = a.query_start_loc = PTR
+    size = ctypes.c_size_t(7)
+    assert ti.load_library().ti_select_pages_workspace_bytes(ctypes.byref(a), ctypes.byref(size)) == 0
+    return size.value
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(32, 8), (8, 8), (64, 2), (128, 2), (300, 300), (24, 4)])
+def test_select_workspace(heads, kv_heads):
+    """Bounded (4096 tokens over 8192 table entries of 8 KV heads took 1 GiB), growing with tokens and entries, the
+    same for every split of the tokens into sequences, and never less than one token's."""
+    size = lambda *a, **kw: select_size(*a, heads=heads, kv_heads=kv_heads, **kw)
+    strides = [1, 100, 256, 257, 1032, 2048, 2049, 8192, 8193, 16384, 32768, 40000, 131072, 10 ** 6, 10 ** 7]
+    tokens = [1, 2, 3, 15, 31, 32, 33, 127, 255, 256, 512, 4096, 70000]
+    for i, w in enumerate(strides):
+        one = 4 * kv_heads * w
+        for j, t in enumerate(tokens):
+            b = size(t, w)
+            assert one <= b <= max(128 << 20, 4 * kv_heads * ((w + 255) // 256 * 256))
+            assert i == 0 or size(t, strides[i - 1]) <= b
+            assert j == 0 or size(tokens[j - 1], w) <= b
+            assert size(t, w, seqs=min(t, 9), n=t) == b and size(t, w, seqs=min(t, 9), n=1) == b

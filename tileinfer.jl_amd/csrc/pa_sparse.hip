@@ -13,6 +13,8 @@
 // Pairs take consecutive work-groups with the KV heads innermost: with 8 KV heads (a multiple of
 // the 8 XCDs in general) all tokens of a KV head run on one XCD, and the pages that the tokens of
 // a step share are read through one L2.
+#include <algorithm>
+
 #include "pa_decode.hpp"
 
 using namespace ti;
@@ -193,7 +195,7 @@ size_t ti_sparse_bound(const ti_sparse_attention_args *a, const ti_kv_cache *c) 
     long long tokens = 0;   // times splits
     for (int tg = 1; splits > 1 && tg <= most; tg++) {
         const long long groups = ((long long)a->total_tokens + tg - 1) / tg;
-        tokens = max(tokens, tg * min(groups * splits, (split_target(f32, int8, tg) - 1) / c->kv_heads * 2));
+        tokens = std::max(tokens, tg * std::min(groups * splits, (split_target(f32, int8, tg) - 1) / c->kv_heads * 2));
     }
     return (size_t)tokens * a->q_heads * (c->head_dim + 2) * sizeof(float);
 }

@@ -16,6 +16,8 @@
 // Two forms. select_kernel holds a token tile's keys in LDS and does both steps in one launch.
 // scores_kernel and keep_kernel share a tile's pages out over several work-groups, the keys going
 // through the workspace, for few tokens over wide tables and for tables that LDS does not hold.
+#include <algorithm>
+
 #include "page_bounds.hpp"
 
 using namespace ti;
@@ -34,9 +36,10 @@ struct SelectParams {
     const float *scale;
     const int32_t *positions, *qsl, *bt;
     int32_t *tables, *lengths;
-    uint32_t *keys;   // two launches: [total][Hk][pitch]
+    uint32_t *keys;   // two launches: [end - first][Hk][pitch]
     int bt_stride, num_pages, P, Hk, Hq, G, nmax, total, keep, sinks, window, causal, f32, pshift;
     int pitch, split;   // keys per (token, KV head); work-groups that share a token tile's pages
+    int first, end;     // two launches: the rows of the packed tokens that they work on
 };
 
 // What one token sees: pages [0, seen), of which [c0, c1) are up for choice and `need` kept by score.
@@ -137,9 +140,9 @@ __device__ __forceinline__ void quantize_rows(const SelectParams &p, const Step 
 // the heads of a token are a lane's registers (and those of other 16-lane groups for GP > 4), its page's
 // scale is at hand, and few vector instructions are left beside the loads: with the operands the other
 // way round (heads in lanes) they bound the kernel (512 tokens on 64k: 17 us of scores, 2048 pages
-// 11.6). dst(t, page) is where the key of token t0 + t goes.
+// 11.6). dst(t, page) is where the key of token t0 + t goes, from <= t < tokens.
 template <int D, int GP, int RT, bool WIDE, typename Dst>
-__device__ __forceinline__ void score_pages(const SelectParams &p, int b, int h, int tokens, int lane, int first, int step, int ntiles,
+__device__ __forceinline__ void score_pages(const SelectParams &p, int b, int h, int from, int tokens, int lane, int first, int step, int ntiles,
                                             int most, const int8_t (*w)[2 * D], const float *forth, Dst dst) {
     constexpr int NK = 2 * D / 64;
     constexpr int HL = GP < 4 ? GP : 4, TL = 4 / HL;   // heads and tokens of a lane's four rows
@@ -183,7 +186,7 @@ __device__ __forceinline__ void score_pages(const SelectParams &p, int b, int h,
 #pragma unroll
             for (int n = 0; n < TL; n++) {
                 const int t = WIDE ? 0 : (rt * 16 + 4 * kg + n * HL) / GP;
-                if (4 * kg % GP == 0 && t < tokens) *dst(t, j * 16 + r16) = order_key(s[n] * pg.scale);
+                if (4 * kg % GP == 0 && t >= from && t < tokens) *dst(t, j * 16 + r16) = order_key(s[n] * pg.scale);
             }
         }
     };
@@ -498,7 +501,7 @@ __global__ void __launch_bounds__(W * 64) select_kernel(SelectParams p) {
         const int span = (most + ROUND - 1) / ROUND * ROUND;
         quantize_rows<D, GP, RT, WIDE, W>(p, st, h, t0, tid, w, forth);
         __syncthreads();
-        score_pages<D, GP, RT, WIDE>(p, b, h, tokens, lane, wv, W, ntiles, most, w, forth,
+        score_pages<D, GP, RT, WIDE>(p, b, h, 0, tokens, lane, wv, W, ntiles, most, w, forth,
                                      [&](int t, int page) { return keys + t * p.pitch + page; });
         __syncthreads();
         const int32_t *bt = p.bt + (size_t)b * p.bt_stride;
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(W * 64) select_kernel(SelectParams p) {
     }
 }
 
-// The keys of a token tile to the workspace: grid (Hk x split, token tiles, B).
+// The keys of a token tile to the workspace, for tokens first .. end - 1: grid (Hk x split, token tiles, B).
 template <int D, int GP, int RT, bool WIDE, int W>
 __global__ void __launch_bounds__(W * 64) scores_kernel(SelectParams p) {
     using TL = Tile<GP, RT, WIDE>;
@@ -527,31 +530,33 @@ __global__ void __launch_bounds__(W * 64) scores_kernel(SelectParams p) {
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % p.Hk, part = blockIdx.x / p.Hk, b = blockIdx.z;
     const Step st = step_of(p.qsl, p.positions, b, p.nmax, p.total);
-    for (int t0 = blockIdx.y * TL::TT; t0 < st.n; t0 += gridDim.y * TL::TT) {
+    const int end = min(st.n, p.end - st.tok0);
+    for (int t0 = max(p.first - st.tok0, 0) / TL::TT * TL::TT + blockIdx.y * TL::TT; t0 < end; t0 += gridDim.y * TL::TT) {
         __syncthreads();
-        const int tokens = min(TL::TT, st.n - t0);
+        const int tokens = min(TL::TT, end - t0);
         const int most = Seen(p, st, t0 + tokens - 1).seen, ntiles = (most + 15) >> 4;
         quantize_rows<D, GP, RT, WIDE, W>(p, st, h, t0, tid, w, forth);
         __syncthreads();
-        score_pages<D, GP, RT, WIDE>(p, b, h, tokens, lane, part * W + wv, p.split * W, ntiles, most, w, forth, [&](int t, int page) {
-            return p.keys + ((size_t)(st.tok0 + t0 + t) * p.Hk + h) * p.pitch + page;
-        });
+        const int row = st.tok0 + t0 - p.first;   // the tile's first tokens may be before p.first
+        score_pages<D, GP, RT, WIDE>(p, b, h, max(-row, 0), tokens, lane, part * W + wv, p.split * W, ntiles, most, w, forth,
+                                     [&](int t, int page) { return p.keys + ((size_t)(row + t) * p.Hk + h) * p.pitch + page; });
     }
 }
 
 // Kept pages of one token and KV head from the workspace: grid (Hk, tokens, B). The keys are read into LDS
-// where it holds them (`lds` of them).
+// where it holds them (`lds` of them). Tokens as scores_kernel.
 template <int W> __global__ void __launch_bounds__(W * 64) keep_kernel(SelectParams p, int lds) {
     __shared__ SearchLds<W> search;
     extern __shared__ __attribute__((aligned(16))) uint32_t held[];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x, b = blockIdx.z;
     const Step st = step_of(p.qsl, p.positions, b, p.nmax, p.total);
-    for (int t = blockIdx.y; t < st.n; t += gridDim.y) {
+    const int end = min(st.n, p.end - st.tok0);
+    for (int t = max(p.first - st.tok0, 0) + blockIdx.y; t < end; t += gridDim.y) {
         const Seen s(p, st, t);
         const int span = (s.seen + ROUND - 1) / ROUND * ROUND;
         const size_t pair = (size_t)(st.tok0 + t) * p.Hk + h;
-        uint32_t *keys = p.keys + pair * p.pitch;
+        uint32_t *keys = p.keys + ((size_t)(st.tok0 + t - p.first) * p.Hk + h) * p.pitch;
         __syncthreads();   // the token before this one is done with LDS
         const int32_t *bt = p.bt + (size_t)b * p.bt_stride;
         if (span <= lds) {
@@ -581,6 +586,18 @@ template <int TT> bool fits_one_launch(const SelectParams &p, long long groups) 
     return key_bytes(p, TT) <= (size_t)LDS_KEYS && (groups >= 256 || p.bt_stride <= 768);
 }
 
+// Bytes of a token's keys in the workspace, and of the workspace. Where LDS holds the keys of a tile of TT tokens, two
+// launches are taken for fewer than 256 work-groups only, for at most 255 / Hk tiles. Where it does not, longer steps
+// are worked on in parts of PART_BYTES (with 4 tokens a tile at least 255 work-groups each up to 32768 table entries;
+// beyond, a tile's pages are shared out over several).
+constexpr size_t PART_BYTES = 128u << 20;
+size_t row_bytes(int Hk, int pitch) { return (size_t)Hk * pitch * sizeof(uint32_t); }
+size_t scratch_bytes(int total, int Hk, int pitch, int TT) {
+    const size_t row = row_bytes(Hk, pitch);
+    const size_t most = (size_t)TT * pitch * sizeof(uint32_t) <= LDS_KEYS ? 255u / Hk * TT * row : PART_BYTES;
+    return std::min(total * row, std::max(row, most));
+}
+
 template <int D, int GP, int RT, bool WIDE, int W>
 int launch_one(const SelectParams &p, unsigned y, int num_seqs, hipStream_t s) {
     const size_t bytes = key_bytes(p, Tile<GP, RT, WIDE>::TT);
@@ -604,14 +621,21 @@ int launch(SelectParams p, int num_seqs, hipStream_t s) {
         return launch_one<D, GP, RT, WIDE, W>(p, y, num_seqs, s);
     }
     if constexpr (RT == 1 || WIDE) {   // launch_rows takes tiles of several tokens' blocks for one launch only
-        p.split = 1;
-        while (groups * p.split < 256 && p.split * W * 32 < p.bt_stride) p.split <<= 1;
-        scores_kernel<D, GP, RT, WIDE, W><<<dim3(p.Hk * p.split, y, num_seqs), W * 64, 0, s>>>(p);
-        if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
-        const size_t held = min((size_t)p.pitch * sizeof(uint32_t), (size_t)LDS_KEYS);
+        const size_t held = std::min((size_t)p.pitch * sizeof(uint32_t), (size_t)LDS_KEYS);
         if (!allow_lds((const void *)keep_kernel<W>, held)) return TI_ERR_LAUNCH;
-        keep_kernel<W><<<dim3(p.Hk, min(p.nmax, 32768), num_seqs), W * 64, held, s>>>(p, (int)(held / sizeof(uint32_t)));
-        return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
+        // as many tokens at a time as the workspace holds; a part of a sequence may begin inside a tile
+        const int rows = (int)(scratch_bytes(p.total, p.Hk, p.pitch, TT) / row_bytes(p.Hk, p.pitch));
+        const long long most = std::min(tiles, ((long long)rows + TT - 1) / TT + 1);
+        p.split = 1;
+        while (std::min(groups, most * num_seqs * p.Hk) * p.split < 256 && p.split * W * 32 < p.bt_stride) p.split <<= 1;
+        for (p.first = 0;; p.first = p.end) {
+            p.end = p.total - p.first > rows ? p.first + rows : p.total;
+            scores_kernel<D, GP, RT, WIDE, W><<<dim3(p.Hk * p.split, min(y, (unsigned)most), num_seqs), W * 64, 0, s>>>(p);
+            if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
+            keep_kernel<W><<<dim3(p.Hk, min(min(p.nmax, rows), 32768), num_seqs), W * 64, held, s>>>(p, (int)(held / sizeof(uint32_t)));
+            if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
+            if (p.end == p.total) return TI_OK;
+        }
     }
     return TI_ERR_LAUNCH;
 }
@@ -642,7 +666,9 @@ int key_pitch(const ti_select_args *a) { return (int)(((long long)a->block_table
 }  // namespace
 
 size_t ti_select_bytes(const ti_select_args *a) {
-    return (size_t)a->total_tokens * a->kv_heads * key_pitch(a) * sizeof(uint32_t);
+    const int G = a->q_heads / a->kv_heads;
+    const int TT = G > 8 ? 1 : G > 4 ? 2 : G > 2 ? 4 : G > 1 ? 8 : 16;   // a tile's tokens in two launches (launch_heads)
+    return scratch_bytes(a->total_tokens, a->kv_heads, key_pitch(a), TT);
 }
 
 int ti_launch_select_pages(const ti_select_args *a, hipStream_t s) {

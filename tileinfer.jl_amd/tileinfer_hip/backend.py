@@ -372,8 +372,8 @@ def _select_args(q, bounds: KeyBounds, stride, B, n, keep, sinks, window, causal
 
 
 def select_pages_workspace(be: HipBackend, q, bounds: KeyBounds, block_tables):
-    """Scratch of select_pages_ for queries shaped like q: a byte tensor (4 bytes per query token, KV head
-    and block-table entry)."""
+    """Scratch of select_pages_: a byte tensor, enough for every call with q's heads of at most as many tokens as q
+    has and block tables at most as wide (4 bytes per token, KV head and entry, up to 128 MiB or one token's)."""
     a = _select_args(q, bounds, block_tables.shape[-1], 1, q.shape[0], 1, 0, 1, True)
     a.q = a.bounds.bounds = a.bounds.scale = a.positions = a.block_tables = a.tables = a.lengths = 16
     return _workspace(_lib.load().ti_select_pages_workspace_bytes, q.device, ctypes.byref(a))
