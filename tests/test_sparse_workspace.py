@@ -106,3 +106,17 @@ def test_select_workspace(heads, kv_heads):
             assert i == 0 or size(t, strides[i - 1]) <= b
             assert j == 0 or size(tokens[j - 1], w) <= b
             assert size(t, w, seqs=min(t, 9), n=t) == b and size(t, w, seqs=min(t, 9), n=1) == b
+
+
+def test_select_widest_table():
+    """A width is rounded up to 256 entries in 32 bits: one that cannot be is refused (it gave a size near 2^64)."""
+    a, size = _lib.SelectArgs(), ctypes.c_size_t(7)
+    a.dtype, a.q_heads, a.kv_heads, a.head_dim, a.page_size, a.num_pages = 1, 8, 8, 128, 16, 100
+    a.num_seqs, a.max_query_len, a.total_tokens, a.keep, a.sinks, a.window, a.causal = 1, 1, 1, 8, 1, 2, 1
+    a.q = a.bounds.bounds = a.bounds.scale = a.positions = a.block_tables = a.tables = a.lengths = PTR
+    L = ti.load_library()
+    for stride, want in ((2 ** 31 - 256, _lib.TI_OK), (2 ** 31 - 255, _lib.TI_ERR_UNSUPPORTED), (2 ** 31 - 1, _lib.TI_ERR_UNSUPPORTED)):
+        a.block_table_stride = stride
+        assert L.ti_select_pages_workspace_bytes(ctypes.byref(a), ctypes.byref(size)) == want
+        assert size.value == (8 * 4 * stride if want == _lib.TI_OK else 0)
+        assert L.ti_select_pages(ctypes.byref(a), None) == (_lib.TI_ERR_WORKSPACE if want == _lib.TI_OK else want)

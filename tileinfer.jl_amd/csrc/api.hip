@@ -116,8 +116,9 @@ int check_select(const ti_select_args *a) {
     const int st = check_step(a->num_seqs, a->max_query_len, a->total_tokens, a->query_start_loc);
     if (st) return st;
     if (a->head_dim != 64 && a->head_dim != 128) return TI_ERR_UNSUPPORTED;
-    // lengths are 32-bit
-    if (a->q_heads / a->kv_heads > 64 || (long long)a->keep * a->page_size > 0x7fffffffLL) return TI_ERR_UNSUPPORTED;
+    // lengths are 32-bit, and so is a table's width rounded to 256
+    if (a->q_heads / a->kv_heads > 64 || (long long)a->keep * a->page_size > 0x7fffffffLL || a->block_table_stride > 0x7fffff00)
+        return TI_ERR_UNSUPPORTED;
     return TI_OK;
 }
 
