@@ -120,3 +120,20 @@ def test_select_widest_table():
         assert L.ti_select_pages_workspace_bytes(ctypes.byref(a), ctypes.byref(size)) == want
         assert size.value == (8 * 4 * stride if want == _lib.TI_OK else 0)
         assert L.ti_select_pages(ctypes.byref(a), None) == (_lib.TI_ERR_WORKSPACE if want == _lib.TI_OK else want)
+
+
+@pytest.mark.parametrize("P,width", [(1, 2 ** 31 - 1), (1, 2 ** 31 - 255), (65537, 32767), (2 ** 31 - 1, 1)])
+def test_attend_longest_table(P, width):
+    """Key counts are 32-bit and rounded up to tiles: a table that holds 2^31 keys but for a few is refused (a full
+    one of 2^31 - 1 keys wrapped to none); one of 2^31 - 256 is not."""
+    L, size = ti.load_library(), ctypes.c_size_t(7)
+    c, a = _lib.KVCache(), _lib.SparseAttentionArgs()
+    c.kind, c.head_dim, c.page_size, c.kv_heads, c.num_pages, c.k_pages, c.v_pages = 0, 128, P, 8, 100, PTR, PTR
+    a.dtype, a.q_heads, a.total_tokens, a.table_width, a.num_seqs, a.max_query_len, a.scale = 1, 32, 4, width, 4, 1, 0.1
+    a.q = a.out = a.tables = a.lengths = PTR
+    assert L.ti_sparse_attention(ctypes.byref(a), ctypes.byref(c), None) == _lib.TI_ERR_UNSUPPORTED
+    for name in ("bytes", "bound"):
+        assert getattr(L, f"ti_sparse_attention_workspace_{name}")(ctypes.byref(a), ctypes.byref(c), ctypes.byref(size)) == _lib.TI_ERR_UNSUPPORTED
+        assert size.value == 0
+    c.page_size, a.table_width = 1, 2 ** 31 - 256
+    assert L.ti_sparse_attention(ctypes.byref(a), ctypes.byref(c), None) == _lib.TI_ERR_WORKSPACE

@@ -130,8 +130,9 @@ int check_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
     if (!(a->scale > 0.0f) || a->scale == INFINITY) return TI_ERR_INVALID_ARG;
     const int st = check_step(a->num_seqs, a->max_query_len, a->total_tokens, a->query_start_loc);
     if (st) return st;
-    // lengths, work-groups (at most 32 a pair) and rows of q are counted in 32 bits; query heads take grid y
-    if ((long long)a->table_width * c->page_size > 0x7fffffffLL ||
+    // lengths (and up to 4 tiles of 16 past them), work-groups (at most 32 a pair) and rows of q are counted in 32 bits;
+    // query heads take grid y
+    if ((long long)a->table_width * c->page_size > 0x7fffff00LL ||
         (long long)a->total_tokens * a->q_heads * 32 > 0x7fffffffLL || a->q_heads > 65535)
         return TI_ERR_UNSUPPORTED;
     return a->dtype == TI_BF16 && a->q_heads / c->kv_heads > 64 ? TI_ERR_UNSUPPORTED : TI_OK;
