@@ -110,3 +110,30 @@ def test_selection_in_parts(gpu, G, D):
     for r, b, t in ((0, 0, 0), (140, 4, 2), (total - 1, 6, 129)):
         want, want_len = ref.select(q[r].double().cpu().numpy(), hb, hs, ht[b], starts[b] + t, P, 40, 2, 3)
         assert np.array_equal(out[r].cpu().numpy(), want) and np.array_equal(lengths[r].cpu().numpy(), want_len)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8", "fp32"])
+@pytest.mark.parametrize("n", [1, 6])
+@pytest.mark.parametrize("P", [8, 16, 64])
+def test_garbage_in_pages_that_no_key_is_in(gpu, kv, n, P):
+    """NaN and infinities behind each row's last key, in the pages of the entries behind it, in the first page (that
+    of zero entries) and in every page that no table names."""
+    c = Cache(kv, 128, 2, P, [100 * P], seed=53)
+    torch.manual_seed(53)
+    q = torch.randn((6, 8, 128), device="cuda", dtype=T[kv])
+    ids = torch.randperm(c.pages - 1, generator=torch.Generator().manual_seed(53)) + 2    # not the first page
+    tables = torch.zeros((6, 2, 8), dtype=torch.int32)
+    for r in range(6):
+        tables[r, :, :4] = ids[3 * r:3 * r + 4]        # neighbours share one
+        tables[r, :, 4] = ids[30 + r]                  # 5 keys, then garbage
+        tables[r, :, 5] = ids[40 + r]                  # garbage; then two entries of zero
+    tables, lengths = tables.cuda(), torch.full((6, 2), 4 * P + 5, dtype=torch.int32, device="cuda")
+    used = torch.zeros(c.pages, dtype=torch.bool)
+    used[tables[:, :, :5].cpu().long().reshape(-1) - 1] = True
+    assert not used[0] and not used[tables[:, :, 5].cpu().long() - 1].any() and (~used).sum() > 50
+    last = tables[:, 0, 4].long() - 1
+    keys, values = (c.k.scale, c.v.scale) if kv == "int8" else (c.k, c.v)
+    for i, (a, b) in enumerate([(math.nan, math.inf), (math.inf, math.nan), (-math.inf, math.nan)]):
+        keys[~used.cuda()], values[~used.cuda()] = a, b
+        keys[last, :, 5:], values[last, :, 5:] = a, b
+        check_attend(c, q, tables, lengths, n=n)

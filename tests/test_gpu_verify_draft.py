@@ -158,3 +158,17 @@ def test_refusals(gpu):
     refused(acc, tok, ws, x, p, q, u, torch.zeros(3, dtype=torch.int32, device="cuda"))
     refused(acc, tok, ws, x, p[:, :, ::2], q[:, :, ::2], u)
     refused(acc, tok, ws, x.cpu(), p, q, u)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("given", [True, False])
+def test_uniforms_that_are_nan(gpu, dtype, given):
+    """A last uniform of NaN exceeds nothing: the last token with weight; one of a draft's accepts nothing."""
+    p, q, x, u = inputs(6, 2, 9000, dtype, seed=11, given=given)
+    p[:, :, :5] = 0
+    p[:, :, -4100:] = 0
+    u[:, -1] = math.nan
+    acc, tok = check(p, q, x, u)
+    u[:3, 0] = math.nan
+    acc, tok = check(p, q, x, u)
+    assert (acc[:3] == 0).all()
