@@ -231,10 +231,15 @@ int ti_attention_inputs(int dtype, void *q_out, const ti_kv_cache *cache, const 
 
 /* Bounds of the keys of a layer's pages, kept beside its cache: for each page and KV head the keys'
  * largest (first row) and smallest element in each dimension, rounded outward to whole multiples
- * of the page's power of two `scale`. 16-byte aligned. */
+ * of the page's power of two `scale`. 16-byte aligned.
+ * One power of two serves all of a head's dimensions, so a few dimensions with keys much larger than the rest
+ * leave these a step or two wide, and the selection loses pages for it (ti_select_pages). `channel` takes that out:
+ * keys are divided by their dimension's power of two before they are bounded, queries multiplied by it before
+ * they are rounded, which leaves every product of the two as it is. The same pointer in both calls. */
 typedef struct {
     int8_t *bounds;             /* [num_pages][Hk][2][D] */
     float *scale;               /* [num_pages][Hk] */
+    const float *channel;       /* [Hk][D] powers of two, about the dimensions' largest |k|; or NULL: ones */
 } ti_key_bounds;
 
 /*
@@ -243,7 +248,8 @@ typedef struct {
  * the cache holds in them up to the step's end. Called after the step's keys are written
  * (ti_attention_inputs, ti_store_kv). The result depends on the cached keys alone, so a step that
  * is taken back and written again needs no other call. For an INT8 cache a key is its value times
- * scale times smoothing, rounded to float after each product. A page with a key that is not finite
+ * scale times smoothing, rounded to float after each product; with `channel` a key is what its channel leaves of
+ * it (exactly, above 2^-126). A page with a key that is not finite
  * gets bounds 127 and -127 and an infinite scale, and is kept by every selection that reaches
  * its score. Pages whose id lies outside the pool, or past the block-table row, are skipped. Two
  * sequences of a call that write into one page, or two entries of a block-table row that name one,
@@ -278,10 +284,15 @@ typedef struct {
 
 /*
  * For each query token and KV head the `keep` pages of its sequence whose keys can matter most.
- * A query head is taken as whole numbers w = rint(q / 2^e) (to even), 2^e the least power of two
+ * A query head (times bounds.channel) is taken as whole numbers w = rint(q / 2^e) (to even), 2^e the least power of two
  * (from 2^-126 on) with |q| <= 127 2^e; a page's score is the largest over the KV head's query heads of
- * 2^e scale sum_d (w_d hi_d where w_d > 0, else w_d lo_d), which no key inside the bounds exceeds
- * (it is the sum of max(w_d hi_d, w_d lo_d), since hi_d >= lo_d). The first `sinks`
+ * 2^e scale sum_d (w_d hi_d where w_d > 0, else w_d lo_d), which no key inside the bounds exceeds with the
+ * rounded query 2^e w (it is the sum of max(w_d hi_d, w_d lo_d), since hi_d >= lo_d). With the query itself a key may
+ * exceed it by 2^(e - 1) scale sum_d max |hi_d|, |lo_d|, and it may itself exceed the score of unrounded bounds by
+ * as much and by scale 2^e sum_d |w_d|: a page that would be kept can be left out for others within these
+ * distances. Of 64 pages kept of 512 (random keys about a mean of the page's own, 4 query heads) 62 are
+ * those of the unrounded score; with two of 128 dimensions 5 or 10 times as large 49, and 60 to 61 with `channel`.
+ * The first `sinks`
  * and the last `window` visible pages are kept, then pages by score, equal ones in order; the sums
  * are exact, so which are kept does not depend on how they are made. A query head with an element
  * that is not finite scores 0 everywhere.

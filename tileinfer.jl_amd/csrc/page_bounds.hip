@@ -5,7 +5,8 @@
 //   e = least integer in [-126, 127] with |k| <= 127 2^e for every element k of the page's keys
 //   hi_d = ceil(max k_d 2^-e), lo_d = floor(min k_d 2^-e)
 // Multiplying by a power of two is exact and so are ceil and floor, so the bounds are a function of
-// the keys alone, whatever the order they are read in, and no key lies outside them. They depend
+// the keys alone, whatever the order they are read in, and no key lies outside them. Divided by powers of two of their
+// dimensions first (`channel`, where a few would decide e for all), they stay exact. They depend
 // only on what the cache holds below the sequence's length: after a step is taken back (a rejected
 // draft) and written again they come out as if it had never been.
 #include <type_traits>
@@ -20,7 +21,7 @@ namespace {
 struct BoundsParams {
     const void *kp;
     const int8_t *lq;
-    const float *ls, *smooth;
+    const float *ls, *smooth, *channel;
     int8_t *bounds;
     float *scale;
     const int32_t *positions, *qsl, *bt;
@@ -129,6 +130,15 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(BoundsParams p) {
             odd = __builtin_fmaf(a, 0.0f, __builtin_fmaf(b, 0.0f, odd));
         }
     }
+    if (p.channel) {   // positive powers of two: the largest key divided is the largest of the divided ones
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            const float s = 1.0f / p.channel[h * D + c + i];
+            up[i] *= s;
+            dn[i] *= s;
+            odd = __builtin_fmaf(up[i], 0.0f, __builtin_fmaf(dn[i], 0.0f, odd));
+        }
+    }
     // lanes 0 - 31: up, 32 - 63: dn
     constexpr int N = LPK <= 16 ? E / 2 : E;   // elements a lane is left with
     float v[N];
@@ -180,6 +190,7 @@ int ti_launch_key_bounds(int dtype, const ti_kv_cache *c, const ti_key_bounds *k
     p.smooth = c->smooth;
     p.bounds = kb->bounds;
     p.scale = kb->scale;
+    p.channel = kb->channel;
     p.positions = positions;
     p.qsl = qsl;
     p.bt = bt;

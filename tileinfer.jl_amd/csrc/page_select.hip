@@ -1,6 +1,6 @@
 // The pages that a query keeps by the bounds of their keys (page_bounds.hip).
 //
-// A query row q (one token, one query head) as whole numbers w_d = rint(q_d 2^-e), e the least exponent
+// A query row q (one token, one query head; times its dimensions' channels) as whole numbers w_d = rint(q_d 2^-e), e the least exponent
 // with |q| <= 127 2^e, has with any key inside a page's bounds at most the product
 //   2^e 2^e_page sum_d (w_d hi_d where w_d > 0, else w_d lo_d) = 2^e 2^e_page (relu(w) . hi + min(w, 0) . lo):
 // one int8 matrix product of depth 2 D, whose sums stay below 2^22 and are exact. The score of a page
@@ -33,7 +33,7 @@ constexpr int ONE = 8 * ROUND;   // the most keys that one wave searches (they s
 struct SelectParams {
     const void *q;
     const int8_t *bounds;
-    const float *scale;
+    const float *scale, *channel;
     const int32_t *positions, *qsl, *bt;
     int32_t *tables, *lengths;
     uint32_t *keys;   // two launches: [end - first][Hk][pitch]
@@ -104,6 +104,10 @@ __device__ __forceinline__ void quantize_rows(const SelectParams &p, const Step 
         } else {
 #pragma unroll
             for (int i = 0; i < E; i++) x[i] = Elt<uint16_t>::ld((const uint16_t *)p.q, src + i);
+        }
+        if (p.channel) {
+#pragma unroll
+            for (int i = 0; i < E; i++) x[i] *= p.channel[h * D + c + i];
         }
 #pragma unroll
         for (int i = 0; i < E; i++) {
@@ -676,6 +680,7 @@ int ti_launch_select_pages(const ti_select_args *a, hipStream_t s) {
     p.q = a->q;
     p.bounds = a->bounds.bounds;
     p.scale = a->bounds.scale;
+    p.channel = a->bounds.channel;
     p.positions = a->positions;
     p.qsl = a->query_start_loc;
     p.bt = a->block_tables;

@@ -30,7 +30,7 @@ decltype(&ti_select_pages) f_select;
 decltype(&ti_sparse_attention) f_sparse;
 decltype(&ti_verify_draft) f_verify;
 PyObject *int8_pages, *key_bounds;   // Int8Pages, KeyBounds
-PyObject *n_layer_q, *n_layer_scale, *n_smooth, *n_half, *n_cos_sin, *n_bounds, *n_scale, *n_page_size;   // attribute names
+PyObject *n_layer_q, *n_layer_scale, *n_smooth, *n_half, *n_cos_sin, *n_bounds, *n_scale, *n_channel, *n_page_size;   // attribute names
 
 struct NotPlain {};   // leave the call to backend.py
 
@@ -129,17 +129,19 @@ struct OneGpu {
 
 // The tensors of a KeyBounds; its shape is (pages, kv_heads, page_size, D).
 struct Bounds {
-    Attr b, s;
+    Attr b, s, c;
     ti_key_bounds ptr;
     int64_t pages, heads, page, D;
     Bounds(PyObject *o, const OneGpu &gpu)
-        : b((require((PyObject *)Py_TYPE(o) == key_bounds), o), n_bounds), s(o, n_scale) {
-        const at::Tensor &bt = gpu(b.o), &st = gpu(s.o);
+        : b((require((PyObject *)Py_TYPE(o) == key_bounds), o), n_bounds), s(o, n_scale), c(o, n_channel) {
+        const at::Tensor &bt = gpu(b.o), &st = gpu(s.o), *ct = gpu.or_none(c.o);
         const Attr p(o, n_page_size);
         require(bt.dim() == 4 && bt.scalar_type() == at::kChar && st.scalar_type() == at::kFloat && bt.size(2) == 2);
         require(st.dim() == 2 && st.size(0) == bt.size(0) && st.size(1) == bt.size(1));
         pages = bt.size(0), heads = bt.size(1), page = integer(p.o), D = bt.size(3);
-        ptr = {static_cast<int8_t *>(bt.data_ptr()), static_cast<float *>(st.data_ptr())};
+        require(!ct || (ct->scalar_type() == at::kFloat && ct->dim() == 2 && ct->size(0) == heads && ct->size(1) == D));
+        ptr = {static_cast<int8_t *>(bt.data_ptr()), static_cast<float *>(st.data_ptr()),
+               ct ? static_cast<const float *>(ct->data_ptr()) : nullptr};
     }
 };
 
@@ -422,6 +424,7 @@ PyMODINIT_FUNC PyInit__calls() {
     n_cos_sin = PyUnicode_InternFromString("cos_sin");
     n_bounds = PyUnicode_InternFromString("bounds");
     n_scale = PyUnicode_InternFromString("scale");
+    n_channel = PyUnicode_InternFromString("channel");
     n_page_size = PyUnicode_InternFromString("page_size");
     PyObject *m = PyModule_Create(&module);
     // the torch and Python whose layouts this was compiled for; _lib.py compares

@@ -52,7 +52,7 @@ class AttentionArgs(ctypes.Structure):
 
 class KeyBoundsArgs(ctypes.Structure):
     """ti_key_bounds: the bounds of a layer's pages (device pointers)."""
-    _fields_ = [("bounds", ctypes.c_void_p), ("scale", ctypes.c_void_p)]
+    _fields_ = [("bounds", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("channel", ctypes.c_void_p)]
 
 
 def _fields(*groups):

@@ -312,6 +312,12 @@ def _cache_tensors(k_pages, v_pages):
     return k_pages, v_pages
 
 
+def _bounds_struct(b: KeyBounds) -> KeyBoundsArgs:
+    if b.channel is not None and (b.channel.dtype != torch.float32 or b.channel.shape != (b.bounds.shape[1], b.bounds.shape[3])):
+        raise ArgumentError("channel must be float32 [kv_heads][D]")
+    return KeyBoundsArgs(_ptr(b.bounds), _ptr(b.scale), _ptr(b.channel))
+
+
 def _step(block_tables, positions, query_start_loc, max_query_len):
     """(block tables as rows, sequences, most queries of one) of a step, as paged_attention_ takes it."""
     bts = block_tables if block_tables.dim() == 2 else block_tables.view(1, -1)
@@ -346,13 +352,13 @@ def update_key_bounds_(be: HipBackend, bounds: KeyBounds, k_pages, v_pages, bloc
     pages there is nothing else to call. Returns bounds."""
     if _done(_lib.native().update_key_bounds(bounds, k_pages, v_pages, block_tables, positions, query_start_loc, max_query_len)):
         return bounds
-    on = _one_device(bounds.bounds, bounds.scale, *_cache_tensors(k_pages, v_pages), block_tables, positions, query_start_loc)
+    on = _one_device(bounds.bounds, bounds.scale, bounds.channel, *_cache_tensors(k_pages, v_pages), block_tables, positions, query_start_loc)
     bts, B, n = _step(block_tables, positions, query_start_loc, max_query_len)
     c = kv_cache_struct(k_pages, v_pages)
     if bounds.shape != (c.num_pages, c.kv_heads, c.page_size, c.head_dim):
         raise ArgumentError("bounds do not belong to pools of this shape")
     dtype = _lib.TI_BF16 if c.kind == _lib.TI_KV_INT8 else _dtype(k_pages)
-    kb = KeyBoundsArgs(_ptr(bounds.bounds), _ptr(bounds.scale))
+    kb = _bounds_struct(bounds)
     with on:
         check(_lib.load().ti_update_key_bounds(
             dtype, ctypes.byref(c), ctypes.byref(kb), _ptr(bts), bts.shape[1], _ptr(positions), _ptr(query_start_loc), B, n,
@@ -387,12 +393,14 @@ def select_pages_(be: HipBackend, tables, lengths, workspace, q, bounds: KeyBoun
     int32: 1-based page ids in order of position, zero-padded; lengths [n][kv_heads] int32: the
     keys they hold, as sparse_attention_ takes both. The first `sinks` and the last `window` visible
     pages are always kept, the others by the largest product that a key inside their bounds could have
-    with any of the KV head's queries (rounded to whole numbers); equal ones in order. Rows that belong
-    to no sequence are left as they were. Returns (tables, lengths)."""
+    with any of the KV head's queries (rounded to whole numbers); equal ones in order. Bounds and queries are
+    rounded to 8 bits per head, which loses pages where a few dimensions are much larger than the rest
+    unless the bounds have a channel (KeyBounds). Rows that belong to no sequence are left as they were.
+    Returns (tables, lengths)."""
     if _done(_lib.native().select_pages(tables, lengths, workspace, q, bounds, block_tables, positions, sinks, window, causal,
                                         query_start_loc, max_query_len)):
         return tables, lengths
-    on = _one_device(q, bounds.bounds, bounds.scale, block_tables, positions, query_start_loc, tables, lengths, workspace)
+    on = _one_device(q, bounds.bounds, bounds.scale, bounds.channel, block_tables, positions, query_start_loc, tables, lengths, workspace)
     bts, B, n = _step(block_tables, positions, query_start_loc, max_query_len)
     _i32(tables, "tables")
     _i32(lengths, "lengths")
@@ -402,7 +410,7 @@ def select_pages_(be: HipBackend, tables, lengths, workspace, q, bounds: KeyBoun
     if tables.dim() != 3 or tables.shape[:2] != (q.shape[0], H) or lengths.shape != (q.shape[0], H):
         raise ArgumentError("tables must be [n][kv_heads][keep] and lengths [n][kv_heads]")
     a = _select_args(q, bounds, bts.shape[1], B, n, tables.shape[2], int(sinks), int(window), causal)
-    a.q, a.bounds.bounds, a.bounds.scale, a.positions = _ptr(q), _ptr(bounds.bounds), _ptr(bounds.scale), _ptr(positions)
+    a.q, a.bounds, a.positions = _ptr(q), _bounds_struct(bounds), _ptr(positions)
     a.query_start_loc, a.block_tables, a.tables, a.lengths = _ptr(query_start_loc), _ptr(bts), _ptr(tables), _ptr(lengths)
     _give_workspace(a, workspace)
     with on:

@@ -147,13 +147,19 @@ class KeyBounds:
     """Bounds of the keys of a layer's pages, beside its pools of either kind: for each page and KV
     head the keys' largest and smallest element in each dimension as whole multiples of the page's
     power of two. `bounds` [pages][H][2][D] int8 (largest first), `scale` [pages][H] f32;
-    update_key_bounds_ writes them, select_pages_ scores pages by them."""
+    update_key_bounds_ writes them, select_pages_ scores pages by them.
 
-    def __init__(self, bounds: torch.Tensor, scale: torch.Tensor, page_size: int):
+    channel: what keys of each dimension are about as large as ([D] or [H][D], positive), rounded here to powers
+    of two between 2^-30 and 2^30: keys are divided by them before they are bounded, queries multiplied, so that
+    dimensions with large keys do not take the others' precision. Good values are the largest |k| of each dimension over
+    sample keys, or key_smoothing(k_norm); None where keys are about alike. Kept as `channel` [H][D] f32 or None."""
+
+    def __init__(self, bounds: torch.Tensor, scale: torch.Tensor, page_size: int, channel: Optional[torch.Tensor] = None):
         if bounds.dtype != torch.int8 or scale.dtype != torch.float32 or bounds.dim() != 4 or bounds.shape[2] != 2 \
                 or scale.shape != bounds.shape[:2] or page_size <= 0:
             raise ArgumentError("bounds must be int8 [pages][kv_heads][2][D] and scale float32 [pages][kv_heads]")
         self.bounds, self.scale, self.page_size = bounds, scale, int(page_size)
+        self.channel = None if channel is None else _channel(channel, bounds)
 
     @property
     def shape(self):
@@ -162,24 +168,38 @@ class KeyBounds:
         return (pages, H, self.page_size, D)
 
 
-def key_bounds(head_dim: int, page_size: int, kv_heads: int, num_pages: int, device="cuda") -> KeyBounds:
+def _channel(channel: torch.Tensor, bounds: torch.Tensor) -> torch.Tensor:
+    """The nearest powers of two (by ratio), [H][D] on the bounds' device."""
+    H, D = bounds.shape[1], bounds.shape[3]
+    if channel.shape not in ((D,), (H, D)):
+        raise ArgumentError("channel must be [D] or [kv_heads][D]")
+    c = channel.detach().double().cpu()
+    if not bool(((c > 0) & torch.isfinite(c)).all()):
+        raise ArgumentError("channel must be positive and finite")
+    e = torch.log2(c).round().clamp(-30, 30)
+    return torch.exp2(e).float().expand(H, D).contiguous().to(bounds.device)
+
+
+def key_bounds(head_dim: int, page_size: int, kv_heads: int, num_pages: int, device="cuda",
+               channel: Optional[torch.Tensor] = None) -> KeyBounds:
     """The zeroed KeyBounds of one layer."""
     return KeyBounds(torch.zeros((num_pages, kv_heads, 2, head_dim), dtype=torch.int8, device=device),
-                     torch.zeros((num_pages, kv_heads), dtype=torch.float32, device=device), page_size)
+                     torch.zeros((num_pages, kv_heads), dtype=torch.float32, device=device), page_size, channel)
 
 
 class PagedKVCache:
     """Key/value pools for every layer and their page allocator (src/kv/paged_cache.jl:18-36).
     quantize=None: pools in `dtype`; quantize="int8": Int8Pages pairs. bounds=True: a KeyBounds
-    for every layer in `bounds`, for attention over chosen pages."""
+    for every layer in `bounds`, for attention over chosen pages; bounds_channel: the channel of each layer's."""
 
     def __init__(self, num_layers: int, head_dim: int, kv_heads: int, num_pages: int,
                  page_size: int = DEFAULT_PAGE_SIZE, dtype=torch.bfloat16, quantize=None,
-                 key_smoothing=None, device="cuda", bounds: bool = False):
+                 key_smoothing=None, device="cuda", bounds: bool = False, bounds_channel=None):
         self.blocks = BlockManager(num_pages, page_size)
         self.quantize = quantize
-        self.bounds = [key_bounds(head_dim, page_size, kv_heads, num_pages, device) for _ in range(num_layers)] \
-            if bounds else None
+        self.bounds = [key_bounds(head_dim, page_size, kv_heads, num_pages, device,
+                                  None if bounds_channel is None else bounds_channel[l])
+                       for l in range(num_layers)] if bounds else None
         if quantize is None:
             shape = (num_pages, kv_heads, page_size, head_dim)
             self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
