@@ -253,7 +253,7 @@ typedef struct {
  * gets bounds 127 and -127 and an infinite scale, and is kept by every selection that reaches
  * its score. Pages whose id lies outside the pool, or past the block-table row, are skipped. Two
  * sequences of a call that write into one page, or two entries of a block-table row that name one,
- * are not supported: the page's bounds are one of the two's.
+ * are not supported: each part of the page's bounds is one of the two's.
  * head_dim 64 or 128. dtype: of dense pools.
  */
 int ti_update_key_bounds(int dtype, const ti_kv_cache *cache, const ti_key_bounds *bounds,

@@ -137,3 +137,22 @@ def test_attend_longest_table(P, width):
         assert size.value == 0
     c.page_size, a.table_width = 1, 2 ** 31 - 256
     assert L.ti_sparse_attention(ctypes.byref(a), ctypes.byref(c), None) == _lib.TI_ERR_WORKSPACE
+
+
+def test_launches_past_32_bits_of_threads():
+    """Work-groups times 256 threads have to fit 32 bits: refused before any HIP call, not a failed launch."""
+    L, size = ti.load_library(), ctypes.c_size_t(7)
+    c, a = _lib.KVCache(), _lib.SparseAttentionArgs()
+    c.kind, c.head_dim, c.page_size, c.kv_heads, c.num_pages, c.k_pages, c.v_pages = 0, 128, 16, 8, 100, PTR, PTR
+    a.dtype, a.q_heads, a.table_width, a.num_seqs, a.max_query_len, a.scale = 1, 8, 64, 1, 1, 0.1
+    a.q = a.out = a.tables = a.lengths = a.query_start_loc = PTR
+    call = lambda: L.ti_sparse_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(c), ctypes.byref(size))
+    a.total_tokens = 2 ** 21
+    assert call() == _lib.TI_ERR_UNSUPPORTED and L.ti_sparse_attention(ctypes.byref(a), ctypes.byref(c), None) == _lib.TI_ERR_UNSUPPORTED
+    a.total_tokens = 2 ** 21 - 1
+    assert call() == _lib.TI_OK
+    a.total_tokens, a.max_query_len = 2 ** 23 - 1, 2 ** 20     # 16 tokens together
+    assert call() == _lib.TI_OK
+    kb = _lib.KeyBoundsArgs(PTR, PTR)
+    assert L.ti_update_key_bounds(1, ctypes.byref(c), ctypes.byref(kb), PTR, 2 ** 24, PTR, None, 1, 2 ** 28, 2 ** 28, None) \
+        == _lib.TI_ERR_UNSUPPORTED

@@ -135,7 +135,8 @@ int check_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
     if ((long long)a->table_width * c->page_size > 0x7fffff00LL ||
         (long long)a->total_tokens * a->q_heads * 32 > 0x7fffffffLL || a->q_heads > 65535)
         return TI_ERR_UNSUPPORTED;
-    return a->dtype == TI_BF16 && a->q_heads / c->kv_heads > 64 ? TI_ERR_UNSUPPORTED : TI_OK;
+    if (a->dtype == TI_BF16 && a->q_heads / c->kv_heads > 64) return TI_ERR_UNSUPPORTED;
+    return ti_sparse_groups(a, c) * 256 > MAX_THREADS ? TI_ERR_UNSUPPORTED : TI_OK;
 }
 
 int check_verify(const ti_verify_args *a) {

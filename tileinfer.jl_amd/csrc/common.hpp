@@ -117,6 +117,9 @@ __device__ __forceinline__ int clamp_page(int raw, int num_pages) { return min(m
 
 }  // namespace ti
 
+// The most threads of a launch in one dimension of its grid.
+constexpr long long MAX_THREADS = 0xffffffffLL;
+
 // Launchers implemented per kernel file, dispatched by api.hip.
 int ti_launch_rmsnorm(int dtype, void *y, const void *x, const void *w, int rows, int H, float eps,
                       hipStream_t s);
@@ -185,6 +188,7 @@ struct ti_sparse_plan {
 };
 ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c);
 size_t ti_sparse_bytes(const ti_sparse_attention_args *a, const ti_kv_cache *c);
+long long ti_sparse_groups(const ti_sparse_attention_args *a, const ti_kv_cache *c);   // work-groups of the launch
 size_t ti_sparse_bound(const ti_sparse_attention_args *a, const ti_kv_cache *c);
 int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c, hipStream_t s);
 bool ti_sparse_f32_mfma(const ti_sparse_attention_args *a, const ti_kv_cache *c);

@@ -589,7 +589,7 @@ int ti_launch_sparse_f32(const ti_sparse_attention_args *a, const ti_kv_cache *c
         f.qtiles = 1;
         f.splits = splits;
         f.scale_log2 = a->scale * LOG2E;
-        const unsigned grid = (unsigned)(((long long)a->total_tokens + pl.tg - 1) / pl.tg * c->kv_heads * splits);
+        const unsigned grid = (unsigned)ti_sparse_groups(a, c);
         if (pl.tg > 1) {
             const size_t lds = (size_t)pl.tg * pl.tg * a->table_width * sizeof(uint16_t);
             if (c->head_dim == 128) attn_f32_kernel<128, false, true, true><<<grid, 256, lds, s>>>(f);

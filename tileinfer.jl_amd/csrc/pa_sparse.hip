@@ -179,6 +179,11 @@ ti_sparse_plan ti_plan_sparse(const ti_sparse_attention_args *a, const ti_kv_cac
     return pl;
 }
 
+long long ti_sparse_groups(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
+    const ti_sparse_plan pl = ti_plan_sparse(a, c);
+    return ((long long)a->total_tokens + pl.tg - 1) / pl.tg * c->kv_heads * pl.splits;
+}
+
 size_t ti_sparse_bytes(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
     const ti_sparse_plan pl = ti_plan_sparse(a, c);
     if (pl.splits == 1) return 0;
@@ -228,7 +233,7 @@ int ti_launch_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_ca
     p.nmax = 1;
     p.splits = pl.splits;
     p.scale_log2 = a->scale * LOG2E;
-    const unsigned grid = (unsigned)(((long long)a->total_tokens + pl.tg - 1) / pl.tg * c->kv_heads * p.splits);
+    const unsigned grid = (unsigned)ti_sparse_groups(a, c);
     if (a->dtype == TI_F32) {
         p.min_tiles = ti_launch_sparse_f32(a, c, pl, s);
         if (p.min_tiles < 0) return TI_ERR_LAUNCH;

@@ -202,7 +202,7 @@ int ti_launch_key_bounds(int dtype, const ti_kv_cache *c, const ti_key_bounds *k
     p.total = total;
     const long long pages = min(((long long)nmax + c->page_size - 2) / c->page_size + 1, (long long)bt_stride);
     const long long groups = (pages * c->kv_heads + 3) / 4;
-    if (pages * c->kv_heads > 0x7fffff00LL) return TI_ERR_UNSUPPORTED;
+    if (groups * 256 > MAX_THREADS) return TI_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)groups, num_seqs);
     const bool wide = c->head_dim == 128;
     if (c->kind == TI_KV_INT8) {
