@@ -375,10 +375,8 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
     }
     const int q0 = GROUP && p.qsl ? max(p.qsl[0], 0) : 0, q1 = GROUP ? (p.qsl ? min(p.qsl[p.B], p.total) : p.total) : 0;
     int len = start + nb;
-    if constexpr (GROUP) {
-        __shared__ int red[1 + NW];
-        len = group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem_raw), lim, red, tok0, h, q0, q1) * p.P;
-    }
+    __shared__ int red[2 + NW];   // GROUP
+    if constexpr (GROUP) len = group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem_raw), lim, red, tok0, h, q0, q1) * p.P;
     const int ntiles = (len + 15) >> 4;
     const int per = (ntiles + nsp - 1) / nsp;
     const int j0 = s * per, j1 = min(j0 + per, ntiles);
@@ -801,7 +799,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
         l[rb] += __shfl_xor(l[rb], 16);
         l[rb] += __shfl_xor(l[rb], 32);
     }
-    bool fine = true;   // GROUP: no value that is not finite has come in
+    bool fine = true;   // GROUP: no value that is not finite has come in (rows of tokens without keys: none does, they are zeros)
 #pragma unroll
     for (int hb = 0; hb < ROWB; hb += HB) {
         __syncthreads();   // every wave is done with its V tile
@@ -833,9 +831,17 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
                 acc += *reinterpret_cast<const f32x4 *>(src + d4) * wgt;
             }
             if constexpr (GROUP && !INT8) {
-                fine &= fabsf(lsum) < INFINITY;
+                bool finite = fabsf(lsum) < INFINITY;
 #pragma unroll
-                for (int e = 0; e < 4; e++) fine &= fabsf(acc[e]) < INFINITY;
+                for (int e = 0; e < 4; e++) finite &= fabsf(acc[e]) < INFINITY;
+                if (!finite) {
+                    if (red[1 + NW] >> (r / p.G) & 1) {
+                        fine = false;
+                    } else {
+                        acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+                        lsum = 0.0f;
+                    }
+                }
             }
             if (nsp == 1) {
                 // One split: this group saw every key; normalize and write the output rows.
@@ -861,7 +867,6 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
     if constexpr (GROUP && !INT8) {
         // The slabs have overwritten the joined list: it is made again.
         if (__syncthreads_or(!fine)) {
-            __shared__ int red[1 + NW];
             group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem_raw), lim, red, tok0, h, q0, q1);
             group_rows<D>(p, reinterpret_cast<const int2 *>(smem_raw), lim, tok0, h, q0, q1, j0, j1, nsp, unit, w, NW, lane);
         }

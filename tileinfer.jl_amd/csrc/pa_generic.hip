@@ -245,9 +245,11 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     }
     int len = start + nb;
     const int q0 = GROUP && p.qsl ? max(p.qsl[0], 0) : 0, q1 = GROUP ? (p.qsl ? min(p.qsl[p.B], p.total) : p.total) : 0;
+    uint32_t keyed = 0;   // GROUP: the tokens with keys; the others' queries may hold anything
     if constexpr (GROUP) {
-        __shared__ int red[1 + NW];
+        __shared__ int red[2 + NW];
         len = group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem), lim, red, tok0, h, q0, q1) * p.P;
+        keyed = (uint32_t)__builtin_amdgcn_readfirstlane(red[1 + NW]);
     }
     // splits cut the sequence's 16-key tiles (the combine derives the same count; GROUP: every split writes a
     // partial); this q-tile's keys end after its last token's position
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     const GroupMap gm{reinterpret_cast<const int2 *>(smem), p.P, p.pshift, p.Hk, h, len};
     const int j0 = s * as.per, j1 = min(j0 + as.per, (kend + 15) >> 4);   // may be empty: (m, l) = (NEG_BIG, 0)
     const int r = 16 * qt + r16, t = r / p.G, g = r - t * p.G;
-    const bool ok = r < p.M && t < nb && (!GROUP || (tok0 + t >= q0 && tok0 + t < q1));
+    const bool ok = r < p.M && (GROUP ? (keyed >> t & 1) != 0 : t < nb);
     const int qpos = p.causal && ok ? start + t : len - 1;
     const int mask_from = p.causal ? start + t_first : len - 1;   // keys up to here are visible to every row
     f32x4 qv[NJ];
@@ -424,7 +426,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     if constexpr (GROUP) {
         // as the bf16 kernel: the slabs have overwritten the joined list, which is made again
         if (__syncthreads_or(!fine)) {
-            __shared__ int red[1 + NW];
+            __shared__ int red[2 + NW];
             group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem), lim, red, tok0, h, q0, q1);
             group_rows<D>(p, reinterpret_cast<const int2 *>(smem), lim, tok0, h, q0, q1, j0, j1, p.splits, unit, w, NW, lane);
         }

@@ -39,7 +39,8 @@ struct GroupMap {
 // that a page that several tokens keep is read and multiplied once for all their rows. An entry's place is
 // that of its first mention (position in the table first, then token): found with a hash table in LDS whose
 // slots keep the smallest mention, so the list does not depend on the order of the threads. Where a token
-// names a page twice, every entry is a page of its own.
+// names a page twice, every entry is a page of its own. red: 2 + NT / 64 words of LDS; the last one then holds the
+// tokens that have keys, a bit each.
 constexpr int GROUP_PAGES = 1024, GROUP_SLOTS = 2 * GROUP_PAGES;
 struct GroupLds {
     int2 pages[GROUP_PAGES];             // {page, keys that some token sees}
@@ -78,6 +79,8 @@ __device__ __forceinline__ int group_pages(const Params &p, GroupLds &g, uint16_
         keys[n] = x < entries && tok >= q0 && tok < q1 ? min(len - a * p.P, p.P) : 0;
         id[n] = clamp_page(id[n], p.num_pages);
     }
+    const unsigned long long keyed = __ballot(tid < TG && keys[0] > 0);   // wave 0: the tokens' first entries
+    if (tid == 0) red[1 + NT / 64] = (int)keyed;
 #pragma unroll
     for (int n = 0; n < EACH; n++) {
         if (keys[n] <= 0) continue;
