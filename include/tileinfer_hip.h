@@ -329,6 +329,8 @@ typedef struct {
  * of them visible: the last entry in use may hold fewer than page_size keys. A token without keys
  * (length <= 0) gets zeros; longer lengths read as table_width * page_size. An entry outside the
  * pool is clamped into it, as in ti_attention; a page that a table names twice counts twice.
+ * Over INT8 caches a weight (at most 1) times its value's scale is held in 16 bits, as in ti_attention: value
+ * scales above 65504 overflow, and products below 2^-14 are rounded to multiples of 2^-24.
  * ti_sparse_attention_workspace_bytes is what a call of exactly these sizes needs: fewer tokens, or another
  * max_query_len, may need more, because keys are split where work-groups are few. ..._workspace_bound is enough
  * for every call with these heads, types and pages of at most total_tokens tokens, max_query_len tokens a sequence

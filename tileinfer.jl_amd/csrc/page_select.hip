@@ -619,7 +619,9 @@ int launch(SelectParams p, int num_seqs, hipStream_t s) {
     if (fits_one_launch<TT>(p, groups)) {
         // 4 waves for short tables, whose pages give 16 waves little to do, and for several work-groups per CU,
         // which wait for each other less (while LDS holds four): 128 pages and 64 work-groups 7.1 us and 7.8 with
-        // 16, 512 and 512 19.2 and 25.2, 2048 and 512 68 and 76; 2048 and 128 27.7 and 25.9.
+        // 16, 512 and 512 19.2 and 25.2, 2048 and 512 68 and 76; 2048 and 128 27.7 and 25.9. Single tokens of 1 to 32
+        // sequences (8 to 256 work-groups): 64 pages 5.5 and 6.2, 256 9.3-11.0 and 12.9-13.3, 512 11.7-13.4 and
+        // 15.3-16.6; 768 14.2-17.0 and 17.4-20.0, where tiles of several tokens were not measured.
         if constexpr (RT == 1)
             if (key_bytes(p, TT) <= (32u << 10) && (p.bt_stride <= 512 || groups >= 512)) return launch_one<D, GP, RT, WIDE, 4>(p, y, num_seqs, s);
         return launch_one<D, GP, RT, WIDE, W>(p, y, num_seqs, s);
