@@ -155,3 +155,31 @@ def test_queries_of_tokens_without_keys_are_not_read(gpu, kv, rows, heads, width
     q[pad] = math.nan
     got = ti.sparse_attention(BE, q, c.k, c.v, tables, lengths, 0.09, None, rows)
     assert torch.equal(got, want) and (got[pad] == 0).all()
+
+
+@pytest.mark.parametrize("P,width", [(16, 1500), (1, 33500)])
+def test_selection_with_many_rows_of_no_sequence(gpu, P, width):
+    """A few tokens far behind the start of an array of 3000 rows, over tables that take two launches (with and
+    without LDS for a tile's keys): the same as those tokens alone, the other rows as they were."""
+    pages, H, first, counts = 4000, 8, 1700, [3, 0, 2, 1]
+    starts = [width * P - 4, 0, 50, width * P // 2]
+    g = torch.Generator().manual_seed(57)
+    tables = torch.randint(1, pages + 1, (4, width), generator=g, dtype=torch.int32).cuda()
+    kb = random_bounds(pages, H, 64, P, 57)
+    torch.manual_seed(57)
+    rows, n = 3000, sum(counts)
+    q = torch.randn((rows, H * 4, 64), device="cuda", dtype=torch.bfloat16)
+    pos = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    pos[first:first + n] = positions(starts, counts)
+    out = torch.full((rows, H, 20), -5, dtype=torch.int32, device="cuda")
+    lengths = torch.full((rows, H), -5, dtype=torch.int32, device="cuda")
+    ws = ti.select_pages_workspace(BE, q, kb, tables)
+    ti.select_pages_(BE, out, lengths, ws, q, kb, tables, pos, 1, 2, True, offsets(counts) + first, 3)
+    a = slice(first, first + n)
+    want = ti.select_pages(BE, q[a], kb, tables, pos[a], 20, 1, 2, True, offsets(counts), 3)
+    assert torch.equal(out[a], want[0]) and torch.equal(lengths[a], want[1])
+    assert (out[:first] == -5).all() and (out[first + n:] == -5).all() and (lengths[:first] == -5).all()
+    hb, hs, ht = kb.bounds.cpu().numpy(), kb.scale.cpu().numpy(), tables.cpu().numpy()
+    for r, b, t in ((0, 0, 0), (4, 2, 1), (5, 3, 0)):
+        table, length = ref.select(q[first + r].double().cpu().numpy(), hb, hs, ht[b], starts[b] + t, P, 20, 1, 2)
+        assert np.array_equal(want[0][r].cpu().numpy(), table) and np.array_equal(want[1][r].cpu().numpy(), length)

@@ -36,10 +36,20 @@ struct SelectParams {
     const float *scale, *channel;
     const int32_t *positions, *qsl, *bt;
     int32_t *tables, *lengths;
-    uint32_t *keys;   // two launches: [end - first][Hk][pitch]
+    uint32_t *keys;   // two launches: [rows][Hk][pitch] (Part)
     int bt_stride, num_pages, P, Hk, Hq, G, nmax, total, keep, sinks, window, causal, f32, pshift;
     int pitch, split;   // keys per (token, KV head); work-groups that share a token tile's pages
-    int first, end;     // two launches: the rows of the packed tokens that they work on
+    int first, end;     // two launches: the packed tokens that they work on; end 0: all, a sequence's from row b nmax on
+};
+
+// Two launches: the tokens begin .. end - 1 of a sequence that they work on, and the workspace's row of its token 0.
+struct Part {
+    int begin, end, row;
+    __device__ Part(const SelectParams &p, const Step &st, int b) {
+        begin = p.end ? max(p.first - st.tok0, 0) : 0;
+        end = p.end ? min(st.n, p.end - st.tok0) : st.n;
+        row = p.end ? st.tok0 - p.first : b * p.nmax;
+    }
 };
 
 // What one token sees: pages [0, seen), of which [c0, c1) are up for choice and `need` kept by score.
@@ -525,7 +535,7 @@ __global__ void __launch_bounds__(W * 64) select_kernel(SelectParams p) {
     }
 }
 
-// The keys of a token tile to the workspace, for tokens first .. end - 1: grid (Hk x split, token tiles, B).
+// The keys of a token tile to the workspace: grid (Hk x split, token tiles, B).
 template <int D, int GP, int RT, bool WIDE, int W>
 __global__ void __launch_bounds__(W * 64) scores_kernel(SelectParams p) {
     using TL = Tile<GP, RT, WIDE>;
@@ -534,33 +544,32 @@ __global__ void __launch_bounds__(W * 64) scores_kernel(SelectParams p) {
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % p.Hk, part = blockIdx.x / p.Hk, b = blockIdx.z;
     const Step st = step_of(p.qsl, p.positions, b, p.nmax, p.total);
-    const int end = min(st.n, p.end - st.tok0);
-    for (int t0 = max(p.first - st.tok0, 0) / TL::TT * TL::TT + blockIdx.y * TL::TT; t0 < end; t0 += gridDim.y * TL::TT) {
+    const Part own(p, st, b);
+    for (int t0 = own.begin / TL::TT * TL::TT + blockIdx.y * TL::TT; t0 < own.end; t0 += gridDim.y * TL::TT) {
         __syncthreads();
-        const int tokens = min(TL::TT, end - t0);
+        const int tokens = min(TL::TT, own.end - t0);
         const int most = Seen(p, st, t0 + tokens - 1).seen, ntiles = (most + 15) >> 4;
         quantize_rows<D, GP, RT, WIDE, W>(p, st, h, t0, tid, w, forth);
         __syncthreads();
-        const int row = st.tok0 + t0 - p.first;   // the tile's first tokens may be before p.first
-        score_pages<D, GP, RT, WIDE>(p, b, h, max(-row, 0), tokens, lane, part * W + wv, p.split * W, ntiles, most, w, forth,
-                                     [&](int t, int page) { return p.keys + ((size_t)(row + t) * p.Hk + h) * p.pitch + page; });
+        score_pages<D, GP, RT, WIDE>(p, b, h, max(own.begin - t0, 0), tokens, lane, part * W + wv, p.split * W, ntiles, most, w, forth,
+                                     [&](int t, int page) { return p.keys + ((size_t)(own.row + t0 + t) * p.Hk + h) * p.pitch + page; });
     }
 }
 
 // Kept pages of one token and KV head from the workspace: grid (Hk, tokens, B). The keys are read into LDS
-// where it holds them (`lds` of them). Tokens as scores_kernel.
+// where it holds them (`lds` of them).
 template <int W> __global__ void __launch_bounds__(W * 64) keep_kernel(SelectParams p, int lds) {
     __shared__ SearchLds<W> search;
     extern __shared__ __attribute__((aligned(16))) uint32_t held[];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x, b = blockIdx.z;
     const Step st = step_of(p.qsl, p.positions, b, p.nmax, p.total);
-    const int end = min(st.n, p.end - st.tok0);
-    for (int t = max(p.first - st.tok0, 0) + blockIdx.y; t < end; t += gridDim.y) {
+    const Part own(p, st, b);
+    for (int t = own.begin + blockIdx.y; t < own.end; t += gridDim.y) {
         const Seen s(p, st, t);
         const int span = (s.seen + ROUND - 1) / ROUND * ROUND;
         const size_t pair = (size_t)(st.tok0 + t) * p.Hk + h;
-        uint32_t *keys = p.keys + ((size_t)(st.tok0 + t - p.first) * p.Hk + h) * p.pitch;
+        uint32_t *keys = p.keys + ((size_t)(own.row + t) * p.Hk + h) * p.pitch;
         __syncthreads();   // the token before this one is done with LDS
         const int32_t *bt = p.bt + (size_t)b * p.bt_stride;
         if (span <= lds) {
@@ -629,18 +638,21 @@ int launch(SelectParams p, int num_seqs, hipStream_t s) {
     if constexpr (RT == 1 || WIDE) {   // launch_rows takes tiles of several tokens' blocks for one launch only
         const size_t held = std::min((size_t)p.pitch * sizeof(uint32_t), (size_t)LDS_KEYS);
         if (!allow_lds((const void *)keep_kernel<W>, held)) return TI_ERR_LAUNCH;
-        // as many tokens at a time as the workspace holds; a part of a sequence may begin inside a tile
+        // All tokens at once where the workspace has a row for each that the sequences can have (always, where LDS holds
+        // a tile's keys), or for each row of the packed tokens, else as many rows at a time as it has. A part of a
+        // sequence may begin inside a tile.
         const int rows = (int)(scratch_bytes(p.total, p.Hk, p.pitch, TT) / row_bytes(p.Hk, p.pitch));
+        const bool whole = (long long)num_seqs * p.nmax <= rows;
         const long long most = std::min(tiles, ((long long)rows + TT - 1) / TT + 1);
         p.split = 1;
         while (std::min(groups, most * num_seqs * p.Hk) * p.split < 256 && p.split * W * 32 < p.bt_stride) p.split <<= 1;
         for (p.first = 0;; p.first = p.end) {
-            p.end = p.total - p.first > rows ? p.first + rows : p.total;
+            p.end = whole ? 0 : p.total - p.first > rows ? p.first + rows : p.total;
             scores_kernel<D, GP, RT, WIDE, W><<<dim3(p.Hk * p.split, min(y, (unsigned)most), num_seqs), W * 64, 0, s>>>(p);
             if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
             keep_kernel<W><<<dim3(p.Hk, min(min(p.nmax, rows), 32768), num_seqs), W * 64, held, s>>>(p, (int)(held / sizeof(uint32_t)));
             if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
-            if (p.end == p.total) return TI_OK;
+            if (whole || p.end == p.total) return TI_OK;
         }
     }
     return TI_ERR_LAUNCH;
