@@ -183,3 +183,55 @@ def test_selection_with_many_rows_of_no_sequence(gpu, P, width):
     for r, b, t in ((0, 0, 0), (4, 2, 1), (5, 3, 0)):
         table, length = ref.select(q[first + r].double().cpu().numpy(), hb, hs, ht[b], starts[b] + t, P, 20, 1, 2)
         assert np.array_equal(want[0][r].cpu().numpy(), table) and np.array_equal(want[1][r].cpu().numpy(), length)
+
+
+def shifted(x, by=1):
+    """The same values, `by` elements behind an aligned address."""
+    flat = torch.empty(x.numel() + by, dtype=x.dtype, device=x.device)
+    flat[by:] = x.reshape(-1)
+    return flat[by:].view(x.shape)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp32", "int8"])
+@pytest.mark.parametrize("rows", [1, 20])
+def test_tensors_aligned_to_their_elements_only(gpu, kv, rows):
+    """Queries, outputs, pools, tables, positions and probabilities that begin one element behind an aligned address
+    (workspaces and bounds have to be aligned): the bits of aligned ones."""
+    D, H, P = 128, 2, 16
+    c = Cache(kv, D, H, P, [600], seed=58)
+    torch.manual_seed(58)
+    q = torch.randn((rows, 8, D), device="cuda", dtype=T[kv])
+    pos = positions([600 - rows], [rows])
+    results = []
+    for f in (lambda x: x, shifted):
+        k, v = c.k, c.v
+        if kv == "int8":
+            lq, ls, sm = f(k.layer_q), f(k.layer_scale), f(k.smooth)
+            k, v = ti.Int8Pages(lq, ls, sm, 0), ti.Int8Pages(lq, ls, v.smooth, 1)
+        else:
+            k, v = f(k), f(v)
+        kb = ti.key_bounds(D, P, H, c.pages)
+        kb.scale = f(kb.scale)
+        bt, qq = f(c.tables), f(q)
+        ti.update_key_bounds_(BE, kb, k, v, bt, f(positions([0], [600])), max_query_len=600)
+        tables, lengths = f(torch.zeros((rows, H, 9), dtype=torch.int32, device="cuda")), f(torch.zeros((rows, H), dtype=torch.int32, device="cuda"))
+        ti.select_pages_(BE, tables, lengths, ti.select_pages_workspace(BE, q, kb, bt), qq, kb, bt, f(pos), max_query_len=rows)
+        out = f(torch.zeros_like(q))
+        ti.sparse_attention_(BE, out, ti.sparse_attention_workspace(BE, q, k, tables, rows), qq, k, v, tables, lengths, 0.09, None, rows)
+        results.append((kb.bounds, kb.scale, tables, lengths, out))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    check_attend(c, q, results[0][2], results[0][3], scale=0.09, n=rows)
+
+
+@pytest.mark.parametrize("kv,D", [("bf16", 128), ("int8", 128), ("fp32", 64), ("int8_fp32", 64), ("bf16", 64)])
+@pytest.mark.parametrize("rows", [1, 2])
+def test_long_tables(gpu, kv, D, rows):
+    """200000 keys a token, the pages of a small pool named again and again."""
+    c = Cache(kv, D, 1, 16, [300 * 16], seed=59)
+    g = torch.Generator().manual_seed(59)
+    torch.manual_seed(59)
+    q = torch.randn((rows, 4, D), device="cuda", dtype=T[kv])
+    tables = torch.randint(1, c.pages + 1, (rows, 1, 12500), generator=g, dtype=torch.int32).cuda()
+    lengths = i32([[200000], [199991]][:rows])
+    check_attend(c, q, tables, lengths, n=rows)

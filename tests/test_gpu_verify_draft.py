@@ -172,3 +172,14 @@ def test_uniforms_that_are_nan(gpu, dtype, given):
     u[:3, 0] = math.nan
     acc, tok = check(p, q, x, u)
     assert (acc[:3] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tensors_aligned_to_their_elements_only(gpu, dtype):
+    """Rows that begin one element behind an aligned address."""
+    def shifted(x):
+        flat = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+        flat[1:] = x.reshape(-1)
+        return flat[1:].view(x.shape)
+
+    check(*(shifted(t) for t in inputs(7, 3, 5000, dtype, seed=12)))
