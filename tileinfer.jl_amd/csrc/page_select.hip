@@ -1,7 +1,8 @@
 // The pages that a query keeps by the bounds of their keys (page_bounds.hip).
 //
-// A query row q (one token, one query head; times its dimensions' channels) as whole numbers w_d = rint(q_d 2^-e), e the least exponent
-// with |q| <= 127 2^e, has with any key inside a page's bounds at most the product
+// A query row q (one token, one query head; times its dimensions' channels) becomes whole numbers
+// w_d = rint(q_d 2^-e), e the least exponent with |q| <= 127 2^e; the row 2^e w so rounded has with any key
+// inside a page's bounds at most the product
 //   2^e 2^e_page sum_d (w_d hi_d where w_d > 0, else w_d lo_d) = 2^e 2^e_page (relu(w) . hi + min(w, 0) . lo):
 // one int8 matrix product of depth 2 D, whose sums stay below 2^22 and are exact. The score of a page
 // for a token and KV head is the largest over the G query heads, two multiplications by powers of
