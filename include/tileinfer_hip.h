@@ -5,7 +5,7 @@
  * The entry points of paged attention and the cache replace one method each of the reference's
  * op interface (src/ops/interface.jl) for its TileBackend kernels; each declaration cites the
  * reference function it stands in for. Page bounds, page selection, attention over selected pages
- * and draft verification (last in this file) have no counterpart there: they work on the same
+ * and draft verification have no counterpart there: they work on the same
  * caches, block tables and steps. All pointers are device pointers unless noted;
  * calls enqueue work on `stream` and return without synchronizing. The library never
  * allocates device memory: the caller owns pools, inputs, outputs and the workspace.
@@ -20,6 +20,9 @@
  *     layer_q     (D, P, Hk, pages, 2) int8             -> [2][pages][Hk][P][D] (keys first)
  *     layer_scale (P, Hk, pages, 2) Float32             -> [2][pages][Hk][P]
  *     smooth      (D,) Float32 (the keys' smoothing; values use ones)
+ *   8-bit block layer arrays (TI_KV_FP8):
+ *     layer_q     [2][pages][Hk][P][D] e4m3 (keys first)
+ *     layer_scale [2][pages][Hk] Float32 powers of two
  *   rotary table cos_sin (D, 2 max_len)                 -> [max_len][2][D] (cos, then sin)
  *   block tables: int32, 1-based page ids, zero-padded past a sequence's pages
  *   slots: int32, 1-based, slot s = offset (s-1) % P of page (s-1) / P + 1
@@ -44,7 +47,7 @@ typedef enum {
 } ti_status;
 
 typedef enum { TI_F32 = 0, TI_BF16 = 1 } ti_dtype;      /* activations / dense pools */
-typedef enum { TI_KV_DENSE = 0, TI_KV_INT8 = 1 } ti_kv_kind;
+typedef enum { TI_KV_DENSE = 0, TI_KV_INT8 = 1, TI_KV_FP8 = 2 } ti_kv_kind;
 
 /* Path selection for ti_attention. AUTO follows the reference's rule
  * (src/ops/tile/attention.jl:265, :351-352): split-KV decode for short steps, the prefill
@@ -75,8 +78,16 @@ typedef enum {
     TI_PATH_PREFILL_PAIRED16 = 7,
 } ti_path;
 
-/* One layer's KV cache: dense pools in the activations' type, or an INT8 layer
- * (Int8Pages pair: src/ops/quant.jl:86-92). Host struct of device pointers. */
+/* One layer's KV cache: dense pools in the activations' type, an INT8 layer
+ * (Int8Pages pair: src/ops/quant.jl:86-92), or an 8-bit block layer. Host struct of device pointers.
+ *
+ * 8-bit block layers (TI_KV_FP8) hold e4m3 values and one scale for each block, the keys (or the values)
+ * of a page and KV head: a value stands for itself times the scale, a power of two between 2^-120 and 2^120.
+ * head_dim 64 or 128, pages of 2^k keys from 16 to 1024. ti_store_kv and ti_attention_inputs write them,
+ * ti_attention, ti_attention_noalloc and ti_window_attention read them; page bounds and sparse attention do not
+ * take them (TI_ERR_UNSUPPORTED). `path` names no variants for them: other than TI_PATH_DECODE, the library's pick
+ * runs. Where a product meets a value that is not finite, the rows of its work-group are done again key by
+ * key over what each of them sees (as in ti_window_attention): slow, and right. */
 typedef struct {
     int32_t kind;               /* ti_kv_kind */
     int32_t head_dim;           /* D: 64 or 128 */
@@ -85,8 +96,8 @@ typedef struct {
     int32_t num_pages;          /* pages in the pool; page ids are 1..num_pages */
     void *k_pages;              /* dense: [num_pages][Hk][P][D] */
     void *v_pages;
-    int8_t *layer_q;            /* int8: [2][num_pages][Hk][P][D] */
-    float *layer_scale;         /* int8: [2][num_pages][Hk][P] */
+    int8_t *layer_q;            /* int8, fp8: [2][num_pages][Hk][P][D] */
+    float *layer_scale;         /* int8: [2][num_pages][Hk][P]; fp8: [2][num_pages][Hk] */
     const float *smooth;        /* int8: [D] keys' smoothing factors */
 } ti_kv_cache;
 
@@ -179,6 +190,14 @@ int ti_attention_noalloc(const ti_attention_args *args, const ti_kv_cache *cache
  * (src/ops/tile/elementwise.jl:133-140 and :180-188; reference
  * src/ops/reference.jl:64-74, src/ops/quant.jl:147-159).
  * k, v: [n][Hk][D] in dtype. Slots outside the pool are skipped.
+ *
+ * 8-bit block layers: a block's scale is the least 2^e (e from -120 to 120) with |x| <= 448 2^e for every finite
+ * element that its rows were written with, and a row holds x 2^-e rounded to the nearest e4m3 value (ties to even);
+ * an element that is not finite is held as NaN. Rows are written from a page's first on: a call that writes a page's
+ * first row begins the block anew, with the scale of this call's rows alone (other rows of the page then hold
+ * nothing). Otherwise the scale only grows; where it does, the rows that the block holds are divided by the
+ * growth, which is exact but for values that become subnormal (each time rounded again, by at most 2^-10 of the
+ * new scale). The rows of one page may be anywhere among the call's; of two for one slot the later stays.
  */
 int ti_store_kv(int dtype, const ti_kv_cache *cache, const void *k, const void *v,
                 const int32_t *slots, int n, void *stream);
@@ -216,7 +235,7 @@ int ti_rope(int dtype, void *y, const void *x, const void *cos_table, const void
  * qkv: [n][q_heads + 2 Hk][D]; q_out: [n][q_heads][D]; q_norm, k_norm: [D] or both NULL;
  * cos_sin: [table_len][2][D]. A token whose position lies outside [0, table_len) writes
  * nothing (its q_out rows are left untouched and its K/V slot is not written); a token
- * whose slot lies outside the pool writes no K/V row.
+ * whose slot lies outside the pool writes no K/V row. 8-bit block layers are written as by ti_store_kv.
  */
 int ti_attention_inputs(int dtype, void *q_out, const ti_kv_cache *cache, const void *qkv,
                         const void *q_norm, const void *k_norm, const void *cos_sin,
@@ -366,6 +385,60 @@ typedef struct {
  */
 int ti_verify_draft_workspace_bytes(const ti_verify_args *args, size_t *bytes);
 int ti_verify_draft(const ti_verify_args *args, void *stream);
+
+/* ---- attention with a sliding window ----------------------------------------------------------
+ *
+ * ti_attention with causal = 1, where the query at position p sees the keys p - window + 1 .. p and the keys
+ * 0 .. sinks - 1 (never past p): window >= 1, sinks >= 0. Arguments, caches and steps as in ti_attention (path:
+ * TI_PATH_AUTO; workspace of ti_window_attention_workspace_bytes, which depends on the window too, mandatory
+ * where that is not 0). Block-table entries of pages that hold no visible key of any of the sequence's queries are not
+ * used: their pages may have been given back. Rows of q and out that belong to no sequence are left as they were.
+ *
+ * A key that a query does not see leaves its output as it is whatever the cache holds there, NaN and infinities
+ * among it. The rows of a work-group are worked on together, so where a product is not finite they are done
+ * again row by row over the keys that each sees: right, but slow (a cache with NaN in it takes hundreds of times as long).
+ */
+int ti_window_attention_workspace_bytes(const ti_attention_args *args, int window, int sinks, const ti_kv_cache *cache,
+                                        size_t *bytes);
+int ti_window_attention(const ti_attention_args *args, int window, int sinks, const ti_kv_cache *cache, void *stream);
+
+/* ---- the page bookkeeping of a step, on the device ----------------------------------------------
+ *
+ * The pages of a pool and the sequences that hold them, as device arrays: what BlockManager (src/kv/block_manager.jl:39-100)
+ * keeps on the host. A step can be reserved, run and taken back in one captured graph.
+ * Page i of sequence b (positions i P .. i P + P - 1) is tables[b][i]. With a window, release gives back the pages that
+ * no later query can see, those from page ceil(sinks / P) up to behind[b]; their entries are 0.
+ * Calls on one pool must not overlap. `ticket` is 0 between calls. */
+typedef struct {
+    int32_t num_pages, page_size;
+    int32_t num_seqs;                 /* S: 1 to 4096 */
+    int32_t table_width;              /* W */
+    int32_t window, sinks;            /* of the attention over the pool: window 0: none, every page is kept */
+    int32_t *free;                    /* [num_pages] stack of free page ids, 1-based, the next one on top */
+    int32_t *free_count;              /* [1] ids on the stack */
+    int32_t *tables;                  /* [S][W] page ids, 0 where none */
+    int32_t *lengths;                 /* [S] positions */
+    int32_t *behind;                  /* [S]; NULL without a window */
+    int32_t *ticket;                  /* [1] */
+} ti_page_pool;
+
+/*
+ * counts[b] more positions for each sequence (a negative count is 0): pages off the stack in order of sequence and position
+ * into the tables, lengths moved on, and the step's arrays: query_start_loc [S + 1]; positions and slots [tokens]
+ * of the step's tokens, 0 behind them (slot 0 writes nothing).
+ * short_of [1]: 0; or the pages that were missing; or -1 where a sequence would outgrow its table or the step
+ * `tokens`. Unless it is 0 nothing is reserved: pool unchanged, query_start_loc, positions and slots 0.
+ */
+int ti_reserve_pages(const ti_page_pool *pool, const int32_t *counts, int tokens, int32_t *positions, int32_t *slots,
+                     int32_t *query_start_loc, int32_t *short_of, void *stream);
+
+/*
+ * Sequences cut to keep[b] positions (0 .. lengths[b]; others are clamped): pages that only later positions use
+ * go back, and with a window those that a query at position keep[b] or later does not see. The stack gets them in
+ * the opposite order to that in which ti_reserve_pages takes them, so a step taken back whole leaves the pool as it was.
+ * A sequence must not be cut to below a position whose window reaches into pages given back before.
+ */
+int ti_release_pages(const ti_page_pool *pool, const int32_t *keep, void *stream);
 
 #ifdef __cplusplus
 }

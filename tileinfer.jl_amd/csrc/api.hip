@@ -34,13 +34,20 @@ int device_scratch(void **out) {
 
 bool bad_cache(const ti_kv_cache *c) {
     if (!c) return true;
-    if (c->kind != TI_KV_DENSE && c->kind != TI_KV_INT8) return true;
+    if (c->kind != TI_KV_DENSE && c->kind != TI_KV_INT8 && c->kind != TI_KV_FP8) return true;
     if (c->head_dim <= 0 || (c->head_dim & 1) || c->page_size <= 0 || c->kv_heads <= 0 ||
         c->num_pages <= 0)
         return true;
     if (c->kind == TI_KV_DENSE && (!c->k_pages || !c->v_pages)) return true;
     if (c->kind == TI_KV_INT8 && (!c->layer_q || !c->layer_scale || !c->smooth)) return true;
+    if (c->kind == TI_KV_FP8 && (!c->layer_q || !c->layer_scale || ((uintptr_t)c->layer_q & 15))) return true;
     return false;
+}
+
+// An 8-bit block layer of a shape that no kernel takes.
+bool odd_fp8(const ti_kv_cache *c) {
+    const int P = c->page_size;
+    return c->kind == TI_KV_FP8 && ((c->head_dim != 64 && c->head_dim != 128) || P < 16 || P > 1024 || (P & (P - 1)));
 }
 
 bool bad_dtype(int dtype) { return dtype != TI_F32 && dtype != TI_BF16; }
@@ -53,6 +60,7 @@ bool bad_dtype(int dtype) { return dtype != TI_F32 && dtype != TI_BF16; }
 int resolve_path(const ti_attention_args *a, const ti_kv_cache *c) {
     const int G = a->q_heads / c->kv_heads;
     if (a->dtype == TI_F32) return 0;
+    if (c->kind == TI_KV_FP8) return a->path < TI_PATH_AUTO || a->path > TI_PATH_PREFILL_PAIRED16 ? -TI_ERR_INVALID_ARG : 0;
     const int rows = G * a->max_query_len;
     const bool decode_ok = rows <= 64;
     const bool decode_auto = a->max_query_len <= 16 && (rows <= 32 || (a->max_query_len == 1 && decode_ok));
@@ -71,7 +79,7 @@ int resolve_path(const ti_attention_args *a, const ti_kv_cache *c) {
 
 int check_attention(const ti_attention_args *a, const ti_kv_cache *c) {
     if (!a || bad_cache(c) || bad_dtype(a->dtype)) return TI_ERR_INVALID_ARG;
-    if (c->head_dim != 64 && c->head_dim != 128) return TI_ERR_UNSUPPORTED;
+    if ((c->head_dim != 64 && c->head_dim != 128) || odd_fp8(c)) return TI_ERR_UNSUPPORTED;
     if (a->q_heads <= 0 || a->q_heads % c->kv_heads) return TI_ERR_INVALID_ARG;
     if (a->num_seqs <= 0 || a->max_query_len <= 0 || a->total_tokens <= 0 ||
         a->block_table_stride <= 0)
@@ -124,7 +132,7 @@ int check_select(const ti_select_args *a) {
 
 int check_sparse(const ti_sparse_attention_args *a, const ti_kv_cache *c) {
     if (!a || bad_cache(c) || bad_dtype(a->dtype)) return TI_ERR_INVALID_ARG;
-    if (c->head_dim != 64 && c->head_dim != 128) return TI_ERR_UNSUPPORTED;
+    if ((c->head_dim != 64 && c->head_dim != 128) || c->kind == TI_KV_FP8) return TI_ERR_UNSUPPORTED;
     if (a->q_heads <= 0 || a->q_heads % c->kv_heads || a->table_width <= 0) return TI_ERR_INVALID_ARG;
     if (!a->q || !a->out || !a->tables || !a->lengths) return TI_ERR_INVALID_ARG;
     if (!(a->scale > 0.0f) || a->scale == INFINITY) return TI_ERR_INVALID_ARG;
@@ -146,6 +154,22 @@ int check_verify(const ti_verify_args *a) {
     if (a->max_drafts > 0 && !a->draft_tokens) return TI_ERR_INVALID_ARG;
     // entries of a row are counted in 32 bits, sequences take grid y
     return a->num_seqs > 65535 || a->vocab > 0x7fff0000 || a->max_drafts > 0xffff ? TI_ERR_UNSUPPORTED : TI_OK;
+}
+
+int check_window(const ti_attention_args *a, int window, int sinks, const ti_kv_cache *c) {
+    const int st = check_attention(a, c);
+    if (st) return st;
+    if (window < 1 || sinks < 0 || !a->causal) return TI_ERR_INVALID_ARG;
+    return a->path != TI_PATH_AUTO ? TI_ERR_UNSUPPORTED : TI_OK;
+}
+
+int check_pool(const ti_page_pool *p) {
+    if (!p || p->num_pages <= 0 || p->page_size <= 0 || p->num_seqs <= 0 || p->table_width <= 0 || p->window < 0 || p->sinks < 0)
+        return TI_ERR_INVALID_ARG;
+    if (!p->free || !p->free_count || !p->tables || !p->lengths || !p->ticket || (p->window > 0 && !p->behind))
+        return TI_ERR_INVALID_ARG;
+    // slots are 32-bit, sequences' sums sit in LDS
+    return p->num_seqs > 4096 || (long long)p->num_pages * p->page_size > 0x7fffffffLL ? TI_ERR_UNSUPPORTED : TI_OK;
 }
 
 int check_workspace(const void *ws, size_t have, size_t need) {
@@ -247,9 +271,10 @@ int ti_attention_noalloc(const ti_attention_args *a, const ti_kv_cache *c, void 
 int ti_store_kv(int dtype, const ti_kv_cache *c, const void *k, const void *v,
                 const int32_t *slots, int n, void *stream) {
     if (bad_dtype(dtype) || bad_cache(c) || n < 0) return TI_ERR_INVALID_ARG;
-    if (c->head_dim > 512) return TI_ERR_UNSUPPORTED;
+    if (c->head_dim > 512 || odd_fp8(c)) return TI_ERR_UNSUPPORTED;
     if (n == 0) return TI_OK;
     if (!k || !v || !slots) return TI_ERR_INVALID_ARG;
+    if (c->kind == TI_KV_FP8) return ti_launch_store_fp8(dtype, c, k, v, slots, n, (hipStream_t)stream);
     return ti_launch_store_kv(dtype, c, k, v, slots, n, (hipStream_t)stream);
 }
 
@@ -279,10 +304,13 @@ int ti_attention_inputs(int dtype, void *q_out, const ti_kv_cache *c, const void
                         int q_heads, float eps, void *stream) {
     if (bad_dtype(dtype) || bad_cache(c) || n < 0 || q_heads <= 0 || table_len <= 0)
         return TI_ERR_INVALID_ARG;
-    if (c->head_dim > 128) return TI_ERR_UNSUPPORTED;
+    if (c->head_dim > 128 || odd_fp8(c)) return TI_ERR_UNSUPPORTED;
     if ((q_norm == nullptr) != (k_norm == nullptr)) return TI_ERR_INVALID_ARG;
     if (n == 0) return TI_OK;
     if (!q_out || !qkv || !cos_sin || !positions || !slots) return TI_ERR_INVALID_ARG;
+    if (c->kind == TI_KV_FP8)
+        return ti_launch_inputs_fp8(dtype, q_out, c, qkv, q_norm, k_norm, cos_sin, table_len, positions, slots, n, q_heads, eps,
+                                    (hipStream_t)stream);
     return ti_launch_attention_inputs(dtype, q_out, c, qkv, q_norm, k_norm, cos_sin, table_len,
                                       positions, slots, n, q_heads, eps, (hipStream_t)stream);
 }
@@ -294,7 +322,7 @@ int ti_update_key_bounds(int dtype, const ti_kv_cache *c, const ti_key_bounds *k
     if (!block_tables || block_table_stride <= 0 || !positions || misaligned(kb->bounds)) return TI_ERR_INVALID_ARG;
     const int st = check_step(num_seqs, max_query_len, total_tokens, query_start_loc);
     if (st) return st;
-    if (c->head_dim != 64 && c->head_dim != 128) return TI_ERR_UNSUPPORTED;
+    if ((c->head_dim != 64 && c->head_dim != 128) || c->kind == TI_KV_FP8) return TI_ERR_UNSUPPORTED;
     return ti_launch_key_bounds(dtype, c, kb, block_tables, block_table_stride, positions, query_start_loc, num_seqs,
                                 max_query_len, total_tokens, (hipStream_t)stream);
 }
@@ -336,6 +364,36 @@ int ti_sparse_attention(const ti_sparse_attention_args *a, const ti_kv_cache *c,
     int st = check_sparse(a, c);
     if (!st) st = check_workspace(a->workspace, a->workspace_bytes, ti_sparse_bytes(a, c));
     return st ? st : ti_launch_sparse_attention(a, c, (hipStream_t)stream);
+}
+
+int ti_window_attention_workspace_bytes(const ti_attention_args *a, int window, int sinks, const ti_kv_cache *c, size_t *bytes) {
+    if (!bytes) return TI_ERR_INVALID_ARG;
+    *bytes = 0;
+    const int st = check_window(a, window, sinks, c);
+    if (st) return st;
+    ti_plan_generic(a, c, bytes);
+    return TI_OK;
+}
+
+int ti_window_attention(const ti_attention_args *a, int window, int sinks, const ti_kv_cache *c, void *stream) {
+    size_t need = 0;
+    int st = ti_window_attention_workspace_bytes(a, window, sinks, c, &need);
+    if (!st) st = check_workspace(a->workspace, a->workspace_bytes, need);
+    return st ? st : ti_launch_generic(a, c, (hipStream_t)stream, ti_window{window, sinks});
+}
+
+int ti_reserve_pages(const ti_page_pool *pool, const int32_t *counts, int tokens, int32_t *positions, int32_t *slots,
+                     int32_t *query_start_loc, int32_t *short_of, void *stream) {
+    const int st = check_pool(pool);
+    if (st) return st;
+    if (!counts || tokens < 0 || (tokens > 0 && (!positions || !slots)) || !query_start_loc || !short_of) return TI_ERR_INVALID_ARG;
+    return ti_launch_reserve(pool, counts, tokens, positions, slots, query_start_loc, short_of, (hipStream_t)stream);
+}
+
+int ti_release_pages(const ti_page_pool *pool, const int32_t *keep, void *stream) {
+    const int st = check_pool(pool);
+    if (st) return st;
+    return !keep ? TI_ERR_INVALID_ARG : ti_launch_release(pool, keep, (hipStream_t)stream);
 }
 
 int ti_verify_draft_workspace_bytes(const ti_verify_args *a, size_t *bytes) {

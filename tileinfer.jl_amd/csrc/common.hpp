@@ -133,6 +133,22 @@ int ti_launch_attention_inputs(int dtype, void *q_out, const ti_kv_cache *c, con
                                int table_len, const int32_t *positions, const int32_t *slots,
                                int n, int q_heads, float eps, hipStream_t s);
 
+// Writes into 8-bit block caches (kv_fp8.hip).
+int ti_launch_store_fp8(int dtype, const ti_kv_cache *c, const void *k, const void *v, const int32_t *slots, int n,
+                        hipStream_t s);
+int ti_launch_inputs_fp8(int dtype, void *q_out, const ti_kv_cache *c, const void *qkv, const void *q_norm, const void *k_norm,
+                         const void *cos_sin, int table_len, const int32_t *positions, const int32_t *slots, int n,
+                         int q_heads, float eps, hipStream_t s);
+// Page bookkeeping (step_pages.hip).
+int ti_launch_reserve(const ti_page_pool *pool, const int32_t *counts, int tokens, int32_t *positions, int32_t *slots,
+                      int32_t *qsl, int32_t *short_of, hipStream_t s);
+int ti_launch_release(const ti_page_pool *pool, const int32_t *keep, hipStream_t s);
+
+// The keys that a query at position p sees: all up to p (size 0), or the last `size` of these and the first `sinks`.
+struct ti_window {
+    int size = 0, sinks = 0;
+};
+
 struct ti_decode_plan {
     int splits;      // split-KV work-groups per (sequence, KV head)
     int waves;       // waves per work-group (4 or 8)
@@ -179,7 +195,7 @@ int ti_launch_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, const
                          hipStream_t s);
 // fp32 path: its key splits and workspace bytes (host shapes only).
 int ti_plan_generic(const ti_attention_args *a, const ti_kv_cache *c, size_t *bytes);
-int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStream_t s);
+int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStream_t s, ti_window win = ti_window{});
 
 // Attention over chosen pages (pa_sparse.hip, its fp32 kernels in pa_generic.hip).
 struct ti_sparse_plan {

@@ -32,11 +32,14 @@ struct GenericParams {
     float scale_log2;
     const int32_t *lengths;      // SPARSE: keys of each (token, KV head)
     int B;
+    int window, sinks;           // WIN
 };
 
 // SPARSE: (token, KV head) pairs with a table row and a length each (pa_sparse.hip), grid
 // (tokens x splits, Hq); the token's own row of partials.
-template <typename T, bool INT8, int D, bool SPARSE = false>
+// FP8: an 8-bit block cache. WIN: the query's own keys (the last p.window and the first p.sinks) counted through, so
+// that nothing else is touched.
+template <typename T, bool INT8, int D, bool SPARSE = false, bool FP8 = false, bool WIN = false>
 __global__ void __launch_bounds__(64) generic_attention_kernel(GenericParams p) {
     using E = Elt<T>;
     const int t0 = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
@@ -58,6 +61,13 @@ __global__ void __launch_bounds__(64) generic_attention_kernel(GenericParams p) 
         last = p.causal ? start + t : len - 1;
     }
     // this split's keys: [k0, k1) of the sequence's len, cut at the query's last key
+    int first = 0, sunk = 0;   // WIN: the window's first key, the keys in front of it
+    if constexpr (WIN) {
+        first = max(last - p.window + 1, 0);
+        sunk = min(first, p.sinks);
+        len = last = sunk + last + 1 - first;
+        last--;
+    }
     const int per = (len + p.splits - 1) / p.splits;
     const int k0 = split * per, k1 = min(k0 + per, last + 1);
     const int32_t *bt = p.bt + (size_t)b * p.bt_stride;
@@ -77,15 +87,24 @@ __global__ void __launch_bounds__(64) generic_attention_kernel(GenericParams p) 
     for (int j = 0; j < PER; j++) acc[j] = 0.0f;
     float m = NEG_BIG, l = 0.0f;
     for (int c0 = k0; c0 < k1; c0 += WAVE) {
-        const int key = c0 + lane;
+        int key = c0 + lane;
         const bool valid = key < k1;
+        if (WIN && key >= sunk) key += first - sunk;
         float s = -INFINITY;
         long long row = 0;
         if (valid) {
             const int pg = page_of(bt, key / p.P, p.bt_stride, p.num_pages);
             row = ((long long)pg * p.Hk + g) * p.P + key % p.P;
             float dot = 0.0f;
-            if (INT8) {
+            if constexpr (FP8) {
+                const uint32_t *kr = reinterpret_cast<const uint32_t *>(p.lq + row * D);
+                for (int d = 0; d < D; d += 4) {
+                    const int w = (int)kr[d / 4];
+                    dot += __builtin_amdgcn_cvt_f32_fp8(w, 0) * qs[d] + __builtin_amdgcn_cvt_f32_fp8(w, 1) * qs[d + 1] +
+                           __builtin_amdgcn_cvt_f32_fp8(w, 2) * qs[d + 2] + __builtin_amdgcn_cvt_f32_fp8(w, 3) * qs[d + 3];
+                }
+                dot *= p.ls[row / p.P];   // a power of two
+            } else if (INT8) {
                 const int8_t *kr = p.lq + row * D;
                 const float sk = p.ls[row];
                 for (int d = 0; d < D; d++) dot += ((float)kr[d] * sk) * p.smooth[d] * qs[d];
@@ -113,8 +132,11 @@ __global__ void __launch_bounds__(64) generic_attention_kernel(GenericParams p) 
             for (int j = 0; j < PER; j++) {
                 const int d = lane + WAVE * j;
                 if (d < D) {
-                    const float v = INT8 ? (float)p.lq[half_q + r * D + d] * p.ls[half_s + r]
-                                         : E::ld((const T *)p.vp + r * D, d);
+                    float v;
+                    if constexpr (FP8)
+                        v = __builtin_amdgcn_cvt_f32_fp8((int)(uint8_t)p.lq[half_q + r * D + d], 0) * p.ls[(half_s + r) / p.P];
+                    else
+                        v = INT8 ? (float)p.lq[half_q + r * D + d] * p.ls[half_s + r] : E::ld((const T *)p.vp + r * D, d);
                     acc[j] += pk * v;
                 }
             }
@@ -433,10 +455,15 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     }
 }
 
-template <typename T, bool INT8>
+template <typename T, bool INT8, bool FP8 = false>
 void launch(const GenericParams &p, int D, dim3 grid, hipStream_t s) {
-    if (D == 128) generic_attention_kernel<T, INT8, 128><<<grid, 64, 0, s>>>(p);
-    else generic_attention_kernel<T, INT8, 64><<<grid, 64, 0, s>>>(p);
+    if (p.window) {
+        if (D == 128) generic_attention_kernel<T, INT8, 128, false, FP8, true><<<grid, 64, 0, s>>>(p);
+        else generic_attention_kernel<T, INT8, 64, false, FP8, true><<<grid, 64, 0, s>>>(p);
+        return;
+    }
+    if (D == 128) generic_attention_kernel<T, INT8, 128, false, FP8><<<grid, 64, 0, s>>>(p);
+    else generic_attention_kernel<T, INT8, 64, false, FP8><<<grid, 64, 0, s>>>(p);
 }
 
 }  // namespace
@@ -477,8 +504,8 @@ int ti_plan_generic(const ti_attention_args *a, const ti_kv_cache *c, size_t *by
     return sp;
 }
 
-int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStream_t s) {
-    if (f32_mfma(a, c)) {
+int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStream_t s, ti_window win) {
+    if (f32_mfma(a, c) && !win.size) {
         F32Params f;
         f.q = (const float *)a->q;
         f.out = (float *)a->out;
@@ -539,6 +566,8 @@ int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStrea
     p.G = a->q_heads / c->kv_heads;
     p.nmax = a->max_query_len;
     p.causal = a->causal;
+    p.window = win.size;
+    p.sinks = win.sinks;
     p.scale_log2 = a->scale * LOG2E;
     size_t bytes = 0;
     p.splits = ti_plan_generic(a, c, &bytes);
@@ -546,7 +575,10 @@ int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStrea
     p.part = (float *)a->workspace;
     dim3 grid(a->max_query_len * p.splits, a->q_heads, a->num_seqs);
     const bool int8 = c->kind == TI_KV_INT8;
-    if (a->dtype == TI_BF16) {
+    if (c->kind == TI_KV_FP8) {
+        if (a->dtype == TI_BF16) launch<uint16_t, false, true>(p, c->head_dim, grid, s);
+        else launch<float, false, true>(p, c->head_dim, grid, s);
+    } else if (a->dtype == TI_BF16) {
         if (int8) launch<uint16_t, true>(p, c->head_dim, grid, s);
         else launch<uint16_t, false>(p, c->head_dim, grid, s);
     } else {

@@ -29,7 +29,11 @@ decltype(&ti_update_key_bounds) f_bounds;
 decltype(&ti_select_pages) f_select;
 decltype(&ti_sparse_attention) f_sparse;
 decltype(&ti_verify_draft) f_verify;
-PyObject *int8_pages, *key_bounds;   // Int8Pages, KeyBounds
+decltype(&ti_window_attention) f_window;
+decltype(&ti_reserve_pages) f_reserve;
+decltype(&ti_release_pages) f_release;
+PyObject *int8_pages, *key_bounds, *fp8_pages, *page_pool;   // Int8Pages, KeyBounds, Fp8Pages, PagePool
+PyObject *n_free, *n_free_count, *n_tables, *n_lengths, *n_behind, *n_ticket, *n_window, *n_sinks;
 PyObject *n_layer_q, *n_layer_scale, *n_smooth, *n_half, *n_cos_sin, *n_bounds, *n_scale, *n_channel, *n_page_size;   // attribute names
 
 struct NotPlain {};   // leave the call to backend.py
@@ -76,8 +80,26 @@ struct Attr {
     Attr(const Attr &) = delete;
 };
 
-// The layer's cache: dense pools [pages][H][P][D] of element type `like`, or an Int8Pages pair.
+// An 8-bit block layer, on the current GPU (as OneGpu below).
+ti_kv_cache fp8_cache_of(PyObject *k, PyObject *v) {
+    require(Py_TYPE(k) == Py_TYPE(v));
+    Attr lq(k, n_layer_q), lq2(v, n_layer_q), ls(k, n_layer_scale), ls2(v, n_layer_scale), h0(k, n_half), h1(v, n_half);
+    require(lq.o == lq2.o && ls.o == ls2.o && integer(h0.o) == 0 && integer(h1.o) == 1);
+    const at::Tensor &q = dev(lq.o), &s = dev(ls.o);
+    require(q.dim() == 5 && q.size(0) == 2 && q.element_size() == 1 && s.scalar_type() == at::kFloat && s.sizes() == q.sizes().slice(0, 3));
+    require(q.device() == s.device() && q.device().index() == c10::hip::current_device());
+    ti_kv_cache c{};
+    c.kind = TI_KV_FP8;
+    c.layer_q = static_cast<int8_t *>(q.data_ptr());
+    c.layer_scale = static_cast<float *>(s.data_ptr());
+    c.num_pages = (int32_t)q.size(1), c.kv_heads = (int32_t)q.size(2);
+    c.page_size = (int32_t)q.size(3), c.head_dim = (int32_t)q.size(4);
+    return c;
+}
+
+// The layer's cache: dense pools [pages][H][P][D] of element type `like`, an Int8Pages or an Fp8Pages pair.
 ti_kv_cache cache_of(PyObject *k, PyObject *v, at::ScalarType like) {
+    if ((PyObject *)Py_TYPE(k) == fp8_pages || (PyObject *)Py_TYPE(v) == fp8_pages) return fp8_cache_of(k, v);
     ti_kv_cache c{};
     if ((PyObject *)Py_TYPE(k) == int8_pages || (PyObject *)Py_TYPE(v) == int8_pages) {
         require(Py_TYPE(k) == Py_TYPE(v));
@@ -119,6 +141,9 @@ struct OneGpu {
         const ti_kv_cache c = cache_of(k, v, like);
         if (c.kind == TI_KV_DENSE) {
             (*this)(k), (*this)(v);
+        } else if (c.kind == TI_KV_FP8) {
+            Attr q(k, n_layer_q), s(k, n_layer_scale);
+            (*this)(q.o), (*this)(s.o);
         } else {
             Attr q(k, n_layer_q), s(k, n_layer_scale), m(k, n_smooth);
             (*this)(q.o), (*this)(s.o), (*this)(m.o);
@@ -195,6 +220,7 @@ PyObject *py_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
         g.dtype = dtype_of(q);
         g.positions = i32(pos);
         g.block_tables = i32(bt);
+        require(c.kind != TI_KV_FP8 || q.device().index() == c10::hip::current_device());
         require(pos.numel() == q.size(0) && q.size(2) == c.head_dim && PyBool_Check(a[8]));
         const bool rows = bt.dim() == 2 && a[12] != Py_True;
         const int64_t B = rows ? bt.size(0) : 1;
@@ -226,6 +252,7 @@ PyObject *py_inputs(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
         require(q.dim() == 3 && !qn == !kn);
         const int64_t n = q.size(0), nq = q.size(1), D = q.size(2);
         const ti_kv_cache c = cache_of(a[1], a[2], q.scalar_type());
+        require(c.kind != TI_KV_FP8 || q.device().index() == c10::hip::current_device());
         require(qkv.scalar_type() == q.scalar_type() && qkv.numel() == n * (nq + 2 * (int64_t)c.kv_heads) * D && D == c.head_dim);
         require(cs.scalar_type() == q.scalar_type() && cs.dim() == 3 && cs.size(1) == 2 && cs.size(2) == D);
         require(pos.numel() == n && slots.numel() == n);
@@ -245,6 +272,7 @@ PyObject *py_store_kv(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
         const at::Tensor &k = dev(a[2]), &v = dev(a[3]), &slots = dev(a[4]);
         require(k.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type());
         const ti_kv_cache c = cache_of(a[0], a[1], k.scalar_type());
+        require(c.kind != TI_KV_FP8 || k.device().index() == c10::hip::current_device());
         require(k.size(1) == c.kv_heads && k.size(2) == c.head_dim && slots.numel() == k.size(0));
         const int dtype = dtype_of(k);
         const int32_t *sl = i32(slots);
@@ -382,19 +410,102 @@ PyObject *py_verify(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     });
 }
 
-// bind(Int8Pages, KeyBounds, addresses of ti_attention, ti_attention_inputs, ti_store_kv, ti_rope, ti_rmsnorm,
-//      ti_update_key_bounds, ti_select_pages, ti_sparse_attention, ti_verify_draft)
+// (out, workspace, q, k_pages, v_pages, block_tables, positions, scale, window, sinks, query_start_loc, max_query_len)
+PyObject *py_window(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded(nargs, 12, [&]() -> long {
+        const at::Tensor &q = dev(a[2]);
+        const OneGpu gpu(q);
+        const at::Tensor &out = gpu(a[0]), *ws = gpu.or_none(a[1]);
+        require(q.dim() == 3 && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type());
+        const ti_kv_cache c = gpu.cache(a[3], a[4], q.scalar_type());
+        const StepArgs t(gpu, a[5], a[6], a[10], a[11]);
+        require(t.total == q.size(0) && q.size(2) == c.head_dim);
+        ti_attention_args g{};
+        g.dtype = dtype_of(q);
+        g.q_heads = (int32_t)q.size(1);
+        g.num_seqs = t.seqs, g.max_query_len = t.n, g.total_tokens = t.total, g.block_table_stride = t.stride;
+        g.q = q.data_ptr(), g.out = out.data_ptr();
+        g.positions = t.positions, g.query_start_loc = t.qsl, g.block_tables = t.tables;
+        g.scale = number(a[7]);
+        g.causal = 1;
+        g.workspace = ws ? ws->data_ptr() : nullptr, g.workspace_bytes = ws ? (size_t)ws->nbytes() : 0;
+        const long window = integer(a[8]), sinks = integer(a[9]);
+        require(window >= 1 && window <= 0x7fffffff && sinks >= 0 && sinks <= 0x7fffffff);
+        void *s = stream_of(q);
+        return unlocked([&] { return f_window(&g, (int)window, (int)sinks, &c, s); });
+    });
+}
+
+// A PagePool's arrays, and its GPU.
+struct Pool {
+    Attr free, count, tables, lengths, behind, ticket;
+    OneGpu gpu;
+    ti_page_pool p{};
+    Pool(PyObject *o)
+        : free((require((PyObject *)Py_TYPE(o) == page_pool), o), n_free), count(o, n_free_count), tables(o, n_tables),
+          lengths(o, n_lengths), behind(o, n_behind), ticket(o, n_ticket), gpu(dev(free.o)) {
+        const Attr size(o, n_page_size), window(o, n_window), sinks(o, n_sinks);
+        const at::Tensor &t = gpu(tables.o), &f = gpu(free.o), *b = gpu.or_none(behind.o);
+        require(t.dim() == 2 && f.numel() <= 0x7fffffff);
+        const int64_t S = t.size(0);
+        require(gpu(lengths.o).numel() == S && gpu(count.o).numel() == 1 && gpu(ticket.o).numel() == 1 && (!b || b->numel() == S));
+        p.num_pages = (int32_t)f.numel(), p.page_size = (int32_t)integer(size.o), p.num_seqs = (int32_t)S, p.table_width = (int32_t)t.size(1);
+        p.window = (int32_t)integer(window.o), p.sinks = (int32_t)integer(sinks.o);
+        p.free = out(free.o), p.free_count = out(count.o), p.tables = out(tables.o), p.lengths = out(lengths.o);
+        p.behind = b ? out(behind.o) : nullptr, p.ticket = out(ticket.o);
+    }
+    int32_t *out(PyObject *o) const { return const_cast<int32_t *>(i32(gpu(o))); }
+};
+
+// (pool, counts, positions, slots, query_start_loc, short)
+PyObject *py_reserve(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded(nargs, 6, [&]() -> long {
+        const Pool pool(a[0]);
+        const at::Tensor &counts = pool.gpu(a[1]), &pos = pool.gpu(a[2]), &slots = pool.gpu(a[3]);
+        const int64_t S = pool.p.num_seqs, T = pos.numel();
+        require(counts.dim() == 1 && counts.numel() == S && pos.dim() == 1 && slots.dim() == 1 && slots.numel() == T && T <= 0x7fffffff);
+        require(pool.gpu(a[4]).dim() == 1 && pool.gpu(a[4]).numel() == S + 1 && pool.gpu(a[5]).numel() == 1);
+        const int32_t *n = i32(counts);
+        int32_t *x = pool.out(a[2]), *y = pool.out(a[3]), *z = pool.out(a[4]), *w = pool.out(a[5]);
+        void *s = stream_of(counts);
+        return unlocked([&] { return f_reserve(&pool.p, n, (int)T, x, y, z, w, s); });
+    });
+}
+
+// (pool, lengths)
+PyObject *py_release(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded(nargs, 2, [&]() -> long {
+        const Pool pool(a[0]);
+        const at::Tensor &keep = pool.gpu(a[1]);
+        require(keep.dim() == 1 && keep.numel() == pool.p.num_seqs);
+        const int32_t *n = i32(keep);
+        void *s = stream_of(keep);
+        return unlocked([&] { return f_release(&pool.p, n, s); });
+    });
+}
+
+void hold(PyObject *&to, PyObject *o) {
+    Py_INCREF(o);
+    Py_XDECREF(to);
+    to = o;
+}
+
+// bind(Int8Pages, KeyBounds, Fp8Pages, PagePool, addresses of ti_attention, ti_attention_inputs, ti_store_kv, ti_rope,
+//      ti_rmsnorm, ti_update_key_bounds, ti_select_pages, ti_sparse_attention, ti_verify_draft, ti_window_attention,
+//      ti_reserve_pages, ti_release_pages)
 PyObject *py_bind(PyObject *, PyObject *args) {
-    PyObject *pages, *bounds;
-    unsigned long long f[9];
-    if (!PyArg_ParseTuple(args, "OOKKKKKKKKK", &pages, &bounds, &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6], &f[7], &f[8]))
+    PyObject *pages, *bounds, *fp8, *pool;
+    unsigned long long f[12];
+    if (!PyArg_ParseTuple(args, "OOOOKKKKKKKKKKKK", &pages, &bounds, &fp8, &pool, &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6], &f[7],
+                          &f[8], &f[9], &f[10], &f[11]))
         return nullptr;
-    Py_INCREF(pages);
-    Py_XDECREF(int8_pages);
-    int8_pages = pages;
-    Py_INCREF(bounds);
-    Py_XDECREF(key_bounds);
-    key_bounds = bounds;
+    hold(int8_pages, pages);
+    hold(key_bounds, bounds);
+    hold(fp8_pages, fp8);
+    hold(page_pool, pool);
+    f_window = reinterpret_cast<decltype(f_window)>(f[9]);
+    f_reserve = reinterpret_cast<decltype(f_reserve)>(f[10]);
+    f_release = reinterpret_cast<decltype(f_release)>(f[11]);
     f_bounds = reinterpret_cast<decltype(f_bounds)>(f[5]);
     f_select = reinterpret_cast<decltype(f_select)>(f[6]);
     f_sparse = reinterpret_cast<decltype(f_sparse)>(f[7]);
@@ -410,7 +521,9 @@ PyObject *py_bind(PyObject *, PyObject *args) {
 #define FAST(name, f) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST("attention", py_attention), FAST("attention_inputs", py_inputs), FAST("store_kv", py_store_kv),
                          FAST("rope", py_rope), FAST("rmsnorm", py_rmsnorm), FAST("update_key_bounds", py_bounds),
-                         FAST("select_pages", py_select), FAST("sparse_attention", py_sparse), FAST("verify_draft", py_verify), {"bind", py_bind, METH_VARARGS, nullptr},
+                         FAST("select_pages", py_select), FAST("sparse_attention", py_sparse), FAST("verify_draft", py_verify),
+                         FAST("window_attention", py_window), FAST("reserve_pages", py_reserve), FAST("release_pages", py_release),
+                         {"bind", py_bind, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods};
 
@@ -426,6 +539,14 @@ PyMODINIT_FUNC PyInit__calls() {
     n_scale = PyUnicode_InternFromString("scale");
     n_channel = PyUnicode_InternFromString("channel");
     n_page_size = PyUnicode_InternFromString("page_size");
+    n_free = PyUnicode_InternFromString("free");
+    n_free_count = PyUnicode_InternFromString("free_count");
+    n_tables = PyUnicode_InternFromString("tables");
+    n_lengths = PyUnicode_InternFromString("lengths");
+    n_behind = PyUnicode_InternFromString("behind");
+    n_ticket = PyUnicode_InternFromString("ticket");
+    n_window = PyUnicode_InternFromString("window");
+    n_sinks = PyUnicode_InternFromString("sinks");
     PyObject *m = PyModule_Create(&module);
     // the torch and Python whose layouts this was compiled for; _lib.py compares
     if (m && PyModule_AddStringConstant(m, "built_for", BUILT_FOR) < 0) {

@@ -16,7 +16,7 @@ LIB_PATH = os.path.join(HERE, "libtileinfer_hip.so")
 
 TI_OK, TI_ERR_INVALID_ARG, TI_ERR_UNSUPPORTED, TI_ERR_WORKSPACE, TI_ERR_LAUNCH = range(5)
 TI_F32, TI_BF16 = 0, 1
-TI_KV_DENSE, TI_KV_INT8 = 0, 1
+TI_KV_DENSE, TI_KV_INT8, TI_KV_FP8 = 0, 1, 2
 (TI_PATH_AUTO, TI_PATH_DECODE, TI_PATH_PREFILL, TI_PATH_PREFILL_STAGED, TI_PATH_PREFILL_DIRECT,
  TI_PATH_PREFILL_PINGPONG, TI_PATH_PREFILL_PAIRED, TI_PATH_PREFILL_PAIRED16) = range(8)
 
@@ -25,12 +25,13 @@ EXPORTS = ("ti_version", "ti_status_string", "ti_attention_workspace_bytes", "ti
            "ti_attention_noalloc", "ti_store_kv", "ti_rmsnorm", "ti_rope", "ti_attention_inputs",
            "ti_update_key_bounds", "ti_select_pages_workspace_bytes", "ti_select_pages",
            "ti_sparse_attention_workspace_bytes", "ti_sparse_attention_workspace_bound", "ti_sparse_attention",
-           "ti_verify_draft_workspace_bytes", "ti_verify_draft")
+           "ti_verify_draft_workspace_bytes", "ti_verify_draft", "ti_window_attention_workspace_bytes",
+           "ti_window_attention", "ti_reserve_pages", "ti_release_pages")
 NOALLOC_SCRATCH_BYTES = 32 << 20   # TI_NOALLOC_SCRATCH_BYTES
 
 
 class KVCache(ctypes.Structure):
-    """ti_kv_cache: one layer's dense pools or INT8 layer arrays (device pointers)."""
+    """ti_kv_cache: one layer's dense pools, INT8 or 8-bit block layer arrays (device pointers)."""
     _fields_ = [("kind", ctypes.c_int32), ("head_dim", ctypes.c_int32),
                 ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
                 ("num_pages", ctypes.c_int32), ("k_pages", ctypes.c_void_p),
@@ -85,6 +86,13 @@ class VerifyArgs(ctypes.Structure):
         (ctypes.c_size_t, "workspace_bytes"))
 
 
+class PagePoolArgs(ctypes.Structure):
+    """ti_page_pool."""
+    _fields_ = _fields(
+        (ctypes.c_int32, "num_pages page_size num_seqs table_width window sinks"),
+        (ctypes.c_void_p, "free free_count tables lengths behind ticket"))
+
+
 _lib = None
 
 
@@ -124,7 +132,11 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
                         ("ti_sparse_attention_workspace_bound", [P(SparseAttentionArgs), P(KVCache), size]),
                         ("ti_sparse_attention", [P(SparseAttentionArgs), P(KVCache), vp]),
                         ("ti_verify_draft_workspace_bytes", [P(VerifyArgs), size]),
-                        ("ti_verify_draft", [P(VerifyArgs), vp])):
+                        ("ti_verify_draft", [P(VerifyArgs), vp]),
+                        ("ti_window_attention_workspace_bytes", [P(AttentionArgs), i32, i32, P(KVCache), size]),
+                        ("ti_window_attention", [P(AttentionArgs), i32, i32, P(KVCache), vp]),
+                        ("ti_reserve_pages", [P(PagePoolArgs), vp, i32, vp, vp, vp, vp, vp]),
+                        ("ti_release_pages", [P(PagePoolArgs), vp, vp])):
         getattr(L, name).restype = i32
         getattr(L, name).argtypes = types
     _bind_calls(L)
@@ -148,7 +160,7 @@ def _bind_calls(L: ctypes.CDLL) -> None:
     ctypes, with a warning."""
     global calls
     import torch
-    from .kv import Int8Pages, KeyBounds
+    from .kv import Fp8Pages, Int8Pages, KeyBounds, PagePool
     here = f"torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
     try:
         from . import _calls
@@ -159,9 +171,10 @@ def _bind_calls(L: ctypes.CDLL) -> None:
                       "build it with `python tileinfer.jl_amd/build.py`", RuntimeWarning, stacklevel=2)
         calls = _NoCalls()
         return
-    _calls.bind(Int8Pages, KeyBounds, *(ctypes.cast(f, ctypes.c_void_p).value for f in
+    _calls.bind(Int8Pages, KeyBounds, Fp8Pages, PagePool, *(ctypes.cast(f, ctypes.c_void_p).value for f in
                                         (L.ti_attention, L.ti_attention_inputs, L.ti_store_kv, L.ti_rope, L.ti_rmsnorm,
-                                         L.ti_update_key_bounds, L.ti_select_pages, L.ti_sparse_attention, L.ti_verify_draft)))
+                                         L.ti_update_key_bounds, L.ti_select_pages, L.ti_sparse_attention, L.ti_verify_draft,
+                                         L.ti_window_attention, L.ti_reserve_pages, L.ti_release_pages)))
     calls = _calls
 
 

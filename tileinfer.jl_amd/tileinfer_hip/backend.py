@@ -14,14 +14,16 @@ zero-padded; positions int32 [n], 0-based; slots int32 [n], 1-based.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional
 
 import torch
 
 from . import _lib
-from ._lib import ArgumentError, AttentionArgs, KeyBoundsArgs, KVCache, SelectArgs, SparseAttentionArgs, VerifyArgs, check
-from .kv import Int8Pages, KeyBounds, layer_arrays
+from ._lib import (ArgumentError, AttentionArgs, KeyBoundsArgs, KVCache, PagePoolArgs, SelectArgs, SparseAttentionArgs,
+                   VerifyArgs, check)
+from .kv import Fp8Pages, Int8Pages, KeyBounds, PagePool, fp8_layer_arrays, layer_arrays
 from .rope import RotaryTable
 
 
@@ -43,7 +45,7 @@ class HipBackend:
 
 _OPS = {"attention", "attention!", "store_kv!", "rmsnorm", "rmsnorm!", "rope", "rope!", "attention_inputs!",
         "update_key_bounds!", "select_pages", "select_pages!", "sparse_attention", "sparse_attention!", "verify_draft",
-        "verify_draft!"}
+        "verify_draft!", "window_attention", "window_attention!", "reserve_pages!", "release_pages!"}
 
 
 def supports_graphs(be: HipBackend) -> bool:
@@ -88,8 +90,15 @@ def _stream(t: torch.Tensor) -> int:
 
 
 def kv_cache_struct(k_pages, v_pages, dtype: Optional[torch.dtype] = None) -> KVCache:
-    """The ti_kv_cache of a layer: dense pools [pages][H][P][D] or an Int8Pages pair."""
+    """The ti_kv_cache of a layer: dense pools [pages][H][P][D], an Int8Pages or an Fp8Pages pair."""
     c = KVCache()
+    if isinstance(k_pages, Fp8Pages) or isinstance(v_pages, Fp8Pages):
+        lq, ls = fp8_layer_arrays(k_pages, v_pages)
+        _dev(lq, ls)
+        _, pages, H, P, D = lq.shape
+        c.kind, c.layer_q, c.layer_scale = _lib.TI_KV_FP8, lq.data_ptr(), ls.data_ptr()
+        c.head_dim, c.page_size, c.kv_heads, c.num_pages = D, P, H, pages
+        return c
     if isinstance(k_pages, Int8Pages) or isinstance(v_pages, Int8Pages):
         lq, ls, sm = layer_arrays(k_pages, v_pages)
         _dev(lq, ls, sm)
@@ -105,6 +114,21 @@ def kv_cache_struct(k_pages, v_pages, dtype: Optional[torch.dtype] = None) -> KV
         c.kind, c.k_pages, c.v_pages = _lib.TI_KV_DENSE, k_pages.data_ptr(), v_pages.data_ptr()
     c.head_dim, c.page_size, c.kv_heads, c.num_pages = D, P, H, pages
     return c
+
+
+def _pool_dtype(k_pages, like) -> Optional[torch.dtype]:
+    """The element type that dense pools must have."""
+    return None if isinstance(k_pages, (Int8Pages, Fp8Pages)) else like.dtype
+
+
+def _fp8_device(c: KVCache, k_pages, *ts):
+    """Where the library launches on an 8-bit block layer: its GPU, that of every tensor ts too. Else the current one."""
+    if c.kind != _lib.TI_KV_FP8:
+        return contextlib.nullcontext()
+    for t in ts:
+        if t is not None and t.device != k_pages.layer_q.device:
+            raise ArgumentError("tensors must be on one GPU")
+    return torch.cuda.device(k_pages.layer_q.device)
 
 
 def _attention_args(out, q, block_tables, positions, scale, causal, path, num_seqs,
@@ -128,18 +152,24 @@ def _attention_args(out, q, block_tables, positions, scale, causal, path, num_se
     return a
 
 
+def _shape_only(k_pages) -> KVCache:
+    """A ti_kv_cache of the pools' shape and kind, for size queries."""
+    c = KVCache()
+    if isinstance(k_pages, Int8Pages):
+        c.kind, c.layer_q, c.layer_scale, c.smooth = _lib.TI_KV_INT8, 16, 16, 16
+    elif isinstance(k_pages, Fp8Pages):
+        c.kind, c.layer_q, c.layer_scale = _lib.TI_KV_FP8, 16, 16
+    else:
+        c.kind, c.k_pages, c.v_pages = _lib.TI_KV_DENSE, 16, 16
+    c.num_pages, c.kv_heads, c.page_size, c.head_dim = k_pages.shape
+    return c
+
+
 def workspace_bytes(q, k_pages, num_seqs: int = 1, max_query_len: Optional[int] = None,
                     path: int = _lib.TI_PATH_AUTO) -> int:
     """Bytes of split-KV scratch ti_attention needs for these query shapes (0 for none)."""
     # A shape-only query: the library validates and sizes, it never dereferences pointers.
-    c = KVCache()
-    if isinstance(k_pages, Int8Pages):
-        pages, H, P, D = k_pages.q.shape
-        c.kind, c.layer_q, c.layer_scale, c.smooth = _lib.TI_KV_INT8, 1, 1, 1
-    else:
-        pages, H, P, D = k_pages.shape
-        c.kind, c.k_pages, c.v_pages = _lib.TI_KV_DENSE, 1, 1
-    c.head_dim, c.page_size, c.kv_heads, c.num_pages = D, P, H, pages
+    c = _shape_only(k_pages)
     n = max_query_len if max_query_len is not None else q.shape[0] // num_seqs
     a = AttentionArgs()
     a.dtype, a.q_heads, a.num_seqs, a.max_query_len = _dtype(q), q.shape[1], num_seqs, n
@@ -177,7 +207,7 @@ def paged_attention_(be: HipBackend, out, workspace, q, k_pages, v_pages, block_
         raise ArgumentError("q and out must be matching [n][heads][D] tensors")
     if positions.numel() != q.shape[0]:
         raise ArgumentError("one position per query token")
-    c = kv_cache_struct(k_pages, v_pages, None if isinstance(k_pages, Int8Pages) else q.dtype)
+    c = kv_cache_struct(k_pages, v_pages, _pool_dtype(k_pages, q))
     if q.shape[2] != c.head_dim:
         raise ArgumentError("q's head_dim differs from the pools'")
     if query_start_loc is not None:
@@ -187,7 +217,8 @@ def paged_attention_(be: HipBackend, out, workspace, q, k_pages, v_pages, block_
     n = max_query_len if max_query_len is not None else q.shape[0] // B
     a = _attention_args(out, q, bts, positions, scale, causal, path, B, n, query_start_loc,
                         workspace)
-    check(_lib.load().ti_attention(ctypes.byref(a), ctypes.byref(c), _stream(q)))
+    with _fp8_device(c, k_pages, q, out, bts, positions, query_start_loc, workspace):
+        check(_lib.load().ti_attention(ctypes.byref(a), ctypes.byref(c), _stream(q)))
     return out
 
 
@@ -212,18 +243,20 @@ def attention(be: HipBackend, q, k_pages, v_pages, block_table, positions, scale
 
 def store_kv_(be: HipBackend, k_pages, v_pages, k, v, slots):
     """store_kv!(::TileBackend, k_pages, v_pages, k, v, slots)
-    (src/ops/tile/elementwise.jl:133-140, :180-188)."""
+    (src/ops/tile/elementwise.jl:133-140, :180-188). Into Fp8Pages a page's rows go from the first on: writing
+    row 0 begins the page anew, later rows can only make its scale grow."""
     if _done(_lib.native().store_kv(k_pages, v_pages, k, v, slots)):
         return
     _dev(k, v, slots)
     _i32(slots, "slots")
     if k.shape != v.shape or k.dtype != v.dtype or k.dim() != 3:
         raise ArgumentError("k and v must be matching [n][kv_heads][D] tensors")
-    c = kv_cache_struct(k_pages, v_pages, None if isinstance(k_pages, Int8Pages) else k.dtype)
+    c = kv_cache_struct(k_pages, v_pages, _pool_dtype(k_pages, k))
     if k.shape[1] != c.kv_heads or k.shape[2] != c.head_dim or slots.numel() != k.shape[0]:
         raise ArgumentError("k/v/slots shapes do not match the pools")
-    check(_lib.load().ti_store_kv(_dtype(k), ctypes.byref(c), _ptr(k), _ptr(v), _ptr(slots),
-                                  k.shape[0], _stream(k)))
+    with _fp8_device(c, k_pages, k, v, slots):
+        check(_lib.load().ti_store_kv(_dtype(k), ctypes.byref(c), _ptr(k), _ptr(v), _ptr(slots),
+                                      k.shape[0], _stream(k)))
 
 
 def rmsnorm_(be: HipBackend, y, x, w, eps: float):
@@ -278,7 +311,7 @@ def attention_inputs_(be: HipBackend, q, k_pages, v_pages, qkv, q_norm, k_norm,
     _i32(positions, "positions")
     _i32(slots, "slots")
     n, nq, D = q.shape
-    c = kv_cache_struct(k_pages, v_pages, None if isinstance(k_pages, Int8Pages) else q.dtype)
+    c = kv_cache_struct(k_pages, v_pages, _pool_dtype(k_pages, q))
     if qkv.dtype != q.dtype or qkv.numel() != n * (nq + 2 * c.kv_heads) * D or D != c.head_dim:
         raise ArgumentError("qkv must be [n][(heads + 2 kv_heads) D] in q's element type")
     if table.cos_sin.dtype != q.dtype or table.cos_sin.shape[1:] != (2, D):
@@ -287,10 +320,11 @@ def attention_inputs_(be: HipBackend, q, k_pages, v_pages, qkv, q_norm, k_norm,
         raise ArgumentError("q_norm and k_norm go together")
     if positions.numel() != n or slots.numel() != n:
         raise ArgumentError("one position and one slot per token")
-    check(_lib.load().ti_attention_inputs(
-        _dtype(q), _ptr(q), ctypes.byref(c), _ptr(qkv), _ptr(q_norm), _ptr(k_norm),
-        _ptr(table.cos_sin), table.cos_sin.shape[0], _ptr(positions), _ptr(slots), n, nq,
-        float(eps), _stream(q)))
+    with _fp8_device(c, k_pages, q, qkv, q_norm, k_norm, table.cos_sin, positions, slots):
+        check(_lib.load().ti_attention_inputs(
+            _dtype(q), _ptr(q), ctypes.byref(c), _ptr(qkv), _ptr(q_norm), _ptr(k_norm),
+            _ptr(table.cos_sin), table.cos_sin.shape[0], _ptr(positions), _ptr(slots), n, nq,
+            float(eps), _stream(q)))
     return q
 
 
@@ -309,6 +343,8 @@ def _one_device(first: torch.Tensor, *ts):
 def _cache_tensors(k_pages, v_pages):
     if isinstance(k_pages, Int8Pages) or isinstance(v_pages, Int8Pages):
         return layer_arrays(k_pages, v_pages)
+    if isinstance(k_pages, Fp8Pages) or isinstance(v_pages, Fp8Pages):
+        return fp8_layer_arrays(k_pages, v_pages)
     return k_pages, v_pages
 
 
@@ -357,7 +393,7 @@ def update_key_bounds_(be: HipBackend, bounds: KeyBounds, k_pages, v_pages, bloc
     c = kv_cache_struct(k_pages, v_pages)
     if bounds.shape != (c.num_pages, c.kv_heads, c.page_size, c.head_dim):
         raise ArgumentError("bounds do not belong to pools of this shape")
-    dtype = _lib.TI_BF16 if c.kind == _lib.TI_KV_INT8 else _dtype(k_pages)
+    dtype = _lib.TI_BF16 if c.kind != _lib.TI_KV_DENSE else _dtype(k_pages)
     kb = _bounds_struct(bounds)
     with on:
         check(_lib.load().ti_update_key_bounds(
@@ -448,12 +484,7 @@ def _sparse_step(q, query_start_loc, max_query_len):
 
 
 def _sparse_workspace(size_of, q, k_pages, tables, max_query_len):
-    c = KVCache()
-    if isinstance(k_pages, Int8Pages):
-        c.kind, c.layer_q, c.layer_scale, c.smooth = _lib.TI_KV_INT8, 16, 16, 16
-    else:
-        c.kind, c.k_pages, c.v_pages = _lib.TI_KV_DENSE, 16, 16
-    c.num_pages, c.kv_heads, c.page_size, c.head_dim = k_pages.shape
+    c = _shape_only(k_pages)
     a = _sparse_args(q, tables.shape[-1], 1, int(max_query_len), 1.0)
     a.q = a.out = a.tables = a.lengths = a.query_start_loc = 16
     return _workspace(size_of, q.device, ctypes.byref(a), ctypes.byref(c))
@@ -482,7 +513,7 @@ def sparse_attention_(be: HipBackend, out, workspace, q, k_pages, v_pages, table
     _i32(lengths, "lengths")
     if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype:
         raise ArgumentError("q and out must be matching [n][heads][D] tensors")
-    c = kv_cache_struct(k_pages, v_pages, None if isinstance(k_pages, Int8Pages) else q.dtype)
+    c = kv_cache_struct(k_pages, v_pages, _pool_dtype(k_pages, q))
     if q.shape[2] != c.head_dim:
         raise ArgumentError("q's head_dim differs from the pools'")
     if tables.dim() != 3 or tables.shape[:2] != (q.shape[0], c.kv_heads) or lengths.shape != (q.shape[0], c.kv_heads):
@@ -562,3 +593,109 @@ def verify_draft(be: HipBackend, draft_tokens, target, draft, uniforms, draft_le
     accepted = torch.empty(B, dtype=torch.int32, device=target.device)
     tokens = torch.empty((B, N1), dtype=torch.int32, device=target.device)
     return verify_draft_(be, accepted, tokens, verify_draft_workspace(be, target), draft_tokens, target, draft, uniforms, draft_lens)
+
+
+# ---- attention with a sliding window, and the page bookkeeping of a step -------------------------
+
+def _window_args(q, window, sinks, B, n):
+    a = AttentionArgs()
+    a.dtype, a.q_heads, a.num_seqs, a.max_query_len = _dtype(q), q.shape[1], B, n
+    a.total_tokens, a.causal, a.path = q.shape[0], 1, _lib.TI_PATH_AUTO
+    if isinstance(window, bool) or isinstance(sinks, bool) or int(window) != window or int(sinks) != sinks \
+            or not 1 <= window < 1 << 31 or not 0 <= sinks < 1 << 31:
+        raise ArgumentError("window must be a whole number from 1 on, sinks from 0 on")
+    return a
+
+
+def window_attention_workspace(be: HipBackend, q, k_pages, window: int, sinks: int = 0, num_seqs: int = 1,
+                               max_query_len: Optional[int] = None):
+    """Scratch of window_attention_ for steps of these sizes, or None where there is none: a byte tensor."""
+    a = _window_args(q, window, sinks, num_seqs, max_query_len if max_query_len is not None else q.shape[0] // max(num_seqs, 1))
+    a.block_table_stride, a.scale = 1, 1.0
+    a.q = a.out = a.positions = a.block_tables = a.query_start_loc = 16
+    c = _shape_only(k_pages)
+    return _workspace(_lib.load().ti_window_attention_workspace_bytes, q.device, ctypes.byref(a), int(window), int(sinks), ctypes.byref(c))
+
+
+def window_attention_(be: HipBackend, out, workspace, q, k_pages, v_pages, block_tables, positions, scale: float, window: int,
+                      sinks: int = 0, query_start_loc: Optional[torch.Tensor] = None, max_query_len: Optional[int] = None):
+    """Causal attention where the query at position p sees the keys p - window + 1 .. p and the first `sinks`; caches of any
+    kind and steps as paged_attention_ takes them. Table entries of pages that hold no visible key are not used
+    (release_pages_ gives such pages back), and a key that a query does not see never reaches its output, whatever the
+    cache holds there. Rows that belong to no sequence are left as they were."""
+    if _done(_lib.native().window_attention(out, workspace, q, k_pages, v_pages, block_tables, positions, scale, window, sinks,
+                                            query_start_loc, max_query_len)):
+        return out
+    on = _one_device(q, out, *_cache_tensors(k_pages, v_pages), block_tables, positions, query_start_loc, workspace)
+    bts, B, n = _step(block_tables, positions, query_start_loc, max_query_len)
+    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype:
+        raise ArgumentError("q and out must be matching [n][heads][D] tensors")
+    if positions.numel() != q.shape[0]:
+        raise ArgumentError("one position per query token")
+    c = kv_cache_struct(k_pages, v_pages, _pool_dtype(k_pages, q))
+    if q.shape[2] != c.head_dim:
+        raise ArgumentError("q's head_dim differs from the pools'")
+    a = _window_args(q, window, sinks, B, n)
+    a.block_table_stride, a.scale = bts.shape[1], float(scale)
+    a.q, a.out, a.positions, a.query_start_loc, a.block_tables = _ptr(q), _ptr(out), _ptr(positions), _ptr(query_start_loc), _ptr(bts)
+    _give_workspace(a, workspace)
+    with on:
+        check(_lib.load().ti_window_attention(ctypes.byref(a), int(window), int(sinks), ctypes.byref(c), _stream(q)))
+    return out
+
+
+def window_attention(be: HipBackend, q, k_pages, v_pages, block_tables, positions, scale: float, window: int, sinks: int = 0,
+                     query_start_loc: Optional[torch.Tensor] = None, max_query_len: Optional[int] = None):
+    """Allocating window_attention_: rows that belong to no sequence are zero."""
+    out = torch.empty_like(q) if query_start_loc is None else torch.zeros_like(q)
+    B = block_tables.shape[0] if block_tables.dim() == 2 else 1
+    return window_attention_(be, out, window_attention_workspace(be, q, k_pages, window, sinks, B, max_query_len), q, k_pages, v_pages,
+                             block_tables, positions, scale, window, sinks, query_start_loc, max_query_len)
+
+
+def _pool_args(pool: PagePool, *ts):
+    """The ti_page_pool and a context with its GPU as the current one; ts on it too."""
+    state = (pool.free_count, pool.tables, pool.lengths, pool.behind, pool.ticket)
+    on = _one_device(pool.free, *state, *ts)
+    for t in (pool.free, *state, *ts):
+        if t is not None:
+            _i32(t, "a pool's and a step's tensors")
+    S, W = pool.tables.shape
+    if pool.free_count.numel() != 1 or pool.lengths.shape != (S,) or (pool.behind is not None and pool.behind.shape != (S,)):
+        raise ArgumentError("a pool has one length per sequence")
+    a = PagePoolArgs(pool.free.numel(), pool.page_size, S, W, pool.window, pool.sinks, _ptr(pool.free), _ptr(pool.free_count),
+                     _ptr(pool.tables), _ptr(pool.lengths), _ptr(pool.behind), _ptr(pool.ticket))
+    return a, on
+
+
+def reserve_pages_(be: HipBackend, pool: PagePool, counts, positions, slots, query_start_loc, short):
+    """reserve and slots (src/kv/block_manager.jl:58-65, 97-100) for every sequence of a step, on the GPU: counts [sequences]
+    int32 more positions each. Writes the step's query_start_loc [sequences + 1], and the positions and slots [tokens] of
+    its tokens, 0 behind them (slot 0 writes nothing); pool.tables and pool.lengths then hold the step. short [1] int32: 0,
+    or the pages that were missing, or -1 where a sequence would outgrow its table or the step the token arrays: then
+    nothing is reserved and the step is empty. Calls on one pool must not overlap. Returns (positions, slots, query_start_loc, short)."""
+    if _done(_lib.native().reserve_pages(pool, counts, positions, slots, query_start_loc, short)):
+        return positions, slots, query_start_loc, short
+    a, on = _pool_args(pool, counts, positions, slots, query_start_loc, short)
+    S = pool.tables.shape[0]
+    if counts.shape != (S,) or query_start_loc.shape != (S + 1,) or short.numel() != 1 or positions.dim() != 1 or slots.shape != positions.shape:
+        raise ArgumentError("counts must be [sequences], query_start_loc [sequences + 1], positions and slots [tokens], short [1]")
+    with on:
+        check(_lib.load().ti_reserve_pages(ctypes.byref(a), _ptr(counts), positions.numel(), _ptr(positions), _ptr(slots),
+                                           _ptr(query_start_loc), _ptr(short), _stream(pool.free)))
+    return positions, slots, query_start_loc, short
+
+
+def release_pages_(be: HipBackend, pool: PagePool, lengths):
+    """truncate (src/kv/block_manager.jl:74-81) for every sequence, on the GPU: sequence b keeps its first lengths[b]
+    positions (all, where that is more), unused pages go back, and with a window those that no query at a kept
+    position's successor or later sees. The stack gets them in the opposite order to that in which reserve_pages_ takes them: a
+    step taken back whole leaves the pool as it was. Calls on one pool must not overlap. Returns pool."""
+    if _done(_lib.native().release_pages(pool, lengths)):
+        return pool
+    a, on = _pool_args(pool, lengths)
+    if lengths.shape != pool.lengths.shape:
+        raise ArgumentError("lengths must be [sequences]")
+    with on:
+        check(_lib.load().ti_release_pages(ctypes.byref(a), _ptr(lengths), _stream(pool.free)))
+    return pool

@@ -8,7 +8,9 @@ Pools are torch tensors in C order, the reference's column-major shapes reversed
 dense (head_dim, page_size, kv_heads, pages) -> [pages][kv_heads][page_size][head_dim];
 an INT8 layer's values `layer_q` (D, P, H, pages, 2) -> [2][pages][H][P][D] (keys first)
 and scales `layer_scale` (P, H, pages, 2) -> [2][pages][H][P]. Page ids and slots are
-1-based, as in the reference, so block tables and slots pass through unchanged.
+1-based, as in the reference, so block tables and slots pass through unchanged. Fp8Pages (8-bit pages
+with one scale per page and KV head) and PagePool (the bookkeeping of the pages on the GPU) have no
+counterpart there.
 """
 from __future__ import annotations
 
@@ -143,6 +145,79 @@ def layer_arrays(k: Int8Pages, v: Int8Pages):
     return k.layer_q, k.layer_scale, k.smooth
 
 
+class Fp8Pages:
+    """One half (keys or values) of an 8-bit block layer: e4m3 values with one scale for each block, the rows
+    of a page and KV head. `q` [pages][H][P][D] torch.float8_e4m3fn and `scale` [pages][H] f32 (powers of two) are
+    views of the layer arrays `layer_q` [2][pages][H][P][D] (uint8 or float8_e4m3fn; keys first) and `layer_scale`
+    [2][pages][H]. head_dim 64 or 128, pages of 2^k rows from 16 to 1024. store_kv_ and attention_inputs_
+    write them, page by page from the first row on; attention_, paged_attention_ and window_attention_ read them."""
+
+    def __init__(self, layer_q: torch.Tensor, layer_scale: torch.Tensor, half: int):
+        if layer_q.dim() != 5 or layer_q.shape[0] != 2 or layer_q.dtype not in (torch.uint8, torch.float8_e4m3fn) \
+                or layer_scale.dtype != torch.float32 or layer_scale.shape != layer_q.shape[:3] or half not in (0, 1):
+            raise ArgumentError("layer_q must be e4m3 [2][pages][kv_heads][P][D] and layer_scale float32 [2][pages][kv_heads]")
+        self.layer_q, self.layer_scale, self.half = layer_q, layer_scale, half
+        self.q = layer_q[half].view(torch.float8_e4m3fn)
+        self.scale = layer_scale[half]
+
+    @property
+    def shape(self):
+        return tuple(self.q.shape)
+
+    def size(self, d: Optional[int] = None):
+        return self.q.size() if d is None else self.q.size(d)
+
+    def values(self) -> torch.Tensor:
+        """What the pages stand for, in Float32."""
+        return self.q.float() * self.scale[..., None, None]
+
+
+def fp8_kv_pools(head_dim: int, page_size: int, kv_heads: int, num_pages: int, device="cuda"):
+    """The zeroed key and value Fp8Pages of one layer."""
+    q = torch.zeros((2, num_pages, kv_heads, page_size, head_dim), dtype=torch.uint8, device=device)
+    s = torch.zeros((2, num_pages, kv_heads), dtype=torch.float32, device=device)
+    return Fp8Pages(q, s, 0), Fp8Pages(q, s, 1)
+
+
+def fp8_layer_arrays(k: Fp8Pages, v: Fp8Pages):
+    """The layer arrays behind a key/value pair; both must be the halves of one layer (fp8_kv_pools)."""
+    if not (isinstance(k, Fp8Pages) and isinstance(v, Fp8Pages) and k.layer_q.data_ptr() == v.layer_q.data_ptr()
+            and k.layer_scale.data_ptr() == v.layer_scale.data_ptr() and k.layer_q.shape == v.layer_q.shape
+            and k.half == 0 and v.half == 1):
+        raise ArgumentError("keys and values must be the halves of one layer's pools (fp8_kv_pools)")
+    return k.layer_q, k.layer_scale
+
+
+class PagePool:
+    """The pages of a cache and the sequences that hold them, on the GPU: what BlockManager and Sequence keep on the
+    host. `free` [num_pages] int32 is the stack of free page ids (1-based), `free_count` [1] its height, `tables`
+    [sequences][width] int32 the sequences' pages (0: none), `lengths` [sequences] int32 their positions.
+    reserve_pages_ and release_pages_ change them in place.
+
+    window, sinks: of the attention over the cache (window_attention_); release_pages_ then gives back the pages that no later
+    query sees. `behind` [sequences] counts a sequence's pages up to the first that it still holds past its sinks."""
+
+    def __init__(self, free: torch.Tensor, free_count: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, page_size: int,
+                 window: int = 0, sinks: int = 0):
+        if any(t.dtype != torch.int32 for t in (free, free_count, tables, lengths)) or free.dim() != 1 or free_count.numel() != 1 \
+                or tables.dim() != 2 or lengths.shape != tables.shape[:1]:
+            raise ArgumentError("free, free_count, tables and lengths must be int32 [pages], [1], [sequences][width] and [sequences]")
+        if page_size <= 0 or window < 0 or sinks < 0:
+            raise ArgumentError("page_size must be positive, window and sinks not negative")
+        self.free, self.free_count, self.tables, self.lengths = free, free_count, tables, lengths
+        self.page_size, self.window, self.sinks = int(page_size), int(window), int(sinks)
+        self.behind = torch.full_like(lengths, -(-self.sinks // self.page_size)) if window else None
+        self.ticket = torch.zeros(1, dtype=torch.int32, device=free.device)
+
+
+def page_pool(num_pages: int, page_size: int, num_seqs: int, max_pages: int, window: int = 0, sinks: int = 0, device="cuda") -> PagePool:
+    """A PagePool whose pages are all free, handed out in increasing order as a new BlockManager's, for num_seqs
+    sequences of at most max_pages pages."""
+    i32 = dict(dtype=torch.int32, device=device)
+    return PagePool(torch.arange(num_pages, 0, -1, **i32), torch.full((1,), num_pages, **i32),
+                    torch.zeros((num_seqs, max_pages), **i32), torch.zeros(num_seqs, **i32), page_size, window, sinks)
+
+
 class KeyBounds:
     """Bounds of the keys of a layer's pages, beside its pools of either kind: for each page and KV
     head the keys' largest and smallest element in each dimension as whole multiples of the page's
@@ -189,7 +264,7 @@ def key_bounds(head_dim: int, page_size: int, kv_heads: int, num_pages: int, dev
 
 class PagedKVCache:
     """Key/value pools for every layer and their page allocator (src/kv/paged_cache.jl:18-36).
-    quantize=None: pools in `dtype`; quantize="int8": Int8Pages pairs. bounds=True: a KeyBounds
+    quantize=None: pools in `dtype`; "int8": Int8Pages pairs; "fp8": Fp8Pages pairs. bounds=True: a KeyBounds
     for every layer in `bounds`, for attention over chosen pages; bounds_channel: the channel of each layer's."""
 
     def __init__(self, num_layers: int, head_dim: int, kv_heads: int, num_pages: int,
@@ -210,8 +285,14 @@ class PagedKVCache:
                      for l in range(num_layers)]
             self.k = [p[0] for p in pairs]
             self.v = [p[1] for p in pairs]
+        elif quantize == "fp8":
+            if bounds:
+                raise ArgumentError("page bounds are of dense and INT8 caches")
+            pairs = [fp8_kv_pools(head_dim, page_size, kv_heads, num_pages, device) for _ in range(num_layers)]
+            self.k = [p[0] for p in pairs]
+            self.v = [p[1] for p in pairs]
         else:
-            raise ArgumentError(f"unsupported KV cache quantization {quantize} (only 'int8')")
+            raise ArgumentError(f"unsupported KV cache quantization {quantize} (only 'int8' and 'fp8')")
 
     def page_size(self) -> int:
         return self.blocks.page_size
@@ -226,7 +307,9 @@ class PagedKVCache:
 def bytes_per_token(num_layers: int, kv_heads: int, head_dim: int, elt_bytes: int = 2,
                     quantize=None) -> int:
     """Cache bytes per cached position (src/kv/paged_cache.jl:43-47), without KeyBounds (2 head_dim + 4
-    bytes a page, layer and KV head)."""
+    bytes a page, layer and KV head) and the scales of Fp8Pages (8 bytes a page, layer and KV head)."""
+    if quantize == "fp8":
+        return 2 * num_layers * kv_heads * head_dim
     if quantize == "int8":
         return 2 * num_layers * kv_heads * (head_dim + 4)
     return 2 * num_layers * kv_heads * head_dim * elt_bytes
