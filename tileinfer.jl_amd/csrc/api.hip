@@ -60,19 +60,18 @@ bool bad_dtype(int dtype) { return dtype != TI_F32 && dtype != TI_BF16; }
 int resolve_path(const ti_attention_args *a, const ti_kv_cache *c) {
     const int G = a->q_heads / c->kv_heads;
     if (a->dtype == TI_F32) return 0;
-    if (c->kind == TI_KV_FP8) return a->path < TI_PATH_AUTO || a->path > TI_PATH_PREFILL_PAIRED16 ? -TI_ERR_INVALID_ARG : 0;
     const int rows = G * a->max_query_len;
     const bool decode_ok = rows <= 64;
     const bool decode_auto = a->max_query_len <= 16 && (rows <= 32 || (a->max_query_len == 1 && decode_ok));
     switch (a->path) {
-        case TI_PATH_AUTO: return decode_auto ? 1 : (G <= 64 ? 2 : -TI_ERR_UNSUPPORTED);
+        case TI_PATH_AUTO: return decode_auto ? 1 : (G <= 64 ? c->kind == TI_KV_FP8 ? 0 : 2 : -TI_ERR_UNSUPPORTED);
         case TI_PATH_DECODE: return decode_ok ? 1 : -TI_ERR_UNSUPPORTED;
         case TI_PATH_PREFILL:
         case TI_PATH_PREFILL_STAGED:
         case TI_PATH_PREFILL_DIRECT:
         case TI_PATH_PREFILL_PINGPONG:
         case TI_PATH_PREFILL_PAIRED:
-        case TI_PATH_PREFILL_PAIRED16: return G <= 64 ? 2 : -TI_ERR_UNSUPPORTED;
+        case TI_PATH_PREFILL_PAIRED16: return G <= 64 ? c->kind == TI_KV_FP8 ? 0 : 2 : -TI_ERR_UNSUPPORTED;
         default: return -TI_ERR_INVALID_ARG;
     }
 }
@@ -234,6 +233,7 @@ int ti_attention(const ti_attention_args *a, const ti_kv_cache *c, void *stream)
     }
     const ti_decode_plan pl = ti_plan_decode(a, c);
     if (pl.bytes > 0 && (!a->workspace || a->workspace_bytes < pl.bytes)) return TI_ERR_WORKSPACE;
+    if (c->kind == TI_KV_FP8) return ti_launch_decode_window(a, c, pl, ti_window{}, s);
     return ti_launch_decode(a, c, pl, s);
 }
 
@@ -371,7 +371,9 @@ int ti_window_attention_workspace_bytes(const ti_attention_args *a, int window, 
     *bytes = 0;
     const int st = check_window(a, window, sinks, c);
     if (st) return st;
-    ti_plan_generic(a, c, bytes);
+    const ti_window win{window, sinks};
+    if (a->dtype == TI_BF16 && ti_window_decodes(a, c)) *bytes = ti_plan_decode(a, c, win).bytes;
+    else ti_plan_generic(a, c, bytes);
     return TI_OK;
 }
 
@@ -379,7 +381,11 @@ int ti_window_attention(const ti_attention_args *a, int window, int sinks, const
     size_t need = 0;
     int st = ti_window_attention_workspace_bytes(a, window, sinks, c, &need);
     if (!st) st = check_workspace(a->workspace, a->workspace_bytes, need);
-    return st ? st : ti_launch_generic(a, c, (hipStream_t)stream, ti_window{window, sinks});
+    if (st) return st;
+    const ti_window win{window, sinks};
+    hipStream_t s = (hipStream_t)stream;
+    if (a->dtype == TI_BF16 && ti_window_decodes(a, c)) return ti_launch_decode_window(a, c, ti_plan_decode(a, c, win), win, s);
+    return ti_launch_generic(a, c, s, win);
 }
 
 int ti_reserve_pages(const ti_page_pool *pool, const int32_t *counts, int tokens, int32_t *positions, int32_t *slots,

@@ -157,7 +157,10 @@ struct ti_decode_plan {
     size_t meta;     // flat: byte offset of the per-sequence {first work-group, pieces} table
     size_t bytes;    // workspace bytes
 };
-ti_decode_plan ti_plan_decode(const ti_attention_args *a, const ti_kv_cache *c);
+ti_decode_plan ti_plan_decode(const ti_attention_args *a, const ti_kv_cache *c, ti_window win = ti_window{});
+bool ti_window_decodes(const ti_attention_args *a, const ti_kv_cache *c);
+// With a window, or over an 8-bit block cache (pa_window.hip).
+int ti_launch_decode_window(const ti_attention_args *a, const ti_kv_cache *c, const ti_decode_plan &p, ti_window win, hipStream_t s);
 int ti_launch_decode(const ti_attention_args *a, const ti_kv_cache *c, const ti_decode_plan &p,
                      hipStream_t s);
 // Merge split partials [B][Hk][splits][rows][D + 2] from a->workspace into a->out; flat

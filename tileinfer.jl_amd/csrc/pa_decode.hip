@@ -138,7 +138,7 @@ void launch_decode_p(const DecodeParams &p, int rowb, int waves, dim3 grid, hipS
 // combine launch); smaller ones split the keys into a power of two of 4-wave groups (at
 // most 16, about 8 waves per CU over the 256 CUs) merged by the combine kernel. Depends only
 // on host shapes, never on context length, so a captured graph stays valid.
-ti_decode_plan ti_plan_decode(const ti_attention_args *a, const ti_kv_cache *c) {
+ti_decode_plan ti_plan_decode(const ti_attention_args *a, const ti_kv_cache *c, ti_window win) {
     ti_decode_plan pl;
     const int G = a->q_heads / c->kv_heads;
     pl.rows = G * a->max_query_len;
@@ -157,6 +157,9 @@ ti_decode_plan ti_plan_decode(const ti_attention_args *a, const ti_kv_cache *c) 
     int sp = 1, nw = 4;
     if (pairs < 256 || pl.rows > 32) {
         while (sp < max_splits && pairs * sp < target) sp <<= 1;
+        // A window bounds the keys: no more splits than leave every wave of each a tile.
+        const long long tiles = ((long long)win.size + a->max_query_len + 30) / 16 + ((long long)win.sinks + 15) / 16;
+        while (win.size && sp > 1 && 4LL * (sp / 2) >= tiles) sp >>= 1;
     }
     // Split batches of 4-64 sequences with at least 4 splits each share their work-groups out
     // by length (flat mode): the same B x splits work-groups per KV head, cut in proportion
@@ -176,33 +179,7 @@ ti_decode_plan ti_plan_decode(const ti_attention_args *a, const ti_kv_cache *c) 
 
 int ti_launch_decode(const ti_attention_args *a, const ti_kv_cache *c, const ti_decode_plan &pl,
                      hipStream_t s) {
-    DecodeParams p;
-    p.q = (const uint16_t *)a->q;
-    p.out = (uint16_t *)a->out;
-    p.kp = (const uint16_t *)c->k_pages;
-    p.vp = (const uint16_t *)c->v_pages;
-    p.lq = c->layer_q;
-    p.ls = c->layer_scale;
-    p.smooth = c->smooth;
-    p.positions = a->positions;
-    p.qsl = a->query_start_loc;
-    p.bt = a->block_tables;
-    p.part = (float *)a->workspace;
-    p.meta = pl.flat ? reinterpret_cast<int *>((char *)a->workspace + pl.meta) : nullptr;
-    p.B = a->num_seqs;
-    p.flat = pl.flat;
-    p.bt_stride = a->block_table_stride;
-    p.num_pages = c->num_pages;
-    p.P = c->page_size;
-    p.pshift = (c->page_size & (c->page_size - 1)) == 0 ? __builtin_ctz(c->page_size) : -1;
-    p.Hk = c->kv_heads;
-    p.Hq = a->q_heads;
-    p.G = a->q_heads / c->kv_heads;
-    p.nmax = a->max_query_len;
-    p.M = pl.rows;
-    p.splits = pl.splits;
-    p.causal = a->causal;
-    p.scale_log2 = a->scale * LOG2E;
+    const DecodeParams p = decode_params(a, c, pl);
     const int rowb = (pl.rows + 15) / 16;
     const dim3 grid = pl.flat ? dim3(pl.flat, c->kv_heads, 1) : dim3(pl.splits, c->kv_heads, a->num_seqs);
     const bool int8 = c->kind == TI_KV_INT8;

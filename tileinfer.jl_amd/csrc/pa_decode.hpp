@@ -46,6 +46,7 @@
 #include <type_traits>
 
 #include "pa_group.hpp"
+#include "pa_window.hpp"
 
 using namespace ti;
 
@@ -68,7 +69,14 @@ struct DecodeParams {
     int min_tiles;   // > 0: splits of at least this many 16-key tiles (f32_active_splits)
     float scale_log2;
     const int32_t *lengths;   // SPARSE: keys of each (token, KV head); bt holds a table row for each
-    int tg, total;            // GROUP: tokens of a group, tokens of the call
+    union {
+        int tg;               // GROUP: tokens of a group
+        int window;           // WIN
+    };
+    union {
+        int total;            // GROUP: tokens of the call
+        int sinks;            // WIN
+    };
 };
 
 // Flat mode: the W = p.flat work-groups of a KV head are shared out over the B sequences
@@ -81,6 +89,7 @@ struct DecodeParams {
 struct FlatPiece {
     int b, lo, n, tok0, nb, start;
 };
+template <bool WIN = false>
 __device__ inline FlatPiece flat_piece(const DecodeParams &p, int x, int lane) {
     int tok0 = 0, nb = 0, st = 0, nt = 0;
     if (lane < p.B) {
@@ -89,6 +98,7 @@ __device__ inline FlatPiece flat_piece(const DecodeParams &p, int x, int lane) {
         if (nb > 0) {
             st = max(p.positions[tok0], 0);
             nt = (st + nb + 15) >> 4;
+            if constexpr (WIN) nt -= WindowTiles::of<4>(st, p.window, p.sinks).skip;
         }
     }
     int incl = nt;
@@ -209,10 +219,27 @@ struct RowMap {
         return ((long long)pg * Hk + h) * P + (pos & (P - 1));
     }
     __device__ __forceinline__ int last(int pos) const { return len - 1 - pos; }   // last key of the tile at pos
+    __device__ __forceinline__ int first_key(int) const { return 0; }             // and first
+    __device__ __forceinline__ int pos(int j) const { return j * 16; }            // the tile's first position
 };
 
-// PART: 1 the keys, 2 the values, 3 both (1 and 2 for whole tiles).
-template <int D, bool INT8, bool PG16, int PART = 3, typename Map>
+// The tiles that a window leaves (WindowTiles). Keys that no row of the work-group sees are read as a neighbour that
+// one does, so that what they hold does not matter.
+struct WindowMap : RowMap {
+    WindowTiles t;
+    int sinks;
+    __device__ __forceinline__ int pos(int j) const { return t.tile(j) * 16; }
+    __device__ __forceinline__ int last(int pos) const { return min(len, pos < t.lo && pos + 16 <= t.lo ? min(sinks, t.lo) : len) - 1 - pos; }
+    __device__ __forceinline__ int first_key(int pos) const { return pos < sinks ? 0 : max(t.lo - pos, 0); }
+    __device__ __forceinline__ long long row(int pos) const {
+        if (pos < t.lo && pos >= sinks) pos = (pos & ~15) + 15 < t.lo ? min(sinks, t.lo) - 1 : t.lo;
+        return RowMap::row(pos);
+    }
+};
+
+// PART: 1 the keys, 2 the values, 3 both (1 and 2 for whole tiles). FP8: 8-bit block caches, whose tiles are as INT8 ones
+// (TileRegs<D, true>) but for the scales, one of a tile's keys and one of its values.
+template <int D, bool INT8, bool PG16, int PART = 3, bool FP8 = false, typename Map>
 __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodeParams &p,
                                           const Map &rm, int j, int r16, int kg, int vg,
                                           int vc, size_t half_q, size_t half_s) {
@@ -222,12 +249,18 @@ __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodePara
         // (scalar-base addressing, no 64-bit vector math). Keys past len read the last
         // valid key's row, whose finite values meet p = 0 (never stale memory that could
         // hold NaN).
-        const long long r0 = rm.row_s(j * 16);
-        const int last = rm.last(j * 16);
-        const uint32_t kr = (uint32_t)min(r16, last);
+        const long long r0 = rm.row_s(rm.pos(j));
+        const int last = rm.last(rm.pos(j));
+        uint32_t kr = (uint32_t)min(r16, last);
         uint32_t vr[KPL];
 #pragma unroll
         for (int e = 0; e < KPL; e++) vr[e] = (uint32_t)min(vg * KPL + e, last);
+        if constexpr (std::is_same_v<Map, WindowMap>) {
+            const uint32_t first = (uint32_t)rm.first_key(rm.pos(j));
+            kr = max(kr, first);
+#pragma unroll
+            for (int e = 0; e < KPL; e++) vr[e] = max(vr[e], first);
+        }
         // Values are streamed with non-temporal loads: each value row is read once per
         // split, and keeping them out of the caches measured 8-10% faster on bf16 pages and
         // 4% on INT8 pages. Keys keep normal loads (non-temporal keys measured 26% slower on
@@ -256,16 +289,21 @@ __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodePara
                 const u32x2 r = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(vb + (vr[e] * D + vc * 8)));
                 t.v[e] = (u32x4){r[0], r[1], 0u, 0u};
             }
-            const float *sb = p.ls + r0;
-            if (PART & 1) t.sk = sb[kr];
-            if (PART & 2) t.sv = sb[half_s + kr];
+            if constexpr (FP8) {
+                if (PART & 1) t.sk = sloadf(p.ls, r0 >> p.pshift);
+                if (PART & 2) t.sv = sloadf(p.ls, (long long)((r0 + (long long)half_s) >> p.pshift));
+            } else {
+                const float *sb = p.ls + r0;
+                if (PART & 1) t.sk = sb[kr];
+                if (PART & 2) t.sv = sb[half_s + kr];
+            }
         }
         return;
     }
     long long krow, vrow[KPL];
-    krow = rm.row(j * 16 + r16);
+    krow = rm.row(rm.pos(j) + r16);
 #pragma unroll
-    for (int e = 0; e < KPL; e++) vrow[e] = rm.row(j * 16 + vg * KPL + e);
+    for (int e = 0; e < KPL; e++) vrow[e] = rm.row(rm.pos(j) + vg * KPL + e);
     if (!INT8) {
 #pragma unroll
         for (int i = 0; i < NKB; i++)
@@ -295,7 +333,9 @@ __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodePara
 // pairs' splits, KV heads innermost. GROUP (SPARSE, whole tiles): p.tg neighbouring tokens' pairs at a time
 // over the joined list of their pages, packed rows g + G t of the group. (32 rows of INT8 caches take 8 registers
 // too many for two waves a SIMD by themselves, 112 and 72 us for 512 tokens.)
-template <int D, int ROWB, bool INT8, bool PG16, int NW, int RS, bool JOINT = false, bool SPARSE = false, bool GROUP = false>
+// FP8: an 8-bit block cache (whole tiles). WIN: the window of pa_window.hpp; keys are cut into tiles of the list that it leaves.
+template <int D, int ROWB, bool INT8, bool PG16, int NW, int RS, bool JOINT = false, bool SPARSE = false, bool GROUP = false,
+          bool FP8 = false, bool WIN = false>
 __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) decode_kernel(DecodeParams p) {
     constexpr int NKB = D / 32;          // 32-wide head-dim blocks (QK MFMAs per tile)
     constexpr int NDT = D / 16;          // 16-wide head-dim tiles (PV MFMAs per tile)
@@ -306,7 +346,9 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
     // Tiles loaded per step (TPI: see the loop) and worked on together (JT). JOINT: a whole step
     // runs its tiles through one softmax, so their score chains overlap and one max decides the
     // rescale. GROUP: two, whose values are one product of depth 32 (INT8, 512 tokens: 100 -> 88 us).
-    constexpr int TPI = GROUP ? 2 : INT8 ? (ROWB == 1 ? 3 : 2) : 1, JT = JOINT || GROUP ? TPI : 1;
+    constexpr int TPI = GROUP ? 2 : INT8 || FP8 ? (ROWB == 1 ? 3 : 2) : 1, JT = JOINT || GROUP ? TPI : 1;
+    constexpr bool B8 = INT8 || FP8, SAFE = FP8 || WIN;   // SAFE: rows are done again where a product is not finite
+    static_assert(!FP8 || (PG16 && !INT8 && !SPARSE), "8-bit block caches: whole tiles of one page");
 
     // Per-wave transposed V tiles during the key loop; afterwards the same LDS holds each
     // wave's (O, m, l) slab for the merge (rows of D + 4 floats, 16-B aligned).
@@ -353,7 +395,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
             return;
         }
     } else if (p.flat) {
-        const FlatPiece f = flat_piece(p, blockIdx.x, lane);
+        const FlatPiece f = flat_piece<WIN>(p, blockIdx.x, lane);
         b = f.b;
         s = blockIdx.x - f.lo;
         nsp = f.n;
@@ -377,13 +419,17 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
     int len = start + nb;
     __shared__ int red[2 + NW];   // GROUP
     if constexpr (GROUP) len = group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem_raw), lim, red, tok0, h, q0, q1) * p.P;
-    const int ntiles = (len + 15) >> 4;
+    WindowTiles wt{};
+    if constexpr (WIN) wt = WindowTiles::of<4>(start, p.window, p.sinks);
+    const int ntiles = ((len + 15) >> 4) - wt.skip;
     const int per = (ntiles + nsp - 1) / nsp;
     const int j0 = s * per, j1 = min(j0 + per, ntiles);
     const size_t half_q = (size_t)p.num_pages * p.Hk * p.P * D;
     const size_t half_s = (size_t)p.num_pages * p.Hk * p.P;
     const auto rm = [&] {
         if constexpr (GROUP) return GroupMap{reinterpret_cast<const int2 *>(smem_raw), p.P, p.pshift, p.Hk, h, len};
+        else if constexpr (WIN)
+            return WindowMap{{p.bt + (size_t)b * p.bt_stride, p.P, p.pshift, p.Hk, h, p.num_pages, len, p.bt_stride}, wt, p.sinks};
         else return RowMap{p.bt + (size_t)b * p.bt_stride, p.P, p.pshift, p.Hk, h, p.num_pages, len, p.bt_stride};
     }();
     // Keys up to mask_from are visible to every row; later tiles need the mask.
@@ -404,8 +450,12 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
         const uint16_t *qr = p.q + ((size_t)(tok0 + t) * p.Hq + h * p.G + g) * D;
         if constexpr (!INT8) {
 #pragma unroll
-            for (int i = 0; i < NKB; i++)
-                qreg[rb][i] = ok ? *reinterpret_cast<const u32x4 *>(qr + i * 32 + kg * 8) : (u32x4){0u, 0u, 0u, 0u};
+            for (int i = 0; i < NKB; i++) {
+                if constexpr (FP8)   // the keys' 16-B loads' order
+                    qreg[rb][i] = ok ? *reinterpret_cast<const u32x4 *>(qr + (i >> 1) * 64 + kg * 16 + (i & 1) * 8) : (u32x4){0u, 0u, 0u, 0u};
+                else
+                    qreg[rb][i] = ok ? *reinterpret_cast<const u32x4 *>(qr + i * 32 + kg * 8) : (u32x4){0u, 0u, 0u, 0u};
+            }
         } else {
             float qf[NKB][8], amax = 0.0f;
 #pragma unroll
@@ -464,7 +514,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
     const int vc = lane % CPR, vg = lane / CPR;   // V load: chunk, key group
 
     // NT tiles j .. j + NT - 1: their scores, one softmax over them, their values.
-    auto compute = [&](const TileRegs<D, INT8> *t, int j, auto count) {
+    auto compute = [&](const TileRegs<D, B8> *t, int j, auto count) {
         constexpr int NT = decltype(count)::value;
         // ---- V rows -> row-major LDS tiles (INT8: biased fp16, exact) ----
         u32x4 vrows[NT][KPL];
@@ -472,7 +522,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int e = 0; e < KPL; e++)
-                vrows[n][e] = INT8 ? i8x8_to_f16b(t[n].v[e][0], t[n].v[e][1]) : t[n].v[e];
+                vrows[n][e] = FP8 ? e4m3x8_to_bf16(t[n].v[e][0], t[n].v[e][1], t[n].sv) : INT8 ? i8x8_to_f16b(t[n].v[e][0], t[n].v[e][1]) : t[n].v[e];
         lds_fence();   // the previous step's reads of myvt are done before overwriting
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -485,7 +535,8 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
         for (int n = 0; n < NT; n++) {
             u32x4 kreg[NKB];
 #pragma unroll
-            for (int i = 0; i < NKB; i++) kreg[i] = INT8 ? i8x8_to_f16b(t[n].k[i][0], t[n].k[i][1]) : t[n].k[i];
+            for (int i = 0; i < NKB; i++)
+                kreg[i] = FP8 ? e4m3x8_to_bf16(t[n].k[i][0], t[n].k[i][1], t[n].sk) : INT8 ? i8x8_to_f16b(t[n].k[i][0], t[n].k[i][1]) : t[n].k[i];
 #pragma unroll
             for (int rb = 0; rb < ROWB; rb++) {
                 sc[n][rb] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -509,7 +560,12 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
         // it by more than RESCALE_LOG2 (then p <= 2^RESCALE_LOG2, safe in bf16 and fp32);
         // l and O always use the same reference, so the result is exact. INT8 moves m
         // with every larger max (p <= 1, so p times a value scale stays within fp16).
-        const bool need_mask = (j + NT) * 16 - 1 > mask_from;
+        bool need_mask = (WIN ? rm.pos(j + NT - 1) + 16 : (j + NT) * 16) - 1 > mask_from;
+        if constexpr (WIN) {
+            // tiles in front of the last row's window, and those of sinks that end inside one
+#pragma unroll
+            for (int n = 0; n < NT; n++) need_mask |= rm.pos(j + n) < len - p.window && rm.pos(j + n) + 15 >= p.sinks;
+        }
         s16x4 pop[NT][ROWB];
         float x[ROWB][4 * NT], mt[ROWB];
         bool grow = false;
@@ -522,8 +578,13 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
                 if (INT8) v = (v - qcorr[rb]) * skk[e >> 2][e & 3] * qsl[rb];
                 else v *= p.scale_log2;
                 if (need_mask) {
-                    const int kp = (j + (e >> 2)) * 16 + kg * 4 + (e & 3);
-                    v = (kp <= qpos[rb] && kp < len) ? v : -INFINITY;
+                    if constexpr (WIN) {
+                        const int kp = rm.pos(j + (e >> 2)) + kg * 4 + (e & 3);
+                        v = (kp <= qpos[rb] && (kp > qpos[rb] - p.window || kp < p.sinks)) ? v : -INFINITY;
+                    } else {
+                        const int kp = (j + (e >> 2)) * 16 + kg * 4 + (e & 3);
+                        v = (kp <= qpos[rb] && kp < len) ? v : -INFINITY;
+                    }
                 }
                 x[rb][e] = v;
                 mt[rb] = fmaxf(mt[rb], v);
@@ -728,13 +789,13 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
     // unconditionally (past the last tile it re-reads that tile, unused) so the count of
     // loads in flight is static and each wait covers only the tiles in use.
     constexpr int STRIDE = NKW * TPI;
-    TileRegs<D, INT8> ta[TPI], tb[TPI];
-    auto ld = [&](TileRegs<D, INT8> (&t)[TPI], int jj) {
+    TileRegs<D, B8> ta[TPI], tb[TPI];
+    auto ld = [&](TileRegs<D, B8> (&t)[TPI], int jj) {
 #pragma unroll
         for (int e = 0; e < TPI; e++)
-            load_tile<D, INT8, PG16>(t[e], p, rm, min(jj + e, j1 - 1), r16, kg, vg, vc, half_q, half_s);
+            load_tile<D, B8, PG16, 3, FP8>(t[e], p, rm, min(jj + e, j1 - 1), r16, kg, vg, vc, half_q, half_s);
     };
-    auto run = [&](const TileRegs<D, INT8> (&t)[TPI], int jj) {
+    auto run = [&](const TileRegs<D, B8> (&t)[TPI], int jj) {
         if constexpr (JT > 1) {
             if (jj + JT <= j1) return compute(t, jj, std::integral_constant<int, JT>{});
         }
@@ -799,7 +860,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
         l[rb] += __shfl_xor(l[rb], 16);
         l[rb] += __shfl_xor(l[rb], 32);
     }
-    bool fine = true;   // GROUP: no value that is not finite has come in (rows of tokens without keys: none does, they are zeros)
+    bool fine = true;   // GROUP, SAFE: no value that is not finite has come in (GROUP's rows of tokens without keys: none does, they are zeros)
 #pragma unroll
     for (int hb = 0; hb < ROWB; hb += HB) {
         __syncthreads();   // every wave is done with its V tile
@@ -843,6 +904,11 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
                     }
                 }
             }
+            if constexpr (SAFE) {
+                fine &= fabsf(lsum) < INFINITY;
+#pragma unroll
+                for (int e = 0; e < 4; e++) fine &= fabsf(acc[e]) < INFINITY;
+            }
             if (nsp == 1) {
                 // One split: this group saw every key; normalize and write the output rows.
                 const int t = r / p.G, g = r - t * p.G;
@@ -864,6 +930,32 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
             }
         }
     }
+    if constexpr (SAFE) {
+        if (__syncthreads_or(!fine)) {
+            constexpr int PER = D / 64;
+            for (int r = w; r < min(p.M, nb * p.G); r += NW) {
+                const int t = r / p.G, last = p.causal ? start + t : len - 1;
+                const size_t qrow = (size_t)(tok0 + t) * p.Hq + h * p.G + (r - t * p.G);
+                float m, l, acc[PER];
+                exact_row<D, INT8, FP8>(p, rm.bt, h, p.q + qrow * D, j0 * 16, j1 * 16, [&](int v) {
+                    const int key = rm.pos(v >> 4) + (v & 15);
+                    return key <= last && (!WIN || key > last - p.window || key < p.sinks) ? key : -1;
+                }, m, l, acc);
+                if (nsp == 1) {
+#pragma unroll
+                    for (int k = 0; k < PER; k++) Elt<uint16_t>::st(p.out, qrow * D + lane + 64 * k, acc[k] / l);
+                } else {
+                    float *dst = p.part + (unit * (size_t)p.M + r) * (D + 2);
+#pragma unroll
+                    for (int k = 0; k < PER; k++) dst[lane + 64 * k] = acc[k];
+                    if (lane == 0) {
+                        dst[D] = m;
+                        dst[D + 1] = l;
+                    }
+                }
+            }
+        }
+    }
     if constexpr (GROUP && !INT8) {
         // The slabs have overwritten the joined list: it is made again.
         if (__syncthreads_or(!fine)) {
@@ -871,6 +963,38 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
             group_rows<D>(p, reinterpret_cast<const int2 *>(smem_raw), lim, tok0, h, q0, q1, j0, j1, nsp, unit, w, NW, lane);
         }
     }
+}
+
+// A step's parameters for the kernel and its combine.
+inline DecodeParams decode_params(const ti_attention_args *a, const ti_kv_cache *c, const ti_decode_plan &pl) {
+    DecodeParams p{};
+    p.q = (const uint16_t *)a->q;
+    p.out = (uint16_t *)a->out;
+    p.kp = (const uint16_t *)c->k_pages;
+    p.vp = (const uint16_t *)c->v_pages;
+    p.lq = c->layer_q;
+    p.ls = c->layer_scale;
+    p.smooth = c->smooth;
+    p.positions = a->positions;
+    p.qsl = a->query_start_loc;
+    p.bt = a->block_tables;
+    p.part = (float *)a->workspace;
+    p.meta = pl.flat ? reinterpret_cast<int *>((char *)a->workspace + pl.meta) : nullptr;
+    p.B = a->num_seqs;
+    p.flat = pl.flat;
+    p.bt_stride = a->block_table_stride;
+    p.num_pages = c->num_pages;
+    p.P = c->page_size;
+    p.pshift = (c->page_size & (c->page_size - 1)) == 0 ? __builtin_ctz(c->page_size) : -1;
+    p.Hk = c->kv_heads;
+    p.Hq = a->q_heads;
+    p.G = a->q_heads / c->kv_heads;
+    p.nmax = a->max_query_len;
+    p.M = pl.rows;
+    p.splits = pl.splits;
+    p.causal = a->causal;
+    p.scale_log2 = a->scale * LOG2E;
+    return p;
 }
 
 }  // namespace ti_decode

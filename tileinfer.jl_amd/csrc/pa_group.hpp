@@ -32,6 +32,7 @@ struct GroupMap {
         return most - 1 - first(pos, most);
     }
     __device__ __forceinline__ long long row(int) const { return 0; }   // whole tiles only
+    __device__ __forceinline__ int pos(int j) const { return j * 16; }
 };
 
 // Groups of tokens over chosen pages. The tables of up to GROUP_PAGES entries in all are joined into one
