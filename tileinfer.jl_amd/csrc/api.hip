@@ -64,14 +64,14 @@ int resolve_path(const ti_attention_args *a, const ti_kv_cache *c) {
     const bool decode_ok = rows <= 64;
     const bool decode_auto = a->max_query_len <= 16 && (rows <= 32 || (a->max_query_len == 1 && decode_ok));
     switch (a->path) {
-        case TI_PATH_AUTO: return decode_auto ? 1 : (G <= 64 ? c->kind == TI_KV_FP8 ? 0 : 2 : -TI_ERR_UNSUPPORTED);
+        case TI_PATH_AUTO: return decode_auto ? 1 : (G <= 64 ? 2 : -TI_ERR_UNSUPPORTED);
         case TI_PATH_DECODE: return decode_ok ? 1 : -TI_ERR_UNSUPPORTED;
         case TI_PATH_PREFILL:
         case TI_PATH_PREFILL_STAGED:
         case TI_PATH_PREFILL_DIRECT:
         case TI_PATH_PREFILL_PINGPONG:
         case TI_PATH_PREFILL_PAIRED:
-        case TI_PATH_PREFILL_PAIRED16: return G <= 64 ? c->kind == TI_KV_FP8 ? 0 : 2 : -TI_ERR_UNSUPPORTED;
+        case TI_PATH_PREFILL_PAIRED16: return G <= 64 ? 2 : -TI_ERR_UNSUPPORTED;
         default: return -TI_ERR_INVALID_ARG;
     }
 }
@@ -95,10 +95,24 @@ int check_attention(const ti_attention_args *a, const ti_kv_cache *c) {
     return TI_OK;
 }
 
+// The plan of a prefill. An 8-bit block cache has no variants to pin.
+ti_prefill_plan prefill_plan(const ti_attention_args *a, const ti_kv_cache *c, bool bound_keys, ti_window win = ti_window{}) {
+    ti_attention_args local = *a;
+    if (c->kind == TI_KV_FP8) local.path = TI_PATH_PREFILL;
+    return ti_plan_prefill(&local, c, bound_keys, win);
+}
+
 // Grid y of a prefill launch: paired plans hold two q-tiles per work-group, the others one
 // q-tile per key split. At most 65535.
 long long prefill_grid_y(const ti_prefill_plan &pl) {
     return pl.pair ? (pl.qtiles + 1LL) / 2 : (long long)pl.qtiles * pl.splits;
+}
+
+int window_prefill(const ti_attention_args *a, const ti_kv_cache *c, ti_window win, bool bound_keys, ti_prefill_plan *pl) {
+    if (a->q_heads / c->kv_heads > 64) return TI_ERR_UNSUPPORTED;
+    *pl = prefill_plan(a, c, bound_keys, win);
+    if (prefill_grid_y(*pl) > 65535) pl->splits = 1, pl->bytes = 0;   // unsplit
+    return prefill_grid_y(*pl) > 65535 ? TI_ERR_UNSUPPORTED : TI_OK;
 }
 
 bool misaligned(const void *p) { return ((uintptr_t)p & 15) != 0; }
@@ -204,7 +218,7 @@ int ti_attention_workspace_bytes(const ti_attention_args *a, const ti_kv_cache *
     if (path == 0) ti_plan_generic(a, c, bytes);
     if (path == 1) *bytes = ti_plan_decode(a, c).bytes;
     if (path == 2) {
-        ti_prefill_plan pp = ti_plan_prefill(a, c, false);
+        ti_prefill_plan pp = prefill_plan(a, c, false);
         if (prefill_grid_y(pp) > 65535) pp.splits = 1, pp.bytes = 0;   // runs unsplit
         if (prefill_grid_y(pp) > 65535) return TI_ERR_UNSUPPORTED;
         *bytes = pp.bytes;
@@ -222,7 +236,7 @@ int ti_attention(const ti_attention_args *a, const ti_kv_cache *c, void *stream)
     if (path == 2) {
         // The prefill path never requires a workspace (the reference runs its prefill
         // kernel exactly when none is passed); without one it runs unsplit.
-        ti_prefill_plan pp = ti_plan_prefill(a, c, true);
+        ti_prefill_plan pp = prefill_plan(a, c, true);
         if (prefill_grid_y(pp) > 65535) pp.splits = 1, pp.bytes = 0;
         if (prefill_grid_y(pp) > 65535) return TI_ERR_UNSUPPORTED;   // q-tiles share grid y
         if (pp.bytes > 0 && (!a->workspace || a->workspace_bytes < pp.bytes)) {
@@ -372,9 +386,12 @@ int ti_window_attention_workspace_bytes(const ti_attention_args *a, int window, 
     const int st = check_window(a, window, sinks, c);
     if (st) return st;
     const ti_window win{window, sinks};
-    if (a->dtype == TI_BF16 && ti_window_decodes(a, c)) *bytes = ti_plan_decode(a, c, win).bytes;
-    else ti_plan_generic(a, c, bytes);
-    return TI_OK;
+    if (a->dtype == TI_F32) return ti_plan_generic(a, c, bytes), TI_OK;
+    if (ti_window_decodes(a, c)) return *bytes = ti_plan_decode(a, c, win).bytes, TI_OK;
+    ti_prefill_plan pl;
+    const int ok = window_prefill(a, c, win, false, &pl);
+    if (!ok) *bytes = pl.bytes;
+    return ok;
 }
 
 int ti_window_attention(const ti_attention_args *a, int window, int sinks, const ti_kv_cache *c, void *stream) {
@@ -384,8 +401,11 @@ int ti_window_attention(const ti_attention_args *a, int window, int sinks, const
     if (st) return st;
     const ti_window win{window, sinks};
     hipStream_t s = (hipStream_t)stream;
-    if (a->dtype == TI_BF16 && ti_window_decodes(a, c)) return ti_launch_decode_window(a, c, ti_plan_decode(a, c, win), win, s);
-    return ti_launch_generic(a, c, s, win);
+    if (a->dtype == TI_F32) return ti_launch_generic(a, c, s, win);
+    if (ti_window_decodes(a, c)) return ti_launch_decode_window(a, c, ti_plan_decode(a, c, win), win, s);
+    ti_prefill_plan pl;
+    st = window_prefill(a, c, win, true, &pl);
+    return st ? st : ti_launch_prefill(a, c, pl, s, win);
 }
 
 int ti_reserve_pages(const ti_page_pool *pool, const int32_t *counts, int tokens, int32_t *positions, int32_t *slots,

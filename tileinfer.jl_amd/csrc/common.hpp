@@ -148,6 +148,8 @@ int ti_launch_release(const ti_page_pool *pool, const int32_t *keep, hipStream_t
 struct ti_window {
     int size = 0, sinks = 0;
 };
+// The most 32-key tiles that `tq` neighbouring queries see.
+inline long long window_tiles(ti_window w, long long tq) { return (w.size + tq + 62LL) / 32 + (w.sinks + 31LL) / 32; }
 
 struct ti_decode_plan {
     int splits;      // split-KV work-groups per (sequence, KV head)
@@ -188,14 +190,15 @@ struct ti_prefill_plan {
 };
 // bound_keys: limit the key splits by the keys the block tables can hold (a launch); the
 // workspace query passes false and sizes for the most splits any block-table width allows.
-ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c, bool bound_keys);
+ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c, bool bound_keys, ti_window win = ti_window{});
 int ti_launch_prefill(const ti_attention_args *a, const ti_kv_cache *c, const ti_prefill_plan &p,
-                      hipStream_t s);
+                      hipStream_t s, ti_window win = ti_window{});
 // The ping-pong form a prefill on `path` takes (AUTO, PREFILL: the library's pick; bound_keys as
 // in ti_plan_prefill).
 int ti_pick_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, int path, bool bound_keys);
+int ti_pick_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, int path, bool bound_keys, ti_window win);
 int ti_launch_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, const ti_prefill_plan &p,
-                         hipStream_t s);
+                         hipStream_t s, ti_window win = ti_window{});
 // fp32 path: its key splits and workspace bytes (host shapes only).
 int ti_plan_generic(const ti_attention_args *a, const ti_kv_cache *c, size_t *bytes);
 int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStream_t s, ti_window win = ti_window{});

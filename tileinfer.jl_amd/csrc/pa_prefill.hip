@@ -28,7 +28,9 @@
 // multiplied by the keys' smoothing and rounded to bf16 (attention.jl:68-95).
 #include <stdlib.h>
 
-#include "common.hpp"
+#include <algorithm>
+
+#include "pa_window.hpp"
 
 using namespace ti;
 
@@ -44,6 +46,7 @@ struct PrefillParams {
     float *part;                       // split partials [B][Hk][splits][M][D + 2]
     int bt_stride, num_pages, P, pshift, Hk, Hq, G, gshift, TQ, nmax, qtiles, causal, splits, M;
     float scale_log2;
+    int window, sinks;                 // WIN
 };
 
 constexpr int KT = 32;                 // keys per LDS tile
@@ -137,6 +140,11 @@ struct Stage {
     float s;
 };
 
+// FP8: the scales of a staged tile's page halves, keys' and values'.
+struct HalfScales {
+    float k[2], v[2];
+};
+
 // Page ids (0-based, clamped into the pool) of the two 16-key halves of tile kt, read with
 // scalar loads; fetched one tile ahead of use so their latency hides behind compute.
 struct TilePages {
@@ -166,7 +174,8 @@ __device__ __forceinline__ TilePages tile_pages(const PrefillParams &p, const in
     return tp;
 }
 
-template <int D, bool INT8, bool PG16, int GT>
+// INT8 also for 8-bit block caches (FP8), whose scales are found apart.
+template <int D, bool INT8, bool PG16, int GT, bool FP8 = false>
 __device__ __forceinline__ void load_tile(Stage<D, INT8, GT> &st, const PrefillParams &p,
                                           const int32_t *bt, int h, int kt, int kend, int gtid,
                                           const TilePages &tp) {
@@ -200,7 +209,7 @@ __device__ __forceinline__ void load_tile(Stage<D, INT8, GT> &st, const PrefillP
                 st.v[u] = (u32x4){b.x, b.y, 0u, 0u};
             }
         }
-        if (INT8 && gtid < 2 * KT) {
+        if (INT8 && !FP8 && gtid < 2 * KT) {
             // keys past kend take the last key's scale: a stale one may be NaN, and p = 0 times NaN
             // is NaN
             const int key = min(gtid % KT, kend - 1 - kt * KT);
@@ -241,33 +250,42 @@ __device__ __forceinline__ u32x4 i8x8_to_bf16x8(uint32_t x, uint32_t y) {
     return r;
 }
 
-template <int D, bool INT8, int GT>
+// h0, h1: WIN: the tile's keys from h0 to h1 - 1 are seen by no row. FP8: with the scales of its page halves.
+template <int D, bool INT8, int GT, bool FP8 = false, bool WIN = false>
 __device__ __forceinline__ void store_tile(const Stage<D, INT8, GT> &st, Smem<D> &sm, int buf, int gtid,
-                                           int valid_keys) {
+                                           int valid_keys, int h0 = 0, int h1 = 0, const HalfScales &sc = HalfScales{}) {
     constexpr int CPR = D / 8;
-    const bool partial = valid_keys < KT;      // wave-uniform: only the last tile
+    const bool partial = valid_keys < KT || (WIN && h1 > 0 && h0 < KT);   // wave-uniform: only the last tile, or edges of a window
 #pragma unroll
     for (int u = 0; u < Stage<D, INT8, GT>::PER; u++) {
         const int c = gtid + GT * u, key = c / CPR, ch = c % CPR;
         if (c < Stage<D, INT8, GT>::CH) {
-            const u32x4 kv = INT8 ? i8x8_to_bf16x8(st.k[u][0], st.k[u][1]) : st.k[u];
-            const u32x4 vv = INT8 ? i8x8_to_bf16x8(st.v[u][0], st.v[u][1]) : st.v[u];
+            u32x4 kv, vv;
+            if constexpr (FP8) {
+                kv = e4m3x8_to_bf16(st.k[u][0], st.k[u][1], key & 16 ? sc.k[1] : sc.k[0]);
+                vv = e4m3x8_to_bf16(st.v[u][0], st.v[u][1], key & 16 ? sc.v[1] : sc.v[0]);
+            } else {
+                kv = INT8 ? i8x8_to_bf16x8(st.k[u][0], st.k[u][1]) : st.k[u];
+                vv = INT8 ? i8x8_to_bf16x8(st.v[u][0], st.v[u][1]) : st.v[u];
+            }
             *reinterpret_cast<u32x4 *>(&sm.k[buf][key * Smem<D>::KROW + ch * 8]) = kv;
             if (partial) {
                 // Only the last tile has keys past the step's end (their values meet p = 0 and
                 // must be finite); the empty asm keeps this a real branch, so full tiles skip
                 // the selects.
                 asm volatile("");
-                const uint32_t keep = key < valid_keys ? ~0u : 0u;
+                const uint32_t keep = key < valid_keys && !(WIN && key >= h0 && key < h1) ? ~0u : 0u;
                 *reinterpret_cast<u32x4 *>(&sm.v[buf][key * Smem<D>::VROW + ch * 8]) = vv & keep;
             } else {
                 *reinterpret_cast<u32x4 *>(&sm.v[buf][key * Smem<D>::VROW + ch * 8]) = vv;
             }
         }
     }
-    if (INT8 && gtid < 2 * KT) {
-        if (gtid < KT) sm.sk[buf][gtid] = st.s;
-        else sm.sv[buf][gtid - KT] = st.s;
+    if (INT8 && !FP8 && gtid < 2 * KT) {
+        const int key = gtid % KT;
+        const float x = WIN && key >= h0 && key < h1 ? 0.0f : st.s;
+        if (gtid < KT) sm.sk[buf][gtid] = x;
+        else sm.sv[buf][gtid - KT] = x;
     }
 }
 
@@ -299,8 +317,14 @@ __device__ __forceinline__ u32x2 lds_tr16(const uint16_t *p) {
 // (the light tile's keys are the first tiles of the heavy one's: they share the LDS
 // tiles). Waves 0-3 are the groups' heavy waves, 4-7 the light ones, one of each per SIMD;
 // a light wave past its keys only issues its share of the tile loads.
-template <int D, bool INT8, bool PG16, int WPG, int NG, bool DL, bool PAIR = false>
+//
+// FP8: an 8-bit block cache, converted on the way into LDS. WIN: the window of pa_window.hpp; the groups walk the list of
+// tiles that it leaves for the work-group's rows (`actual` maps them).
+template <int D, bool INT8, bool PG16, int WPG, int NG, bool DL, bool PAIR = false, bool FP8 = false, bool WIN = false>
 __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p) {
+    static_assert(!FP8 || (!INT8 && PG16 && !DL), "8-bit block caches: staged, whole pages of 2^k");
+    static_assert(!WIN || !PAIR, "q-tiles of a pair see different windows");
+    constexpr bool B8 = INT8 || FP8;
     static_assert(!DL || (!INT8 && PG16 && D == 128 && (WPG == 2 || WPG == 4)), "direct loads: bf16, D 128, 2^k pages");
     static_assert(!PAIR || (DL && WPG == 2 && NG == 4), "paired q-tiles: direct loads, 2 x 4 waves");
     constexpr int NQB = D / 16;          // QK MFMAs (16 head-dim elements each)
@@ -367,7 +391,7 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
     }
 
     TilePages spec{};
-    if constexpr (DL) {
+    if constexpr (DL && !WIN) {
         if (p.splits == 1) spec = raw_pages(p, bt, grp);
     }
     const int start = max(sload(p.positions, nb > 0 ? tok0 : 0), 0), len = start + nb;   // a negative position reads as 0
@@ -377,11 +401,22 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
     // this wave's own keys (PAIR: the light wave's end before the work-group's)
     const int kend_w = PAIR && p.causal ? start + min(t_first_w + p.TQ, nb) : kend;
     const int kt_hi_w = (kend_w + KT - 1) / KT;
-    const int nkt = (kend + KT - 1) / KT;
+    int nkt = (kend + KT - 1) / KT;
+    WindowTiles wt{};
+    if constexpr (WIN) {
+        wt = WindowTiles::of<5>(start + t_first, p.window, p.sinks);
+        nkt -= wt.skip;
+    }
+    auto actual = [&](int kt) {
+        if constexpr (WIN) return wt.tile(kt);
+        else return kt;
+    };
     // This work-group's split: key tiles [kt_lo, kt_hi) of the q-tile's nkt.
     const int per = (nkt + p.splits - 1) / p.splits;
     const int kt_lo = min(split * per, nkt), kt_hi = min(kt_lo + per, nkt);
     const int steps = (kt_hi - kt_lo + NG - 1) / NG;       // same for every group
+    // WIN: the last key in front of the row's window, the first of the last row's
+    const int before = WIN ? (row_ok ? start + t : len - 1) - p.window : 0, last_lo = WIN ? start + t_last - p.window + 1 : 0;
     const size_t unit = ((size_t)b * p.Hk + h) * p.splits + split;
     Smem<D> &sm = smg[grp];
     DlSmem &dsm = reinterpret_cast<DlSmem *>(smem_raw)[grp];
@@ -470,7 +505,9 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
         // the buffer holds, fully masked, so the next loads and the score MFMAs share one
         // scheduling region; its PV stage is skipped.
         const bool valid = kt < (PAIR ? kt_hi_w : kt_hi);
-        const bool need_mask = !valid || kt * KT + KT - 1 > mask_from;
+        const int kt_at = actual(kt);
+        bool need_mask = !valid || kt_at * KT + KT - 1 > mask_from;
+        if constexpr (WIN) need_mask |= kt_at * KT < last_lo && kt_at * KT + KT > p.sinks;
         // INT8: the scales of this lane's 16 score keys, 8 q + 4 kg + (0..3) for q = 0..3,
         // as four 16-B reads per array
         f32x4 skq[4], svq[4];
@@ -489,8 +526,8 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
             float v = sc[e];
             if constexpr (INT8) v *= skq[e >> 2][e & 3];
             if (need_mask) {
-                const int kpos = kt * KT + key;
-                v = (valid && kpos <= qpos && kpos < kend_w) ? v : -INFINITY;
+                const int kpos = kt_at * KT + key;
+                v = (valid && kpos <= qpos && kpos < kend_w && (!WIN || kpos > before || kpos < p.sinks)) ? v : -INFINITY;
             }
             x[e] = v;
             mt = fmaxf(mt, v);
@@ -572,7 +609,7 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
         };
         auto dl_load = [&](int kt, int buf, const TilePages &tp) {
             typedef __attribute__((address_space(3))) void *lds_ptr;
-            const int pos0 = kt * KT, last = kend - 1 - pos0;   // >= 0 for every tile loaded
+            const int pos0 = actual(kt) * KT, last = kend - 1 - pos0;   // >= 0 for every tile loaded
             uint16_t *kd = &dsm.k[buf][dx * 2048], *vd = &dsm.v[buf][dx * 2048];
             if (last >= KT - 1) {
                 // every key of the tile is a step key: a scalar base and fixed offsets
@@ -607,12 +644,12 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
         // the tile after next at its end, so the scalar loads' wait falls on the closing
         // barrier instead of on the step's LDS reads
         const int ft = min(tile_of(0), kt_hi - 1);
-        TilePages pn = p.splits == 1 && ft == grp ? spec : raw_pages(p, bt, ft);
+        TilePages pn = !WIN && p.splits == 1 && ft == grp ? spec : raw_pages(p, bt, actual(ft));
         auto issue = [&](int i, int buf) {
             if (i < steps) dl_load(min(tile_of(i), kt_hi - 1), buf, pn);
         };
         auto next_pages = [&](int i) {
-            if (i < steps) pn = raw_pages(p, bt, min(tile_of(i), kt_hi - 1));
+            if (i < steps) pn = raw_pages(p, bt, actual(min(tile_of(i), kt_hi - 1)));
         };
         issue(0, 0);
         next_pages(1);
@@ -628,6 +665,40 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
             next_pages(i + 3);
         }
         __syncthreads();   // every wave is done with the tiles before the merge reuses the LDS
+    } else if constexpr (FP8 || WIN) {   // as below
+        Stage<D, B8, GT> s0, s1;
+        HalfScales c0{}, c1{};   // FP8: of the tiles in s0 and s1
+        // Page ids of the next tile to load, fetched one load ahead.
+        TilePages pnext = PG16 ? tile_pages(p, bt, actual(min(tile_of(0), kt_hi - 1))) : TilePages{};
+        auto ld = [&](Stage<D, B8, GT> &stg, HalfScales &sc, int i) {
+            load_tile<D, B8, PG16, GT, FP8>(stg, p, bt, h, actual(min(tile_of(i), kt_hi - 1)), kend, gtid, pnext);
+            if constexpr (FP8) {
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const long long at = (long long)pnext.pg[x] * p.Hk + h;
+                    sc.k[x] = sloadf(p.ls, at);
+                    sc.v[x] = sloadf(p.ls, (long long)p.num_pages * p.Hk + at);
+                }
+            }
+            if (PG16) pnext = tile_pages(p, bt, actual(min(tile_of(i + 1), kt_hi - 1)));
+        };
+        auto put = [&](const Stage<D, B8, GT> &stg, const HalfScales &sc, int buf, int i) {
+            const int pos0 = actual(tile_of(i)) * KT;
+            store_tile<D, B8, GT, FP8, WIN>(stg, sm, buf, gtid, kend - pos0, WIN ? max(p.sinks - pos0, 0) : 0, WIN ? wt.lo - pos0 : 0, sc);
+        };
+        ld(s0, c0, 0);
+        ld(s1, c1, 1);
+        if (tile_of(0) < kt_hi) put(s0, c0, 0, 0);
+        __syncthreads();
+        for (int i = 0; i < steps; i += 2) {
+            compute(tile_of(i), 0, [&] { ld(s0, c0, i + 2); });
+            if (tile_of(i + 1) < kt_hi) put(s1, c1, 1, i + 1);
+            __syncthreads();
+            if (i + 1 >= steps) break;
+            compute(tile_of(i + 1), 1, [&] { ld(s1, c1, i + 3); });
+            if (tile_of(i + 2) < kt_hi) put(s0, c0, 0, i + 2);
+            __syncthreads();
+        }
     } else {
         // Loads are issued unconditionally (a step past the group's last tile re-reads its
         // last tile, never used) so the number of loads in flight is static and the waits
@@ -653,6 +724,37 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
             __syncthreads();
         }
     }
+    // A product that is not finite (FP8, WIN): the rows once more, each over the keys that it sees.
+    auto again = [&](bool fine) {
+        if (!__syncthreads_or(!fine)) return false;
+        for (int x = w; x < RPG; x += WPG * NG) {
+            const int xt = t_first + x / p.G;
+            if (x / p.G >= p.TQ || xt >= nb) continue;
+            const size_t qrow = (size_t)(tok0 + xt) * p.Hq + h * p.G + x % p.G;
+            const int last = p.causal ? start + xt : len - 1;
+            float xm, xl, acc[D / 64];
+            exact_row<D, INT8, FP8>(p, bt, h, p.q + qrow * D, kt_lo * KT, kt_hi * KT, [&](int v) {
+                const int key = actual(v / KT) * KT + v % KT;
+                return key <= last && (!WIN || key > last - p.window || key < p.sinks) ? key : -1;
+            }, xm, xl, acc);
+            float *dst = p.part + (unit * p.M + (size_t)xt * p.G + x % p.G) * (D + 2);
+#pragma unroll
+            for (int k = 0; k < D / 64; k++) {
+                if (p.splits > 1) dst[lane + 64 * k] = acc[k];
+                else Elt<uint16_t>::st(p.out, qrow * D + lane + 64 * k, acc[k] / xl);
+            }
+            if (p.splits > 1 && lane == 0) *reinterpret_cast<float2 *>(dst + D) = make_float2(xm, xl);
+        }
+        return true;
+    };
+    if constexpr ((FP8 || WIN) && NG == 1) {
+        bool fine = fabsf(l) < INFINITY;
+#pragma unroll
+        for (int db = 0; db < NDB; db++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) fine &= fabsf(o[db][e]) < INFINITY;
+        if (again(fine || !row_ok)) return;
+    }
     l += __shfl_xor(l, 32);
     if (NG > 1) {
         // Merge the groups' states (same rows, disjoint keys): every group writes its
@@ -673,6 +775,7 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
         // before any arithmetic so their LDS latencies overlap.
         constexpr int NT = 64 * WPG * NG, IT = RPG * (D / 4) / NT;
         static_assert(IT * NT == RPG * (D / 4), "merge items must divide evenly");
+        bool all_fine = true;
         float2 ml[IT][NG];
         f32x4 dv[IT][NG];
 #pragma unroll
@@ -704,6 +807,11 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
                 acc += dv[it][gi] * wgt;
             }
             if (ttl >= p.TQ || tt >= nb) continue;
+            if constexpr (FP8 || WIN) {
+                all_fine &= fabsf(lsum) < INFINITY;
+#pragma unroll
+                for (int e = 0; e < 4; e++) all_fine &= fabsf(acc[e]) < INFINITY;
+            }
             if (p.splits > 1) {
                 // The split's partial for packed row tt * G + gg: (acc, m, l).
                 float *dst = p.part + (unit * p.M + (size_t)tt * p.G + gg) * (D + 2);
@@ -716,6 +824,7 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
             *reinterpret_cast<u32x2 *>(orow) = (u32x2){pack_bf16x2(acc[0] * inv, acc[1] * inv),
                                                        pack_bf16x2(acc[2] * inv, acc[3] * inv)};
         }
+        if constexpr (FP8 || WIN) again(all_fine);
         return;
     }
     if (!row_ok) return;
@@ -1176,45 +1285,62 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     }
 }
 
-template <int D, bool INT8, bool PG16, bool DL>
+template <int D, bool INT8, bool PG16, bool DL, bool FP8, bool WIN>
 void launch_prefill_w2(const PrefillParams &p, int ng, dim3 grid, hipStream_t s, bool pair = false) {
-    if constexpr (DL) {
+    if constexpr (DL && !WIN) {
         if (pair) return (void)(prefill_kernel<D, INT8, PG16, 2, 4, true, true><<<grid, 512, 0, s>>>(p));
     }
     switch (ng) {
-        case 1: prefill_kernel<D, INT8, PG16, 2, 1, DL><<<grid, 128, 0, s>>>(p); break;
-        case 2: prefill_kernel<D, INT8, PG16, 2, 2, DL><<<grid, 256, 0, s>>>(p); break;
-        default: prefill_kernel<D, INT8, PG16, 2, 4, DL><<<grid, 512, 0, s>>>(p); break;
+        case 1: prefill_kernel<D, INT8, PG16, 2, 1, DL, false, FP8, WIN><<<grid, 128, 0, s>>>(p); break;
+        case 2: prefill_kernel<D, INT8, PG16, 2, 2, DL, false, FP8, WIN><<<grid, 256, 0, s>>>(p); break;
+        default: prefill_kernel<D, INT8, PG16, 2, 4, DL, false, FP8, WIN><<<grid, 512, 0, s>>>(p); break;
     }
 }
 
-template <int D, bool INT8, bool PG16, bool DL>
+template <int D, bool INT8, bool PG16, bool DL, bool FP8, bool WIN>
 void launch_prefill_w4(const PrefillParams &p, int ng, dim3 grid, hipStream_t s) {
     switch (ng) {
-        case 1: prefill_kernel<D, INT8, PG16, 4, 1, DL><<<grid, 256, 0, s>>>(p); break;
-        default: prefill_kernel<D, INT8, PG16, 4, 2, DL><<<grid, 512, 0, s>>>(p); break;
+        case 1: prefill_kernel<D, INT8, PG16, 4, 1, DL, false, FP8, WIN><<<grid, 256, 0, s>>>(p); break;
+        default: prefill_kernel<D, INT8, PG16, 4, 2, DL, false, FP8, WIN><<<grid, 512, 0, s>>>(p); break;
     }
 }
 
-template <int D, bool INT8, bool PG16>
+template <int D, bool INT8, bool PG16, bool FP8, bool WIN>
 void launch_prefill_g(const PrefillParams &p, int wpg, int ng, bool dl, dim3 grid, hipStream_t s, bool pair) {
     if (wpg == 2) {
-        if constexpr (!INT8 && PG16 && D == 128) {
-            if (dl) return launch_prefill_w2<D, INT8, PG16, true>(p, ng, grid, s, pair);
+        if constexpr (!INT8 && !FP8 && PG16 && D == 128) {
+            if (dl) return launch_prefill_w2<D, INT8, PG16, true, FP8, WIN>(p, ng, grid, s, pair);
         }
-        launch_prefill_w2<D, INT8, PG16, false>(p, ng, grid, s);
+        launch_prefill_w2<D, INT8, PG16, false, FP8, WIN>(p, ng, grid, s);
     } else {
-        if constexpr (!INT8 && PG16 && D == 128) {
-            if (dl) return launch_prefill_w4<D, INT8, PG16, true>(p, ng, grid, s);
+        if constexpr (!INT8 && !FP8 && PG16 && D == 128 && !WIN) {
+            if (dl) return launch_prefill_w4<D, INT8, PG16, true, FP8, WIN>(p, ng, grid, s);
         }
-        launch_prefill_w4<D, INT8, PG16, false>(p, ng, grid, s);
+        launch_prefill_w4<D, INT8, PG16, false, FP8, WIN>(p, ng, grid, s);
     }
 }
 
-template <int D, bool INT8>
+template <int D, bool INT8, bool FP8, bool WIN>
 void launch_prefill_d(const PrefillParams &p, int wpg, int ng, bool dl, dim3 grid, hipStream_t s, bool pair) {
-    if (p.P % 16 == 0 && p.pshift >= 0) launch_prefill_g<D, INT8, true>(p, wpg, ng, dl, grid, s, pair);
-    else launch_prefill_g<D, INT8, false>(p, wpg, ng, dl, grid, s, false);
+    if constexpr (FP8) {
+        launch_prefill_g<D, INT8, true, FP8, WIN>(p, wpg, ng, dl, grid, s, false);
+    } else {
+        if (p.P % 16 == 0 && p.pshift >= 0) launch_prefill_g<D, INT8, true, FP8, WIN>(p, wpg, ng, dl, grid, s, pair);
+        else launch_prefill_g<D, INT8, false, FP8, WIN>(p, wpg, ng, dl, grid, s, false);
+    }
+}
+
+template <int D>
+void launch_prefill_kind(const PrefillParams &p, int kind, int wpg, int ng, bool dl, dim3 grid, hipStream_t s, bool pair) {
+    if (p.window) {
+        if (kind == TI_KV_FP8) launch_prefill_d<D, false, true, true>(p, wpg, ng, dl, grid, s, false);
+        else if (kind == TI_KV_INT8) launch_prefill_d<D, true, false, true>(p, wpg, ng, dl, grid, s, false);
+        else launch_prefill_d<D, false, false, true>(p, wpg, ng, dl, grid, s, false);
+    } else {
+        if (kind == TI_KV_FP8) launch_prefill_d<D, false, true, false>(p, wpg, ng, dl, grid, s, false);
+        else if (kind == TI_KV_INT8) launch_prefill_d<D, true, false, false>(p, wpg, ng, dl, grid, s, false);
+        else launch_prefill_d<D, false, false, false>(p, wpg, ng, dl, grid, s, pair);
+    }
 }
 
 }  // namespace
@@ -1223,13 +1349,13 @@ void launch_prefill_d(const PrefillParams &p, int wpg, int ng, bool dl, dim3 gri
 // per work-group, and key splits across work-groups, chosen so small prefills and verify
 // steps still spread over the 256 CUs. Depends only on host shapes (the block-table
 // width bounds the keys), never on positions, so a captured graph stays valid.
-ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c, bool bound_keys) {
+ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c, bool bound_keys, ti_window win) {
     ti_prefill_plan pl;
     const int G = a->q_heads / c->kv_heads;
     const long long pairs = (long long)c->kv_heads * a->num_seqs;
-    const long long key_tiles = ((long long)a->block_table_stride * c->page_size + 31) / 32;
+    long long key_tiles = ((long long)a->block_table_stride * c->page_size + 31) / 32;
     const bool auto_path = a->path == TI_PATH_PREFILL || a->path == TI_PATH_AUTO;
-    pl.pp = ti_pick_prefill_pp(a, c, a->path, bound_keys);
+    pl.pp = ti_pick_prefill_pp(a, c, a->path, bound_keys, win);
     pl.dl = 0;
     pl.pair = 0;
     pl.r16 = 0;
@@ -1254,6 +1380,12 @@ ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c
     pl.TQ = 32 * pl.wpg / G;
     pl.qtiles = (a->max_query_len + pl.TQ - 1) / pl.TQ;
     const long long wgs = (long long)pl.qtiles * pairs;
+    if (win.size) {
+        // a window bounds a q-tile's keys too, whatever the tables hold
+        const long long most = window_tiles(win, pl.TQ);
+        key_tiles = bound_keys ? std::min(key_tiles, most) : most;
+        bound_keys = true;
+    }
     pl.ng = wgs >= 1024 ? 1 : (wgs >= 512 ? 2 : 4);
     if (pl.wpg == 4 && pl.ng > 2) pl.ng = 2;   // 16 waves of this kernel do not fit one CU's registers
     // Split the keys while work-groups are fewer than the CUs and every split keeps at
@@ -1285,7 +1417,7 @@ ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c
     // (INT8 caches pair on the 16-row kernel only, its tiles staged through registers)
     const bool i8_ok = c->kind == TI_KV_INT8 && a->dtype == TI_BF16 && c->head_dim == 128 &&
                        c->page_size >= 16 && (c->page_size & (c->page_size - 1)) == 0;
-    const bool pair_ok = (dl_ok || i8_ok) && a->causal && pl.splits == 1 && 32 % G == 0;
+    const bool pair_ok = (dl_ok || i8_ok) && a->causal && pl.splits == 1 && 32 % G == 0 && !win.size;
     // (32 % G == 0 in pair_ok: G <= 32, so 32 / G >= 1)
     const long long pair_wgs = pair_ok ? pairs * (((a->max_query_len + 32 / G - 1) / (32 / G) + 1) / 2) : 0;
     pl.r16 = pair_ok && (a->path == TI_PATH_PREFILL_PAIRED16 || (auto_path && R16_BY_DEFAULT && pair_wgs <= 512));
@@ -1301,9 +1433,11 @@ ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c
 }
 
 int ti_launch_prefill(const ti_attention_args *a, const ti_kv_cache *c, const ti_prefill_plan &pl,
-                      hipStream_t s) {
-    if (pl.pp) return ti_launch_prefill_pp(a, c, pl, s);
+                      hipStream_t s, ti_window win) {
+    if (pl.pp) return ti_launch_prefill_pp(a, c, pl, s, win);
     PrefillParams p;
+    p.window = win.size;
+    p.sinks = win.sinks;
     p.q = (const uint16_t *)a->q;
     p.out = (uint16_t *)a->out;
     p.kp = (const uint16_t *)c->k_pages;
@@ -1337,15 +1471,8 @@ int ti_launch_prefill(const ti_attention_args *a, const ti_kv_cache *c, const ti
         else prefill16_kernel<false><<<grid, 1024, 0, s>>>(p);
         return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
     }
-    const bool int8 = c->kind == TI_KV_INT8;
-    const bool dl = pl.dl;
-    if (c->head_dim == 128) {
-        if (int8) launch_prefill_d<128, true>(p, wpg, ng, dl, grid, s, false);
-        else launch_prefill_d<128, false>(p, wpg, ng, dl, grid, s, pl.pair);
-    } else {
-        if (int8) launch_prefill_d<64, true>(p, wpg, ng, dl, grid, s, false);
-        else launch_prefill_d<64, false>(p, wpg, ng, dl, grid, s, false);
-    }
+    if (c->head_dim == 128) launch_prefill_kind<128>(p, c->kind, wpg, ng, pl.dl, grid, s, pl.pair);
+    else launch_prefill_kind<64>(p, c->kind, wpg, ng, pl.dl, grid, s, false);
     if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
     return pl.splits > 1 ? ti_launch_combine(a, c, pl.rows, pl.splits, s) : TI_OK;
 }

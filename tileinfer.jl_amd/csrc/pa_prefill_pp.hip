@@ -46,9 +46,11 @@
 // four-wave prefill kernel (pa_prefill.hip).
 #include <stdlib.h>
 
+#include <algorithm>
+
 #include <type_traits>
 
-#include "common.hpp"
+#include "pa_window.hpp"
 
 using namespace ti;
 
@@ -71,6 +73,7 @@ struct PPParams {
     int bt_stride, num_pages, P, pshift, Hk, Hq, G, TQ, nmax, qtiles, causal, splits, sshift, M;   // splits = 2^sshift
     int eager;                         // first steps that rescale to every larger maximum
     float scale_log2;
+    int window, sinks;                 // WIN
 };
 
 // One tile stream's double-buffered tiles. Row strides (bf16): D + 8 for K (16-B reads by 16
@@ -102,10 +105,12 @@ __device__ __forceinline__ void unroll(F &&f) {
     }
 }
 
-template <int D, bool INT8, int FORM>
+// FP8: an 8-bit block cache, converted as INT8 tiles are, with its blocks' scales. WIN: the window of pa_window.hpp; tiles are
+// those of the list that it leaves for the work-group's rows (`tile` maps them).
+template <int D, bool INT8, int FORM, bool FP8 = false, bool WIN = false>
 __global__ void __launch_bounds__(FORM == TI_PP_SOLO ? 256 : 512, FORM == TI_PP_SOLO && D == 64 ? 3 : 2)
 prefill_pp_kernel(PPParams p) {
-    constexpr bool KS = FORM == TI_PP_KSPLIT, SOLO = FORM == TI_PP_SOLO;
+    constexpr bool KS = FORM == TI_PP_KSPLIT, SOLO = FORM == TI_PP_SOLO, B8 = INT8 || FP8;
     static_assert(D == 128 || KS || SOLO, "head_dim 64 stages a tile with one team");
     constexpr int NW = SOLO ? 4 : 8;
     constexpr int NQB = D / 16;        // score MFMAs per tile (16 head-dim elements each)
@@ -118,7 +123,7 @@ prefill_pp_kernel(PPParams p) {
     // D = 128 stages two chunks per thread and has registers for one step's values only.
     constexpr int LV = D == 128 && GT == 256 ? 1 : 2;
     using Tiles = PPTiles<D, INT8>;
-    using Chunk = std::conditional_t<INT8, u32x2, u32x4>;
+    using Chunk = std::conditional_t<B8, u32x2, u32x4>;
     constexpr int KROW = Tiles::KROW, VROW = Tiles::VROW;
     constexpr int SLAB = KS ? NW * 64 * (NDB / 2 * 64 + 8) : 0;   // the merge's exchange area (bytes)
     constexpr int TILES = (KS ? 2 : 1) * (int)sizeof(Tiles);
@@ -143,10 +148,10 @@ prefill_pp_kernel(PPParams p) {
     constexpr int KPU = GT / CPR;
     const int wave_half = __builtin_amdgcn_readfirstlane(ckey >> 4);
     auto half_of = [&](int u) { return NC == 2 ? u : wave_half; };
-    const uint32_t chunk_off = (uint32_t)((ckey & 15) * D + cch * 8) * (INT8 ? 1 : 2);
+    const uint32_t chunk_off = (uint32_t)((ckey & 15) * D + cch * 8) * (B8 ? 1 : 2);
     // Block-table entries of a tile's halves (raw: scalar loads, looked up a phase before use).
     // NH = 1: only this wave's half (its chunks lie in one, and there are no scales to find).
-    constexpr int NH = NC == 2 || INT8 ? 2 : 1, EB = INT8 ? 1 : 2;
+    constexpr int NH = NC == 2 || INT8 ? 2 : 1, EB = B8 ? 1 : 2;
     struct Pages {
         int pg[NH];
     };
@@ -160,11 +165,15 @@ prefill_pp_kernel(PPParams p) {
     // Without key splits the first tiles' entries do not depend on the sequence's position:
     // their loads go out together with those of the query counts.
     Pages rp[4];
+    WindowTiles wt{};
     auto first_pages = [&](int lo) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) rp[j] = pages_at(KS ? lo + 2 * j + team : lo + j);
+        for (int j = 0; j < 4; j++) {
+            if constexpr (WIN) rp[j] = pages_at(wt.tile(KS ? lo + 2 * j + team : lo + j));
+            else rp[j] = pages_at(KS ? lo + 2 * j + team : lo + j);
+        }
     };
-    if (p.splits == 1) first_pages(0);
+    if (!WIN && p.splits == 1) first_pages(0);
     const int tok0 = p.qsl ? sload(p.qsl, b) : b * p.nmax;
     const int nb = p.qsl ? min(sload(p.qsl, b + 1) - tok0, p.nmax) : p.nmax;   // at most max_query_len
     const int t_first = qt * p.TQ;
@@ -172,7 +181,11 @@ prefill_pp_kernel(PPParams p) {
     const int start = max(sload(p.positions, tok0), 0), len = start + nb;   // a negative position reads as 0
     const int t_last = min(t_first + p.TQ, nb) - 1;
     const int kend = p.causal ? start + t_last + 1 : len;
-    const int nkt = (kend + KT - 1) / KT;
+    int nkt = (kend + KT - 1) / KT;
+    if constexpr (WIN) {
+        wt = WindowTiles::of<5>(start + t_first, p.window, p.sinks);
+        nkt -= wt.skip;
+    }
     const int per = (nkt + p.splits - 1) / p.splits;
     const int kt_lo = min(split * per, nkt), kt_hi = min(kt_lo + per, nkt);
     const int N = KS ? (kt_hi - kt_lo + 1) / 2 : kt_hi - kt_lo;   // steps of this work-group
@@ -190,7 +203,11 @@ prefill_pp_kernel(PPParams p) {
     }
 
     // Key tile of step j (this team's, KS; its odd tile out is masked by position).
-    auto tile = [&](int j) { return KS ? kt_lo + 2 * j + team : kt_lo + j; };
+    auto tile = [&](int j) {
+        const int kt = KS ? kt_lo + 2 * j + team : kt_lo + j;
+        if constexpr (WIN) return wt.tile(kt);
+        else return kt;
+    };
 
     // Row offsets of a tile's halves in bytes from the KV head's first row (page clamped into
     // the pool; an entry of 0 or less wraps and reads the last page). Tiles past the last are
@@ -198,10 +215,27 @@ prefill_pp_kernel(PPParams p) {
     struct Bases {
         uint64_t e[NH];
     };
+    // FP8: the scales of a tile's halves, keys' and values', found with the offsets and used when the tile is stored.
+    struct Scales {
+        float k[NH], v[NH];
+    };
+    Scales sc8[5];   // of tiles i .. i + 4
+    const long long half_b = (long long)p.num_pages * p.Hk;
+    auto scales = [&](const Pages &r) {
+        Scales o;
+#pragma unroll
+        for (int x = 0; x < NH; x++) {
+            const long long at = (long long)min((uint32_t)(r.pg[x] - 1), (uint32_t)p.num_pages - 1) * p.Hk + h;
+            o.k[x] = sloadf(p.ls, at);
+            o.v[x] = sloadf(p.ls, half_b + at);
+        }
+        return o;
+    };
+    auto scale_of = [&](const float (&o)[NH], int u) { return NH == 2 && half_of(u) ? o[NH - 1] : o[0]; };
     const uint32_t pstride = (uint32_t)p.Hk * p.P * D * EB;
     const size_t hoff = (size_t)h * p.P * D * EB, half_q = (size_t)p.num_pages * p.Hk * p.P * D;
-    const char *kbase = (INT8 ? (const char *)p.lq : (const char *)p.kp) + hoff;
-    const char *vbase_g = INT8 ? kbase + half_q : (const char *)p.vp + hoff;
+    const char *kbase = (B8 ? (const char *)p.lq : (const char *)p.kp) + hoff;
+    const char *vbase_g = B8 ? kbase + half_q : (const char *)p.vp + hoff;
     auto bases = [&](const Pages &r, int j) {
         Bases o;
 #pragma unroll
@@ -231,8 +265,10 @@ prefill_pp_kernel(PPParams p) {
         // static), one wave of the staging threads stores them
         r = sbase[(r32 >> 4 ? o.e[NH - 1] : o.e[0]) / D];
     };
-    auto bf16_chunk = [&](const Chunk &r) -> u32x4 {
-        if constexpr (INT8) {
+    auto bf16_chunk = [&](const Chunk &r, float scale) -> u32x4 {
+        if constexpr (FP8) {
+            return e4m3x8_to_bf16(r[0], r[1], scale);
+        } else if constexpr (INT8) {
             u32x4 o;
             uint32_t a, b2, c, d;
             i8x4_to_bf16(r[0], a, b2);
@@ -243,20 +279,24 @@ prefill_pp_kernel(PPParams p) {
             return r;
         }
     };
-    auto store_k = [&](const Chunk &r, int buf, int u) {
-        *reinterpret_cast<u32x4 *>(&sm.k[buf][(ckey + KPU * u) * KROW + cch * 8]) = bf16_chunk(r);
+    // FP8: x is the place of the tile's scales in sc8
+    auto store_k = [&](const Chunk &r, int buf, int u, int x) {
+        *reinterpret_cast<u32x4 *>(&sm.k[buf][(ckey + KPU * u) * KROW + cch * 8]) = bf16_chunk(r, FP8 ? scale_of(sc8[x].k, u) : 1.0f);
     };
+    // WIN: keys that no row of the work-group sees
+    auto hidden = [&](int key) { return WIN && key < wt.lo && key >= p.sinks; };
     auto store_v = [&](const Chunk &r, int buf, int j, int u) {
         // Keys past kend in the last tile may hold any bits (even NaN) of an allocated
         // page: their probabilities are 0 and their values must be finite. Branch-free,
         // so the stage registers are never rewritten while loads are pending.
-        const uint32_t keep = tile(j) * KT + ckey + KPU * u < kend ? ~0u : 0u;
-        *reinterpret_cast<u32x4 *>(&sm.v[buf][(ckey + KPU * u) * VROW + cch * 8]) = bf16_chunk(r) & keep;
+        const int key = tile(j) * KT + ckey + KPU * u;
+        const uint32_t keep = key < kend && !hidden(key) ? ~0u : 0u;
+        *reinterpret_cast<u32x4 *>(&sm.v[buf][(ckey + KPU * u) * VROW + cch * 8]) = bf16_chunk(r, FP8 ? scale_of(sc8[0].v, u) : 1.0f) & keep;
     };
     const float smul = kg ? 1.0f : p.scale_log2;
     auto store_s = [&](float r, int j) {
         // scales of keys past kend may hold any bits too: zero
-        if (w == (KS ? 4 * team : 0)) sm.s[j & 3][lane] = tile(j) * KT + r32 < kend ? r * smul : 0.0f;
+        if (w == (KS ? 4 * team : 0)) sm.s[j & 3][lane] = tile(j) * KT + r32 < kend && !hidden(tile(j) * KT + r32) ? r * smul : 0.0f;
     };
 
     // Query rows (B operand of S^T = K Q^T): wave w holds rows 32 w .. 32 w + 31 (KS: both
@@ -264,7 +304,12 @@ prefill_pp_kernel(PPParams p) {
     const int r = (KS ? w & 3 : w) * 32 + r32, tl = r / p.G, g = r - tl * p.G, t = t_first + tl;
     const bool row_ok = tl < p.TQ && t < nb;
     // last visible key of the row (KS: of this split too, whose odd tile out is masked by it)
-    const int qpos = min(p.causal && row_ok ? start + t : len - 1, kt_hi * KT - 1);
+    int qpos = min(p.causal && row_ok ? start + t : len - 1, kt_hi * KT - 1);
+    int before = 0;                                // WIN: the last key in front of the row's window
+    if constexpr (WIN) {
+        before = (row_ok ? start + t : len - 1) - p.window;
+        qpos = min(row_ok ? start + t : len - 1, wt.tile(kt_hi - 1) * KT + KT - 1);
+    }
 
     // Prologue: K of tiles 0 and 1 in LDS; K of tiles 2, 3 and V of tiles 0 .. LV - 1 in
     // flight (in the order of their stores, so the waits before each store count exactly the
@@ -273,9 +318,12 @@ prefill_pp_kernel(PPParams p) {
     Pages raw4;                                    // block-table entries of tile i + 4
     bf16x8 qreg[NQB];
     {
-        if (p.splits != 1) first_pages(kt_lo);
+        if (WIN || p.splits != 1) first_pages(kt_lo);
 #pragma unroll
-        for (int j = 0; j < 4; j++) bs[j] = bases(rp[j], j);
+        for (int j = 0; j < 4; j++) {
+            bs[j] = bases(rp[j], j);
+            if constexpr (FP8) sc8[j] = scales(rp[j]);
+        }
         Chunk k0[NC], k1[NC];
         float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
@@ -303,10 +351,10 @@ prefill_pp_kernel(PPParams p) {
         __builtin_amdgcn_sched_barrier(0);
         raw4 = pages_at(tile(4));
 #pragma unroll
-        for (int u = 0; u < NC; u++) store_k(k0[u], 0, u);
+        for (int u = 0; u < NC; u++) store_k(k0[u], 0, u, 0);
         if constexpr (INT8) store_s(s0, 0);
 #pragma unroll
-        for (int u = 0; u < NC; u++) store_k(k1[u], 1, u);
+        for (int u = 0; u < NC; u++) store_k(k1[u], 1, u, 1);
         if constexpr (INT8) store_s(s1, 1);
         const uint32_t keep = row_ok ? ~0u : 0u;
 #pragma unroll
@@ -360,7 +408,9 @@ prefill_pp_kernel(PPParams p) {
     };
     // Online softmax of step j's scores (exp2 domain, lazy rescale after the first p.eager steps)
     // -> pb. Only tiles reaching past mask_from (the diagonal / last tiles) compare key positions.
-    const int jm = min(mask_from + 1, kt_hi * KT); // first key position that a row may not see
+    int jm = min(mask_from + 1, kt_hi * KT);       // first key position that a row may not see
+    if constexpr (WIN) jm = min(mask_from + 1, wt.tile(kt_hi - 1) * KT + KT);
+    const int last_lo = start + t_last - p.window + 1;   // WIN: the last row's window begins here
     auto softmax = [&](int j) {
         const int kt = tile(j);
         f32x4 svq[4];
@@ -384,6 +434,18 @@ prefill_pp_kernel(PPParams p) {
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 sc[e] = 8 * (e >> 2) + (e & 3) <= lim ? sc[e] : -INFINITY;
+        }
+        if constexpr (WIN) {
+            // tiles that some row's window begins behind, but for those of sinks alone
+            if (kt * KT < last_lo && kt * KT + KT > p.sinks) {
+                asm volatile("");
+                const int lim = before - kt * KT - 4 * kg, sunk = p.sinks - kt * KT - 4 * kg;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int key = 8 * (e >> 2) + (e & 3);
+                    sc[e] = key > lim || key < sunk ? sc[e] : -INFINITY;
+                }
+            }
         }
         float mt = -INFINITY;
 #pragma unroll
@@ -459,11 +521,15 @@ prefill_pp_kernel(PPParams p) {
                     } else if constexpr (X < O_SK) {
                         store_v(sv[SV][X - O_SV], S, i, X - O_SV);
                     } else if constexpr (X < O_SS) {
-                        store_k(sk[S][X - O_SK], S, X - O_SK);
+                        store_k(sk[S][X - O_SK], S, X - O_SK, 2);
                     } else if constexpr (X < O_BA) {
                         store_s(ss[S], i + 2);
                     } else if constexpr (X < O_LV) {
                         b4.e[X - O_BA] = bases(raw4, i + 4).e[X - O_BA];
+                        if constexpr (FP8) {
+                            const Scales n = scales(raw4);
+                            sc8[4].k[X - O_BA] = n.k[X - O_BA], sc8[4].v[X - O_BA] = n.v[X - O_BA];
+                        }
                     } else if constexpr (X < O_LK) {
                         load_v(sv[SV][X - O_LV], bs[LV], X - O_LV);
                     } else if constexpr (X < O_LS) {
@@ -478,6 +544,7 @@ prefill_pp_kernel(PPParams p) {
             __builtin_amdgcn_sched_barrier(0);
         });
         bs[1] = bs[2], bs[2] = bs[3], bs[3] = b4;
+        if constexpr (FP8) sc8[0] = sc8[1], sc8[1] = sc8[2], sc8[2] = sc8[3], sc8[3] = sc8[4];
     };
     auto phase_y = [&](int i) {
         raw4 = pages_at(tile(i + 5));
@@ -568,6 +635,35 @@ prefill_pp_kernel(PPParams p) {
         l = l * wa + oml.y * wb;
         db0 = team * NOUT;
     }
+    if constexpr (FP8 || WIN) {
+        // a product that is not finite: the rows once more, each over the keys that it sees
+        bool fine = fabsf(l) < INFINITY;
+#pragma unroll
+        for (int db = 0; db < NOUT; db++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) fine &= fabsf(o[db][e]) < INFINITY;
+        if (__syncthreads_or(row_ok && !fine)) {
+            for (int x = w; x < RW; x += NW) {
+                const int xt = t_first + x / p.G;
+                if (x / p.G >= p.TQ || xt >= nb) continue;
+                const size_t qrow = (size_t)(tok0 + xt) * p.Hq + h * p.G + x % p.G;
+                const int last = p.causal ? start + xt : len - 1;
+                float xm, xl, acc[D / 64];
+                exact_row<D, INT8, FP8>(p, bt, h, p.q + qrow * D, kt_lo * KT, kt_hi * KT, [&](int v) {
+                    const int key = (WIN ? wt.tile(v / KT) : v / KT) * KT + v % KT;
+                    return key <= last && (!WIN || key > last - p.window || key < p.sinks) ? key : -1;
+                }, xm, xl, acc);
+                float *dst = p.part + (unit * p.M + (size_t)xt * p.G + x % p.G) * (D + 2);
+#pragma unroll
+                for (int k = 0; k < D / 64; k++) {
+                    if (p.splits > 1) dst[lane + 64 * k] = acc[k];
+                    else Elt<uint16_t>::st(p.out, qrow * D + lane + 64 * k, acc[k] / xl);
+                }
+                if (p.splits > 1 && lane == 0) *reinterpret_cast<float2 *>(dst + D) = make_float2(xm, xl);
+            }
+            return;
+        }
+    }
     if (!row_ok) return;
     if (p.splits > 1) {
         float *dst = p.part + (unit * p.M + (size_t)t * p.G + g) * (D + 2);
@@ -593,18 +689,21 @@ prefill_pp_kernel(PPParams p) {
         }
 }
 
-template <int D, bool INT8, int FORM>
+template <int D, bool INT8, int FORM, bool FP8, bool WIN>
 void launch_pp(const PPParams &p, int B, hipStream_t s) {
-    prefill_pp_kernel<D, INT8, FORM><<<dim3(p.Hk, p.qtiles * p.splits, B), FORM == TI_PP_SOLO ? 256 : 512, 0, s>>>(p);
+    prefill_pp_kernel<D, INT8, FORM, FP8, WIN><<<dim3(p.Hk, p.qtiles * p.splits, B), FORM == TI_PP_SOLO ? 256 : 512, 0, s>>>(p);
 }
 
-template <int D, bool INT8>
+template <int D, bool INT8, bool FP8 = false, bool WIN = false>
 void launch_pp_form(const PPParams &p, int form, int B, hipStream_t s) {
-    if constexpr (D == 128 && !INT8) {
-        if (form == TI_PP_SHARED) return launch_pp<D, INT8, TI_PP_SHARED>(p, B, s);
+    if constexpr (!WIN) {
+        if (p.window) return launch_pp_form<D, INT8, FP8, true>(p, form, B, s);
     }
-    if (form == TI_PP_SOLO) launch_pp<D, INT8, TI_PP_SOLO>(p, B, s);
-    else launch_pp<D, INT8, TI_PP_KSPLIT>(p, B, s);
+    if constexpr (D == 128 && !INT8) {
+        if (form == TI_PP_SHARED) return launch_pp<D, INT8, TI_PP_SHARED, FP8, WIN>(p, B, s);
+    }
+    if (form == TI_PP_SOLO) launch_pp<D, INT8, TI_PP_SOLO, FP8, WIN>(p, B, s);
+    else launch_pp<D, INT8, TI_PP_KSPLIT, FP8, WIN>(p, B, s);
 }
 
 }  // namespace
@@ -657,12 +756,13 @@ void launch_pp_form(const PPParams &p, int form, int B, hipStream_t s) {
 // take 0.87 times as long in the mean as on the kernels that took them before this one had forms.
 // Slower by more than 3 %: 14, mostly batches of W < 200 whose contexts are ragged, which the host
 // cannot see (7 x 66 on 200 to 930 21.6 against 18.5; 5 x 110 on 1000 each 23.6 against 36.0).
-int ti_pick_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, int path, bool bound_keys) {
+int ti_pick_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, int path, bool bound_keys, ti_window win) {
     const int G = a->q_heads / c->kv_heads, P = c->page_size, D = c->head_dim;
     if (a->dtype != TI_BF16 || (D != 64 && D != 128) || P < 16 || (P & (P - 1)) || G > 64 ||
         2ull * c->kv_heads * P * D > 0xffffffffull)
         return TI_PP_NONE;
-    const bool dense = c->kind == TI_KV_DENSE, dense128 = dense && D == 128;
+    // 8-bit block caches as dense ones: e4m3 tiles cost a conversion of four instructions per chunk, and no scales in LDS
+    const bool dense = c->kind != TI_KV_INT8, dense128 = dense && D == 128;
     if (path == TI_PATH_PREFILL_PINGPONG && dense128 && 256 % G == 0) return TI_PP_SHARED;
     if (path != TI_PATH_AUTO && path != TI_PATH_PREFILL) return TI_PP_NONE;
     const long long pairs = (long long)c->kv_heads * a->num_seqs, n = a->max_query_len;
@@ -670,7 +770,8 @@ int ti_pick_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, int pat
     // grids hold 65535 q-tiles: 256-row ones where those have been taken, none where not
     if (T > 65535) return dense128 && 256 % G == 0 ? TI_PP_SHARED : TI_PP_NONE;
     long long W = T * pairs;
-    const long long tiles = bound_keys ? ((long long)a->block_table_stride * P + 31) / 32 : 1LL << 40;
+    long long tiles = bound_keys ? ((long long)a->block_table_stride * P + 31) / 32 : 1LL << 40;
+    if (win.size) tiles = std::min(tiles, window_tiles(win, TQ));
     // Only here does the four-wave plan split keys, and only from 32 tiles: a workspace query
     // (unbounded tiles) that answers KSPLIT is right for narrower tables too.
     if (q64 < 256)
@@ -695,9 +796,15 @@ int ti_pick_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, int pat
     return dense128 && T > 6 && !padded ? TI_PP_SHARED : TI_PP_SOLO;
 }
 
+int ti_pick_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, int path, bool bound_keys) {
+    return ti_pick_prefill_pp(a, c, path, bound_keys, ti_window{});
+}
+
 int ti_launch_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, const ti_prefill_plan &pl,
-                         hipStream_t s) {
+                         hipStream_t s, ti_window win) {
     PPParams p;
+    p.window = win.size;
+    p.sinks = win.sinks;
     p.q = (const uint16_t *)a->q;
     p.out = (uint16_t *)a->out;
     p.kp = (const uint16_t *)c->k_pages;
@@ -730,14 +837,17 @@ int ti_launch_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, const
     // 80.5), five of 512 at head_dim 64 0.00198 (SOLO without 0.00204, four-wave 0.00200) for 20.8
     // -> 21.3.
     const long long T = (a->max_query_len + 128 / p.G - 1) / (128 / p.G), W = T * p.Hk * a->num_seqs;
-    const bool dense128 = c->kind == TI_KV_DENSE && c->head_dim == 128;
+    const bool dense128 = c->kind != TI_KV_INT8 && c->head_dim == 128;
     if (pl.pp == TI_PP_KSPLIT) p.eager = W > 256 ? 0 : T == 1 ? 8 : 3;
     else p.eager = W < 1024 && !(T == 1 && dense128) && a->path != TI_PATH_PREFILL_PINGPONG ? 4 : 0;
     p.M = pl.rows;
     p.TQ = pl.TQ;
     p.qtiles = pl.qtiles;
     const bool int8 = c->kind == TI_KV_INT8;
-    if (c->head_dim == 64) {
+    if (c->kind == TI_KV_FP8) {
+        if (c->head_dim == 64) launch_pp_form<64, false, true>(p, pl.pp, a->num_seqs, s);
+        else launch_pp_form<128, false, true>(p, pl.pp, a->num_seqs, s);
+    } else if (c->head_dim == 64) {
         if (int8) launch_pp_form<64, true>(p, pl.pp, a->num_seqs, s);
         else launch_pp_form<64, false>(p, pl.pp, a->num_seqs, s);
     } else {
