@@ -386,7 +386,7 @@ int ti_window_attention_workspace_bytes(const ti_attention_args *a, int window, 
     const int st = check_window(a, window, sinks, c);
     if (st) return st;
     const ti_window win{window, sinks};
-    if (a->dtype == TI_F32) return ti_plan_generic(a, c, bytes), TI_OK;
+    if (a->dtype == TI_F32) return ti_plan_generic(a, c, bytes, win), TI_OK;
     if (ti_window_decodes(a, c)) return *bytes = ti_plan_decode(a, c, win).bytes, TI_OK;
     ti_prefill_plan pl;
     const int ok = window_prefill(a, c, win, false, &pl);

@@ -200,7 +200,7 @@ int ti_pick_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, int pat
 int ti_launch_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, const ti_prefill_plan &p,
                          hipStream_t s, ti_window win = ti_window{});
 // fp32 path: its key splits and workspace bytes (host shapes only).
-int ti_plan_generic(const ti_attention_args *a, const ti_kv_cache *c, size_t *bytes);
+int ti_plan_generic(const ti_attention_args *a, const ti_kv_cache *c, size_t *bytes, ti_window win = ti_window{});
 int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStream_t s, ti_window win = ti_window{});
 
 // Attention over chosen pages (pa_sparse.hip, its fp32 kernels in pa_generic.hip).

@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
                 if (need_mask) {
                     if constexpr (WIN) {
                         const int kp = rm.pos(j + (e >> 2)) + kg * 4 + (e & 3);
-                        v = (kp <= qpos[rb] && (kp > qpos[rb] - p.window || kp < p.sinks)) ? v : -INFINITY;
+                        v = window_sees(kp, qpos[rb], p.window, p.sinks) ? v : -INFINITY;
                     } else {
                         const int kp = (j + (e >> 2)) * 16 + kg * 4 + (e & 3);
                         v = (kp <= qpos[rb] && kp < len) ? v : -INFINITY;
@@ -939,7 +939,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
                 float m, l, acc[PER];
                 exact_row<D, INT8, FP8>(p, rm.bt, h, p.q + qrow * D, j0 * 16, j1 * 16, [&](int v) {
                     const int key = rm.pos(v >> 4) + (v & 15);
-                    return key <= last && (!WIN || key > last - p.window || key < p.sinks) ? key : -1;
+                    return (WIN ? window_sees(key, last, p.window, p.sinks) : key <= last) ? key : -1;
                 }, m, l, acc);
                 if (nsp == 1) {
 #pragma unroll

@@ -14,6 +14,7 @@
 #include <stddef.h>
 
 #include "pa_group.hpp"
+#include "pa_window.hpp"
 
 using namespace ti;
 using namespace ti_group;
@@ -197,6 +198,7 @@ struct F32Params {
     float scale_log2;
     const int32_t *lengths;   // SPARSE: keys of each (token, KV head)
     int tg, total;            // GROUP: tokens of a group, tokens of the call
+    int window, sinks;        // WIN
 };
 
 // Each split takes at least this many 16-key tiles (one per wave), so short contexts run on
@@ -206,7 +208,8 @@ constexpr int F32_MIN_TILES = 4;
 // QT: more than one q-tile per (sequence, KV head). SPARSE (one q-tile): (token, KV head) pairs with a
 // table row and a length each (pa_sparse.hip), 1-D grid of the pairs' splits. GROUP (SPARSE): p.tg
 // neighbouring tokens' pairs at a time over the joined list of their pages (pa_group.hpp), packed rows g + G t.
-template <int D, bool QT, bool SPARSE = false, bool GROUP = false>
+// WIN: the window of pa_window.hpp; the splits cut the list of tiles that it leaves for the q-tile, and each writes a partial.
+template <int D, bool QT, bool SPARSE = false, bool GROUP = false, bool WIN = false>
 __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     constexpr int NJ = D / 16, NDB = D / 16, NW = 4, MROW = D + 4;
     // GROUP: the joined list, in the merge's LDS; the tokens' keys of each page in dynamic LDS
@@ -277,11 +280,19 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     // partial); this q-tile's keys end after its last token's position
     ActiveSplits as = f32_active_splits((len + 15) >> 4, p.splits, F32_MIN_TILES);
     if constexpr (GROUP) as = ActiveSplits{((len >> 4) + p.splits - 1) / p.splits, p.splits};
+    if constexpr (WIN) as.active = p.splits;
     if (s >= as.active) return;   // no keys for this split
     const int t_last = QT ? min((16 * qt + 15) / p.G, nb - 1) : nb - 1;
     const int kend = p.causal ? start + t_last + 1 : len;
     const GroupMap gm{reinterpret_cast<const int2 *>(smem), p.P, p.pshift, p.Hk, h, len};
-    const int j0 = s * as.per, j1 = min(j0 + as.per, (kend + 15) >> 4);   // may be empty: (m, l) = (NEG_BIG, 0)
+    int ntiles = (kend + 15) >> 4;
+    WindowTiles wt{};
+    if constexpr (WIN) {
+        wt = WindowTiles::of<4>(start + t_first, p.window, p.sinks);
+        ntiles -= wt.skip;
+        as.per = (ntiles + p.splits - 1) / p.splits;
+    }
+    const int j0 = s * as.per, j1 = min(j0 + as.per, ntiles);   // may be empty: (m, l) = (NEG_BIG, 0)
     const int r = 16 * qt + r16, t = r / p.G, g = r - t * p.G;
     const bool ok = r < p.M && (GROUP ? (keyed >> t & 1) != 0 : t < nb);
     const int qpos = p.causal && ok ? start + t : len - 1;
@@ -303,35 +314,41 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         float v[4][NDB];
     };
     auto load = [&](int j, Tile &tl) {
-        const int pos0 = j * 16;
+        const int pos0 = (WIN ? wt.tile(j) : j) * 16;
         int last;   // keys past it read its row
+        int first = 0;   // WIN: and keys in front of it
         long long rbase;
         if constexpr (GROUP) {
             last = gm.last(pos0);
             rbase = gm.row_s(pos0);
         } else {
             last = len - 1 - pos0;
+            if constexpr (WIN) {
+                if (pos0 + 16 <= wt.lo) last = min(p.sinks, wt.lo) - 1 - pos0;   // a tile of sinks
+                else if (pos0 >= p.sinks) first = max(wt.lo - pos0, 0);
+            }
             const int pg = page_of_s(bt, pos0 >> p.pshift, p.bt_stride, p.num_pages);
             rbase = ((long long)pg * p.Hk + h) * p.P + (pos0 & (p.P - 1));
         }
-        const float *krow = p.kp + (rbase + min(r16, last)) * D + 4 * kg;
+        const float *krow = p.kp + (rbase + (WIN ? max(min(r16, last), first) : min(r16, last))) * D + 4 * kg;
 #pragma unroll
         for (int jj = 0; jj < NJ; jj++) tl.k[jj] = *reinterpret_cast<const f32x4 *>(krow + 16 * jj);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float *vrow = p.vp + (rbase + min(4 * kg + e, last)) * D + r16;
+            const float *vrow = p.vp + (rbase + (WIN ? max(min(4 * kg + e, last), first) : min(4 * kg + e, last))) * D + r16;
 #pragma unroll
             for (int db = 0; db < NDB; db++) tl.v[e][db] = vrow[16 * db];
         }
     };
     auto compute = [&](int j, const Tile &tl) {
-        const int pos0 = j * 16;
+        const int pos0 = (WIN ? wt.tile(j) : j) * 16;
         f32x4 sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int jj = 0; jj < NJ; jj++)
 #pragma unroll
             for (int c = 0; c < 4; c++) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(tl.k[jj][c], qv[jj][c], sc, 0, 0, 0);
-        const bool need_mask = pos0 + 15 > mask_from;
+        bool need_mask = pos0 + 15 > mask_from;
+        if constexpr (WIN) need_mask |= pos0 <= start + t_last - p.window && pos0 + 15 >= p.sinks;
         int seen = 0, off = 0;   // GROUP: keys of the page that the row sees, the tile's first one
         if constexpr (GROUP) {
             seen = lim[(pos0 >> p.pshift) * p.tg + min(t, p.tg - 1)];
@@ -342,6 +359,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         for (int e = 0; e < 4; e++) {
             const int kpos = pos0 + 4 * kg + e;
             if constexpr (GROUP) x[e] = off + 4 * kg + e < seen ? sc[e] : -INFINITY;
+            else if constexpr (WIN) x[e] = need_mask & !window_sees(kpos, qpos, p.window, p.sinks) ? -INFINITY : sc[e];
             else x[e] = need_mask && kpos > qpos ? -INFINITY : sc[e];
             mt = fmaxf(mt, x[e]);
         }
@@ -409,7 +427,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     __syncthreads();
     const size_t unit = SPARSE ? (size_t)blockIdx.x : ((size_t)b * p.Hk + h) * p.splits + s;
     const int mrows = QT ? 16 : p.M;   // one q-tile: the M <= 16 rows
-    bool fine = true;   // GROUP: no value that is not finite has come in
+    bool fine = true;   // GROUP, WIN: no value that is not finite has come in
     for (int it = threadIdx.x; it < mrows * (D / 4); it += NW * 64) {
         const int rr = it / (D / 4), d4 = (it % (D / 4)) * 4, r = 16 * qt + rr;
         if (r >= p.M) continue;
@@ -427,7 +445,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         }
         const int tr = r / p.G, gr = r - tr * p.G;
         if (tr >= nb || (GROUP && (tok0 + tr < q0 || tok0 + tr >= q1))) continue;
-        if constexpr (GROUP) {
+        if constexpr (GROUP || WIN) {
             fine &= fabsf(lsum) < INFINITY;
 #pragma unroll
             for (int e = 0; e < 4; e++) fine &= fabsf(acc[e]) < INFINITY;
@@ -451,6 +469,31 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
             __shared__ int red[2 + NW];
             group_pages<NW * 64>(p, *reinterpret_cast<GroupLds *>(smem), lim, red, tok0, h, q0, q1);
             group_rows<D>(p, reinterpret_cast<const int2 *>(smem), lim, tok0, h, q0, q1, j0, j1, p.splits, unit, w, NW, lane);
+        }
+    }
+    if constexpr (WIN) {
+        if (__syncthreads_or(!fine)) {
+            for (int rr = w; rr < mrows; rr += NW) {
+                const int r = 16 * qt + rr, t = r / p.G;
+                if (r >= p.M || t >= nb) continue;
+                const size_t qrow = (size_t)(tok0 + t) * p.Hq + h * p.G + (r - t * p.G);
+                const int last = start + t;
+                float m, l, acc[D / 64];
+                exact_row<D, false, false>(p, bt, h, p.q + qrow * D, j0 * 16, j1 * 16, [&](int v) {
+                    const int key = wt.tile(v >> 4) * 16 + (v & 15);
+                    return window_sees(key, last, p.window, p.sinks) ? key : -1;
+                }, m, l, acc);
+                float *dst = p.part + (unit * (size_t)p.M + r) * (D + 2);
+#pragma unroll
+                for (int k = 0; k < D / 64; k++) {
+                    if (as.active == 1) p.out[qrow * D + lane + 64 * k] = acc[k] / l;
+                    else dst[lane + 64 * k] = acc[k];
+                }
+                if (as.active > 1 && lane == 0) {
+                    dst[D] = m;
+                    dst[D + 1] = l;
+                }
+            }
         }
     }
 }
@@ -480,18 +523,21 @@ static bool f32_mfma(const ti_attention_args *a, const ti_kv_cache *c) {
 static int f32_qtiles(const ti_attention_args *a, const ti_kv_cache *c) {
     return (a->q_heads / c->kv_heads * a->max_query_len + 15) / 16;
 }
-static int f32_splits(const ti_attention_args *a, const ti_kv_cache *c) {
+static int f32_splits(const ti_attention_args *a, const ti_kv_cache *c, ti_window win) {
     const long long items = (long long)a->num_seqs * c->kv_heads * f32_qtiles(a, c);
     int sp = 1;
     while (sp < F32_MAX_SPLITS && items * sp < F32_TARGET) sp <<= 1;
+    // a window bounds a q-tile's keys: splits of at least F32_MIN_TILES of them
+    const long long tiles = 2 * window_tiles(win, 16);
+    while (win.size && sp > 1 && (long long)F32_MIN_TILES * sp > tiles) sp >>= 1;
     return sp;
 }
 
 // Key splits for the fp32 path: while the waves (tokens x query heads x sequences) are
 // fewer than about 1024, double the splits (at most 32). Host shapes only (graph-safe).
-int ti_plan_generic(const ti_attention_args *a, const ti_kv_cache *c, size_t *bytes) {
+int ti_plan_generic(const ti_attention_args *a, const ti_kv_cache *c, size_t *bytes, ti_window win) {
     if (f32_mfma(a, c)) {
-        const int sp = f32_splits(a, c);
+        const int sp = f32_splits(a, c, win);
         const int rows = a->q_heads / c->kv_heads * a->max_query_len;
         *bytes = sp == 1 ? 0 : (size_t)a->num_seqs * c->kv_heads * sp * rows * (c->head_dim + 2) * sizeof(float);
         return sp;
@@ -505,8 +551,10 @@ int ti_plan_generic(const ti_attention_args *a, const ti_kv_cache *c, size_t *by
 }
 
 int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStream_t s, ti_window win) {
-    if (f32_mfma(a, c) && !win.size) {
+    if (f32_mfma(a, c)) {
         F32Params f;
+        f.window = win.size;
+        f.sinks = win.sinks;
         f.q = (const float *)a->q;
         f.out = (float *)a->out;
         f.kp = (const float *)c->k_pages;
@@ -526,7 +574,7 @@ int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStrea
         f.causal = a->causal;
         f.scale_log2 = a->scale * LOG2E;
         size_t bytes = 0;
-        f.splits = ti_plan_generic(a, c, &bytes);
+        f.splits = ti_plan_generic(a, c, &bytes, win);
         if (bytes > 0 && (!a->workspace || a->workspace_bytes < bytes)) f.splits = 1;   // runs unsplit
         f.part = (float *)a->workspace;
         f.B = a->num_seqs;
@@ -537,6 +585,17 @@ int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStrea
         f.sshift = __builtin_ctz(f.splits);
         f.xcd = pairs % 8 == 0 && f.qtiles > 1;   // decode (one q-tile) reuses no tile across work-groups
         const dim3 grid = f.xcd ? dim3((unsigned)wgs) : dim3((unsigned)(f.splits * f.qtiles), c->kv_heads, a->num_seqs);
+        if (win.size) {
+            if (f.qtiles > 1) {
+                if (c->head_dim == 128) attn_f32_kernel<128, true, false, false, true><<<grid, 256, 0, s>>>(f);
+                else attn_f32_kernel<64, true, false, false, true><<<grid, 256, 0, s>>>(f);
+            } else {
+                if (c->head_dim == 128) attn_f32_kernel<128, false, false, false, true><<<grid, 256, 0, s>>>(f);
+                else attn_f32_kernel<64, false, false, false, true><<<grid, 256, 0, s>>>(f);
+            }
+            if (hipGetLastError() != hipSuccess) return TI_ERR_LAUNCH;
+            return f.splits > 1 ? ti_launch_combine(a, c, f.M, f.splits, s) : TI_OK;
+        }
         if (f.qtiles > 1) {
             if (c->head_dim == 128) attn_f32_kernel<128, true><<<grid, 256, 0, s>>>(f);
             else attn_f32_kernel<64, true><<<grid, 256, 0, s>>>(f);
@@ -570,7 +629,7 @@ int ti_launch_generic(const ti_attention_args *a, const ti_kv_cache *c, hipStrea
     p.sinks = win.sinks;
     p.scale_log2 = a->scale * LOG2E;
     size_t bytes = 0;
-    p.splits = ti_plan_generic(a, c, &bytes);
+    p.splits = ti_plan_generic(a, c, &bytes, win);
     if (bytes > 0 && (!a->workspace || a->workspace_bytes < bytes)) p.splits = 1;   // runs unsplit
     p.part = (float *)a->workspace;
     dim3 grid(a->max_query_len * p.splits, a->q_heads, a->num_seqs);

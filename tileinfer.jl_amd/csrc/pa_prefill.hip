@@ -527,7 +527,8 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
             if constexpr (INT8) v *= skq[e >> 2][e & 3];
             if (need_mask) {
                 const int kpos = kt_at * KT + key;
-                v = (valid && kpos <= qpos && kpos < kend_w && (!WIN || kpos > before || kpos < p.sinks)) ? v : -INFINITY;
+                if constexpr (WIN) v = valid & (kpos <= qpos) & (kpos < kend_w) & ((kpos > before) | (kpos < p.sinks)) ? v : -INFINITY;
+                else v = (valid && kpos <= qpos && kpos < kend_w) ? v : -INFINITY;
             }
             x[e] = v;
             mt = fmaxf(mt, v);
@@ -735,7 +736,7 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
             float xm, xl, acc[D / 64];
             exact_row<D, INT8, FP8>(p, bt, h, p.q + qrow * D, kt_lo * KT, kt_hi * KT, [&](int v) {
                 const int key = actual(v / KT) * KT + v % KT;
-                return key <= last && (!WIN || key > last - p.window || key < p.sinks) ? key : -1;
+                return (WIN ? window_sees(key, last, p.window, p.sinks) : key <= last) ? key : -1;
             }, xm, xl, acc);
             float *dst = p.part + (unit * p.M + (size_t)xt * p.G + x % p.G) * (D + 2);
 #pragma unroll

@@ -284,7 +284,7 @@ prefill_pp_kernel(PPParams p) {
         *reinterpret_cast<u32x4 *>(&sm.k[buf][(ckey + KPU * u) * KROW + cch * 8]) = bf16_chunk(r, FP8 ? scale_of(sc8[x].k, u) : 1.0f);
     };
     // WIN: keys that no row of the work-group sees
-    auto hidden = [&](int key) { return WIN && key < wt.lo && key >= p.sinks; };
+    auto hidden = [&](int key) { return WIN & (key < wt.lo) & (key >= p.sinks); };
     auto store_v = [&](const Chunk &r, int buf, int j, int u) {
         // Keys past kend in the last tile may hold any bits (even NaN) of an allocated
         // page: their probabilities are 0 and their values must be finite. Branch-free,
@@ -443,7 +443,7 @@ prefill_pp_kernel(PPParams p) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int key = 8 * (e >> 2) + (e & 3);
-                    sc[e] = key > lim || key < sunk ? sc[e] : -INFINITY;
+                    sc[e] = (key > lim) | (key < sunk) ? sc[e] : -INFINITY;
                 }
             }
         }
@@ -651,7 +651,7 @@ prefill_pp_kernel(PPParams p) {
                 float xm, xl, acc[D / 64];
                 exact_row<D, INT8, FP8>(p, bt, h, p.q + qrow * D, kt_lo * KT, kt_hi * KT, [&](int v) {
                     const int key = (WIN ? wt.tile(v / KT) : v / KT) * KT + v % KT;
-                    return key <= last && (!WIN || key > last - p.window || key < p.sinks) ? key : -1;
+                    return (WIN ? window_sees(key, last, p.window, p.sinks) : key <= last) ? key : -1;
                 }, xm, xl, acc);
                 float *dst = p.part + (unit * p.M + (size_t)xt * p.G + x % p.G) * (D + 2);
 #pragma unroll

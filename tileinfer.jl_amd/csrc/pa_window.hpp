@@ -35,6 +35,12 @@ struct WindowTiles {
     __device__ __forceinline__ int tile(int j) const { return j < sunk ? j : j + skip; }
 };
 
+// Whether the query at position `at` sees `key`. Without short circuits: hipcc has made of branches around the choice between
+// a matrix product's register and a constant a move of the constant for every lane (attn_f32_kernel's masks, ROCm 7.2).
+__device__ __forceinline__ bool window_sees(int key, int at, int size, int sinks) {
+    return (key <= at) & ((key > at - size) | (key < sinks));
+}
+
 // 8 e4m3 values (two words) times a power of two in bf16.
 __device__ __forceinline__ u32x4 e4m3x8_to_bf16(uint32_t x, uint32_t y, float scale) {
     return (u32x4){__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, false)),
