@@ -30,37 +30,42 @@ __device__ __forceinline__ int pages_of(const PoolParams &p, long long positions
     return (int)(p.pshift >= 0 ? (positions + p.pool.page_size - 1) >> p.pshift : (positions + p.pool.page_size - 1) / p.pool.page_size);
 }
 
-// Running sums of a and b over the sequences (b in `sb`, a in `sa`, both with the total behind): every thread calls it.
+// Running sums of a and b over the sequences, with the totals behind, and what else a sequence is asked for often:
+// every thread calls it.
 struct Sums {
-    int32_t a[MAX_SEQS + 1], b[MAX_SEQS + 1];
+    int32_t a[MAX_SEQS + 1], b[MAX_SEQS + 1], old[MAX_SEQS];
 };
+constexpr uint32_t FULL = 0x7fffffff;   // sums stay here once they get here (neither operand is above it: no wrap)
+__device__ __forceinline__ uint32_t plus(uint32_t x, uint32_t y) { return min(x + y, FULL); }
 template <typename F>
-__device__ __forceinline__ void running_sums(Sums &s, int n, long long &total_a, long long &total_b, F &&value) {
-    __shared__ long long part[2][NT / 64];
+__device__ __forceinline__ void running_sums(Sums &s, int n, uint32_t &total_a, uint32_t &total_b, F &&value) {
+    __shared__ uint2 part[NT / 64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    long long ta = 0, tb = 0;
+    uint32_t ta = 0, tb = 0;
     for (int i0 = 0; i0 < n; i0 += NT) {
         const int i = i0 + (int)threadIdx.x;
-        long long a = 0, b = 0;
+        uint32_t a = 0, b = 0;
         if (i < n) value(i, a, b);
-        long long ia = a, ib = b;
+        uint32_t ia = a, ib = b;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const long long va = __shfl_up(ia, d), vb = __shfl_up(ib, d);
-            if (lane >= d) ia += va, ib += vb;
+            const uint32_t va = __shfl_up(ia, d), vb = __shfl_up(ib, d);
+            if (lane >= d) ia = plus(ia, va), ib = plus(ib, vb);
         }
-        __syncthreads();   // the last round's parts are read
-        if (lane == 63) part[0][w] = ia, part[1][w] = ib;
+        if (i0 > 0) __syncthreads();   // the last round's parts are read
+        if (lane == 63) part[w] = make_uint2(ia, ib);
         __syncthreads();
+        uint32_t before_a = ta, before_b = tb;
 #pragma unroll
         for (int k = 0; k < NT / 64; k++) {
-            if (k < w) ia += part[0][k], ib += part[1][k];
+            const uint2 x = part[k];
+            if (k < w) before_a = plus(before_a, x.x), before_b = plus(before_b, x.y);
+            ta = plus(ta, x.x), tb = plus(tb, x.y);
         }
-        if (i < n) s.a[i] = (int32_t)min(ta + ia - a, 0x7fffffffLL), s.b[i] = (int32_t)min(tb + ib - b, 0x7fffffffLL);
-#pragma unroll
-        for (int k = 0; k < NT / 64; k++) ta += part[0][k], tb += part[1][k];
+        // a sum that is full is of no use to anyone (reserve refuses, release has none)
+        if (i < n) s.a[i] = (int32_t)(plus(before_a, ia) - a), s.b[i] = (int32_t)(plus(before_b, ib) - b);
     }
-    if (threadIdx.x == 0) s.a[n] = (int32_t)min(ta, 0x7fffffffLL), s.b[n] = (int32_t)min(tb, 0x7fffffffLL);
+    if (threadIdx.x == 0) s.a[n] = (int32_t)ta, s.b[n] = (int32_t)tb;
     total_a = ta;
     total_b = tb;
     __syncthreads();
@@ -84,7 +89,9 @@ __device__ __forceinline__ bool last_to_end(int32_t *ticket) {
     if (threadIdx.x == 0) {
         last = 1;
         if (gridDim.x > 1) {
-            const int was = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+            // Nothing is handed over through memory, so no fence (one writes an L2 back: 492 work-groups 20 -> 12 us):
+            // what the others have read is in their registers and LDS.
+            const int was = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             last = was == (int)gridDim.x - 1;
             if (last) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -95,6 +102,8 @@ __device__ __forceinline__ bool last_to_end(int32_t *ticket) {
 
 __device__ __forceinline__ int32_t clamped(int32_t x, int32_t lo, int32_t hi) { return min(max(x, lo), hi); }
 
+// EACH: neighbouring tokens of a thread.
+template <int EACH>
 __global__ void __launch_bounds__(NT) reserve_kernel(PoolParams p) {
     __shared__ Sums s;                // tokens, pages
     __shared__ int wide;
@@ -102,46 +111,72 @@ __global__ void __launch_bounds__(NT) reserve_kernel(PoolParams p) {
     const int S = pool.num_seqs, P = pool.page_size, have = clamped(pool.free_count[0], 0, pool.num_pages);
     if (threadIdx.x == 0) wide = 0;
     __syncthreads();
-    long long tokens, pages;
-    running_sums(s, S, tokens, pages, [&](int b, long long &a, long long &n) {
+    uint32_t tokens, pages;
+    running_sums(s, S, tokens, pages, [&](int b, uint32_t &a, uint32_t &n) {
         const long long old = max(pool.lengths[b], 0);
+        s.old[b] = (int32_t)old;
         a = max(p.counts[b], 0);
         const long long to = old + a;
         const bool fits = to <= (long long)pool.table_width * P && to <= 0x7fffffffLL;
         if (!fits) wide = 1;
         n = fits ? pages_of(p, to) - pages_of(p, old) : 0;
     });
-    const bool outgrown = wide || tokens > p.tokens;
-    const bool ok = !outgrown && pages <= have;
+    const bool outgrown = wide || tokens > (uint32_t)p.tokens || tokens == FULL;
+    const bool ok = !outgrown && pages <= (uint32_t)have;
     const int t_all = ok ? (int)tokens : 0;
     const int wg = blockIdx.x, wgs = gridDim.x;
     if (wg == 0) {
         for (int b = threadIdx.x; b <= S; b += NT) p.qsl[b] = ok ? s.a[b] : 0;
-        if (threadIdx.x == 0) p.short_of[0] = ok ? 0 : (outgrown ? -1 : (int)min(pages - have, 0x7fffffffLL));
+        if (threadIdx.x == 0) p.short_of[0] = ok ? 0 : (outgrown ? -1 : (int)(pages - have));
     }
     // page r of the step's: from the top of the stack down
     auto page_at = [&](int r) { return pool.free[have - 1 - r]; };
     if (ok) {
         for (int r = wg * NT + (int)threadIdx.x; r < (int)pages; r += wgs * NT) {
             const int b = find(s.b, S, r);
-            const int held = pages_of(p, max(pool.lengths[b], 0));
+            const int held = pages_of(p, s.old[b]);
             pool.tables[(size_t)b * pool.table_width + held + (r - s.b[b])] = page_at(r);
         }
     }
-    for (int t = wg * NT + (int)threadIdx.x; t < p.tokens; t += wgs * NT) {
-        int pos = 0, slot = 0;
-        if (t < t_all) {
-            const int b = find(s.a, S, t), old = max(pool.lengths[b], 0);
-            pos = old + (t - s.a[b]);
-            const int i = p.pshift >= 0 ? pos >> p.pshift : pos / P, held = pages_of(p, old);
-            const int page = i < held ? pool.tables[(size_t)b * pool.table_width + i] : page_at(s.b[b] + i - held);
-            slot = (page - 1) * P + (pos - i * P) + 1;
+    // Neighbouring tokens mostly share a sequence and a page: the chain of loads is walked once for them.
+    const bool whole = ((((uintptr_t)p.positions | (uintptr_t)p.slots) & 15) == 0);
+    for (int t0 = EACH * (wg * NT + (int)threadIdx.x); t0 < p.tokens; t0 += EACH * wgs * NT) {
+        int pos[EACH], slot[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; e++) pos[e] = slot[e] = 0;
+        if (t0 < t_all) {
+            int b = find(s.a, S, t0), had = -1, base = 0;
+#pragma unroll
+            for (int e = 0; e < EACH; e++) {
+                const int t = t0 + e;
+                if (t >= t_all) break;
+                while (t >= s.a[b + 1]) b++, had = -1;
+                const int old = s.old[b];
+                pos[e] = old + (t - s.a[b]);
+                const int i = p.pshift >= 0 ? pos[e] >> p.pshift : pos[e] / P;
+                if (i != had) {
+                    const int held = pages_of(p, old);
+                    const int page = i < held ? pool.tables[(size_t)b * pool.table_width + i] : page_at(s.b[b] + i - held);
+                    base = (page - 1 - i) * P + 1;
+                    had = i;
+                }
+                slot[e] = base + pos[e];
+            }
         }
-        p.positions[t] = pos;
-        p.slots[t] = slot;
+        if constexpr (EACH == 4) {
+            if (whole && t0 + 4 <= p.tokens) {
+                *reinterpret_cast<int4 *>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+                *reinterpret_cast<int4 *>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+                continue;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            if (t0 + e < p.tokens) p.positions[t0 + e] = pos[e], p.slots[t0 + e] = slot[e];
+        }
     }
     if (!last_to_end(pool.ticket) || !ok) return;
-    for (int b = threadIdx.x; b < S; b += NT) pool.lengths[b] = max(pool.lengths[b], 0) + (s.a[b + 1] - s.a[b]);
+    for (int b = threadIdx.x; b < S; b += NT) pool.lengths[b] = s.old[b] + (s.a[b + 1] - s.a[b]);
     if (threadIdx.x == 0) pool.free_count[0] = have - (int)pages;
 }
 
@@ -188,12 +223,12 @@ __global__ void __launch_bounds__(NT) release_kernel(PoolParams p) {
     __shared__ Sums s;                // pages; kept positions
     const ti_page_pool &pool = p.pool;
     const int S = pool.num_seqs, have = clamped(pool.free_count[0], 0, pool.num_pages);
-    long long pages, unused;
-    running_sums(s, S, pages, unused, [&](int b, long long &a, long long &n) {
+    uint32_t pages, unused;
+    running_sums(s, S, pages, unused, [&](int b, uint32_t &a, uint32_t &n) {
         a = gone_of(p, b).count();
         n = 0;
     });
-    const int all = (int)min(pages, (long long)(pool.num_pages - have));   // never above the stack's room
+    const int all = (int)min(pages, (uint32_t)(pool.num_pages - have));   // never above the stack's room
     for (int r = blockIdx.x * NT + (int)threadIdx.x; r < all; r += gridDim.x * NT) {
         const int b = find(s.a, S, r);
         int32_t *e = pool.tables + (size_t)b * pool.table_width + gone_of(p, b).entry(r - s.a[b]);
@@ -230,12 +265,14 @@ int ti_launch_reserve(const ti_page_pool *pool, const int32_t *counts, int token
     p.slots = slots;
     p.qsl = qsl;
     p.short_of = short_of;
-    reserve_kernel<<<groups(tokens, 1024, 256), NT, 0, s>>>(p);
+    // one token a thread for steps of a few tokens a sequence, whose chains are the time; four for prompts
+    if (tokens < 65536) reserve_kernel<1><<<groups(tokens, NT, 256), NT, 0, s>>>(p);
+    else reserve_kernel<4><<<groups(tokens, 4 * NT, 512), NT, 0, s>>>(p);
     return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
 }
 
 int ti_launch_release(const ti_page_pool *pool, const int32_t *keep, hipStream_t s) {
     const PoolParams p = params_of(pool, keep);
-    release_kernel<<<groups((long long)pool->num_seqs * pool->table_width, 16384, 32), NT, 0, s>>>(p);
+    release_kernel<<<groups((long long)pool->num_seqs * pool->table_width, 4 * NT, 256), NT, 0, s>>>(p);
     return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
 }
