@@ -13,6 +13,8 @@
 // bit-identical to rmsnorm, rope and store_kv in a row: products and sums are rounded one by one.
 #pragma clang fp contract(off)
 
+#include <type_traits>
+
 #include "kv_rows.hpp"
 
 using namespace ti;
@@ -91,16 +93,48 @@ __device__ __forceinline__ void rotated(const T *x, const T *w, const T *cs, flo
     }
 }
 
+template <int N> using IC = std::integral_constant<int, N>;
+
+// Eight elements held between the passes in their own type's bits (a rotated bf16 key is rounded to bf16 already).
+template <typename T> struct Held;
+template <> struct Held<uint16_t> {
+    u32x4 w;
+    __device__ __forceinline__ void put(const float (&x)[8]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+    }
+    __device__ __forceinline__ void ld(const uint16_t *p) { w = *reinterpret_cast<const u32x4 *>(p); }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    }
+};
+template <> struct Held<float> {
+    f32x4 lo, hi;
+    __device__ __forceinline__ void put(const float (&x)[8]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) lo[e] = x[e], hi[e] = x[4 + e];
+    }
+    __device__ __forceinline__ void ld(const float *p) {
+        lo = *reinterpret_cast<const f32x4 *>(p);
+        hi = *reinterpret_cast<const f32x4 *>(p + 4);
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = lo[e], x[4 + e] = hi[e];
+    }
+};
+
 template <typename T, bool FUSED, bool NORM, int D>
 __global__ void __launch_bounds__(256) fp8_write_kernel(Fp8WriteParams p) {
     constexpr int HALF = D / 2, LPH = D / 8, NT = 256, NG = NT / LPH;
     using V = Vec4<T>;
-    __shared__ int src[MAX_PAGE];              // the token that writes each row of the page, or -1
-    __shared__ int list[MAX_PAGE];             // the rows that are written
-    __shared__ int count;
+    __shared__ int src[MAX_PAGE];                     // the token that writes each row of the page, or -1
+    __shared__ uint16_t lists[NT / 64][MAX_PAGE];     // the rows that are written, a copy for each wave
     __shared__ uint32_t most[2 * MAX_HEADS];
     __shared__ float inv[2 * MAX_HEADS], ratio[2 * MAX_HEADS];
-    const int tid = threadIdx.x, u = tid % LPH, gid = tid / LPH;
+    const int tid = threadIdx.x, lane = tid & 63, u = tid % LPH, gid = tid / LPH;
+    uint16_t *list = lists[tid >> 6];
     if (FUSED && blockIdx.x >= p.page_groups) {
         const long long item = (long long)(blockIdx.x - p.page_groups) * NG + gid;
         const int t = (int)(item / p.nq), j = (int)(item - (long long)t * p.nq);
@@ -116,136 +150,193 @@ __global__ void __launch_bounds__(256) fp8_write_kernel(Fp8WriteParams p) {
         V::st(dst + HALF + 4 * u, hi);
         return;
     }
-    // 0-based page of token j's slot, -1 where the token writes nothing
+    // 0-based page of a slot, -1 for one outside the pool; whether a token writes at all
     const int limit = (int)min((long long)p.pages * p.P, 0x7fffffffLL);
-    auto page_of_token = [&](int j) {
-        const int s = p.slots[j];
-        bool ok = s > 0 && s <= limit;
-        if (FUSED) {
-            const int pos = p.positions[j];
-            ok = ok && pos >= 0 && pos < p.table_len;
-        }
-        return ok ? (s - 1) >> p.pshift : -1;
+    auto page_of_slot = [&](int s) { return s > 0 && s <= limit ? (s - 1) >> p.pshift : -1; };
+    auto writes = [&](int j) {
+        if (!FUSED) return true;
+        const int pos = p.positions[j];
+        return pos >= 0 && pos < p.table_len;
     };
     const int c0 = (int)(blockIdx.x / (unsigned)p.hgroups) * p.chunk, h0 = (int)(blockIdx.x % (unsigned)p.hgroups) * p.hpg;
-    const int heads = min(p.hpg, p.Hk - h0), c1 = min(c0 + p.chunk, p.n);
-    for (int i = c0; i < c1; i++) {
-        const int page = page_of_token(i);
-        if (page < 0 || (i > 0 && page_of_token(i - 1) == page)) continue;
-        bool earlier = false;
-        for (int j = tid; j < i; j += NT) earlier |= page_of_token(j) == page;
-        if (__syncthreads_or(earlier)) continue;   // that one's work-group has the page
-        for (int o = tid; o < p.P; o += NT) src[o] = -1;
-        if (tid < 2 * heads) most[tid] = 0u;
-        __syncthreads();
-        for (int j = i + tid; j < p.n; j += NT)
-            if (page_of_token(j) == page) atomicMax(&src[(p.slots[j] - 1) & (p.P - 1)], j);
-        __syncthreads();
-        if (tid < 64) {
-            int c = 0;
-            for (int o0 = 0; o0 < p.P; o0 += 64) {
-                const int o = o0 + tid;
-                const bool has = o < p.P && src[o] >= 0;
-                const unsigned long long m = __ballot(has);
-                if (has) list[c + __popcll(m & ((1ull << tid) - 1))] = o;
-                c += __popcll(m);
-            }
-            if (tid == 0) count = c;
+    const int heads = min(p.hpg, p.Hk - h0);
+    auto load = [&](int t, int hh, Held<T> &x) {
+        const int half = hh >= heads, h = h0 + hh - half * heads;
+        if constexpr (FUSED) {
+            const T *x0 = (const T *)p.qkv + ((size_t)t * (p.nq + 2 * p.Hk) + p.nq + (size_t)half * p.Hk + h) * D;
+            if (half) return x.ld(x0 + 8 * u);
+            float y[8];
+            rotated<T, NORM, D>(x0, (const T *)p.k_norm, (const T *)p.cos_sin + (size_t)p.positions[t] * 2 * D, p.eps, u, y);
+            x.put(y);
+        } else {
+            x.ld((const T *)(half ? p.v : p.k) + ((size_t)t * p.Hk + h) * D + 8 * u);
         }
+    };
+    // Few tokens: their slots are read once, beside the rows of the work-group's own token.
+    const bool few = p.n <= NT;
+    const int my_slot = few && tid < p.n ? p.slots[tid] : 0;
+    // One token a work-group: its rows are on their way while the slots are looked through.
+    Held<T> mine;
+    if (p.chunk == 1 && (!FUSED || writes(c0))) load(c0, min(gid, 2 * heads - 1), mine);
+    // The chunk's tokens (at most 64) that write to another page than the one in front of them: one lane each.
+    int first_page = -1;
+    if (lane < p.chunk && c0 + lane < p.n && writes(c0 + lane)) {
+        first_page = page_of_slot(p.slots[c0 + lane]);
+        if (c0 + lane > 0 && writes(c0 + lane - 1) && page_of_slot(p.slots[c0 + lane - 1]) == first_page) first_page = -1;
+    }
+    for (unsigned long long starts = __ballot(first_page >= 0); starts; starts &= starts - 1) {
+        const int at = __builtin_ctzll(starts), i = c0 + at, page = __builtin_amdgcn_readlane(first_page, at);
+        // the block's scales, needed below
+        float *sp = nullptr;
+        float old = 0.0f;
+        if (tid < 2 * heads) {
+            const int half = tid >= heads;
+            sp = p.scale + ((size_t)half * p.pages + page) * p.Hk + h0 + tid - half * heads;
+            old = *sp;
+            most[tid] = 0u;
+        }
+        for (int o = tid; o < p.P; o += NT) src[o] = -1;
         __syncthreads();
-        // vectors of the page's new rows: (row, half, head), heads innermost; one per lane group at a time
+        // All tokens of the page, wherever they are; one in front of this one has the page.
+        bool earlier = false;
+        auto take = [&](int s, int j) {
+            if (page_of_slot(s) == page && writes(j)) {
+                if (j < i) earlier = true;
+                else atomicMax(&src[(s - 1) & (p.P - 1)], j);
+            }
+        };
+        if (few) {
+            if (tid < p.n) take(my_slot, tid);
+        } else if (((uintptr_t)p.slots & 15) == 0) {
+            const int quads = p.n >> 2;
+            for (int q0 = tid; q0 < quads; q0 += 4 * NT) {
+                int4 s[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[e] = reinterpret_cast<const int4 *>(p.slots)[min(q0 + e * NT, quads - 1)];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int j = 4 * (q0 + e * NT);
+                    if (q0 + e * NT < quads) take(s[e].x, j), take(s[e].y, j + 1), take(s[e].z, j + 2), take(s[e].w, j + 3);
+                }
+            }
+            if (tid < (p.n & 3)) take(p.slots[4 * quads + tid], 4 * quads + tid);
+        } else {
+            for (int j = tid; j < p.n; j += NT) take(p.slots[j], j);
+        }
+        if (__syncthreads_or(earlier)) continue;
+        int count = 0;
+        for (int o0 = 0; o0 < p.P; o0 += 64) {
+            const int o = o0 + lane;
+            const bool has = o < p.P && src[o] >= 0;
+            const unsigned long long m = __ballot(has);
+            if (has) list[count + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)o;
+            count += __popcll(m);
+        }
+        // Vectors of the page's new rows: (row, half, head), heads innermost; one per lane group at a time. A lane holds
+        // elements 8 u .. 8 u + 7, of a rotated key 4 u .. and D / 2 + 4 u .. .
         const int vectors = count * 2 * heads;
-        auto load = [&](int vec, float (&x)[8], int &row, int &hh) {
+        auto place = [&](int vec, int &row, int &hh) {
             const int r = vec / (2 * heads);
             hh = vec - r * 2 * heads;                // half * heads + head
             row = list[r];
-            const int t = src[row], half = hh >= heads, h = h0 + hh - half * heads;
-            if constexpr (FUSED) {
-                const T *x0 = (const T *)p.qkv + ((size_t)t * (p.nq + 2 * p.Hk) + p.nq + h) * D;
-                if (!half) {
-                    rotated<T, NORM, D>(x0, (const T *)p.k_norm, (const T *)p.cos_sin + (size_t)p.positions[t] * 2 * D, p.eps, u, x);
-                    return;
-                }
-                x0 += (size_t)p.Hk * D;
-                float lo[4], hi[4];
-                V::ld(x0 + 4 * u, lo);
-                V::ld(x0 + HALF + 4 * u, hi);
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = lo[e], x[4 + e] = hi[e];
-            } else {
-                const T *x0 = (const T *)(half ? p.v : p.k) + ((size_t)t * p.Hk + h) * D;
-                float lo[4], hi[4];
-                V::ld(x0 + 4 * u, lo);
-                V::ld(x0 + HALF + 4 * u, hi);
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = lo[e], x[4 + e] = hi[e];
-            }
         };
-        for (int vec = gid; vec < vectors; vec += NG) {
+        auto largest = [&](const Held<T> &held, int hh) {
             float x[8], m = 0.0f;
-            int row, hh;
-            load(vec, x, row, hh);
+            held.get(x);
 #pragma unroll
             for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
             if (u == 0) atomicMax(&most[hh], __float_as_uint(m));   // of no sign: ordered as whole numbers
-        }
-        __syncthreads();
-        bool grown = false;
-        if (tid < 2 * heads) {
-            const int half = tid >= heads, h = h0 + tid - half * heads;
-            float *sp = p.scale + ((size_t)half * p.pages + page) * p.Hk + h;
-            const float old = *sp, need = least_scale(__uint_as_float(most[tid]));
-            const bool fresh = src[0] >= 0 || !(old > 0.0f && old < INFINITY);
-            const float now = fresh ? need : fmaxf(old, need);
-            inv[tid] = inverse(now);
-            ratio[tid] = fresh ? 1.0f : old * inverse(now);
-            grown = ratio[tid] < 1.0f;
-            if (now != old) *sp = now;
-        }
+        };
         uint8_t *base = p.q8 + (((size_t)page * p.Hk + h0) << p.pshift) * D;
         const size_t half_q = (((size_t)p.pages * p.Hk) << p.pshift) * D;
-        if (__syncthreads_or(grown)) {
-            // the held rows of the blocks that grew, 16 bytes at a time
+        auto store = [&](const Held<T> &held, int row, int hh) {
+            float x[8];
+            held.get(x);
+            const int half = hh >= heads;
+            uint8_t *dst = base + half * half_q + ((((size_t)(hh - half * heads)) << p.pshift) + row) * D;
+            const uint32_t lo = to_e4m3(x, inv[hh]), hi = to_e4m3(x + 4, inv[hh]);
+            if (FUSED && !half) {
+                *reinterpret_cast<uint32_t *>(dst + 4 * u) = lo;
+                *reinterpret_cast<uint32_t *>(dst + HALF + 4 * u) = hi;
+            } else {
+                *reinterpret_cast<u32x2 *>(dst + 8 * u) = (u32x2){lo, hi};
+            }
+        };
+        // between the two passes: the blocks' scales, and the rows that they hold already
+        auto scales = [&] {
+            __syncthreads();
+            bool grown = false;
+            if (tid < 2 * heads) {
+                const float need = least_scale(__uint_as_float(most[tid]));
+                const bool fresh = src[0] >= 0 || !(old > 0.0f && old < INFINITY);
+                const float now = fresh ? need : fmaxf(old, need);
+                inv[tid] = inverse(now);
+                ratio[tid] = fresh ? 1.0f : old * inverse(now);
+                grown = ratio[tid] < 1.0f;
+                if (now != old) *sp = now;
+            }
+            if (!__syncthreads_or(grown)) return;
+            // 16 bytes at a time
             for (int c = tid; c < 2 * heads * p.P * (D / 16); c += NT) {
                 const int d16 = c % (D / 16), o = (c / (D / 16)) & (p.P - 1), hh = (c / (D / 16)) >> p.pshift;
                 const float f = ratio[hh];
                 if (src[o] >= 0 || f == 1.0f) continue;
                 const int half = hh >= heads;
-                u32x4 *at = reinterpret_cast<u32x4 *>(base + half * half_q + ((((size_t)(hh - half * heads)) << p.pshift) + o) * D) + d16;
-                u32x4 w = *at;
+                u32x4 *at16 = reinterpret_cast<u32x4 *>(base + half * half_q + ((((size_t)(hh - half * heads)) << p.pshift) + o) * D) + d16;
+                u32x4 w = *at16;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float x[4] = {__builtin_amdgcn_cvt_f32_fp8((int)w[e], 0), __builtin_amdgcn_cvt_f32_fp8((int)w[e], 1),
                                         __builtin_amdgcn_cvt_f32_fp8((int)w[e], 2), __builtin_amdgcn_cvt_f32_fp8((int)w[e], 3)};
                     w[e] = to_e4m3(x, f);
                 }
-                *at = w;
+                *at16 = w;
             }
-        }
-        for (int vec = gid; vec < vectors; vec += NG) {
-            float x[8];
-            int row, hh;
-            load(vec, x, row, hh);
-            const int half = hh >= heads;
-            uint8_t *dst = base + half * half_q + ((((size_t)(hh - half * heads)) << p.pshift) + row) * D;
-            *reinterpret_cast<uint32_t *>(dst + 4 * u) = to_e4m3(x, inv[hh]);
-            *reinterpret_cast<uint32_t *>(dst + HALF + 4 * u) = to_e4m3(x + 4, inv[hh]);
-        }
+        };
+        // KEEP vectors of a lane group stay in registers between the passes, loaded together; more are read twice.
+        auto rows = [&](auto keep) {
+            constexpr int KEEP = decltype(keep)::value;
+            Held<T> x[KEEP];
+            int row[KEEP], hh[KEEP];
+            auto read = [&](int v0) {
+#pragma unroll
+                for (int k = 0; k < KEEP; k++) {
+                    place(min(v0 + k * NG, vectors - 1), row[k], hh[k]);
+                    if (KEEP == 1 && p.chunk == 1 && count == 1 && src[row[k]] == c0) x[k] = mine;
+                    else load(src[row[k]], hh[k], x[k]);
+                }
+            };
+            for (int v0 = gid; v0 < vectors || v0 == gid; v0 += KEEP * NG) {
+                read(v0);
+#pragma unroll
+                for (int k = 0; k < KEEP; k++) largest(x[k], hh[k]);   // (a vector twice is as good as once)
+            }
+            scales();
+            for (int v0 = gid; v0 < vectors; v0 += KEEP * NG) {
+                if (vectors > KEEP * NG) read(v0);
+#pragma unroll
+                for (int k = 0; k < KEEP; k++)
+                    if (v0 + k * NG < vectors) store(x[k], row[k], hh[k]);
+            }
+        };
+        if (vectors <= NG) rows(IC<1>{});
+        else if (vectors <= 4 * NG || FUSED || sizeof(T) == 4) rows(IC<4>{});
+        else rows(IC<8>{});
         __syncthreads();   // the page's lists are read
     }
 }
 
 template <typename T, bool FUSED, bool NORM>
 int launch(Fp8WriteParams &p, int D, hipStream_t s) {
-    // tokens of a work-group: one where there are few, a page's rows for prompts; KV heads: so many that a page's
-    // rows keep its lane groups busy
+    // Tokens of a work-group: one where there are few, a page's rows for prompts. KV heads: so many that a page's rows
+    // are one or eight vectors for each of its lane groups.
+    const int per = 256 / (D / 8);   // lane groups
     p.chunk = p.n <= 256 ? 1 : min(p.P, 64);
-    p.hpg = max(1, min(min(p.Hk, MAX_HEADS), 256 / p.chunk));
+    p.hpg = max(1, min(min(p.Hk, MAX_HEADS), p.n <= 64 ? per / 2 : 4 * per / min(p.P, 64)));
     p.hgroups = (p.Hk + p.hpg - 1) / p.hpg;
     const long long pages = (long long)(p.n + p.chunk - 1) / p.chunk * p.hgroups;
-    const int per = 256 / (D / 8);
     const long long queries = FUSED ? ((long long)p.n * p.nq + per - 1) / per : 0;
     if ((pages + queries) * 256 > MAX_THREADS) return TI_ERR_UNSUPPORTED;
     p.page_groups = (unsigned)pages;
