@@ -168,7 +168,9 @@ ti_decode_plan ti_plan_decode(const ti_attention_args *a, const ti_kv_cache *c, 
     // box): B = 8 (4 splits) 31.0 -> 27.5 us, B = 4 (8 splits) 21.3 vs 21.3 us, but B = 2
     // (16 splits) 16.0 -> 16.9 us and B = 16 (2 splits) 60.8 -> 63.0 us, where the shares
     // balance little and the device-side prefix costs its latency.
-    pl.flat = sp >= 4 && a->num_seqs >= 4 && a->num_seqs <= 64 ? sp * a->num_seqs : 0;
+    // Not with a window: sequences longer than it hold equally many keys, and finding the shares costs its latency (8 INT8
+    // sequences of 8000 to 32767 keys, window 8192: 39.1 -> 32.1 us).
+    pl.flat = sp >= 4 && a->num_seqs >= 4 && a->num_seqs <= 64 && !win.size ? sp * a->num_seqs : 0;
     pl.splits = sp;
     pl.waves = nw;
     pl.bytes = sp == 1 ? 0 : (size_t)pairs * sp * pl.rows * (c->head_dim + 2) * sizeof(float);

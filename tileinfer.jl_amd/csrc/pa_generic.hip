@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         for (int e = 0; e < 4; e++) {
             const int kpos = pos0 + 4 * kg + e;
             if constexpr (GROUP) x[e] = off + 4 * kg + e < seen ? sc[e] : -INFINITY;
-            else if constexpr (WIN) x[e] = need_mask & !window_sees(kpos, qpos, p.window, p.sinks) ? -INFINITY : sc[e];
+            else if constexpr (WIN) x[e] = (need_mask & !window_sees(kpos, qpos, p.window, p.sinks)) ? -INFINITY : sc[e];
             else x[e] = need_mask && kpos > qpos ? -INFINITY : sc[e];
             mt = fmaxf(mt, x[e]);
         }

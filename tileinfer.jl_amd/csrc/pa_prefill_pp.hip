@@ -443,7 +443,7 @@ prefill_pp_kernel(PPParams p) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int key = 8 * (e >> 2) + (e & 3);
-                    sc[e] = (key > lim) | (key < sunk) ? sc[e] : -INFINITY;
+                    sc[e] = ((key > lim) | (key < sunk)) ? sc[e] : -INFINITY;
                 }
             }
         }
