@@ -219,20 +219,29 @@ struct RowMap {
         return ((long long)pg * Hk + h) * P + (pos & (P - 1));
     }
     __device__ __forceinline__ int last(int pos) const { return len - 1 - pos; }   // last key of the tile at pos
-    __device__ __forceinline__ int first_key(int) const { return 0; }             // and first
-    __device__ __forceinline__ int pos(int j) const { return j * 16; }            // the tile's first position
+    __device__ __forceinline__ int pos(int j) const { return j * 16; }            // first position of tile j
 };
 
 // The tiles that a window leaves (WindowTiles). Keys that no row of the work-group sees are read as a neighbour that
 // one does, so that what they hold does not matter.
 struct WindowMap : RowMap {
     WindowTiles t;
-    int sinks;
+    int sinks, sunk_keys;   // sinks in front of the window
+    int first;              // first visible key of the window's first tile
+    int masked0, masked1;   // tiles of the list in which a key up to its query's position may be hidden
+    __device__ __forceinline__ WindowMap(const RowMap &m, const WindowTiles &w, int size, int s) : RowMap(m), t(w), sinks(s) {
+        sunk_keys = min(s, w.lo);
+        const int from = (w.sunk + w.skip) * 16;
+        first = from < s ? 0 : w.lo - from;
+        masked0 = w.sunk - ((sunk_keys & 15) != 0);
+        masked1 = s < len - size ? ((len - size + 15) >> 4) - w.skip : 0;   // the last row's window begins at len - size
+    }
     __device__ __forceinline__ int pos(int j) const { return t.tile(j) * 16; }
-    __device__ __forceinline__ int last(int pos) const { return min(len, pos < t.lo && pos + 16 <= t.lo ? min(sinks, t.lo) : len) - 1 - pos; }
-    __device__ __forceinline__ int first_key(int pos) const { return pos < sinks ? 0 : max(t.lo - pos, 0); }
+    __device__ __forceinline__ int last_key(int j) const { return (j < t.sunk ? sunk_keys : len) - 1 - pos(j); }
+    __device__ __forceinline__ int first_key(int j) const { return j == t.sunk ? first : 0; }
+    __device__ __forceinline__ bool masked(int j) const { return j >= masked0 && j < masked1; }
     __device__ __forceinline__ long long row(int pos) const {
-        if (pos < t.lo && pos >= sinks) pos = (pos & ~15) + 15 < t.lo ? min(sinks, t.lo) - 1 : t.lo;
+        if (pos < t.lo && pos >= sinks) pos = (pos & ~15) + 15 < t.lo ? sunk_keys - 1 : t.lo;
         return RowMap::row(pos);
     }
 };
@@ -250,13 +259,15 @@ __device__ __forceinline__ void load_tile(TileRegs<D, INT8> &t, const DecodePara
         // valid key's row, whose finite values meet p = 0 (never stale memory that could
         // hold NaN).
         const long long r0 = rm.row_s(rm.pos(j));
-        const int last = rm.last(rm.pos(j));
+        int last;
+        if constexpr (std::is_same_v<Map, WindowMap>) last = rm.last_key(j);
+        else last = rm.last(rm.pos(j));
         uint32_t kr = (uint32_t)min(r16, last);
         uint32_t vr[KPL];
 #pragma unroll
         for (int e = 0; e < KPL; e++) vr[e] = (uint32_t)min(vg * KPL + e, last);
         if constexpr (std::is_same_v<Map, WindowMap>) {
-            const uint32_t first = (uint32_t)rm.first_key(rm.pos(j));
+            const uint32_t first = (uint32_t)rm.first_key(j);
             kr = max(kr, first);
 #pragma unroll
             for (int e = 0; e < KPL; e++) vr[e] = max(vr[e], first);
@@ -429,7 +440,8 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
     const auto rm = [&] {
         if constexpr (GROUP) return GroupMap{reinterpret_cast<const int2 *>(smem_raw), p.P, p.pshift, p.Hk, h, len};
         else if constexpr (WIN)
-            return WindowMap{{p.bt + (size_t)b * p.bt_stride, p.P, p.pshift, p.Hk, h, p.num_pages, len, p.bt_stride}, wt, p.sinks};
+            return WindowMap(RowMap{p.bt + (size_t)b * p.bt_stride, p.P, p.pshift, p.Hk, h, p.num_pages, len, p.bt_stride}, wt, p.window,
+                             p.sinks);
         else return RowMap{p.bt + (size_t)b * p.bt_stride, p.P, p.pshift, p.Hk, h, p.num_pages, len, p.bt_stride};
     }();
     // Keys up to mask_from are visible to every row; later tiles need the mask.
@@ -562,9 +574,8 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
         // with every larger max (p <= 1, so p times a value scale stays within fp16).
         bool need_mask = (WIN ? rm.pos(j + NT - 1) + 16 : (j + NT) * 16) - 1 > mask_from;
         if constexpr (WIN) {
-            // tiles in front of the last row's window, and those of sinks that end inside one
 #pragma unroll
-            for (int n = 0; n < NT; n++) need_mask |= rm.pos(j + n) < len - p.window && rm.pos(j + n) + 15 >= p.sinks;
+            for (int n = 0; n < NT; n++) need_mask |= rm.masked(j + n);
         }
         s16x4 pop[NT][ROWB];
         float x[ROWB][4 * NT], mt[ROWB];

@@ -283,20 +283,17 @@ prefill_pp_kernel(PPParams p) {
     auto store_k = [&](const Chunk &r, int buf, int u, int x) {
         *reinterpret_cast<u32x4 *>(&sm.k[buf][(ckey + KPU * u) * KROW + cch * 8]) = bf16_chunk(r, FP8 ? scale_of(sc8[x].k, u) : 1.0f);
     };
-    // WIN: keys that no row of the work-group sees
-    auto hidden = [&](int key) { return WIN & (key < wt.lo) & (key >= p.sinks); };
     auto store_v = [&](const Chunk &r, int buf, int j, int u) {
         // Keys past kend in the last tile may hold any bits (even NaN) of an allocated
         // page: their probabilities are 0 and their values must be finite. Branch-free,
         // so the stage registers are never rewritten while loads are pending.
-        const int key = tile(j) * KT + ckey + KPU * u;
-        const uint32_t keep = key < kend && !hidden(key) ? ~0u : 0u;
+        const uint32_t keep = tile(j) * KT + ckey + KPU * u < kend ? ~0u : 0u;
         *reinterpret_cast<u32x4 *>(&sm.v[buf][(ckey + KPU * u) * VROW + cch * 8]) = bf16_chunk(r, FP8 ? scale_of(sc8[0].v, u) : 1.0f) & keep;
     };
     const float smul = kg ? 1.0f : p.scale_log2;
     auto store_s = [&](float r, int j) {
         // scales of keys past kend may hold any bits too: zero
-        if (w == (KS ? 4 * team : 0)) sm.s[j & 3][lane] = tile(j) * KT + r32 < kend && !hidden(tile(j) * KT + r32) ? r * smul : 0.0f;
+        if (w == (KS ? 4 * team : 0)) sm.s[j & 3][lane] = tile(j) * KT + r32 < kend ? r * smul : 0.0f;
     };
 
     // Query rows (B operand of S^T = K Q^T): wave w holds rows 32 w .. 32 w + 31 (KS: both
