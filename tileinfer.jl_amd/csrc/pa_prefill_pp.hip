@@ -219,7 +219,7 @@ prefill_pp_kernel(PPParams p) {
     struct Scales {
         float k[NH], v[NH];
     };
-    Scales sc8[5];   // of tiles i .. i + 4
+    Scales sc8[4];   // of tiles i .. i + 3
     const long long half_b = (long long)p.num_pages * p.Hk;
     auto scales = [&](const Pages &r) {
         Scales o;
@@ -523,10 +523,6 @@ prefill_pp_kernel(PPParams p) {
                         store_s(ss[S], i + 2);
                     } else if constexpr (X < O_LV) {
                         b4.e[X - O_BA] = bases(raw4, i + 4).e[X - O_BA];
-                        if constexpr (FP8) {
-                            const Scales n = scales(raw4);
-                            sc8[4].k[X - O_BA] = n.k[X - O_BA], sc8[4].v[X - O_BA] = n.v[X - O_BA];
-                        }
                     } else if constexpr (X < O_LK) {
                         load_v(sv[SV][X - O_LV], bs[LV], X - O_LV);
                     } else if constexpr (X < O_LS) {
@@ -541,14 +537,19 @@ prefill_pp_kernel(PPParams p) {
             __builtin_amdgcn_sched_barrier(0);
         });
         bs[1] = bs[2], bs[2] = bs[3], bs[3] = b4;
-        if constexpr (FP8) sc8[0] = sc8[1], sc8[1] = sc8[2], sc8[2] = sc8[3], sc8[3] = sc8[4];
+        if constexpr (FP8) sc8[0] = sc8[1], sc8[1] = sc8[2], sc8[2] = sc8[3];
     };
     auto phase_y = [&](int i) {
+        if constexpr (FP8) sc8[3] = scales(raw4);   // tile i + 4's
         raw4 = pages_at(tile(i + 5));
         softmax(i);
         // the lookup's wait falls here, where the barrier waits for LDS anyway
         asm volatile("" : "+s"(raw4.pg[0]));
         if constexpr (NH == 2) asm volatile("" : "+s"(raw4.pg[NH - 1]));
+        if constexpr (FP8) {
+#pragma unroll
+            for (int x = 0; x < NH; x++) asm volatile("" : "+s"(sc8[3].k[x]), "+s"(sc8[3].v[x]));
+        }
     };
 
     phase_barrier();
@@ -768,6 +769,7 @@ int ti_pick_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, int pat
     if (T > 65535) return dense128 && 256 % G == 0 ? TI_PP_SHARED : TI_PP_NONE;
     long long W = T * pairs;
     long long tiles = bound_keys ? ((long long)a->block_table_stride * P + 31) / 32 : 1LL << 40;
+    const long long held_tiles = tiles;
     if (win.size) tiles = std::min(tiles, window_tiles(win, TQ));
     // Only here does the four-wave plan split keys, and only from 32 tiles: a workspace query
     // (unbounded tiles) that answers KSPLIT is right for narrower tables too.
@@ -788,7 +790,21 @@ int ti_pick_prefill_pp(const ti_attention_args *a, const ti_kv_cache *c, int pat
         return tiles > 40 && (D == 128 || a->num_seqs == 1) ? TI_PP_KSPLIT : TI_PP_NONE;
     }
     if ((D == 64 && W <= 512 ? held : W) < (128 % G == 0 ? 129 : tiles <= 40 ? 176 : 160)) return TI_PP_NONE;
-    if (W <= 512) return TI_PP_KSPLIT;
+    if (W <= 512) {
+        // With a window, and over 8-bit block caches (whose tiles SHARED converts once for twice the rows), the 256 CUs hold
+        // one round of SHARED's work-groups; KSPLIT's second round, of the lighter q-tiles, is as long as the first where
+        // these are not light. The lighter ones' keys against the heaviest's, with contexts as long as the tables hold
+        // (tables wider than sixteen steps say nothing: none): from 0.7 on SHARED (8-bit 1500 on 3000 128.6 -> 115.7 us,
+        // 1500 on 1000, 0.61, 67.1 against 69.3; 2000 tokens with a window of 1024 46.7 -> 39.1, 1500, 0.47, 33.3 against
+        // 36.6). Several sequences go one after the other, heavy q-tiles in the second round too: SHARED (2 x 600 on 2000
+        // 84.9 -> 72.3, 1200 on 8000 274 -> 224, 5 x 350 on 1000 59.4 -> 46.3; 2 x 800 29.6 against 30.2), but for short ones (12 x 130 86 against 119).
+        if (W > 256 && dense128 && T > 6 && (win.size || c->kind == TI_KV_FP8)) {
+            const long long wide = 32 * held_tiles > 16 * n ? n : std::max(32 * held_tiles, n), cap = win.size ? win.size + TQ : wide;
+            const long long rest = std::max(0LL, T - 256 / pairs) * TQ;   // queries of the second round
+            if (a->num_seqs > 1 || 10 * std::min(cap, wide - n + rest) > 7 * std::min(cap, wide)) return TI_PP_SHARED;
+        }
+        return TI_PP_KSPLIT;
+    }
     const bool padded = a->num_seqs >= 8 && W > 1024 && ((T <= 24 && tiles <= 40) || 4 * held < W);
     return dense128 && T > 6 && !padded ? TI_PP_SHARED : TI_PP_SOLO;
 }
