@@ -259,3 +259,39 @@ def test_noalloc_and_graphs(gpu):
             ti.store_kv_(BE, k, v, new, new, n)
             ti.paged_attention_(BE, again, ws, q, k, v, tables, positions, s.scale, True, starts, s.most)
             assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("T", [torch.bfloat16, torch.float32])
+def test_tensors_aligned_to_their_elements_only(gpu, T):
+    def shifted(t):
+        room = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        room[1:].copy_(t.reshape(-1))
+        return room[1:].view(t.shape)
+
+    g = np.random.Generator(np.random.PCG64(8))
+    D, P, H = 128, 16, 2
+    for n in (1, 40, 600):
+        k, v = pools(D, P, H, 40, g)
+        q, scale = k.layer_q.cpu().numpy(), k.layer_scale.cpu().numpy()
+        x, y = rows(g, n, H, D, T), rows(g, n, H, D, T)
+        at = list(g.permutation(40 * P)[:n] + 1)
+        ti.store_kv_(BE, k, v, shifted(x), shifted(y), shifted(i32(at)))
+        store(q, scale, x.float().numpy(), y.float().numpy(), at)
+        same(k, q, scale)
+
+
+def test_positions_that_no_table_holds(gpu):
+    for lens in ([(100, 1), (50, 1)], [(100, 5), (50, 5)], [(100, 60), (50, 60)]):
+        s = Step("fp8", lens, seed=13)
+        want, size = s.want()
+        n = lens[0][1]
+        k, v = s.layer.device()
+        q = s.q.cuda()
+        for first in (2 ** 31 - 1, 10 ** 6):
+            s.positions[0] = first
+            tables, positions, starts = s.args()
+            out = torch.zeros_like(q)
+            ws = ti.attention_workspace(BE, q, k, 2, n)
+            ti.paged_attention_(BE, out, ws, q, k, v, tables, positions, s.scale, True, starts, n)
+            torch.cuda.synchronize()
+            check(out[n:], want[n:], size[n:], s.T)

@@ -222,3 +222,53 @@ def test_same_result_twice(gpu):
         s = Step(kv, [(700, 3), (200, 130), (0, 40)], 100, 4, seed=10)
         a, b = run(s), run(s)
         assert torch.equal(a, b)
+
+
+def test_rows_of_large_values_that_no_query_sees(gpu):
+    """Hidden rows of a tile at a window's edge, finite and huge: no row-by-row path, no trace of them."""
+    for kv, lens in (("bf16", [(200, 9), (90, 1)]), ("fp32", [(200, 9), (90, 1)]), ("fp8", [(200, 9), (90, 1)]), ("bf16", [(0, 200)]),
+                     ("fp8", [(60, 200)]), ("fp32", [(60, 200)])):
+        s = Step(kv, lens, 37, 3, seed=12)
+        want = s.want()
+        big = 3e4 if kv != "fp8" else 448.0
+        for x, half in ((s.layer.k, 0), (s.layer.v, 1)):
+            x[np.isnan(x)] = big
+            if kv == "fp8":
+                s.layer.q[half][s.layer.q[half] == 127] = 126
+        if kv == "fp8":
+            s.layer.scale[np.isnan(s.layer.scale)] = 2.0 ** 100
+        check(run(s), *want, s.T)
+
+
+def test_positions_that_no_table_holds(gpu):
+    """Positions out of contract: every access stays inside, and the call ends; the other sequences are right."""
+    for kv in KINDS:
+        for n in (1, 5, 40):
+            s = Step(kv, [(100, n), (50, n)], 30, 2, seed=13)
+            want, size = s.want()
+            s.positions[:n] = np.resize([2 ** 31 - 1, 2 ** 30, 10 ** 6, -2 ** 31], n)
+            for first in (2 ** 31 - 1, 10 ** 6):
+                s.positions[0] = first
+                got = run(s)
+                torch.cuda.synchronize()
+                check(got[n:], want[n:], size[n:], s.T)
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("lens", [[(300, 1)], [(100, 6), (40, 2)], [(30, 150)], [(100, 700)]])
+def test_tensors_aligned_to_their_elements_only(gpu, kv, lens):
+    def shifted(t):
+        room = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        room[1:].copy_(t.reshape(-1))
+        return room[1:].view(t.shape)
+
+    s = Step(kv, lens, 64, 4, seed=14)
+    k, v = s.layer.device()
+    if kv in ("bf16", "fp32"):
+        k, v = shifted(k), shifted(v)
+    tables, positions, starts = (shifted(t) for t in s.args())
+    q = shifted(s.q.cuda())
+    out = shifted(torch.zeros_like(q))
+    ws = ti.window_attention_workspace(BE, q, k, 64, 4, len(lens), s.most)
+    ti.window_attention_(BE, out, ws, q, k, v, tables, positions, s.scale, 64, 4, starts, s.most)
+    check(out, *s.want(), s.T)

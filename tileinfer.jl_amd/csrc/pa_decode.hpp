@@ -89,14 +89,14 @@ struct DecodeParams {
 struct FlatPiece {
     int b, lo, n, tok0, nb, start;
 };
-template <bool WIN = false>
+template <bool SAFE = false, bool WIN = false>
 __device__ inline FlatPiece flat_piece(const DecodeParams &p, int x, int lane) {
     int tok0 = 0, nb = 0, st = 0, nt = 0;
     if (lane < p.B) {
         tok0 = p.qsl ? p.qsl[lane] : lane * p.nmax;
         nb = p.qsl ? min(p.qsl[lane + 1] - tok0, p.nmax) : p.nmax;
         if (nb > 0) {
-            st = max(p.positions[tok0], 0);
+            st = SAFE ? first_position(p.positions[tok0], p.bt_stride, p.P) : max(p.positions[tok0], 0);
             nt = (st + nb + 15) >> 4;
             if constexpr (WIN) nt -= WindowTiles::of<4>(st, p.window, p.sinks).skip;
         }
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
             return;
         }
     } else if (p.flat) {
-        const FlatPiece f = flat_piece<WIN>(p, blockIdx.x, lane);
+        const FlatPiece f = flat_piece<SAFE, WIN>(p, blockIdx.x, lane);
         b = f.b;
         s = blockIdx.x - f.lo;
         nsp = f.n;
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
         tok0 = p.qsl ? p.qsl[b] : b * p.nmax;
         nb = p.qsl ? min(p.qsl[b + 1] - tok0, p.nmax) : p.nmax;   // at most max_query_len
         if (nb <= 0) return;
-        start = max(p.positions[tok0], 0);   // a negative position reads as 0
+        start = SAFE ? first_position(p.positions[tok0], p.bt_stride, p.P) : max(p.positions[tok0], 0);   // a negative position reads as 0
         unit = ((size_t)b * p.Hk + h) * p.splits + s;
     }
     const int q0 = GROUP && p.qsl ? max(p.qsl[0], 0) : 0, q1 = GROUP ? (p.qsl ? min(p.qsl[p.B], p.total) : p.total) : 0;

@@ -57,7 +57,8 @@ __global__ void __launch_bounds__(64) generic_attention_kernel(GenericParams p) 
         tok0 = p.qsl ? p.qsl[b] : b * p.nmax;
         const int nb = p.qsl ? min(p.qsl[b + 1] - tok0, p.nmax) : p.nmax;   // at most max_query_len
         if (t >= nb) return;
-        const int start = max(p.positions[tok0], 0);   // a negative position reads as 0
+        // a negative position reads as 0
+        const int start = FP8 || WIN ? first_position(p.positions[tok0], p.bt_stride, p.P) : max(p.positions[tok0], 0);
         len = start + nb;
         last = p.causal ? start + t : len - 1;
     }
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         tok0 = p.qsl ? p.qsl[b] : b * p.nmax;
         nb = p.qsl ? min(p.qsl[b + 1] - tok0, p.nmax) : p.nmax;   // at most max_query_len
         if (t_first >= nb) return;   // the q-tile holds no token of this sequence
-        start = max(p.positions[tok0], 0);   // a negative position reads as 0
+        start = WIN ? first_position(p.positions[tok0], p.bt_stride, p.P) : max(p.positions[tok0], 0);   // a negative position reads as 0
     }
     int len = start + nb;
     const int q0 = GROUP && p.qsl ? max(p.qsl[0], 0) : 0, q1 = GROUP ? (p.qsl ? min(p.qsl[p.B], p.total) : p.total) : 0;

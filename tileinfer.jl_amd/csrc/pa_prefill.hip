@@ -394,7 +394,10 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
     if constexpr (DL && !WIN) {
         if (p.splits == 1) spec = raw_pages(p, bt, grp);
     }
-    const int start = max(sload(p.positions, nb > 0 ? tok0 : 0), 0), len = start + nb;   // a negative position reads as 0
+    // a negative position reads as 0
+    const int start = FP8 || WIN ? first_position(sload(p.positions, nb > 0 ? tok0 : 0), p.bt_stride, p.P)
+                                 : max(sload(p.positions, nb > 0 ? tok0 : 0), 0);
+    const int len = start + nb;
     const int qpos = p.causal && row_ok ? start + t : len - 1;
     const int t_last = min(t_first + p.TQ, nb) - 1;
     const int kend = p.causal ? start + t_last + 1 : len;
@@ -1400,7 +1403,8 @@ ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c
     // 512-token prefill and 25.6 -> 23.3 us chunked, bit-identical; for four-wave groups
     // (1024-3072 tokens) no change, so those keep the register-staged loads.
     const bool dl_ok = c->kind == TI_KV_DENSE && a->dtype == TI_BF16 && c->head_dim == 128 &&
-                       c->page_size >= 16 && (c->page_size & (c->page_size - 1)) == 0;
+                       c->page_size >= 16 && (c->page_size & (c->page_size - 1)) == 0 &&
+                       (!win.size || (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15) == 0);
     pl.dl = dl_ok && (a->path == TI_PATH_PREFILL_DIRECT || a->path == TI_PATH_PREFILL_PAIRED ||
                       a->path == TI_PATH_PREFILL_PAIRED16 ||
                       (a->path != TI_PATH_PREFILL_STAGED && pl.wpg == 2));

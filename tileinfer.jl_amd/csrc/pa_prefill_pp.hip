@@ -178,7 +178,9 @@ prefill_pp_kernel(PPParams p) {
     const int nb = p.qsl ? min(sload(p.qsl, b + 1) - tok0, p.nmax) : p.nmax;   // at most max_query_len
     const int t_first = qt * p.TQ;
     if (t_first >= nb) return;
-    const int start = max(sload(p.positions, tok0), 0), len = start + nb;   // a negative position reads as 0
+    // a negative position reads as 0
+    const int start = FP8 || WIN ? first_position(sload(p.positions, tok0), p.bt_stride, p.P) : max(sload(p.positions, tok0), 0);
+    const int len = start + nb;
     const int t_last = min(t_first + p.TQ, nb) - 1;
     const int kend = p.causal ? start + t_last + 1 : len;
     int nkt = (kend + KT - 1) / KT;

@@ -19,6 +19,12 @@
 
 namespace ti {
 
+// The position of a sequence's first query: a negative one reads as 0, one past all that its block-table row can hold as
+// that, so that no count of keys leaves 32 bits and no loop runs on for what no table names.
+__device__ __forceinline__ int first_position(int position, int bt_stride, int P) {
+    return (int)min((long long)max(position, 0), min((long long)bt_stride * P, 1LL << 30));
+}
+
 // Tiles of 2^SHIFT keys that the rows from position `first` on see: `sunk` of them from the cache's start, the others
 // `skip` further on.
 struct WindowTiles {
