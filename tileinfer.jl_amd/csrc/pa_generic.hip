@@ -210,6 +210,9 @@ constexpr int F32_MIN_TILES = 4;
 // table row and a length each (pa_sparse.hip), 1-D grid of the pairs' splits. GROUP (SPARSE): p.tg
 // neighbouring tokens' pairs at a time over the joined list of their pages (pa_group.hpp), packed rows g + G t.
 // WIN: the window of pa_window.hpp; the splits cut the list of tiles that it leaves for the q-tile, and each writes a partial.
+// Values come in 16-byte loads there: MFMA (e, 4 B + c) takes V[key 4 kg + e][64 B + 4 r16 + c], so that block's row i is
+// element 64 B + 4 i + c (512 tokens on 2000 with a window of 512, 16 / 8 heads: 34.4 -> XX us; 32 4-byte loads a tile kept
+// the CU's address units busy).
 template <int D, bool QT, bool SPARSE = false, bool GROUP = false, bool WIN = false>
 __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     constexpr int NJ = D / 16, NDB = D / 16, NW = 4, MROW = D + 4;
@@ -312,7 +315,7 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     const int32_t *bt = p.bt + (size_t)b * p.bt_stride;
     struct Tile {
         f32x4 k[NJ];
-        float v[4][NDB];
+        float v[4][NDB];   // WIN: block 4 B + c at [e][4 B + c]
     };
     auto load = [&](int j, Tile &tl) {
         const int pos0 = (WIN ? wt.tile(j) : j) * 16;
@@ -336,7 +339,17 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
         for (int jj = 0; jj < NJ; jj++) tl.k[jj] = *reinterpret_cast<const f32x4 *>(krow + 16 * jj);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float *vrow = p.vp + (rbase + (WIN ? max(min(4 * kg + e, last), first) : min(4 * kg + e, last))) * D + r16;
+            if constexpr (WIN) {
+                const float *vrow = p.vp + (rbase + max(min(4 * kg + e, last), first)) * D + 4 * r16;
+#pragma unroll
+                for (int B = 0; B < D / 64; B++) {
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(vrow + 64 * B);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) tl.v[e][4 * B + c] = x[c];
+                }
+                continue;
+            }
+            const float *vrow = p.vp + (rbase + min(4 * kg + e, last)) * D + r16;
 #pragma unroll
             for (int db = 0; db < NDB; db++) tl.v[e][db] = vrow[16 * db];
         }
@@ -418,8 +431,17 @@ __global__ void __launch_bounds__(256) attn_f32_kernel(F32Params p) {
     if constexpr (GROUP) __syncthreads();   // the joined list is read
     {
         float *my = slab + ((size_t)w * 16 + r16) * MROW;
+        if constexpr (WIN) {
 #pragma unroll
-        for (int db = 0; db < NDB; db++) *reinterpret_cast<f32x4 *>(my + 16 * db + 4 * kg) = o[db];
+            for (int B = 0; B < D / 64; B++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    *reinterpret_cast<f32x4 *>(my + 64 * B + 16 * kg + 4 * e) =
+                        (f32x4){o[4 * B][e], o[4 * B + 1][e], o[4 * B + 2][e], o[4 * B + 3][e]};
+        } else {
+#pragma unroll
+            for (int db = 0; db < NDB; db++) *reinterpret_cast<f32x4 *>(my + 16 * db + 4 * kg) = o[db];
+        }
         if (kg == 0) {
             my[D] = m;
             my[D + 1] = l;

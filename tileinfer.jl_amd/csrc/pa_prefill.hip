@@ -884,7 +884,7 @@ __device__ __forceinline__ void lds_dma16_v(const void *gptr, uint32_t lds) {
 }
 
 // Paired q-tiles on 16-row waves (bf16 activations, D = 128, pages of 2^k >= 16 tokens,
-// causal, no key splits; dense bf16 cache, or INT8 with INT8 = true). The work of the paired
+// causal, no key splits; dense bf16 cache, INT8 or 8-bit blocks). The work of the paired
 // kernel above — work-group y holds the
 // heavy q-tile qtiles - 1 - y and the light q-tile y, four key groups walk the key tiles
 // through their own double-buffered LDS tiles and merge at the end — with each q-tile's 32
@@ -906,9 +906,10 @@ __device__ __forceinline__ void lds_dma16_v(const void *gptr, uint32_t lds) {
 // and the softmax, and only then reads the values, so key and value operands never occupy
 // registers together. The pair's 64 query rows come through LDS (one direct load per lane),
 // read once into registers after the first tile lands.
-template <bool INT8>
+template <bool INT8, bool FP8 = false>
 __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     constexpr int D = 128, NG = 4, NQB = D / 32, NDB = D / 16;
+    constexpr bool B8 = INT8 || FP8;     // staged through registers
     constexpr int HW = 2, NQ = 2;        // direct loads: waves per 16-key page half, instructions per wave
     constexpr int RPG = 64, MROW = D + 4;
     // a key group's tiles (bf16, swizzled rows) and, for an INT8 cache, their scales
@@ -941,11 +942,13 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     // (dense: a wave loads one 16-key half of each tile, dx, and looks up that half alone)
     const int dx = wl / HW;
     auto raw_half = [&](int kt, int half) { return sload(bt, min((kt * KT + 16 * half) >> p.pshift, p.bt_stride - 1)); };
-    const int spec = INT8 ? 0 : raw_half(grp, dx);
-    const TilePages spec_both = INT8 ? raw_pages(p, bt, grp) : TilePages{};
+    const int spec = B8 ? 0 : raw_half(grp, dx);
+    const TilePages spec_both = B8 ? raw_pages(p, bt, grp) : TilePages{};
     const int tok0 = p.qsl ? sload(p.qsl, b) : b * p.nmax;
     const int nb = p.qsl ? min(sload(p.qsl, b + 1) - tok0, p.nmax) : p.nmax;
-    const int start = max(sload(p.positions, nb > 0 ? tok0 : 0), 0), len = start + nb;
+    const int start = FP8 ? first_position(sload(p.positions, nb > 0 ? tok0 : 0), p.bt_stride, p.P)
+                          : max(sload(p.positions, nb > 0 ? tok0 : 0), 0);
+    const int len = start + nb;
     const int t_first = qt * p.TQ;
     // No early exit for a pair past the sequence's queries (a shorter sequence of a ragged
     // batch): a branch here would let the compiler sink the scalar loads above past it, behind
@@ -1002,7 +1005,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     // Tile grp is whole for any start when the q-tile's last position alone reaches past it
     // (the step's keys end at start + t_last + 1 >= t_last + 1): its loads then go out before
     // the positions load returns.
-    const bool first_full = !INT8 && min(t_first + p.TQ, nb) - 1 - grp * KT >= KT - 1;
+    const bool first_full = !B8 && min(t_first + p.TQ, nb) - 1 - grp * KT >= KT - 1;
     if (first_full) dl_full(grp, 0, spec);
     u32x4 qreg[NQB];
     const int qpos = p.causal && row_ok ? start + t : len - 1;
@@ -1056,7 +1059,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     const size_t half_q = (size_t)p.num_pages * p.Hk * p.P * D;
     const size_t half_s = (size_t)p.num_pages * p.Hk * p.P;
     u32x4 stk = {0u, 0u, 0u, 0u}, stv = {0u, 0u, 0u, 0u};
-    float sts = 0.0f;
+    float sts = 0.0f, stw = 0.0f;   // FP8: the keys' and the values' scale
     auto i8_row = [&](int kt, int key, const TilePages &tp) -> long long {
         const int pos0 = kt * KT, kk = min(key, kend - 1 - pos0);
         const int pg = clamp_page(kk >> 4 ? tp.pg[1] : tp.pg[0], p.num_pages);
@@ -1066,7 +1069,12 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
         const long long row = i8_row(kt, key_l, tp);
         stk = *reinterpret_cast<const u32x4 *>(p.lq + row * D + 16 * part);
         stv = *reinterpret_cast<const u32x4 *>(p.lq + half_q + row * D + 16 * part);
-        if (gl < 2 * KT) {
+        if constexpr (FP8) {
+            // the scales of the wave's keys, all of one page half: vector loads, which no LDS read waits for
+            const float *sp = p.ls + (row >> p.pshift);
+            sts = *sp;
+            stw = sp[(size_t)p.num_pages * p.Hk];
+        } else if (gl < 2 * KT) {
             const long long srow = i8_row(kt, gl & (KT - 1), tp);
             sts = p.ls[(gl < KT ? 0 : half_s) + srow];
         }
@@ -1075,6 +1083,12 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
 #pragma unroll
         for (int c2 = 0; c2 < 2; c2++) {
             const int c = 2 * part + c2;
+            if constexpr (FP8) {
+                const int vs = c ^ (4 * (key_l & 3)) ^ (2 * ((key_l >> 2) & 1));
+                *reinterpret_cast<u32x4 *>(&dsm.k[buf][key_l * D + ((c ^ (key_l & 15)) * 8)]) = e4m3x8_to_bf16(stk[2 * c2], stk[2 * c2 + 1], sts);
+                *reinterpret_cast<u32x4 *>(&dsm.v[buf][key_l * D + vs * 8]) = e4m3x8_to_bf16(stv[2 * c2], stv[2 * c2 + 1], stw);
+                continue;
+            }
             uint32_t a0, a1, a2, a3;
             i8x4_to_bf16(stk[2 * c2], a0, a1);
             i8x4_to_bf16(stk[2 * c2 + 1], a2, a3);
@@ -1084,6 +1098,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
             const int vs = c ^ (4 * (key_l & 3)) ^ (2 * ((key_l >> 2) & 1));
             *reinterpret_cast<u32x4 *>(&dsm.v[buf][key_l * D + vs * 8]) = (u32x4){a0, a1, a2, a3};
         }
+        if (FP8) return;
         if (gl < KT) dsm.sk[buf][gl] = sts;
         else if (gl < 2 * KT) dsm.sv[buf][gl - KT] = sts;
     };
@@ -1169,8 +1184,8 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     // a sequence with no query in the step and no key before it (nkt = 0) looks up tile 0, which
     // nothing uses
     const int last_tile = max(nkt - 1, 0), ft = min(tile_of(0), last_tile);
-    int page = ft == grp ? spec : INT8 ? 0 : raw_half(ft, dx);                             // dense
-    TilePages pages = ft == grp ? spec_both : INT8 ? raw_pages(p, bt, ft) : TilePages{};   // INT8
+    int page = ft == grp ? spec : B8 ? 0 : raw_half(ft, dx);                             // dense
+    TilePages pages = ft == grp ? spec_both : B8 ? raw_pages(p, bt, ft) : TilePages{};   // INT8, FP8
     // A step issues the next tile's loads first and looks up the page ids of the tile after
     // at its end (next_pages), so the scalar loads' wait falls on the step's closing barrier
     // instead of on its LDS reads (both are counted by lgkmcnt).
@@ -1180,7 +1195,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     auto next_pages = [&](int i) {
         if (i < steps) page = raw_half(min(tile_of(i), last_tile), dx);
     };
-    if constexpr (!INT8) {
+    if constexpr (!B8) {
         if (!first_full) issue(0, 0);
         next_pages(1);
     } else {
@@ -1209,7 +1224,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
             if (!row_ok) qreg[i] = (u32x4){0u, 0u, 0u, 0u};
         }
     }
-    if constexpr (!INT8) {
+    if constexpr (!B8) {
         for (int i = 0; i < steps; i += 2) {
             if (i > 0) {
                 wait_direct_loads();
@@ -1252,6 +1267,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     }
     __syncthreads();
     constexpr int NT = 1024, IT = RPG * (D / 4) / NT;
+    bool fine = true;   // FP8
     float2 ml[IT][NG];
     f32x4 dv[IT][NG];
 #pragma unroll
@@ -1282,10 +1298,30 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
             acc += dv[it][gi] * wgt;
         }
         if (ttl >= p.TQ || tt >= nb) continue;
+        if constexpr (FP8) {
+            fine &= fabsf(lsum) < INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4; e++) fine &= fabsf(acc[e]) < INFINITY;
+        }
         const float inv = 1.0f / lsum;
         uint16_t *orow = p.out + ((size_t)(tok0 + tt) * p.Hq + h * p.G + gg) * D + d4;
         *reinterpret_cast<u32x2 *>(orow) = (u32x2){pack_bf16x2(acc[0] * inv, acc[1] * inv),
                                                    pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+    }
+    if constexpr (FP8) {
+        // a product that is not finite: the pair's rows once more, each over the keys that it sees
+        if (__syncthreads_or(!fine)) {
+            for (int x = w; x < RPG; x += 16) {
+                const int rl = x % 32, tt = (x / 32 ? qt_light : qt) * p.TQ + (rl >> p.gshift);
+                if ((rl >> p.gshift) >= p.TQ || tt >= nb || (x >= 32 && qt_light == qt)) continue;
+                const size_t qrow = (size_t)(tok0 + tt) * p.Hq + h * p.G + (rl & (p.G - 1));
+                const int last = p.causal ? start + tt : len - 1;
+                float xm, xl, acc[D / 64];
+                exact_row<D, false, true>(p, bt, h, p.q + qrow * D, 0, nkt * KT, [&](int key) { return key <= last ? key : -1; }, xm, xl, acc);
+#pragma unroll
+                for (int k = 0; k < D / 64; k++) Elt<uint16_t>::st(p.out, qrow * D + lane + 64 * k, acc[k] / xl);
+            }
+        }
     }
 }
 
@@ -1419,8 +1455,8 @@ ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c
     // than 128 work-groups of 128 rows have gone to a ping-pong form before this
     // (ti_pick_prefill_pp). The 32-row paired kernel (pinned with TI_PATH_PREFILL_PAIRED)
     // needs the plan's two-wave, four-group shape.
-    // (INT8 caches pair on the 16-row kernel only, its tiles staged through registers)
-    const bool i8_ok = c->kind == TI_KV_INT8 && a->dtype == TI_BF16 && c->head_dim == 128 &&
+    // (INT8 and 8-bit block caches pair on the 16-row kernel only, its tiles staged through registers)
+    const bool i8_ok = c->kind != TI_KV_DENSE && a->dtype == TI_BF16 && c->head_dim == 128 &&
                        c->page_size >= 16 && (c->page_size & (c->page_size - 1)) == 0;
     const bool pair_ok = (dl_ok || i8_ok) && a->causal && pl.splits == 1 && 32 % G == 0 && !win.size;
     // (32 % G == 0 in pair_ok: G <= 32, so 32 / G >= 1)
@@ -1472,7 +1508,8 @@ int ti_launch_prefill(const ti_attention_args *a, const ti_kv_cache *c, const ti
     const int wpg = pl.wpg, ng = pl.ng;
     dim3 grid(c->kv_heads, pl.pair ? (p.qtiles + 1) / 2 : p.qtiles * pl.splits, a->num_seqs);
     if (pl.r16) {
-        if (c->kind == TI_KV_INT8) prefill16_kernel<true><<<grid, 1024, 0, s>>>(p);
+        if (c->kind == TI_KV_FP8) prefill16_kernel<false, true><<<grid, 1024, 0, s>>>(p);
+        else if (c->kind == TI_KV_INT8) prefill16_kernel<true><<<grid, 1024, 0, s>>>(p);
         else prefill16_kernel<false><<<grid, 1024, 0, s>>>(p);
         return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
     }
