@@ -272,3 +272,61 @@ def test_tensors_aligned_to_their_elements_only(gpu, kv, lens):
     ws = ti.window_attention_workspace(BE, q, k, 64, 4, len(lens), s.most)
     ti.window_attention_(BE, out, ws, q, k, v, tables, positions, s.scale, 64, 4, starts, s.most)
     check(out, *s.want(), s.T)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("lens,at", [([(0, 200)], 77), ([(100, 130), (0, 33)], 160), ([(1000, 500)], 1400)])
+def test_rows_that_only_later_queries_see(gpu, kv, half, value, lens, at):
+    """A window over all that the tables hold: the rows in front of a row that is not finite are as without it."""
+    window = 1 << 20
+    s = Step(kv, lens, window, 0, seed=15)
+    want, size = s.want()
+    s.layer.put(half, int(s.tables[0][at // s.P]) - 1, 1, at % s.P, value)
+    got = run(s).double().cpu().numpy()
+    c, n = lens[0]
+    hit = np.zeros(got.shape[:2], bool)
+    hit[at - c:n, s.G:2 * s.G] = True
+    from window_ref import tolerance
+    assert np.isfinite(got[~hit]).all()
+    assert (np.abs(got - want)[~hit] <= tolerance(s.T, want, size)[~hit]).all()
+    if half == 1:
+        assert not np.isfinite(got[hit]).any()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8", "fp8"])
+@pytest.mark.parametrize("G", [1, 2, 3, 4, 32])
+@pytest.mark.parametrize("lens", [[(0, 512)], [(1000, 200), (0, 0), (17, 65)], [(0, 33)] * 5])
+def test_windows_over_whole_tables(gpu, kv, G, lens):
+    """No key hidden but the later ones: the steps that run on other kernels than with hidden keys, and agree with them."""
+    s = Step(kv, lens, 1 << 20, 0, G=G, seed=16)
+    want = s.want()
+    check(run(s), *want, s.T)
+    most = max(c + n for c, n in lens)
+    check(run(s, window=most), *want, s.T)      # the tables reach past the window, no query does
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [1, 5, 40, 300, 2000])
+@pytest.mark.parametrize("window,G", [(40, 4), (1 << 20, 4), (700, 1)])
+def test_queries_over_int8_caches_keep_11_bits(gpu, D, n, window, G):
+    """Two keys of scores 64 and 64 (1 + 2^-9): half of the smoothing is 1 + 2^-9, which times a query of 1 has 10 bits, and
+    bf16 holds 8. Their weights are to each other as 1 to e^(1/8), their values 1 and -1, so every output is -tanh(1/16);
+    with such queries rounded to 8 bits it were 0. The other keys' scores are 0, their weights e^-64."""
+    H, P, ctx = 2, 64, 70
+    pages = -(-(ctx + n) // P)
+    q8 = np.zeros((2, pages, H, P, D), np.int8)
+    scale = np.full((2, pages, H, P), 1 / 127, np.float32)
+    q8[0, 0, :, 0, :D // 2] = q8[0, 0, :, 1, D // 2:] = 127
+    q8[1, 0, :, 0], q8[1, 0, :, 1] = 127, -127
+    smooth = np.ones(D, np.float32)
+    smooth[D // 2:] += 2.0 ** -9
+    q8, scale, smooth = (torch.from_numpy(x).cuda() for x in (q8, scale, smooth))
+    k, v = ti.Int8Pages(q8, scale, smooth, 0), ti.Int8Pages(q8, scale, torch.ones_like(smooth), 1)
+    q = torch.ones((n, H * G, D), dtype=torch.bfloat16, device="cuda")
+    positions = torch.arange(ctx, ctx + n, dtype=torch.int32, device="cuda")
+    tables = torch.arange(1, pages + 1, dtype=torch.int32, device="cuda")[None]
+    out = ti.window_attention(BE, q, k, v, tables, positions, 128 / D, window, 2).double().cpu()
+    # the weights' rounding and the output's: 2^-8 of (weight times |value|) = 1 and of the output
+    assert float((out + math.tanh(1 / 16)).abs().max()) <= 2.0 ** -8 * (1 + 1 / 16) + 2.0 ** -12

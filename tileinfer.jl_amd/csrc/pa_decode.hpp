@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
                     // bf16(q * smooth) (attention.jl:90-95), kept as float
                     qf[i][2 * e] = __uint_as_float(raw[e] << 16) * p.smooth[d0 + 2 * e];
                     qf[i][2 * e + 1] = __uint_as_float(raw[e] & 0xffff0000u) * p.smooth[d0 + 2 * e + 1];
-                    if constexpr (!SPARSE) {   // SPARSE: rounded once, to fp16's 11 bits
+                    if constexpr (!SPARSE && !WIN) {   // SPARSE, WIN: rounded once, to fp16's 11 bits
                         qf[i][2 * e] = bf2f(f2bf(qf[i][2 * e]));
                         qf[i][2 * e + 1] = bf2f(f2bf(qf[i][2 * e + 1]));
                     }

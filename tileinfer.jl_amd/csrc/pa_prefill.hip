@@ -265,7 +265,7 @@ __device__ __forceinline__ void store_tile(const Stage<D, INT8, GT> &st, Smem<D>
                 kv = e4m3x8_to_bf16(st.k[u][0], st.k[u][1], key & 16 ? sc.k[1] : sc.k[0]);
                 vv = e4m3x8_to_bf16(st.v[u][0], st.v[u][1], key & 16 ? sc.v[1] : sc.v[0]);
             } else {
-                kv = INT8 ? i8x8_to_bf16x8(st.k[u][0], st.k[u][1]) : st.k[u];
+                kv = INT8 && WIN ? i8x8_to_f16x8(st.k[u][0], st.k[u][1]) : INT8 ? i8x8_to_bf16x8(st.k[u][0], st.k[u][1]) : st.k[u];
                 vv = INT8 ? i8x8_to_bf16x8(st.v[u][0], st.v[u][1]) : st.v[u];
             }
             *reinterpret_cast<u32x4 *>(&sm.k[buf][key * Smem<D>::KROW + ch * 8]) = kv;
@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
     // PAIR with an odd count of q-tiles: the middle one pairs with itself (its light wave idles)
     const bool row_ok = tl < p.TQ && t < nb && !(PAIR && wl == 1 && qt_light == qt);
     bf16x8 qreg[NQB];
+    float scale_log2 = p.scale_log2;
     {
         const uint16_t *qr = p.q + ((size_t)(tok0 + (row_ok ? t : 0)) * p.Hq + h * p.G + g) * D;
 #pragma unroll
@@ -378,6 +379,8 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
                 qreg[i] = as_bf16x8((u32x4){0u, 0u, 0u, 0u});
             } else if (!INT8) {
                 qreg[i] = as_bf16x8(*reinterpret_cast<const u32x4 *>(qr + d0));
+            } else if constexpr (INT8 && WIN) {
+                // all elements at once, below
             } else {
                 const u32x4 raw = *reinterpret_cast<const u32x4 *>(qr + d0);
                 u32x4 wv;
@@ -387,6 +390,16 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
                                         __uint_as_float(raw[e] & 0xffff0000u) * p.smooth[d0 + 2 * e + 1]);
                 qreg[i] = as_bf16x8(wv);
             }
+        }
+        if constexpr (INT8 && WIN) {
+            u32x4 raw[NQB];
+#pragma unroll
+            for (int i = 0; i < NQB; i++)
+                raw[i] = row_ok ? *reinterpret_cast<const u32x4 *>(qr + i * 16 + kg * 8) : (u32x4){0u, 0u, 0u, 0u};
+            scale_log2 *= f16_row(raw, p.smooth, [&](int i) { return i * 16 + kg * 8; },
+                                  [](float x) { return fmaxf(x, __shfl_xor(x, 32)); });
+#pragma unroll
+            for (int i = 0; i < NQB; i++) qreg[i] = as_bf16x8(raw[i]);   // bits of fp16
         }
     }
 
@@ -495,7 +508,8 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
         }
 #pragma unroll
         for (int i = 0; i < NQB; i++)
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(ka[i]), qreg[i], sc, 0, 0, 0);
+            sc = INT8 && WIN ? __builtin_amdgcn_mfma_f32_32x32x16_f16(as_f16x8(ka[i]), __builtin_bit_cast(f16x8_t, qreg[i]), sc, 0, 0, 0)
+                             : __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(ka[i]), qreg[i], sc, 0, 0, 0);
         __builtin_amdgcn_sched_group_barrier(0x0100, DL ? NQB + 4 * NDB : NQB, 0);   // all K (and V) reads
 #pragma unroll
         for (int i = 0; i < NQB; i++) {
@@ -536,7 +550,7 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
             x[e] = v;
             mt = fmaxf(mt, v);
         }
-        mt *= p.scale_log2;
+        mt *= scale_log2;
         if (__any(mt > m + RESCALE_LOG2)) {
             mt = fmaxf(mt, __shfl_xor(mt, 32));
             const float mn = fmaxf(m, mt);
@@ -549,7 +563,7 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
         float pe[16], ps = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-            pe[e] = fast_exp2(__builtin_fmaf(x[e], p.scale_log2, -m));
+            pe[e] = fast_exp2(__builtin_fmaf(x[e], scale_log2, -m));
             ps += pe[e];
             if constexpr (INT8) pe[e] *= svq[e >> 2][e & 3];
         }
@@ -906,10 +920,13 @@ __device__ __forceinline__ void lds_dma16_v(const void *gptr, uint32_t lds) {
 // and the softmax, and only then reads the values, so key and value operands never occupy
 // registers together. The pair's 64 query rows come through LDS (one direct load per lane),
 // read once into registers after the first tile lands.
-template <bool INT8, bool FP8 = false>
+// SAFE: rows are done again where a product is not finite (pa_window.hpp): 8-bit block caches, and windows that reach
+// over all that the tables hold.
+template <bool INT8, bool FP8 = false, bool SAFE = FP8>
 __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     constexpr int D = 128, NG = 4, NQB = D / 32, NDB = D / 16;
     constexpr bool B8 = INT8 || FP8;     // staged through registers
+    constexpr bool F16 = INT8 && SAFE;   // fp16 queries and keys (pa_window.hpp)
     constexpr int HW = 2, NQ = 2;        // direct loads: waves per 16-key page half, instructions per wave
     constexpr int RPG = 64, MROW = D + 4;
     // a key group's tiles (bf16, swizzled rows) and, for an INT8 cache, their scales
@@ -946,8 +963,8 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     const TilePages spec_both = B8 ? raw_pages(p, bt, grp) : TilePages{};
     const int tok0 = p.qsl ? sload(p.qsl, b) : b * p.nmax;
     const int nb = p.qsl ? min(sload(p.qsl, b + 1) - tok0, p.nmax) : p.nmax;
-    const int start = FP8 ? first_position(sload(p.positions, nb > 0 ? tok0 : 0), p.bt_stride, p.P)
-                          : max(sload(p.positions, nb > 0 ? tok0 : 0), 0);
+    const int start = SAFE ? first_position(sload(p.positions, nb > 0 ? tok0 : 0), p.bt_stride, p.P)
+                           : max(sload(p.positions, nb > 0 ? tok0 : 0), 0);
     const int len = start + nb;
     const int t_first = qt * p.TQ;
     // No early exit for a pair past the sequence's queries (a shorter sequence of a ragged
@@ -1008,6 +1025,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     const bool first_full = !B8 && min(t_first + p.TQ, nb) - 1 - grp * KT >= KT - 1;
     if (first_full) dl_full(grp, 0, spec);
     u32x4 qreg[NQB];
+    float scale_log2 = p.scale_log2;
     const int qpos = p.causal && row_ok ? start + t : len - 1;
     const int t_last = min(t_first + p.TQ, nb) - 1;
     const int kend = p.causal ? start + t_last + 1 : len;
@@ -1090,9 +1108,14 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
                 continue;
             }
             uint32_t a0, a1, a2, a3;
-            i8x4_to_bf16(stk[2 * c2], a0, a1);
-            i8x4_to_bf16(stk[2 * c2 + 1], a2, a3);
-            *reinterpret_cast<u32x4 *>(&dsm.k[buf][key_l * D + ((c ^ (key_l & 15)) * 8)]) = (u32x4){a0, a1, a2, a3};
+            u32x4 *kdst = reinterpret_cast<u32x4 *>(&dsm.k[buf][key_l * D + ((c ^ (key_l & 15)) * 8)]);
+            if constexpr (F16) {
+                *kdst = i8x8_to_f16x8(stk[2 * c2], stk[2 * c2 + 1]);
+            } else {
+                i8x4_to_bf16(stk[2 * c2], a0, a1);
+                i8x4_to_bf16(stk[2 * c2 + 1], a2, a3);
+                *kdst = (u32x4){a0, a1, a2, a3};
+            }
             i8x4_to_bf16(stv[2 * c2], a0, a1);
             i8x4_to_bf16(stv[2 * c2 + 1], a2, a3);
             const int vs = c ^ (4 * (key_l & 3)) ^ (2 * ((key_l >> 2) & 1));
@@ -1117,7 +1140,8 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
             sc[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < NQB; i++)
-                sc[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(ka[i]), as_bf16x8(qreg[i]), sc[kb], 0, 0, 0);
+                sc[kb] = F16 ? __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(ka[i]), as_f16x8(qreg[i]), sc[kb], 0, 0, 0)
+                             : __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(ka[i]), as_bf16x8(qreg[i]), sc[kb], 0, 0, 0);
         }
         const bool need_mask = kt * KT + KT - 1 > mask_from;
         // INT8: the scales of this lane's 8 score keys, 4 kg + e and 16 + 4 kg + e
@@ -1139,7 +1163,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) mt = fmaxf(mt, x[e]);
-        mt *= p.scale_log2;
+        mt *= scale_log2;
         if (__any(mt > m + RESCALE_LOG2)) {
             mt = fmaxf(mt, __shfl_xor(mt, 16));
             mt = fmaxf(mt, __shfl_xor(mt, 32));
@@ -1153,7 +1177,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
         float pe[8], ps = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            pe[e] = fast_exp2(__builtin_fmaf(x[e], p.scale_log2, -m));
+            pe[e] = fast_exp2(__builtin_fmaf(x[e], scale_log2, -m));
             ps += pe[e];
         }
         l += ps;
@@ -1211,7 +1235,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
 #pragma unroll
         for (int i = 0; i < NQB; i++) {
             const u32x4 raw = *reinterpret_cast<const u32x4 *>(qb + (((4 * i + kg) ^ (qr & 15)) * 8));
-            if constexpr (INT8) {
+            if constexpr (INT8 && !F16) {
                 // bf16(q * smooth) (attention.jl:90-95)
                 const int d0 = 32 * i + 8 * kg;
 #pragma unroll
@@ -1223,6 +1247,11 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
             }
             if (!row_ok) qreg[i] = (u32x4){0u, 0u, 0u, 0u};
         }
+        if constexpr (F16)
+            scale_log2 *= f16_row(qreg, p.smooth, [&](int i) { return 32 * i + 8 * kg; }, [](float x) {
+                x = fmaxf(x, __shfl_xor(x, 16));
+                return fmaxf(x, __shfl_xor(x, 32));
+            });
     }
     if constexpr (!B8) {
         for (int i = 0; i < steps; i += 2) {
@@ -1267,7 +1296,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
     }
     __syncthreads();
     constexpr int NT = 1024, IT = RPG * (D / 4) / NT;
-    bool fine = true;   // FP8
+    bool fine = true;   // SAFE
     float2 ml[IT][NG];
     f32x4 dv[IT][NG];
 #pragma unroll
@@ -1298,7 +1327,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
             acc += dv[it][gi] * wgt;
         }
         if (ttl >= p.TQ || tt >= nb) continue;
-        if constexpr (FP8) {
+        if constexpr (SAFE) {
             fine &= fabsf(lsum) < INFINITY;
 #pragma unroll
             for (int e = 0; e < 4; e++) fine &= fabsf(acc[e]) < INFINITY;
@@ -1308,7 +1337,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
         *reinterpret_cast<u32x2 *>(orow) = (u32x2){pack_bf16x2(acc[0] * inv, acc[1] * inv),
                                                    pack_bf16x2(acc[2] * inv, acc[3] * inv)};
     }
-    if constexpr (FP8) {
+    if constexpr (SAFE) {
         // a product that is not finite: the pair's rows once more, each over the keys that it sees
         if (__syncthreads_or(!fine)) {
             for (int x = w; x < RPG; x += 16) {
@@ -1317,7 +1346,7 @@ __global__ void __launch_bounds__(1024) prefill16_kernel(PrefillParams p) {
                 const size_t qrow = (size_t)(tok0 + tt) * p.Hq + h * p.G + (rl & (p.G - 1));
                 const int last = p.causal ? start + tt : len - 1;
                 float xm, xl, acc[D / 64];
-                exact_row<D, false, true>(p, bt, h, p.q + qrow * D, 0, nkt * KT, [&](int key) { return key <= last ? key : -1; }, xm, xl, acc);
+                exact_row<D, INT8, FP8>(p, bt, h, p.q + qrow * D, 0, nkt * KT, [&](int key) { return key <= last ? key : -1; }, xm, xl, acc);
 #pragma unroll
                 for (int k = 0; k < D / 64; k++) Elt<uint16_t>::st(p.out, qrow * D + lane + 64 * k, acc[k] / xl);
             }
@@ -1509,6 +1538,8 @@ int ti_launch_prefill(const ti_attention_args *a, const ti_kv_cache *c, const ti
     dim3 grid(c->kv_heads, pl.pair ? (p.qtiles + 1) / 2 : p.qtiles * pl.splits, a->num_seqs);
     if (pl.r16) {
         if (c->kind == TI_KV_FP8) prefill16_kernel<false, true><<<grid, 1024, 0, s>>>(p);
+        else if (win.size && c->kind == TI_KV_INT8) prefill16_kernel<true, false, true><<<grid, 1024, 0, s>>>(p);
+        else if (win.size) prefill16_kernel<false, false, true><<<grid, 1024, 0, s>>>(p);
         else if (c->kind == TI_KV_INT8) prefill16_kernel<true><<<grid, 1024, 0, s>>>(p);
         else prefill16_kernel<false><<<grid, 1024, 0, s>>>(p);
         return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;

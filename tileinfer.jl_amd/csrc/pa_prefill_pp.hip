@@ -111,6 +111,7 @@ template <int D, bool INT8, int FORM, bool FP8 = false, bool WIN = false>
 __global__ void __launch_bounds__(FORM == TI_PP_SOLO ? 256 : 512, FORM == TI_PP_SOLO && D == 64 ? 3 : 2)
 prefill_pp_kernel(PPParams p) {
     constexpr bool KS = FORM == TI_PP_KSPLIT, SOLO = FORM == TI_PP_SOLO, B8 = INT8 || FP8;
+    constexpr bool F16 = INT8 && WIN;   // fp16 queries and keys (pa_window.hpp)
     static_assert(D == 128 || KS || SOLO, "head_dim 64 stages a tile with one team");
     constexpr int NW = SOLO ? 4 : 8;
     constexpr int NQB = D / 16;        // score MFMAs per tile (16 head-dim elements each)
@@ -283,7 +284,10 @@ prefill_pp_kernel(PPParams p) {
     };
     // FP8: x is the place of the tile's scales in sc8
     auto store_k = [&](const Chunk &r, int buf, int u, int x) {
-        *reinterpret_cast<u32x4 *>(&sm.k[buf][(ckey + KPU * u) * KROW + cch * 8]) = bf16_chunk(r, FP8 ? scale_of(sc8[x].k, u) : 1.0f);
+        *reinterpret_cast<u32x4 *>(&sm.k[buf][(ckey + KPU * u) * KROW + cch * 8]) = [&] {
+            if constexpr (F16) return i8x8_to_f16x8(r[0], r[1]);
+            else return bf16_chunk(r, FP8 ? scale_of(sc8[x].k, u) : 1.0f);
+        }();
     };
     auto store_v = [&](const Chunk &r, int buf, int j, int u) {
         // Keys past kend in the last tile may hold any bits (even NaN) of an allocated
@@ -316,6 +320,7 @@ prefill_pp_kernel(PPParams p) {
     Bases bs[4];                                   // bases of tiles i + 1 .. i + 3 in 1 .. 3
     Pages raw4;                                    // block-table entries of tile i + 4
     bf16x8 qreg[NQB];
+    float back = 1.0f;   // F16
     {
         if (WIN || p.splits != 1) first_pages(kt_lo);
 #pragma unroll
@@ -356,9 +361,11 @@ prefill_pp_kernel(PPParams p) {
         for (int u = 0; u < NC; u++) store_k(k1[u], 1, u, 1);
         if constexpr (INT8) store_s(s1, 1);
         const uint32_t keep = row_ok ? ~0u : 0u;
+        if constexpr (F16)
+            back = f16_row(raw, p.smooth, [&](int i) { return i * 16 + kg * 8; }, [](float x) { return fmaxf(x, __shfl_xor(x, 32)); });
 #pragma unroll
         for (int i = 0; i < NQB; i++) {
-            if constexpr (INT8) {
+            if constexpr (INT8 && !F16) {
                 // bf16(q * smooth) (attention.jl:90-95)
                 const int d0 = i * 16 + kg * 8;
 #pragma unroll
@@ -403,7 +410,8 @@ prefill_pp_kernel(PPParams p) {
 #pragma unroll
             for (int e = 0; e < 16; e++) sc[e] = 0.0f;
         }
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(ka[i]), qreg[i], sc, 0, 0, 0);
+        if constexpr (F16) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_f16x8(ka[i]), __builtin_bit_cast(f16x8_t, qreg[i]), sc, 0, 0, 0);
+        else sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(ka[i]), qreg[i], sc, 0, 0, 0);
     };
     // Online softmax of step j's scores (exp2 domain, lazy rescale after the first p.eager steps)
     // -> pb. Only tiles reaching past mask_from (the diagonal / last tiles) compare key positions.
@@ -450,6 +458,7 @@ prefill_pp_kernel(PPParams p) {
 #pragma unroll
         for (int e = 0; e < 16; e++) mt = fmaxf(mt, sc[e]);
         if constexpr (!INT8) mt *= p.scale_log2;
+        if constexpr (F16) mt *= back;
         if (__any(mt > m + (j < p.eager ? 0.0f : RESCALE_LOG2))) {
             mt = fmaxf(mt, __shfl_xor(mt, 32));
             const float mn = fmaxf(m, mt);
@@ -462,7 +471,7 @@ prefill_pp_kernel(PPParams p) {
         float pe[16], ps = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-            pe[e] = fast_exp2(INT8 ? sc[e] - m : __builtin_fmaf(sc[e], p.scale_log2, -m));
+            pe[e] = fast_exp2(F16 ? __builtin_fmaf(sc[e], back, -m) : INT8 ? sc[e] - m : __builtin_fmaf(sc[e], p.scale_log2, -m));
             ps += pe[e];
             if constexpr (INT8) pe[e] *= svq[e >> 2][e & 3];
         }

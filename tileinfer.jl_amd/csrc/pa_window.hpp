@@ -7,6 +7,10 @@
 // 8-bit block caches: an e4m3 value times its block's power of two is a bf16 value exactly (v_cvt_scalef32_pk_bf16_fp8),
 // so tiles are converted on their way to the matrix cores and everything behind is the dense kernels'.
 //
+// INT8 caches: the prefill kernels multiply fp16 keys (int8 values exactly) by queries that f16_row rounds once, to fp16's
+// 11 bits, where a step without a window rounds them to bf16's 8: an output's error is then its own rounding's (1.7e-3 of its
+// size, root of the mean square, against 3.3e-3).
+//
 // Masked keys. The matrix products give a masked key the weight 0, and 0 times a value that is not finite is NaN, so
 // a NaN in a row of the cache would reach every row that is worked on together with one that sees it. The kernels look at
 // what they are about to write: where it is not finite, the work-group's rows are done again one by one over the keys that
@@ -40,6 +44,46 @@ struct WindowTiles {
     }
     __device__ __forceinline__ int tile(int j) const { return j < sunk ? j : j + skip; }
 };
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f16x8_t as_f16x8(u32x4 w) { return __builtin_bit_cast(f16x8_t, w); }
+
+// 8 int8 -> 8 fp16 (exact): the bits 0x6400 | (b + 128) are 1152 + b.
+__device__ __forceinline__ u32x4 i8x8_to_f16x8(uint32_t x, uint32_t y) {
+    const f16x2_t bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t bits = __builtin_amdgcn_perm(0x64646464u, (e < 2 ? x : y) ^ 0x80808080u, e & 1 ? 0x04030402u : 0x04010400u);
+        r[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, bits) - bias);
+    }
+    return r;
+}
+
+// A lane's N x 8 elements of a query row (bf16; word i holds elements at(i) on) times the keys' smoothing, as fp16 times the
+// 2^e that brings the row's largest magnitude into [2^14, 2^15); largest: over the row's lanes. Returns 2^-e.
+template <int N, typename At, typename Max>
+__device__ __forceinline__ float f16_row(u32x4 (&q)[N], const float *smooth, At &&at, Max &&largest) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            most = fmaxf(most, fmaxf(fabsf(__uint_as_float(q[i][e] << 16) * smooth[at(i) + 2 * e]),
+                                     fabsf(__uint_as_float(q[i][e] & 0xffff0000u) * smooth[at(i) + 2 * e + 1])));
+    most = largest(most);
+    const int e2 = most > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const f32x2 v = {__builtin_ldexpf(__uint_as_float(q[i][e] << 16) * smooth[at(i) + 2 * e], e2),
+                             __builtin_ldexpf(__uint_as_float(q[i][e] & 0xffff0000u) * smooth[at(i) + 2 * e + 1], e2)};
+            q[i][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+        }
+    return __builtin_ldexpf(1.0f, -e2);
+}
 
 // Whether the query at position `at` sees `key`. Without short circuits: hipcc has made of branches around the choice between
 // a matrix product's register and a constant a move of the constant for every lane (attn_f32_kernel's masks, ROCm 7.2).
