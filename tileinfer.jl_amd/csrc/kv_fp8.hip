@@ -7,7 +7,10 @@
 // divides the rows that the block already holds), and writes the new rows. Nothing depends on the order of threads: the
 // largest magnitude is a maximum, and of two tokens of one slot the later is written.
 //
-// Bound: a prompt's HBM bytes (2 + 1 per element of k and v), one token's chain slots -> rows -> largest -> rows out.
+// Bound: a prompt's bytes (2 + 1 per element of k and v), one token's chain slots -> rows -> largest -> rows out. Measured
+// (8 heads of 128, bf16): 8192 tokens into pages of 16 16.4 us, 3.05 TB/s (rows stay in registers between the two passes; 34.8 us
+// with rows read twice): slots -> page's list -> rows -> largest -> rows out go one after the other in a work-group, and two
+// rounds of work-groups fill the CUs; one token for each of 32 sequences 4.3 us, of which 1.9 are a launch.
 //
 // The fused kernel rotates queries and keys with every rounding of attention_inputs_v_kernel (kv_write.hip), so it is
 // bit-identical to rmsnorm, rope and store_kv in a row: products and sums are rounded one by one.

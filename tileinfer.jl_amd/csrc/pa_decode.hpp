@@ -1,4 +1,5 @@
-// Split-KV paged decode / verify attention on bf16 MFMA (gfx950), dense bf16 or INT8 cache.
+// Split-KV paged decode / verify attention on bf16 MFMA (gfx950), dense bf16 or INT8 cache (FP8, WIN: 8-bit block caches and
+// windows, pa_window.hpp; launched from pa_window.hip).
 //
 // Reference: attention_decode_kernel / decode_body / attention_combine_kernel
 // (src/ops/tile/attention.jl:185-245) and its INT8 variant (:68-95, :194-202).

