@@ -140,6 +140,61 @@ def test_fused_inputs_are_the_ops_in_a_row(gpu, T, norm, D, nq, H, P, n):
     assert torch.equal(a[0].layer_scale, b[0].layer_scale) and torch.equal(a[0].layer_q, b[0].layer_q)
 
 
+def long_slots(g, n, P, pages):
+    """Mostly runs in order, as prompts are; among them single tokens of other sequences, slots again, slots outside."""
+    at, free = [], list(g.permutation(pages) * P)
+    while len(at) < n:
+        run = int(g.integers(1, 6 * P))
+        take = [free.pop() for _ in range(min(-(-run // P), len(free)))]
+        at += [b + o + 1 for b in take for o in range(P)][:run]
+        if not free:
+            free = list(g.permutation(pages) * P)
+    at = np.array(at[:n], np.int64)
+    where = g.integers(0, n, n // 50)
+    at[where] = g.integers(1, pages * P + 1, len(where))
+    where = g.integers(0, n, 40)
+    at[where] = g.choice([0, -1, -2 ** 31, 2 ** 31 - 1, pages * P + 1], 40)
+    return at
+
+
+@pytest.mark.parametrize("T,D,H,P,n,aligned", [(torch.bfloat16, 128, 8, 16, 20000, True), (torch.bfloat16, 64, 8, 64, 40001, True),
+                                               (torch.float32, 64, 5, 32, 17000, True), (torch.bfloat16, 64, 17, 16, 9000, False),
+                                               (torch.bfloat16, 64, 4, 16, 70003, True), (torch.float32, 64, 8, 256, 20000, True)])
+def test_long_calls(gpu, T, D, H, P, n, aligned):
+    """Calls whose work-groups take several heads and pages each, into blocks that hold rows already."""
+    g = np.random.Generator(np.random.PCG64(n))
+    pages = n // P + 50
+    k, v = pools(D, P, H, pages, g)
+    q, scale = k.layer_q.cpu().numpy(), k.layer_scale.cpu().numpy()
+    at = long_slots(g, n, P, pages)
+    x, y = rows(g, n, H, D, T), rows(g, n, H, D, T)
+    slots = torch.empty(n + 1, dtype=torch.int32, device="cuda")[0 if aligned else 1:][:n].copy_(i32(at))
+    ti.store_kv_(BE, k, v, x.cuda(), y.cuda(), slots)
+    store(q, scale, x.float().numpy(), y.float().numpy(), at)
+    same(k, q, scale)
+
+
+@pytest.mark.parametrize("tokens", [(1, 17), (3, 17), (1, 32), (1, 33), (1, 64), (8, 8), (1, 256), (1, 257), (5, 51)])
+@pytest.mark.parametrize("H,P", [(8, 64), (3, 16)])
+def test_few_tokens_of_a_page(gpu, tokens, H, P):
+    """Few tokens, one after the other in a page or more of each sequence."""
+    seqs, each = tokens
+    g = np.random.Generator(np.random.PCG64(seqs * each))
+    pages = seqs * (each // P + 2)
+    k, v = pools(128, P, H, pages, g)
+    q, scale = k.layer_q.cpu().numpy(), k.layer_scale.cpu().numpy()
+    for start in (0, 5):
+        at = [b * (each // P + 2) * P + start + t + 1 for b in range(seqs) for t in range(each)]
+        x, y = rows(g, len(at), H, 128, torch.bfloat16), rows(g, len(at), H, 128, torch.bfloat16)
+        ti.store_kv_(BE, k, v, x.cuda(), y.cuda(), i32(at))
+        store(q, scale, x.float().numpy(), y.float().numpy(), at)
+        same(k, q, scale)
+
+
+def test_long_fused_inputs_are_the_ops_in_a_row(gpu):
+    test_fused_inputs_are_the_ops_in_a_row(gpu, torch.bfloat16, True, 128, 2, 8, 16, 20000)
+
+
 CASES = [
     ([(300, 1)], 4, 16), ([(0, 1)], 4, 16), ([(4000, 1), (1, 1), (999, 1)], 4, 64), ([(200, 5), (40, 0), (3, 2)], 4, 16),
     ([(500, 16), (90, 16)], 4, 64), ([(0, 333)], 4, 16), ([(150, 200), (0, 64)], 4, 64), ([(700, 1)] * 40, 4, 16), ([(64, 1), (10, 1)], 33, 16),

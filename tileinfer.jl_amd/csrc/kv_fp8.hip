@@ -10,7 +10,7 @@
 // Bound: a prompt's bytes (2 + 1 per element of k and v), one token's chain slots -> rows -> largest -> rows out. Measured
 // (8 heads of 128, bf16): 8192 tokens into pages of 16 16.4 us, 3.05 TB/s (rows stay in registers between the two passes; 34.8 us
 // with rows read twice): slots -> page's list -> rows -> largest -> rows out go one after the other in a work-group, and two
-// rounds of work-groups fill the CUs; one token for each of 32 sequences 4.3 us, of which 1.9 are a launch.
+// rounds of work-groups fill the CUs; one token for each of 32 sequences 4.0 us, of which 1.9 are a launch.
 //
 // The fused kernel rotates queries and keys with every rounding of attention_inputs_v_kernel (kv_write.hip), so it is
 // bit-identical to rmsnorm, rope and store_kv in a row: products and sums are rounded one by one.
@@ -24,7 +24,8 @@ using namespace ti;
 
 namespace {
 
-constexpr int MAX_PAGE = 1024, MAX_HEADS = 16;   // keys of a page, KV heads of a work-group
+constexpr int MAX_PAGE = 1024, MAX_HEADS = 16;   // keys of a page, KV heads worked on together
+constexpr int SHARE = 4;   // pages whose rows are looked for in one pass over the slots
 
 struct Fp8WriteParams {
     const void *k, *v;               // store: [n][Hk][D]
@@ -34,7 +35,8 @@ struct Fp8WriteParams {
     float *scale;                    // [2][pages][Hk]
     const int32_t *slots, *positions;
     int n, nq, Hk, P, pshift, pages, table_len;
-    int chunk, hpg, hgroups;         // tokens and KV heads of a work-group, groups of heads
+    int chunk, hpg, hgroups, hloop;  // tokens of a work-group; KV heads worked on together, groups of them, groups of a work-group
+    int hwgs;                        // work-groups of a chunk of tokens: hgroups / hloop, rounded up
     unsigned page_groups;            // work-groups that write pages; the others rotate queries
     float eps;
 };
@@ -128,11 +130,14 @@ template <> struct Held<float> {
     }
 };
 
-template <typename T, bool FUSED, bool NORM, int D>
+// FEW: at most a token for each thread, one for each work-group, whose slots are read once, beside the rows of the
+// work-group's own token.
+template <typename T, bool FUSED, bool NORM, int D, bool FEW>
 __global__ void __launch_bounds__(256) fp8_write_kernel(Fp8WriteParams p) {
     constexpr int HALF = D / 2, LPH = D / 8, NT = 256, NG = NT / LPH;
     using V = Vec4<T>;
-    __shared__ int src[MAX_PAGE];                     // the token that writes each row of the page, or -1
+    __shared__ int srcs[MAX_PAGE];                    // the token that writes each row of up to SHARE pages, or -1
+    __shared__ int taken;                             // those of them that a token in front of the chunk's has
     __shared__ uint16_t lists[NT / 64][MAX_PAGE];     // the rows that are written, a copy for each wave
     __shared__ uint32_t most[2 * MAX_HEADS];
     __shared__ float inv[2 * MAX_HEADS], ratio[2 * MAX_HEADS];
@@ -161,8 +166,9 @@ __global__ void __launch_bounds__(256) fp8_write_kernel(Fp8WriteParams p) {
         const int pos = p.positions[j];
         return pos >= 0 && pos < p.table_len;
     };
-    const int c0 = (int)(blockIdx.x / (unsigned)p.hgroups) * p.chunk, h0 = (int)(blockIdx.x % (unsigned)p.hgroups) * p.hpg;
-    const int heads = min(p.hpg, p.Hk - h0);
+    const int chunk = FEW ? 1 : p.chunk, hloop = FEW ? 1 : p.hloop;
+    const int c0 = (int)(blockIdx.x / (unsigned)p.hwgs) * chunk, g0 = (int)(blockIdx.x % (unsigned)p.hwgs) * hloop;
+    int h0 = g0 * p.hpg, heads = min(p.hpg, p.Hk - h0);   // of the group of heads that is worked on
     auto load = [&](int t, int hh, Held<T> &x) {
         const int half = hh >= heads, h = h0 + hh - half * heads;
         if constexpr (FUSED) {
@@ -175,177 +181,252 @@ __global__ void __launch_bounds__(256) fp8_write_kernel(Fp8WriteParams p) {
             x.ld((const T *)(half ? p.v : p.k) + ((size_t)t * p.Hk + h) * D + 8 * u);
         }
     };
-    // Few tokens: their slots are read once, beside the rows of the work-group's own token.
-    const bool few = p.n <= NT;
-    const int my_slot = few && tid < p.n ? p.slots[tid] : 0;
+    const int my_slot = FEW && tid < p.n ? p.slots[tid] : 0;
     // One token a work-group: its rows are on their way while the slots are looked through.
     Held<T> mine;
-    if (p.chunk == 1 && (!FUSED || writes(c0))) load(c0, min(gid, 2 * heads - 1), mine);
+    if (FEW && (!FUSED || writes(c0))) load(c0, min(gid, 2 * heads - 1), mine);
     // The chunk's tokens (at most 64) that write to another page than the one in front of them: one lane each.
     int first_page = -1;
-    if (lane < p.chunk && c0 + lane < p.n && writes(c0 + lane)) {
+    if (lane < chunk && c0 + lane < p.n && writes(c0 + lane)) {
         first_page = page_of_slot(p.slots[c0 + lane]);
         if (c0 + lane > 0 && writes(c0 + lane - 1) && page_of_slot(p.slots[c0 + lane - 1]) == first_page) first_page = -1;
     }
-    for (unsigned long long starts = __ballot(first_page >= 0); starts; starts &= starts - 1) {
-        const int at = __builtin_ctzll(starts), i = c0 + at, page = __builtin_amdgcn_readlane(first_page, at);
-        // the block's scales, needed below
-        float *sp = nullptr;
-        float old = 0.0f;
+    unsigned long long starts = __ballot(first_page >= 0);
+    // the next page that begins in the chunk: its first token here
+    auto next_start = [&] {
+        const int at = __builtin_ctzll(starts);
+        starts &= starts - 1;
+        return at;
+    };
+    while (starts) {
+        // Up to SHARE pages at a time, whose rows are looked for in one pass over the slots.
+        int at[SHARE], first[SHARE], pages = 0;
+        unsigned span[SHARE];
+        const int fit = FEW ? 1 : min(SHARE, MAX_PAGE >> p.pshift);
+#pragma unroll
+        for (int k = 0; k < SHARE; k++) {
+            at[k] = first[k] = 0;
+            span[k] = 0;
+            if (k < fit && starts) {
+                at[k] = next_start();
+                first[k] = (__builtin_amdgcn_readlane(first_page, at[k]) << p.pshift) + 1;   // the page's first slot
+                span[k] = (unsigned)min(p.P, limit - first[k] + 1);
+                pages = k + 1;
+            }
+        }
+        for (int o = tid; o < pages << p.pshift; o += NT) srcs[o] = -1;
+        if (tid == 0) taken = 0;
+        // (few tokens: the scales are on their way beside the slots)
+        float early = 0.0f;
         if (tid < 2 * heads) {
             const int half = tid >= heads;
-            sp = p.scale + ((size_t)half * p.pages + page) * p.Hk + h0 + tid - half * heads;
-            old = *sp;
+            early = p.scale[((size_t)half * p.pages + ((first[0] - 1) >> p.pshift)) * p.Hk + h0 + tid - half * heads];
             most[tid] = 0u;
         }
-        for (int o = tid; o < p.P; o += NT) src[o] = -1;
         __syncthreads();
-        // All tokens of the page, wherever they are; one in front of this one has the page.
-        bool earlier = false;
-        auto take = [&](int s, int j) {
-            if (page_of_slot(s) == page && writes(j)) {
-                if (j < i) earlier = true;
-                else atomicMax(&src[(s - 1) & (p.P - 1)], j);
-            }
-        };
-        if (few) {
-            if (tid < p.n) take(my_slot, tid);
-        } else if (((uintptr_t)p.slots & 15) == 0) {
-            const int quads = p.n >> 2;
-            for (int q0 = tid; q0 < quads; q0 += 4 * NT) {
-                int4 s[4];
+        // All tokens of the pages, wherever they are; one in front of the chunk's has the page. A slot is of page k where it is
+        // less than `span` past the page's first one, as unsigned numbers: none outside the pool is.
+        int earlier = 0;
+        auto look = [&](auto many) {
+            constexpr int N = decltype(many)::value;
+            auto take = [&](int s, int j) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[e] = reinterpret_cast<const int4 *>(p.slots)[min(q0 + e * NT, quads - 1)];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int j = 4 * (q0 + e * NT);
-                    if (q0 + e * NT < quads) take(s[e].x, j), take(s[e].y, j + 1), take(s[e].z, j + 2), take(s[e].w, j + 3);
-                }
-            }
-            if (tid < (p.n & 3)) take(p.slots[4 * quads + tid], 4 * quads + tid);
-        } else {
-            for (int j = tid; j < p.n; j += NT) take(p.slots[j], j);
-        }
-        if (__syncthreads_or(earlier)) continue;
-        int count = 0;
-        for (int o0 = 0; o0 < p.P; o0 += 64) {
-            const int o = o0 + lane;
-            const bool has = o < p.P && src[o] >= 0;
-            const unsigned long long m = __ballot(has);
-            if (has) list[count + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)o;
-            count += __popcll(m);
-        }
-        // Vectors of the page's new rows: (row, half, head), heads innermost; one per lane group at a time. A lane holds
-        // elements 8 u .. 8 u + 7, of a rotated key 4 u .. and D / 2 + 4 u .. .
-        const int vectors = count * 2 * heads;
-        auto place = [&](int vec, int &row, int &hh) {
-            const int r = vec / (2 * heads);
-            hh = vec - r * 2 * heads;                // half * heads + head
-            row = list[r];
-        };
-        auto largest = [&](const Held<T> &held, int hh) {
-            float x[8], m = 0.0f;
-            held.get(x);
-#pragma unroll
-            for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
-#pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-            if (u == 0) atomicMax(&most[hh], __float_as_uint(m));   // of no sign: ordered as whole numbers
-        };
-        uint8_t *base = p.q8 + (((size_t)page * p.Hk + h0) << p.pshift) * D;
-        const size_t half_q = (((size_t)p.pages * p.Hk) << p.pshift) * D;
-        auto store = [&](const Held<T> &held, int row, int hh) {
-            float x[8];
-            held.get(x);
-            const int half = hh >= heads;
-            uint8_t *dst = base + half * half_q + ((((size_t)(hh - half * heads)) << p.pshift) + row) * D;
-            const uint32_t lo = to_e4m3(x, inv[hh]), hi = to_e4m3(x + 4, inv[hh]);
-            if (FUSED && !half) {
-                *reinterpret_cast<uint32_t *>(dst + 4 * u) = lo;
-                *reinterpret_cast<uint32_t *>(dst + HALF + 4 * u) = hi;
-            } else {
-                *reinterpret_cast<u32x2 *>(dst + 8 * u) = (u32x2){lo, hi};
-            }
-        };
-        // between the two passes: the blocks' scales, and the rows that they hold already
-        auto scales = [&] {
-            __syncthreads();
-            bool grown = false;
-            if (tid < 2 * heads) {
-                const float need = least_scale(__uint_as_float(most[tid]));
-                const bool fresh = src[0] >= 0 || !(old > 0.0f && old < INFINITY);
-                const float now = fresh ? need : fmaxf(old, need);
-                inv[tid] = inverse(now);
-                ratio[tid] = fresh ? 1.0f : old * inverse(now);
-                grown = ratio[tid] < 1.0f;
-                if (now != old) *sp = now;
-            }
-            if (!__syncthreads_or(grown)) return;
-            // 16 bytes at a time
-            for (int c = tid; c < 2 * heads * p.P * (D / 16); c += NT) {
-                const int d16 = c % (D / 16), o = (c / (D / 16)) & (p.P - 1), hh = (c / (D / 16)) >> p.pshift;
-                const float f = ratio[hh];
-                if (src[o] >= 0 || f == 1.0f) continue;
-                const int half = hh >= heads;
-                u32x4 *at16 = reinterpret_cast<u32x4 *>(base + half * half_q + ((((size_t)(hh - half * heads)) << p.pshift) + o) * D) + d16;
-                u32x4 w = *at16;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float x[4] = {__builtin_amdgcn_cvt_f32_fp8((int)w[e], 0), __builtin_amdgcn_cvt_f32_fp8((int)w[e], 1),
-                                        __builtin_amdgcn_cvt_f32_fp8((int)w[e], 2), __builtin_amdgcn_cvt_f32_fp8((int)w[e], 3)};
-                    w[e] = to_e4m3(x, f);
-                }
-                *at16 = w;
-            }
-        };
-        // KEEP vectors of a lane group stay in registers between the passes, loaded together; more are read twice.
-        auto rows = [&](auto keep) {
-            constexpr int KEEP = decltype(keep)::value;
-            Held<T> x[KEEP];
-            int row[KEEP], hh[KEEP];
-            auto read = [&](int v0) {
-#pragma unroll
-                for (int k = 0; k < KEEP; k++) {
-                    place(min(v0 + k * NG, vectors - 1), row[k], hh[k]);
-                    if (KEEP == 1 && p.chunk == 1 && count == 1 && src[row[k]] == c0) x[k] = mine;
-                    else load(src[row[k]], hh[k], x[k]);
+                for (int k = 0; k < N; k++) {
+                    const unsigned o = (unsigned)s - (unsigned)first[k];
+                    if (o < span[k] && writes(j)) {
+                        if (j < c0 + at[k]) earlier |= 1 << k;
+                        else atomicMax(&srcs[(k << p.pshift) + (int)o], j);
+                    }
                 }
             };
-            for (int v0 = gid; v0 < vectors || v0 == gid; v0 += KEEP * NG) {
-                read(v0);
+            if (((uintptr_t)p.slots & 15) == 0) {
+                const int quads = p.n >> 2;
+                for (int q0 = tid; q0 < quads; q0 += 4 * NT) {
+                    int4 s[4];
 #pragma unroll
-                for (int k = 0; k < KEEP; k++) largest(x[k], hh[k]);   // (a vector twice is as good as once)
-            }
-            scales();
-            for (int v0 = gid; v0 < vectors; v0 += KEEP * NG) {
-                if (vectors > KEEP * NG) read(v0);
+                    for (int e = 0; e < 4; e++) s[e] = reinterpret_cast<const int4 *>(p.slots)[min(q0 + e * NT, quads - 1)];
 #pragma unroll
-                for (int k = 0; k < KEEP; k++)
-                    if (v0 + k * NG < vectors) store(x[k], row[k], hh[k]);
+                    for (int e = 0; e < 4; e++) {
+                        const int j = 4 * (q0 + e * NT);
+                        if (q0 + e * NT < quads) take(s[e].x, j), take(s[e].y, j + 1), take(s[e].z, j + 2), take(s[e].w, j + 3);
+                    }
+                }
+                if (tid < (p.n & 3)) take(p.slots[4 * quads + tid], 4 * quads + tid);
+            } else {
+                for (int j = tid; j < p.n; j += NT) take(p.slots[j], j);
             }
         };
-        if (vectors <= NG) rows(IC<1>{});
-        else if (vectors <= 4 * NG || FUSED || sizeof(T) == 4) rows(IC<4>{});
-        else rows(IC<8>{});
-        __syncthreads();   // the page's lists are read
+        if constexpr (FEW) {
+            const unsigned o = (unsigned)my_slot - (unsigned)first[0];
+            if (tid < p.n && o < span[0] && writes(tid)) {
+                if (tid < c0) earlier = 1;
+                else atomicMax(&srcs[o], tid);
+            }
+        } else {
+            if (pages == 1) look(IC<1>{});
+            else look(IC<SHARE>{});
+        }
+        if (earlier) atomicOr(&taken, earlier);
+        __syncthreads();
+        const int done = taken;
+        for (int k = 0; k < pages; k++) {
+            if (done >> k & 1) continue;
+            int slot0 = first[0];
+#pragma unroll
+            for (int j = 1; j < SHARE; j++) slot0 = k == j ? first[j] : slot0;
+            const int page = (slot0 - 1) >> p.pshift;
+            const int *src = srcs + (k << p.pshift);
+            int count = 0;
+            for (int o0 = 0; o0 < p.P; o0 += 64) {
+                const int o = o0 + lane;
+                const bool has = o < p.P && src[o] >= 0;
+                const unsigned long long m = __ballot(has);
+                if (has) list[count + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)o;
+                count += __popcll(m);
+            }
+            for (int hg = 0; hg < hloop && g0 + hg < p.hgroups; hg++) {
+                h0 = (g0 + hg) * p.hpg, heads = min(p.hpg, p.Hk - h0);
+                // the blocks' scales, needed below
+                float *sp = nullptr;
+                float old = 0.0f;
+                if (tid < 2 * heads) {
+                    const int half = tid >= heads;
+                    sp = p.scale + ((size_t)half * p.pages + page) * p.Hk + h0 + tid - half * heads;
+                    old = early;
+                }
+                if (k > 0 || hg > 0) {
+                    if (tid < 2 * heads) old = *sp, most[tid] = 0u;
+                    __syncthreads();
+                }
+                // Vectors of the page's new rows: (row, half, head), heads innermost; one per lane group at a time. A lane holds
+                // elements 8 u .. 8 u + 7, of a rotated key 4 u .. and D / 2 + 4 u .. .
+                const int vectors = count * 2 * heads;
+                auto place = [&](int vec, int &row, int &hh) {
+                    const int r = vec / (2 * heads);
+                    hh = vec - r * 2 * heads;                // half * heads + head
+                    row = list[r];
+                };
+                auto largest = [&](const Held<T> &held, int hh) {
+                    float x[8], m = 0.0f;
+                    held.get(x);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
+#pragma unroll
+                    for (int o = LPH / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+                    if (u == 0) atomicMax(&most[hh], __float_as_uint(m));   // of no sign: ordered as whole numbers
+                };
+                uint8_t *base = p.q8 + (((size_t)page * p.Hk + h0) << p.pshift) * D;
+                const size_t half_q = (((size_t)p.pages * p.Hk) << p.pshift) * D;
+                auto store = [&](const Held<T> &held, int row, int hh) {
+                    float x[8];
+                    held.get(x);
+                    const int half = hh >= heads;
+                    uint8_t *dst = base + half * half_q + ((((size_t)(hh - half * heads)) << p.pshift) + row) * D;
+                    const uint32_t lo = to_e4m3(x, inv[hh]), hi = to_e4m3(x + 4, inv[hh]);
+                    if (FUSED && !half) {
+                        *reinterpret_cast<uint32_t *>(dst + 4 * u) = lo;
+                        *reinterpret_cast<uint32_t *>(dst + HALF + 4 * u) = hi;
+                    } else {
+                        *reinterpret_cast<u32x2 *>(dst + 8 * u) = (u32x2){lo, hi};
+                    }
+                };
+                // between the two passes: the blocks' scales, and the rows that they hold already
+                auto scales = [&] {
+                    __syncthreads();
+                    bool grown = false;
+                    if (tid < 2 * heads) {
+                        const float need = least_scale(__uint_as_float(most[tid]));
+                        const bool fresh = src[0] >= 0 || !(old > 0.0f && old < INFINITY);
+                        const float now = fresh ? need : fmaxf(old, need);
+                        inv[tid] = inverse(now);
+                        ratio[tid] = fresh ? 1.0f : old * inverse(now);
+                        grown = ratio[tid] < 1.0f;
+                        if (now != old) *sp = now;
+                    }
+                    if (!__syncthreads_or(grown)) return;
+                    // 16 bytes at a time
+                    for (int c = tid; c < 2 * heads * p.P * (D / 16); c += NT) {
+                        const int d16 = c % (D / 16), o = (c / (D / 16)) & (p.P - 1), hh = (c / (D / 16)) >> p.pshift;
+                        const float f = ratio[hh];
+                        if (src[o] >= 0 || f == 1.0f) continue;
+                        const int half = hh >= heads;
+                        u32x4 *at16 = reinterpret_cast<u32x4 *>(base + half * half_q + ((((size_t)(hh - half * heads)) << p.pshift) + o) * D) + d16;
+                        u32x4 w = *at16;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float x[4] = {__builtin_amdgcn_cvt_f32_fp8((int)w[e], 0), __builtin_amdgcn_cvt_f32_fp8((int)w[e], 1),
+                                                __builtin_amdgcn_cvt_f32_fp8((int)w[e], 2), __builtin_amdgcn_cvt_f32_fp8((int)w[e], 3)};
+                            w[e] = to_e4m3(x, f);
+                        }
+                        *at16 = w;
+                    }
+                };
+                // KEEP vectors of a lane group stay in registers between the passes, loaded together; more are read twice.
+                auto rows = [&](auto keep) {
+                    constexpr int KEEP = decltype(keep)::value;
+                    Held<T> x[KEEP];
+                    int row[KEEP], hh[KEEP];
+                    auto read = [&](int v0) {
+#pragma unroll
+                        for (int k = 0; k < KEEP; k++) {
+                            place(min(v0 + k * NG, vectors - 1), row[k], hh[k]);
+                            if (KEEP == 1 && FEW && count == 1 && src[row[k]] == c0) x[k] = mine;
+                            else load(src[row[k]], hh[k], x[k]);
+                        }
+                    };
+                    for (int v0 = gid; v0 < vectors || v0 == gid; v0 += KEEP * NG) {
+                        read(v0);
+#pragma unroll
+                        for (int k = 0; k < KEEP; k++) largest(x[k], hh[k]);   // (a vector twice is as good as once)
+                    }
+                    scales();
+                    for (int v0 = gid; v0 < vectors; v0 += KEEP * NG) {
+                        if (vectors > KEEP * NG) read(v0);
+#pragma unroll
+                        for (int k = 0; k < KEEP; k++)
+                            if (v0 + k * NG < vectors) store(x[k], row[k], hh[k]);
+                    }
+                };
+                if (vectors <= NG) rows(IC<1>{});
+                else if (vectors <= 4 * NG || FUSED || sizeof(T) == 4) rows(IC<4>{});
+                else rows(IC<8>{});
+                __syncthreads();   // the lists and scales are read
+            }
+            h0 = g0 * p.hpg, heads = min(p.hpg, p.Hk - h0);
+        }
+        if (starts) __syncthreads();   // `taken` is read
     }
 }
 
+constexpr int LONG_GROUPS = 1024;
+
 template <typename T, bool FUSED, bool NORM>
 int launch(Fp8WriteParams &p, int D, hipStream_t s) {
-    // Tokens of a work-group: one where there are few, a page's rows for prompts. KV heads: so many that a page's rows
-    // are one or eight vectors for each of its lane groups.
+    // Tokens of a work-group: one where there are few, a page's rows for prompts. KV heads worked on together: so many that a
+    // page's rows are one or eight vectors for each of its lane groups. Few tokens may be one of each sequence or all of
+    // one page: two heads up to 32 tokens, one up to 64 (17 tokens of 3 sequences 17.0 -> 6.5 us with two in place of eight, 64
+    // of one 39.2 -> 8.2 with one, one each of 32 and 64 5.4 as before, all by a graph of 6 calls).
     const int per = 256 / (D / 8);   // lane groups
     p.chunk = p.n <= 256 ? 1 : min(p.P, 64);
-    p.hpg = max(1, min(min(p.Hk, MAX_HEADS), p.n <= 64 ? per / 2 : 4 * per / min(p.P, 64)));
+    p.hpg = max(1, min(min(p.Hk, MAX_HEADS), p.n <= 32 ? 2 : p.n <= 64 ? 1 : 4 * per / min(p.P, 64)));
     p.hgroups = (p.Hk + p.hpg - 1) / p.hpg;
-    const long long pages = (long long)(p.n + p.chunk - 1) / p.chunk * p.hgroups;
+    p.hloop = 1;
+    auto groups = [&] { return (long long)(p.n + p.chunk - 1) / p.chunk * ((p.hgroups + p.hloop - 1) / p.hloop); };
+    // Every work-group looks through all slots, so long prompts have fewer of them, but 1024 at least: all heads, then more
+    // pages (32768 tokens in pages of 64 78 -> 52 us, 131072 682 -> 230, in pages of 16 682 -> 329; with 512 8192 take 3 us more).
+    while (p.chunk > 1 && p.hloop < p.hgroups && groups() >= 2 * LONG_GROUPS) p.hloop *= 2;
+    while (p.chunk > 1 && 2 * p.chunk <= 64 && groups() >= 2 * LONG_GROUPS) p.chunk *= 2;
+    p.hwgs = (p.hgroups + p.hloop - 1) / p.hloop;
+    const long long pages = groups();
     const long long queries = FUSED ? ((long long)p.n * p.nq + per - 1) / per : 0;
     if ((pages + queries) * 256 > MAX_THREADS) return TI_ERR_UNSUPPORTED;
     p.page_groups = (unsigned)pages;
     const unsigned grid = (unsigned)(pages + queries);
-    if (D == 128) fp8_write_kernel<T, FUSED, NORM, 128><<<grid, 256, 0, s>>>(p);
-    else fp8_write_kernel<T, FUSED, NORM, 64><<<grid, 256, 0, s>>>(p);
+    const bool few = p.chunk == 1;
+    if (D == 128 && few) fp8_write_kernel<T, FUSED, NORM, 128, true><<<grid, 256, 0, s>>>(p);
+    else if (D == 128) fp8_write_kernel<T, FUSED, NORM, 128, false><<<grid, 256, 0, s>>>(p);
+    else if (few) fp8_write_kernel<T, FUSED, NORM, 64, true><<<grid, 256, 0, s>>>(p);
+    else fp8_write_kernel<T, FUSED, NORM, 64, false><<<grid, 256, 0, s>>>(p);
     return hipGetLastError() == hipSuccess ? TI_OK : TI_ERR_LAUNCH;
 }
 
