@@ -404,8 +404,8 @@ template <typename T, bool FUSED, bool NORM>
 int launch(Fp8WriteParams &p, int D, hipStream_t s) {
     // Tokens of a work-group: one where there are few, a page's rows for prompts. KV heads worked on together: so many that a
     // page's rows are one or eight vectors for each of its lane groups. Few tokens may be one of each sequence or all of
-    // one page: two heads up to 32 tokens, one up to 64 (17 tokens of 3 sequences 17.0 -> 6.5 us with two in place of eight, 64
-    // of one 39.2 -> 8.2 with one, one each of 32 and 64 5.4 as before, all by a graph of 6 calls).
+    // one page: two heads up to 32 tokens, one up to 64 (in place of eight: 17 tokens of 3 sequences 17.0 -> 6.5 us, 64
+    // of one 39.2 -> 8.2, one each of 32 and 64 5.4 as before, all in a graph of 6 calls).
     const int per = 256 / (D / 8);   // lane groups
     p.chunk = p.n <= 256 ? 1 : min(p.P, 64);
     p.hpg = max(1, min(min(p.Hk, MAX_HEADS), p.n <= 32 ? 2 : p.n <= 64 ? 1 : 4 * per / min(p.P, 64)));
