@@ -407,7 +407,8 @@ int ti_window_attention(const ti_attention_args *args, int window, int sinks, co
  * The pages of a pool and the sequences that hold them, as device arrays: what BlockManager (src/kv/block_manager.jl:39-100)
  * keeps on the host. A step can be reserved, run and taken back in one captured graph.
  * Page i of sequence b (positions i P .. i P + P - 1) is tables[b][i]. With a window, release gives back the pages that
- * no later query can see, those from page ceil(sinks / P) up to behind[b]; their entries are 0.
+ * no later query can see, those from page ceil(sinks / P) up to behind[b]; their entries are 0. (behind[b] starts as
+ * ceil(sinks / P). Over tables of which pages went back before, it counts them: entries in front of it are not given back again.)
  * Calls on one pool must not overlap. `ticket` is 0 between calls. */
 typedef struct {
     int32_t num_pages, page_size;

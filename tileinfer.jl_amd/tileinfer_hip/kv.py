@@ -195,10 +195,11 @@ class PagePool:
     reserve_pages_ and release_pages_ change them in place.
 
     window, sinks: of the attention over the cache (window_attention_); release_pages_ then gives back the pages that no later
-    query sees. `behind` [sequences] counts a sequence's pages up to the first that it still holds past its sinks."""
+    query sees. `behind` [sequences] int32 counts a sequence's pages up to the first that it still holds past its sinks: where
+    it is not given, it is taken from the tables, whose entries of pages that went back before are 0."""
 
     def __init__(self, free: torch.Tensor, free_count: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, page_size: int,
-                 window: int = 0, sinks: int = 0):
+                 window: int = 0, sinks: int = 0, behind: Optional[torch.Tensor] = None):
         if any(t.dtype != torch.int32 for t in (free, free_count, tables, lengths)) or free.dim() != 1 or free_count.numel() != 1 \
                 or tables.dim() != 2 or lengths.shape != tables.shape[:1]:
             raise ArgumentError("free, free_count, tables and lengths must be int32 [pages], [1], [sequences][width] and [sequences]")
@@ -206,8 +207,20 @@ class PagePool:
             raise ArgumentError("page_size must be positive, window and sinks not negative")
         self.free, self.free_count, self.tables, self.lengths = free, free_count, tables, lengths
         self.page_size, self.window, self.sinks = int(page_size), int(window), int(sinks)
-        self.behind = torch.full_like(lengths, -(-self.sinks // self.page_size)) if window else None
+        if behind is not None and (not window or behind.dtype != torch.int32 or behind.shape != lengths.shape):
+            raise ArgumentError("behind must be int32 [sequences], of a pool with a window")
+        self.behind = self._behind() if window and behind is None else behind
         self.ticket = torch.zeros(1, dtype=torch.int32, device=free.device)
+
+    def _behind(self) -> torch.Tensor:
+        first = -(-self.sinks // self.page_size)            # pages of sinks
+        none = torch.full_like(self.lengths, first)
+        if first >= self.tables.shape[1]:
+            return none
+        held = self.tables[:, first:] > 0
+        # no page held past the sinks: all that the length reaches into went back
+        all_back = torch.maximum(none, ((self.lengths.long() + (self.page_size - 1)) // self.page_size).to(torch.int32))
+        return torch.where(held.any(1), first + held.int().argmax(1).to(torch.int32), all_back)
 
 
 def page_pool(num_pages: int, page_size: int, num_seqs: int, max_pages: int, window: int = 0, sinks: int = 0, device="cuda") -> PagePool:
