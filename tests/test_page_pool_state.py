@@ -93,3 +93,18 @@ def test_taken_over(gpu, P, window, sinks, given):
         if r in (3, 8):
             b = ti.PagePool(*(t.clone() for t in (a.free, a.free_count, a.tables, a.lengths)), P, window, sinks,
                             **(dict(behind=a.behind.clone()) if given else {}))
+
+
+@pytest.mark.parametrize("what", [dict(window=2 ** 32 + 40), dict(window=2 ** 31), dict(window=40, sinks=2 ** 32), dict(sinks=2 ** 31),
+                                  dict(page_size=2 ** 32 + 16), dict(window=39.5), dict(window=40, sinks=0.5), dict(page_size=16.5),
+                                  dict(window=True), dict(window=-1), dict(sinks=-1), dict(page_size=0)])
+def test_numbers_that_the_library_does_not_hold(what):
+    """A window of 2^32 + 40 would be one of 40 in 32 bits, and pages that later queries see would go back."""
+    with pytest.raises(ti.ArgumentError):
+        ti.page_pool(10, **dict(dict(page_size=16, num_seqs=2, max_pages=4, device="cpu"), **what))
+
+
+def test_whole_numbers_of_other_types():
+    p = ti.page_pool(10, np.int64(16), 2, 4, np.int32(40), 4.0, device="cpu")
+    assert (p.page_size, p.window, p.sinks) == (16, 40, 4) and all(type(x) is int for x in (p.page_size, p.window, p.sinks))
+    assert ti.page_pool(10, 16, 2, 4, 2 ** 31 - 1, 2 ** 31 - 1, device="cpu").window == 2 ** 31 - 1

@@ -203,8 +203,8 @@ class PagePool:
         if any(t.dtype != torch.int32 for t in (free, free_count, tables, lengths)) or free.dim() != 1 or free_count.numel() != 1 \
                 or tables.dim() != 2 or lengths.shape != tables.shape[:1]:
             raise ArgumentError("free, free_count, tables and lengths must be int32 [pages], [1], [sequences][width] and [sequences]")
-        if page_size <= 0 or window < 0 or sinks < 0:
-            raise ArgumentError("page_size must be positive, window and sinks not negative")
+        if any(isinstance(x, bool) or int(x) != x or not low <= x < 1 << 31 for x, low in ((page_size, 1), (window, 0), (sinks, 0))):
+            raise ArgumentError("page_size must be a whole number from 1 on, window and sinks from 0 on")
         self.free, self.free_count, self.tables, self.lengths = free, free_count, tables, lengths
         self.page_size, self.window, self.sinks = int(page_size), int(window), int(sinks)
         if behind is not None and (not window or behind.dtype != torch.int32 or behind.shape != lengths.shape):
