@@ -155,11 +155,14 @@ struct TilePages {
 // The block-table entries (1-based page ids, unclamped) of tile kt's two 16-key halves, as
 // scalar loads: their consumer clamps them (clamp_page), so the wait for these loads can sit
 // where the pages are used, a step later, instead of right after the loads.
-__device__ __forceinline__ TilePages raw_pages(const PrefillParams &p, const int32_t *bt, int kt) {
+// wt: WIN, the tiles that the work-group's rows see.
+template <bool WIN = false>
+__device__ __forceinline__ TilePages raw_pages(const PrefillParams &p, const int32_t *bt, int kt, const WindowTiles &wt = WindowTiles{}) {
     TilePages tp;
 #pragma unroll
     for (int x = 0; x < 2; x++) {
-        const int idx = min((kt * KT + 16 * x) >> p.pshift, p.bt_stride - 1);   // PG16: P = 2^pshift; kt >= 0
+        const int half = WIN && kt == wt.unseen(x, p.sinks) ? x ^ 1 : x;
+        const int idx = min((kt * KT + 16 * half) >> p.pshift, p.bt_stride - 1);   // PG16: P = 2^pshift; kt >= 0
         tp.pg[x] = sload(bt, idx);
     }
     return tp;
@@ -663,12 +666,12 @@ __global__ void __launch_bounds__(64 * WPG * NG) prefill_kernel(PrefillParams p)
         // the tile after next at its end, so the scalar loads' wait falls on the closing
         // barrier instead of on the step's LDS reads
         const int ft = min(tile_of(0), kt_hi - 1);
-        TilePages pn = !WIN && p.splits == 1 && ft == grp ? spec : raw_pages(p, bt, actual(ft));
+        TilePages pn = !WIN && p.splits == 1 && ft == grp ? spec : raw_pages<WIN>(p, bt, actual(ft), wt);
         auto issue = [&](int i, int buf) {
             if (i < steps) dl_load(min(tile_of(i), kt_hi - 1), buf, pn);
         };
         auto next_pages = [&](int i) {
-            if (i < steps) pn = raw_pages(p, bt, actual(min(tile_of(i), kt_hi - 1)));
+            if (i < steps) pn = raw_pages<WIN>(p, bt, actual(min(tile_of(i), kt_hi - 1)), wt);
         };
         issue(0, 0);
         next_pages(1);

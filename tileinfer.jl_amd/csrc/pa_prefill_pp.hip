@@ -158,11 +158,25 @@ prefill_pp_kernel(PPParams p) {
     struct Pages {
         int pg[NH];
     };
+    int unseen[NH];   // WIN: WindowTiles::unseen of the halves
     auto half_pos = [&](int kt, int x) { return kt * KT + 16 * (NH == 2 ? x : wave_half); };
-    auto pages_at = [&](int kt) {
+    auto entries = [&](int kt) {   // indexes into the block table of a tile's halves
         Pages r;
 #pragma unroll
-        for (int x = 0; x < NH; x++) r.pg[x] = sload(bt, min(half_pos(kt, x) >> p.pshift, p.bt_stride - 1));
+        for (int x = 0; x < NH; x++) {
+            int pos = half_pos(kt, x);
+            if constexpr (WIN) {
+                const int at = NH == 2 ? 16 * x : 16 * wave_half;
+                pos = kt * KT + (kt == unseen[x] ? 16 - at : at);
+            }
+            r.pg[x] = min(pos >> p.pshift, p.bt_stride - 1);
+        }
+        return r;
+    };
+    auto pages_at = [&](int kt) {
+        Pages r = entries(kt);
+#pragma unroll
+        for (int x = 0; x < NH; x++) r.pg[x] = sload(bt, r.pg[x]);
         return r;
     };
     // Without key splits the first tiles' entries do not depend on the sequence's position:
@@ -190,6 +204,8 @@ prefill_pp_kernel(PPParams p) {
     if constexpr (WIN) {
         wt = WindowTiles::of<5>(start + t_first, p.window, p.sinks);
         nkt -= wt.skip;
+#pragma unroll
+        for (int x = 0; x < NH; x++) unseen[x] = wt.unseen(NH == 2 ? x : wave_half, p.sinks);
     }
     const int per = (nkt + p.splits - 1) / p.splits;
     const int kt_lo = min(split * per, nkt), kt_hi = min(kt_lo + per, nkt);
@@ -321,6 +337,7 @@ prefill_pp_kernel(PPParams p) {
     // younger loads).
     Bases bs[4];                                   // bases of tiles i + 1 .. i + 3 in 1 .. 3
     Pages raw4;                                    // block-table entries of tile i + 4
+    Pages ahead{};                                 // WIN: where those of tile i + 5 are, found ahead of the softmax that hides their loads
     bf16x8 qreg[NQB];
     float back = 1.0f;   // F16
     {
@@ -356,6 +373,7 @@ prefill_pp_kernel(PPParams p) {
         }
         __builtin_amdgcn_sched_barrier(0);
         raw4 = pages_at(tile(4));
+        if constexpr (WIN) ahead = entries(tile(5));
 #pragma unroll
         for (int u = 0; u < NC; u++) store_k(k0[u], 0, u, 0);
         if constexpr (INT8) store_s(s0, 0);
@@ -554,8 +572,14 @@ prefill_pp_kernel(PPParams p) {
     };
     auto phase_y = [&](int i) {
         if constexpr (FP8) sc8[3] = scales(raw4);   // tile i + 4's
-        raw4 = pages_at(tile(i + 5));
+        if constexpr (WIN) {
+#pragma unroll
+            for (int x = 0; x < NH; x++) raw4.pg[x] = sload(bt, ahead.pg[x]);
+        } else {
+            raw4 = pages_at(tile(i + 5));
+        }
         softmax(i);
+        if constexpr (WIN) ahead = entries(tile(i + 6));
         // the lookup's wait falls here, where the barrier waits for LDS anyway
         asm volatile("" : "+s"(raw4.pg[0]));
         if constexpr (NH == 2) asm volatile("" : "+s"(raw4.pg[NH - 1]));

@@ -43,6 +43,13 @@ struct WindowTiles {
         return t;
     }
     __device__ __forceinline__ int tile(int j) const { return j < sunk ? j : j + skip; }
+    // The 32-key tile whose half x no row sees, or -1: with x = 1 the last one of sinks, with x = 0 the window's first. Such a
+    // half's page may have been given back and be anyone's, so the other half's is read in its place (halves in pages of more
+    // than 16 keys share a page anyhow).
+    __device__ __forceinline__ int unseen(int x, int sinks) const {
+        const int kt = x ? sunk - 1 : sunk + skip, pos = kt * 32 + 16 * x;
+        return kt >= 0 && pos >= sinks && pos + 16 <= lo ? kt : -1;
+    }
 };
 
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
