@@ -18,8 +18,8 @@ class _Window(ctypes.Structure):
 
 
 def pick(kv, lens, window, sinks, D, H, G, P):
-    """The form of the ping-pong kernel that a windowed step over a bf16, INT8 or 8-bit block cache takes, tables as wide as the
-    longest sequence (as window_ref.Step makes them)."""
+    """The form of the ping-pong kernel that a step over a bf16, INT8 or 8-bit block cache takes (window 0: none), tables as wide
+    as the longest sequence (as window_ref.Step makes them)."""
     f = getattr(ti.load_library(), "_Z18ti_pick_prefill_ppPK17ti_attention_argsPK11ti_kv_cacheib9ti_window")
     f.restype, f.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_bool, _Window]
     c = _lib.KVCache()
@@ -64,7 +64,8 @@ FORMS = [
 
 
 def want(s):
-    """s.want() of a window_ref.Step with a causal window, by whole sequences, in float64 on the GPU."""
+    """s.want() of a window_ref.Step, causal, by whole sequences, in float64 on the GPU."""
+    window = s.window or 1 << 30
     q = s.q.double().cuda()
     out, size = torch.zeros_like(q), torch.zeros_like(q)
     at = 0
@@ -76,7 +77,7 @@ def want(s):
         held = np.zeros(c + n, bool)
         held[s.rows[b]] = True
         key, pos = torch.arange(c + n, device="cuda"), torch.arange(c, c + n, device="cuda")[:, None]
-        sees = ((key <= pos) & ((key > pos - s.window) | (key < s.sinks))).repeat_interleave(s.G, 0)
+        sees = ((key <= pos) & ((key > pos - window) | (key < s.sinks))).repeat_interleave(s.G, 0)
         for h in range(s.H):
             k, v = (torch.from_numpy(np.where(held[:, None], x[page, h, off], 0.0)).cuda() for x in (s.layer.k, s.layer.v))
             heads = slice(h * s.G, (h + 1) * s.G)
