@@ -90,7 +90,7 @@ struct DecodeParams {
 struct FlatPiece {
     int b, lo, n, tok0, nb, start;
 };
-template <bool SAFE = false, bool WIN = false>
+template <bool SAFE = false>
 __device__ inline FlatPiece flat_piece(const DecodeParams &p, int x, int lane) {
     int tok0 = 0, nb = 0, st = 0, nt = 0;
     if (lane < p.B) {
@@ -99,7 +99,6 @@ __device__ inline FlatPiece flat_piece(const DecodeParams &p, int x, int lane) {
         if (nb > 0) {
             st = SAFE ? first_position(p.positions[tok0], p.bt_stride, p.P) : max(p.positions[tok0], 0);
             nt = (st + nb + 15) >> 4;
-            if constexpr (WIN) nt -= WindowTiles::of<4>(st, p.window, p.sinks).skip;
         }
     }
     int incl = nt;
@@ -406,8 +405,8 @@ __global__ void __launch_bounds__(NW * 64, GROUP && INT8 && ROWB == 2 ? 2 : 1) d
                     *reinterpret_cast<u32x2 *>(p.out + ((size_t)tok0 * p.Hq + h * p.G) * D + 4 * i) = (u32x2){0u, 0u};
             return;
         }
-    } else if (p.flat) {
-        const FlatPiece f = flat_piece<SAFE, WIN>(p, blockIdx.x, lane);
+    } else if (!WIN && p.flat) {   // (windowed steps are not shared out by length)
+        const FlatPiece f = flat_piece<SAFE>(p, blockIdx.x, lane);
         b = f.b;
         s = blockIdx.x - f.lo;
         nsp = f.n;
