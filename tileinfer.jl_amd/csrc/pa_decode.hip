@@ -157,7 +157,7 @@ ti_decode_plan ti_plan_decode(const ti_attention_args *a, const ti_kv_cache *c, 
     int sp = 1, nw = 4;
     if (pairs < 256 || pl.rows > 32) {
         while (sp < max_splits && pairs * sp < target) sp <<= 1;
-        // A window bounds the keys: no more splits than leave every wave of each a tile.
+        // A window bounds the keys: the fewest splits (powers of two) that have a wave for each 16-key tile.
         const long long tiles = ((long long)win.size + a->max_query_len + 30) / 16 + ((long long)win.sinks + 15) / 16;
         while (win.size && sp > 1 && 4LL * (sp / 2) >= tiles) sp >>= 1;
     }
@@ -168,8 +168,8 @@ ti_decode_plan ti_plan_decode(const ti_attention_args *a, const ti_kv_cache *c, 
     // box): B = 8 (4 splits) 31.0 -> 27.5 us, B = 4 (8 splits) 21.3 vs 21.3 us, but B = 2
     // (16 splits) 16.0 -> 16.9 us and B = 16 (2 splits) 60.8 -> 63.0 us, where the shares
     // balance little and the device-side prefix costs its latency.
-    // Not with a window: sequences longer than it hold equally many keys, and finding the shares costs its latency (8 INT8
-    // sequences of 8000 to 32767 keys, window 8192: 39.1 -> 32.1 us).
+    // Not with a window: sequences longer than it hold equally many keys, and finding the shares costs its latency (pa_window.hip
+    // has the figure).
     pl.flat = sp >= 4 && a->num_seqs >= 4 && a->num_seqs <= 64 && !win.size ? sp * a->num_seqs : 0;
     pl.splits = sp;
     pl.waves = nw;
