@@ -10,7 +10,11 @@
 // Bound: a prompt's bytes (2 + 1 per element of k and v), one token's chain slots -> rows -> largest -> rows out. Measured
 // (8 heads of 128, bf16): 8192 tokens into pages of 16 16.4 us, 3.05 TB/s (rows stay in registers between the two passes; 34.8 us
 // with rows read twice): slots -> page's list -> rows -> largest -> rows out go one after the other in a work-group, and two
-// rounds of work-groups fill the CUs; one token for each of 32 sequences 4.0 us, of which 1.9 are a launch.
+// rounds of work-groups fill the CUs; one token for each of 32 sequences 4.0 us, of which 1.9 are a launch. Two forms read full
+// pages twice, as their rows do not fit the registers (KEEP below): Float32 rows (26.3 us, 3.2 TB/s) and fused calls, which norm and
+// rotate each key twice too (32 query heads, 8192 tokens into pages of 16 84 us, of 64 94, where the dense cache's fused write
+// takes 40 and INT8's 47; a token for each of 32 sequences 4.9). A work-group has all of a page, so large pages leave CUs idle: 8192
+// tokens into pages of 64 / 128 / 256 / 1024 16.3 / 27 / 47 / 160 us, fused into pages of 1024 655.
 //
 // The fused kernel rotates queries and keys with every rounding of attention_inputs_v_kernel (kv_write.hip), so it is
 // bit-identical to rmsnorm, rope and store_kv in a row: products and sums are rounded one by one.
@@ -361,7 +365,8 @@ __global__ void __launch_bounds__(256) fp8_write_kernel(Fp8WriteParams p) {
                         *at16 = w;
                     }
                 };
-                // KEEP vectors of a lane group stay in registers between the passes, loaded together; more are read twice.
+                // KEEP vectors of a lane group stay in registers between the passes, loaded together; more are read twice (a full page
+                // is 8: bf16 rows fit, Float32 and rotated ones do not).
                 auto rows = [&](auto keep) {
                     constexpr int KEEP = decltype(keep)::value;
                     Held<T> x[KEEP];

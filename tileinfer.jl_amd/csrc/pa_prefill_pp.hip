@@ -1,7 +1,8 @@
 // Paged causal / chunked / non-causal prefill attention, ping-pong form (gfx950, bf16
 // MFMA, dense bf16 or INT8 cache, head_dim 64 or 128, power-of-two pages of >= 16 tokens; FP8, WIN: 8-bit block caches
-// and windows, pa_window.hpp: 1500 tokens on 3000 keys of an 8-bit block cache 115 us, 800 TFLOP/s; a prompt of 8192
-// tokens with a window of 2048 260-273 us, 882-925 TFLOP/s).
+// and windows, pa_window.hpp: 1500 tokens on 3000 keys of an 8-bit block cache 115 us, 800 TFLOP/s, and 126 us with block
+// tables wider than sixteen steps; a prompt of 8192 tokens with a window of 2048 257-269 us, 895-935 TFLOP/s, over INT8 347 and 8-bit
+// blocks 285).
 //
 // Reference: attention_prefill_kernel / prefill_body (src/ops/tile/attention.jl:130-177)
 // and attention_prefill_int8_kernel (:139-147). Query t of the step sits at position
