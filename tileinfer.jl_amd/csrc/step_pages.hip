@@ -134,15 +134,16 @@ __global__ void __launch_bounds__(NT) reserve_kernel(PoolParams p) {
     // page r of the step's: from the top of the stack down
     auto page_at = [&](int r) { return pool.free[have - 1 - r]; };
     if (ok) {
-        for (int r = wg * NT + (int)threadIdx.x; r < (int)pages; r += wgs * NT) {
+        for (uint32_t r = wg * NT + threadIdx.x; r < pages; r += wgs * NT) {   // (32 bits with no sign: a step further does not wrap)
             const int b = find(s.b, S, r);
             const int held = pages_of(p, s.old[b]);
-            pool.tables[(size_t)b * pool.table_width + held + (r - s.b[b])] = page_at(r);
+            pool.tables[(size_t)b * pool.table_width + held + ((int)r - s.b[b])] = page_at((int)r);
         }
     }
     // Neighbouring tokens mostly share a sequence and a page: the chain of loads is walked once for them.
     const bool whole = ((((uintptr_t)p.positions | (uintptr_t)p.slots) & 15) == 0);
-    for (int t0 = EACH * (wg * NT + (int)threadIdx.x); t0 < p.tokens; t0 += EACH * wgs * NT) {
+    for (uint32_t u0 = EACH * (wg * NT + threadIdx.x); u0 < (uint32_t)p.tokens; u0 += EACH * wgs * NT) {
+        const int t0 = (int)u0;
         int pos[EACH], slot[EACH];
 #pragma unroll
         for (int e = 0; e < EACH; e++) pos[e] = slot[e] = 0;
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(NT) reserve_kernel(PoolParams p) {
             }
         }
         if constexpr (EACH == 4) {
-            if (whole && t0 + 4 <= p.tokens) {
+            if (whole && t0 <= p.tokens - 4) {
                 *reinterpret_cast<int4 *>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
                 *reinterpret_cast<int4 *>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
                 continue;
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(NT) reserve_kernel(PoolParams p) {
         }
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
-            if (t0 + e < p.tokens) p.positions[t0 + e] = pos[e], p.slots[t0 + e] = slot[e];
+            if (t0 < p.tokens - e) p.positions[t0 + e] = pos[e], p.slots[t0 + e] = slot[e];
         }
     }
     if (!last_to_end(pool.ticket) || !ok) return;
@@ -231,8 +232,8 @@ __global__ void __launch_bounds__(NT) release_kernel(PoolParams p) {
         n = 0;
     });
     const int all = (int)min(pages, (uint32_t)(pool.num_pages - have));   // never above the stack's room
-    for (int r = blockIdx.x * NT + (int)threadIdx.x; r < all; r += gridDim.x * NT) {
-        const int b = find(s.a, S, r);
+    for (uint32_t r0 = blockIdx.x * NT + threadIdx.x; r0 < (uint32_t)all; r0 += gridDim.x * NT) {
+        const int r = (int)r0, b = find(s.a, S, r);
         int32_t *e = pool.tables + (size_t)b * pool.table_width + gone_of(p, b).entry(r - s.a[b]);
         pool.free[have + all - 1 - r] = *e;
         *e = 0;
