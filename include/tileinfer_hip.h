@@ -83,9 +83,9 @@ typedef enum {
  *
  * 8-bit block layers (TI_KV_FP8) hold e4m3 values and one scale for each block, the keys (or the values)
  * of a page and KV head: a value stands for itself times the scale, a power of two between 2^-120 and 2^120.
- * head_dim 64 or 128, pages of 2^k keys from 16 to 1024. ti_store_kv and ti_attention_inputs write them,
- * ti_attention, ti_attention_noalloc and ti_window_attention read them; page bounds and sparse attention do not
- * take them (TI_ERR_UNSUPPORTED). `path` names no variants for them: other than TI_PATH_DECODE, the library's pick
+ * head_dim 64 or 128, pages of 2^k keys from 16 to 1024, block tables of at most 2^30 positions. ti_store_kv and
+ * ti_attention_inputs write them, ti_attention, ti_attention_noalloc and ti_window_attention read them; page bounds and sparse
+ * attention do not take them (TI_ERR_UNSUPPORTED). `path` names no variants for them: other than TI_PATH_DECODE, the library's pick
  * runs. Where a product meets a value that is not finite, the rows of its work-group are done again key by
  * key over what each of them sees (as in ti_window_attention): slow, and right. */
 typedef struct {
@@ -391,8 +391,8 @@ int ti_verify_draft(const ti_verify_args *args, void *stream);
  * ti_attention with causal = 1, where the query at position p sees the keys p - window + 1 .. p and the keys
  * 0 .. sinks - 1 (never past p): window >= 1, sinks >= 0. Arguments, caches and steps as in ti_attention (path:
  * TI_PATH_AUTO; workspace of ti_window_attention_workspace_bytes, which depends on the window too, mandatory
- * where that is not 0). Block-table entries of pages that hold no visible key of any of the sequence's queries are not
- * used: their pages may have been given back. Rows of q and out that belong to no sequence are left as they were.
+ * where that is not 0; block tables of at most 2^30 positions). Block-table entries of pages that hold no visible key of any
+ * of the sequence's queries are not used: their pages may have been given back. Rows of q and out that belong to no sequence are left as they were.
  *
  * A key that a query does not see leaves its output as it is whatever the cache holds there, NaN and infinities
  * among it. The rows of a work-group are worked on together, so where a product is not finite they are done

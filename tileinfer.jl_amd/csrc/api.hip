@@ -50,6 +50,11 @@ bool odd_fp8(const ti_kv_cache *c) {
     return c->kind == TI_KV_FP8 && ((c->head_dim != 64 && c->head_dim != 128) || P < 16 || P > 1024 || (P & (P - 1)));
 }
 
+// Block tables of more positions than the windowed and 8-bit kernels count (first_position, pa_window.hpp).
+bool too_wide(const ti_attention_args *a, const ti_kv_cache *c) {
+    return (long long)a->block_table_stride * c->page_size > 1LL << 30;
+}
+
 bool bad_dtype(int dtype) { return dtype != TI_F32 && dtype != TI_BF16; }
 
 // Resolve the kernel family of an attention call: 0 generic (fp32), 1 decode, 2 prefill,
@@ -92,7 +97,7 @@ int check_attention(const ti_attention_args *a, const ti_kv_cache *c) {
     if (!(a->scale > 0.0f) || a->scale == INFINITY) return TI_ERR_INVALID_ARG;
     // launch grids put sequences in a dimension of at most 65535
     if (a->num_seqs > 65535) return TI_ERR_UNSUPPORTED;
-    return TI_OK;
+    return c->kind == TI_KV_FP8 && too_wide(a, c) ? TI_ERR_UNSUPPORTED : TI_OK;
 }
 
 bool misaligned(const void *p) { return ((uintptr_t)p & 15) != 0; }
@@ -184,7 +189,7 @@ int check_window(const ti_attention_args *a, int window, int sinks, const ti_kv_
     const int st = check_attention(a, c);
     if (st) return st;
     if (window < 1 || sinks < 0 || !a->causal) return TI_ERR_INVALID_ARG;
-    return a->path != TI_PATH_AUTO ? TI_ERR_UNSUPPORTED : TI_OK;
+    return a->path != TI_PATH_AUTO || too_wide(a, c) ? TI_ERR_UNSUPPORTED : TI_OK;
 }
 
 int check_pool(const ti_page_pool *p) {
