@@ -191,13 +191,14 @@ int ti_attention_noalloc(const ti_attention_args *args, const ti_kv_cache *cache
  * src/ops/reference.jl:64-74, src/ops/quant.jl:147-159).
  * k, v: [n][Hk][D] in dtype. Slots outside the pool are skipped.
  *
- * 8-bit block layers: a block's scale is the least 2^e (e from -120 to 120) with |x| <= 448 2^e for every finite
- * element that its rows were written with, and a row holds x 2^-e rounded to the nearest e4m3 value (ties to even);
- * an element that is not finite is held as NaN, one of 248 2^120 (3.3e38) or more as 2^128, infinity in 32 bits. Rows are written from a page's first on: a call that writes a page's
- * first row begins the block anew, with the scale of this call's rows alone (other rows of the page then hold
- * nothing). Otherwise the scale only grows; where it does, the rows that the block holds are divided by the
- * growth, which is exact but for values that become subnormal (each time rounded again, by at most 2^-10 of the
- * new scale). The rows of one page may be anywhere among the call's; of two for one slot the later stays.
+ * 8-bit block layers: a block's scale is the least 2^e (e from -120 to 120) with |x| <= 448 2^e for every finite element
+ * that its rows were written with, and a row holds x 2^-e rounded to the nearest e4m3 value (ties to even); an element
+ * that is not finite is held as NaN, one of 248 2^120 (3.3e38) or more as 2^128, infinity in 32 bits. Rows are written
+ * from a page's first on: a call that writes a page's first row begins the block anew, with the scale of this call's rows
+ * alone (other rows of the page then hold nothing). Otherwise the scale only grows; where it does, the rows that the
+ * block holds are divided by the growth, which is exact but for values that become subnormal (each time rounded again, by
+ * at most 2^-10 of the new scale). The rows of one page may be anywhere among the call's; of two for one slot the later
+ * stays.
  */
 int ti_store_kv(int dtype, const ti_kv_cache *cache, const void *k, const void *v,
                 const int32_t *slots, int n, void *stream);

@@ -123,8 +123,8 @@ bool reaches_all(const ti_attention_args *a, const ti_kv_cache *c, ti_window win
 int window_prefill(const ti_attention_args *a, const ti_kv_cache *c, ti_window win, bool bound_keys, ti_prefill_plan *pl) {
     if (a->q_heads / c->kv_heads > 64) return TI_ERR_UNSUPPORTED;
     // without hidden keys the small causal steps have the 16-row kernel (unsplit), whose pairs of q-tiles share their
-    // keys (512 tokens 13.1 -> 9.6 us, INT8 17.7 -> 12.3); the pools aligned for its direct loads
-    if (bound_keys && reaches_all(a, c, win) && !misaligned(c->k_pages) && !misaligned(c->v_pages)) {
+    // keys (512 tokens 13.1 -> 9.6 us, INT8 17.7 -> 12.3)
+    if (bound_keys && reaches_all(a, c, win)) {
         *pl = prefill_plan(a, c, true);
         if (pl->r16 && prefill_grid_y(*pl) <= 65535) return TI_OK;
     }

@@ -1473,7 +1473,7 @@ ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c
     // (1024-3072 tokens) no change, so those keep the register-staged loads.
     const bool dl_ok = c->kind == TI_KV_DENSE && a->dtype == TI_BF16 && c->head_dim == 128 &&
                        c->page_size >= 16 && (c->page_size & (c->page_size - 1)) == 0 &&
-                       (!win.size || (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15) == 0);
+                       (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15) == 0;   // direct loads: whole 16 bytes
     pl.dl = dl_ok && (a->path == TI_PATH_PREFILL_DIRECT || a->path == TI_PATH_PREFILL_PAIRED ||
                       a->path == TI_PATH_PREFILL_PAIRED16 ||
                       (a->path != TI_PATH_PREFILL_STAGED && pl.wpg == 2));
@@ -1494,7 +1494,8 @@ ti_prefill_plan ti_plan_prefill(const ti_attention_args *a, const ti_kv_cache *c
     const bool pair_ok = (dl_ok || i8_ok) && a->causal && pl.splits == 1 && 32 % G == 0 && !win.size;
     // (32 % G == 0 in pair_ok: G <= 32, so 32 / G >= 1)
     const long long pair_wgs = pair_ok ? pairs * (((a->max_query_len + 32 / G - 1) / (32 / G) + 1) / 2) : 0;
-    pl.r16 = pair_ok && (a->path == TI_PATH_PREFILL_PAIRED16 || (auto_path && R16_BY_DEFAULT && pair_wgs <= 512));
+    // (its queries come through direct loads for every kind of cache)
+    pl.r16 = pair_ok && ((uintptr_t)a->q & 15) == 0 && (a->path == TI_PATH_PREFILL_PAIRED16 || (auto_path && R16_BY_DEFAULT && pair_wgs <= 512));
     pl.pair = pl.r16 || (pair_ok && dl_ok && pl.dl && pl.wpg == 2 && pl.ng == 4 &&
                          (a->path == TI_PATH_PREFILL_PAIRED || (auto_path && PAIR_BY_DEFAULT)));
     if (pl.pair) {
